@@ -580,6 +580,87 @@ int mzk_sparse_mqa_noalloc(const void* q, int64_t B, int64_t S, int H, int D, in
                            void* out, float* lse, const void* rope_cos, const void* rope_sin, int rope_dim,
                            void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Pages and packed sequences: the caches and prompts of a server that runs many sequences of
+ * different lengths.  No counterpart in the reference, whose caches are one tensor per batch
+ * (owlet1/cache.py:84-124) and whose prompts are [B, S].
+ *
+ * A pool holds `pages` pages of `page` entries.  A sequence's table row (int32, row stride
+ * table_stride) names its pages in order, -1 where there is none; its tokens are the first
+ * lens[b] (int64) entries.  refs[p] (int32) counts the table entries that name page p and whatever
+ * else holds it; a page of refs 0 is free.  Table entries outside [0, pages) name no page: nothing
+ * is read or written there.  Packed sequences: cu int64 [B + 1], ascending from 0; sequence b's
+ * tokens are rows cu[b] .. cu[b + 1] - 1.  Everything is read on the device, so calls can be captured.
+ * --------------------------------------------------------------------------------- */
+
+/* Entries of new tokens, the cache write of DeepseekV41CSACache.update (owlet1/cache.py:84-94) into
+ * pages: the i-th of sequence b's n new rows of x (cu NULL: one row per sequence) becomes the entry
+ * at position lens[b] - n + i (lens counts the new tokens).  Positions below 0, past the table or on
+ * no page are skipped.  x [T, D] of `dtype`, rows x_row_stride elements apart; fmt 0: bf16 entries,
+ * 1: FP8-b128 entries (as mzk_pack_latent_fp8_b128; nope a multiple of 128, D - nope in bf16).
+ * D a multiple of 8; pool 16-byte aligned.  No two tokens may have the same entry. */
+int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_row_stride, const int64_t* cu, int64_t B,
+                     const int32_t* tables, int64_t table_stride, int64_t max_pages, const int64_t* lens, int fmt,
+                     int D, int nope, void* pool, int64_t pages, int page, void* stream);
+
+/* The workspace (16-byte aligned, no initialization) that mzk_paged_grow, _fork and _compact take. */
+int mzk_paged_workspace_bytes(int64_t B, int64_t max_pages, int64_t pages, int64_t* bytes);
+
+/* Room for tokens[b] (int64, >= 0) more tokens of each sequence: the lowest free pages, in the order
+ * of the sequences, and lens + tokens.  A partly filled last page that others hold too (refs > 1) is
+ * replaced by a fresh one, and its filled entries are copied in each of the npools pools (host
+ * arrays of base pointers and of bytes per entry, a multiple of 4).  Either every sequence gets its pages or none
+ * does: *missing (int64 on the device) is 0, or the pages that lack, and then nothing changes.
+ * The outputs may be the inputs. */
+int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages, const int64_t* lens,
+                   const int32_t* refs, int64_t pages, const int64_t* tokens, int page, void* const* pools,
+                   const int64_t* entry_bytes, int npools, int32_t* tables_out, int64_t table_out_stride,
+                   int64_t* lens_out, int32_t* refs_out, int64_t* missing, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Sequence i of the rows_out new ones goes on from the tokens of sequence parents[i] (int32; outside
+ * [0, B): from none): it holds the same pages, as far as they hold tokens, and the old sequences hold
+ * theirs no longer -- the paged form of reorder_cache, batch_repeat_interleave and
+ * batch_select_indices (and of freeing, with parent -1).  The outputs may be the inputs (rows_out ==
+ * B); then, and only then, the workspace is needed. */
+int mzk_paged_fork(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages, const int64_t* lens,
+                   const int32_t* refs, int64_t pages, const int32_t* parents, int64_t rows_out, int page,
+                   int32_t* tables_out, int64_t table_out_stride, int64_t* lens_out, int32_t* refs_out,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The used pages moved to the front: of U used ones, the k-th behind page U - 1 moves to the k-th free
+ * one before page U, in the tables, the counts and each of the pools.  The outputs may be the inputs. */
+int mzk_paged_compact(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages, const int32_t* refs,
+                      int64_t pages, int page, void* const* pools, const int64_t* entry_bytes, int npools,
+                      int32_t* tables_out, int64_t table_out_stride, int32_t* refs_out, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Attention of new tokens over their sequences' pages, K == V, scale D^-0.5, sinks as mzk_sparse_mqa.
+ *   q [T, H, D] bf16: one token per sequence (cu NULL, T == B), or the last cu[b+1] - cu[b] tokens of
+ *   each.  Token i of n is at position lens[b] - n + i and sees the positions up to its own, the last
+ *   `window` of them (0: all), or, with idx (int32 [B, idx_row_stride], one token per sequence, window
+ *   0), the positions idx[b, :topk] (outside [0, lens[b]): empty) -- an indexer's selection.
+ *   Positions on no page are empty; a token that sees nothing gets 0, and the sink (or -inf) as lse.
+ *   fmt 0: bf16 entries (D 64, 96, 128, 160, 256, 512, 576), 1: FP8-b128 (512 + 64, 128 + 32).
+ *   out [T, H, D] bf16, lse [T, H] fp32; rows behind the last sequence are left as they are, or, with
+ *   zero_tail, become 0 (lse -inf).
+ *   workspace: mzk_paged_attend_workspace_bytes (16-byte aligned, no initialization). */
+int mzk_paged_attend(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, int fmt, int nope,
+                     const void* pool, int64_t pages, int page, const int32_t* tables, int64_t table_stride,
+                     int64_t max_pages, const int64_t* lens, const int32_t* idx, int64_t idx_row_stride, int topk,
+                     int64_t window, const float* sinks, void* workspace, int64_t workspace_bytes, void* out,
+                     float* lse, int zero_tail, void* stream);
+int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t* bytes);
+
+/* Causal attention over packed prompts: the latent_attn and swa_attn levels
+ * (layers/attn/latent_attn/fwd.py:45, layers/attn/swa_attn/fwd.py:55) without padding.  q [T, H, D]
+ * bf16; kv [T, G, D] bf16 with rows kv_row_stride elements apart (a multiple of 8), head h attends
+ * latent h / (H / G); token i of its sequence sees tokens 0 .. i of it, the last `window` of
+ * them (0: all).  The rest as mzk_paged_attend. */
+int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, const void* kv,
+                   int64_t kv_row_stride, int G, int64_t window, const float* sinks, void* out, float* lse,
+                   int zero_tail, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

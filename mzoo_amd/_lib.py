@@ -88,6 +88,15 @@ _SIGS = {
     "mzk_decode_emit_pair": [_P, _I64, _P, _P, _P, _P, _I32, _P, _F32, _P, _I64, _I64, _P, _P, _F32, _I32, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _F32, _P, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _P, _F32, _P, _I64, _I64, _P],
     "mzk_sparse_mqa_noalloc": [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _I32, _I32, _P, _I64, _I32, _I32,
                                _P, _I64, _I64, _P, _I64, _I32, _P, _I32, _P, _P, _P, _P, _I32, _P],
+    "mzk_paged_append": [_P, _I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I32, _I32, _I32, _P, _I64, _I32, _P],
+    "mzk_paged_workspace_bytes": [_I64, _I64, _I64, ctypes.POINTER(_I64)],
+    "mzk_paged_grow": [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P, _I32, _P, _I64, _P, _P, _P, _P, _I64, _P],
+    "mzk_paged_fork": [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P, _I64, _P, _P, _P, _I64, _P],
+    "mzk_paged_compact": [_P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P, _P, _I64, _P],
+    "mzk_paged_attend": [_P, _I64, _I32, _I32, _P, _I64, _I32, _I32, _P, _I64, _I32, _P, _I64, _I64, _P, _P, _I64, _I32,
+                         _I64, _P, _P, _I64, _P, _P, _I32, _P],
+    "mzk_paged_attend_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, ctypes.POINTER(_I64)],
+    "mzk_packed_mqa": [_P, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32, _I64, _P, _P, _P, _I32, _P],
     "mzk_indexer_decode_fused": [_I32, _P, _P, _P, _P, _I64, _I32, _I32, _I64, _I64, _P, _I32, _P, _I64, _P, _P, _P,
                                  _P, _I32, _P, _P, _F32, _P, _P, _I32, _I32, _P, _I64, _I32, _P],
 }

@@ -12,6 +12,9 @@ Kernel-level drop-ins with the reference's signatures
 query itself (tokens ``t-W+1..t``); ``compress_ratio`` is documentation only: the
 group-causal rule is baked into ``indices`` by the indexer, as in the reference.
 
+* ``packed(q, kv, cu, *, window=None, sinks=None)`` -- causal attention over packed prompts of
+  different lengths, every entry visible (or a sliding window), without padding.
+
 Decode form over the packed caches (used by ``mzoo_amd.decode``):
 
 * ``sparse_mqa_decode(q, positions, win_cache, window, ...)`` -- FP8-b128 (656 B) ring
@@ -150,6 +153,52 @@ def fwd(q: torch.Tensor, kv: torch.Tensor, main_kv: torch.Tensor, indices: torch
 def attn(q, kv, main_kv, indices, *, window: int, compress_ratio: int, causal: bool = True, sinks=None):
     """Forward of ``csa2_attn.attn`` (no autograd: this build is inference-only)."""
     return fwd(q, kv, main_kv, indices, window=window, compress_ratio=compress_ratio, causal=causal, sinks=sinks)[0]
+
+
+def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int | None = None,
+           sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+    """Causal attention over whole prompts of different lengths, packed one after another: the
+    latent_attn / swa_attn levels (``layers/attn/latent_attn/fwd.py:45``, ``layers/attn/swa_attn/fwd.py:55``)
+    without padding.
+
+    q bf16 [T, H, D]; kv bf16 [T, G, D] (K == V), head h on latent ``h // (H // G)``; cu int64 [B + 1],
+    ascending from 0: sequence b is rows ``cu[b] .. cu[b + 1] - 1``.  A token sees its sequence up to
+    itself, or the last ``window`` tokens of that.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D],
+    lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a given ``out``
+    and ``lse``."""
+    _lib.require_gpu(q, kv, cu, sinks, out, lse)
+    if q.dim() != 3 or kv.dim() != 3 or q.dtype != torch.bfloat16 or kv.dtype != torch.bfloat16:
+        raise ValueError(f"packed: q [T, H, D] and kv [T, G, D] in bf16 expected, got {q.dtype} {list(q.shape)} and "
+                         f"{kv.dtype} {list(kv.shape)}")
+    t, h, d = q.shape
+    g = kv.shape[1]
+    if kv.shape[0] != t or kv.shape[2] != d or g < 1 or h < 1 or h % g:
+        raise ValueError(f"packed: kv must be [{t}, G, {d}] with G dividing {h} heads, got {list(kv.shape)}")
+    if cu.dtype != torch.int64 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+        raise ValueError(f"packed: cu must be contiguous int64 [B + 1], got {cu.dtype} {list(cu.shape)}")
+    if window is not None and (not isinstance(window, int) or window < 1):
+        raise ValueError(f"packed: window must be a positive int or None, got {window!r}")
+    if (out is None) != (lse is None):
+        raise ValueError("packed: out and lse go together")
+    for name, x, dt, shape in (("sinks", sinks, torch.float32, (h,)), ("out", out, torch.bfloat16, (t, h, d)),
+                               ("lse", lse, torch.float32, (t, h))):
+        if x is not None and (x.dtype != dt or not x.is_contiguous() or tuple(x.shape) != shape):
+            raise ValueError(f"packed: {name} must be a contiguous {dt} tensor of shape {list(shape)}")
+    for x in (kv, cu, sinks, out, lse):
+        if x is not None and x.device != q.device:
+            raise ValueError(f"packed: tensors on {q.device} and {x.device}")
+    q = q.contiguous()
+    if kv.stride(2) != 1 or (g > 1 and kv.stride(1) != d) or kv.stride(0) % 8 or kv.stride(0) < g * d or kv.data_ptr() % 16:
+        kv = kv.contiguous()
+    given = out is not None
+    if not given:
+        out = torch.empty_like(q)
+        lse = torch.empty(t, h, dtype=torch.float32, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.call("mzk_packed_mqa", q.data_ptr(), t, h, d, cu.data_ptr(), cu.numel() - 1, kv.data_ptr(),
+                  kv.stride(0) if t > 1 else g * d, g, window or 0, _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(),
+                  int(not given), _lib.stream_of(q))
+    return out, lse
 
 
 def sparse_mqa_decode(q: torch.Tensor, positions: torch.Tensor, win_cache: torch.Tensor, window: int, *,

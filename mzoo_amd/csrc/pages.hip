@@ -1,0 +1,658 @@
+// The paged latent cache: entries of new tokens into pages, and the pages themselves.
+//
+// A pool is [P, page, entry bytes]; a sequence's table row names its pages in order (-1: none), and
+// its first `len` entries hold its tokens.  refs[p] counts the table entries that name page p (and
+// whatever else holds it); a page of refs 0 is free.  All of it lives on the device, so a captured
+// decode loop grows its sequences without the host.
+//
+//   append   token i of the n new ones of sequence b -> position len_b - n + i
+//   grow     pages for n_b more tokens each: the lowest free pages, in the order of the sequences;
+//            a partly filled last page that others hold too is replaced by a copy; all or none
+//   fork     sequence i goes on from the tokens of sequence parents[i]
+//   compact  of U used pages, the k-th behind page U moves to the k-th free one before it
+//
+// Results do not depend on the order of workgroups: pages are ranked by prefix sums, and the only
+// atomics add whole numbers.
+#include "common.h"
+
+namespace mzk {
+namespace {
+
+constexpr int kChunk = 4096;  // pages that one workgroup ranks, 16 a thread
+
+__device__ __forceinline__ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- append -------------------------------------------------------------------------------
+
+struct AppendParams {
+  const void* x;
+  int64_t x_stride, T;
+  const int64_t* cu;  // null: one token per sequence
+  int64_t B;
+  const int32_t* tables;
+  int64_t table_stride, max_pages;
+  const int64_t* lens;
+  uint8_t* pool;
+  int64_t P;
+  int page, D, nope;  // nope 0: bf16 entries
+};
+
+// The sequence of packed token t (B: none), counted by the wave: lane l looks at boundaries l, l + 64, ..
+__device__ __forceinline__ int64_t sequence_of(const int64_t* cu, int64_t B, int64_t t, int lane) {
+  int64_t n = 0;
+  for (int64_t i = 0; i <= B; i += 64) {
+    const bool before = i + lane <= B && cu[i + lane] <= t;
+    n += __builtin_popcountll(__ballot(before));
+  }
+  return n - 1;  // -1 or B: the token is in no sequence
+}
+
+typedef uint32_t u32x2a4 __attribute__((ext_vector_type(2), aligned(4)));  // entries of 128 + 32 channels are 196 bytes
+
+// One wave per token.  fp8: a lane quantizes 8 neighbouring channels, 16 lanes share a block of 128.
+template <int DT>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p, bool vec) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (t >= p.T) return;
+  int64_t b = t, pos;
+  if (p.cu) {
+    b = sequence_of(p.cu, p.B, t, lane);
+    if (b < 0 || b >= p.B) return;
+    pos = p.lens[b] - p.cu[b + 1] + t;
+  } else {
+    pos = p.lens[b] - 1;
+  }
+  if (pos < 0 || pos >= p.max_pages * p.page) return;
+  const int64_t pid = p.tables[b * p.table_stride + pos / p.page];
+  if (pid < 0 || pid >= p.P) return;
+  const int eb = p.nope ? p.nope + p.nope / 32 + 2 * (p.D - p.nope) : 2 * p.D;
+  uint8_t* const e = p.pool + (pid * p.page + pos % p.page) * eb;
+  const int64_t x0 = t * p.x_stride;
+  for (int c = 8 * lane; c < p.D; c += 512) {
+    float v[8];
+    {
+      float h[4];
+      load4_as_f32<DT>(p.x, x0 + c, vec, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = h[i];
+      load4_as_f32<DT>(p.x, x0 + c + 4, vec, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 + i] = h[i];
+    }
+    if (c < p.nope) {  // nope is a multiple of 128: 16 lanes are in or out together
+      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+      const float s = fp8_scale_from_amax(group_max(nn_max(abs_max4(lo), abs_max4(hi)), 16));
+      const float inv = s <= 0x1p120f ? pow2_reciprocal(s) : 1.0f / s;  // as the block quantizer
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = clampf(v[i] * inv, 448.0f);
+      int w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+        w[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], w[k], true);
+      }
+      *reinterpret_cast<u32x2a4*>(e + c) = u32x2a4{static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[1])};
+      if ((c & 127) == 0) *reinterpret_cast<float*>(e + p.nope + c / 32) = s;
+    } else {
+      uint8_t* const at = e + (p.nope ? p.nope + p.nope / 32 : 0) + 2 * (c - p.nope);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        *reinterpret_cast<u32x2a4*>(at + 8 * k) =
+            u32x2a4{f32_to_bf16(v[4 * k]) | static_cast<uint32_t>(f32_to_bf16(v[4 * k + 1])) << 16,
+                    f32_to_bf16(v[4 * k + 2]) | static_cast<uint32_t>(f32_to_bf16(v[4 * k + 3])) << 16};
+    }
+  }
+}
+
+template <int DT>
+void launch_append(const AppendParams& p, bool vec, hipStream_t s) {
+  append_kernel<DT><<<static_cast<unsigned>((p.T + 3) / 4), 256, 0, s>>>(p, vec);
+}
+
+// ---- prefix sums over a workgroup of 256 ----------------------------------------------------
+
+// Sum over the workgroup of every thread's v, and of those before this one.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_t* lds4, int tid) {
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d, 64);
+    if ((tid & 63) >= d) x += y;
+  }
+  if ((tid & 63) == 63) lds4[tid >> 6] = x;
+  __syncthreads();
+  int64_t base = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < (tid >> 6)) base += lds4[w];
+    total += lds4[w];
+  }
+  __syncthreads();
+  before = base + x - v;
+  return total;
+}
+
+// This thread's 16 pages of a chunk: bit i of the result is set where page first + i is free (used).
+__device__ __forceinline__ uint32_t page_bits(const int32_t* refs, int64_t P, int64_t first, bool used) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const bool in = first + i < P;
+    const int32_t r = refs[in ? first + i : 0];
+    m |= static_cast<uint32_t>(in && (used ? r > 0 : r == 0)) << i;
+  }
+  return m;
+}
+
+// ---- grow ---------------------------------------------------------------------------------
+
+struct GrowRow {
+  int32_t first, want;  // the fresh table entries: first .. first + want - 1
+  int32_t src, fill;    // the page whose first `fill` entries the first fresh page begins with (-1: none)
+};
+
+struct GrowParams {
+  const int32_t* tables;
+  int32_t* tables_out;
+  int64_t stride, stride_out, B, max_pages;
+  const int64_t* lens;
+  int64_t* lens_out;
+  const int32_t* refs;
+  int32_t* refs_out;
+  int64_t P;
+  const int64_t* tokens;
+  int page;
+  int64_t* missing;
+  // workspace
+  int64_t* begin;   // [B] rank of the row's first fresh page
+  int64_t* old_len; // [B]
+  GrowRow* rows;    // [B]
+  int64_t* over;    // [B] pages past the table's width
+  int64_t* base;    // [chunks] free pages of the chunk, then of those before it
+  int64_t* ok;      // [1]
+  int64_t chunks;
+};
+
+// A count from the device, within what sums of two cannot overflow.
+__device__ __forceinline__ int64_t row_count(int64_t n) { return n < 0 ? 0 : n < (1ll << 60) ? n : 1ll << 60; }
+
+__global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  const int64_t blk = blockIdx.x;
+  if (blk < p.chunks) {
+    int64_t before;
+    const int n = __builtin_popcount(page_bits(p.refs, p.P, blk * kChunk + 16 * tid, false));
+    const int64_t total = block_scan(n, before, lds, tid);
+    if (tid == 0) p.base[blk] = total;
+    return;
+  }
+  const int64_t b = (blk - p.chunks) * 256 + tid;
+  if (b >= p.B) return;
+  const int64_t len = row_count(p.lens[b]), n = row_count(p.tokens[b]);
+  const int64_t held = ceil_div64(len, p.page), end = ceil_div64(len + n, p.page);
+  GrowRow r{0, 0, -1, 0};
+  p.over[b] = n > 0 && end > p.max_pages ? end - p.max_pages : 0;
+  if (n > 0 && end <= p.max_pages) {
+    const int64_t fill = len % p.page;
+    int64_t first = held;
+    if (fill != 0) {
+      const int64_t pid = p.tables[b * p.stride + held - 1];
+      if (pid >= 0 && pid < p.P && p.refs[pid] > 1) {
+        r.src = static_cast<int32_t>(pid);
+        r.fill = static_cast<int32_t>(fill);
+        --first;
+      }
+    }
+    r.first = static_cast<int32_t>(first);
+    r.want = static_cast<int32_t>(end - first);
+  }
+  p.rows[b] = r;
+  p.old_len[b] = len;
+}
+
+__global__ void __launch_bounds__(256) grow_plan_kernel(const GrowParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  int64_t free_pages = 0, want = 0, over = 0;
+  for (int64_t i = 0; i < p.chunks; i += 256) {
+    const int64_t v = i + tid < p.chunks ? p.base[i + tid] : 0;
+    int64_t before;
+    const int64_t total = block_scan(v, before, lds, tid);
+    if (i + tid < p.chunks) p.base[i + tid] = free_pages + before;
+    free_pages += total;
+  }
+  for (int64_t i = 0; i < p.B; i += 256) {
+    const int64_t v = i + tid < p.B ? p.rows[i + tid].want : 0;
+    int64_t before, unused;
+    const int64_t total = block_scan(v, before, lds, tid);
+    if (i + tid < p.B) p.begin[i + tid] = want + before;
+    want += total;
+    over += block_scan(i + tid < p.B ? p.over[i + tid] : 0, unused, lds, tid);
+  }
+  if (tid == 0) {
+    const int64_t lack = over + (want > free_pages ? want - free_pages : 0);
+    *p.missing = lack;
+    *p.ok = lack == 0 ? want : -1;
+  }
+}
+
+__global__ void __launch_bounds__(256) grow_assign_kernel(const GrowParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  const int64_t blk = blockIdx.x;
+  const int64_t want = *p.ok;  // -1: nobody gets any
+  if (blk < p.chunks) {
+    const int64_t first = blk * kChunk + 16 * tid;
+    const uint32_t free_bits = page_bits(p.refs, p.P, first, false);
+    int64_t before;
+    block_scan(__builtin_popcount(free_bits), before, lds, tid);
+    int64_t rank = p.base[blk] + before;
+    for (int i = 0; i < 16; ++i) {
+      if (first + i >= p.P) break;
+      int32_t r = p.refs[first + i];
+      if ((free_bits >> i) & 1u) {
+        if (rank < want) {
+          int64_t lo = 0, hi = p.B - 1;  // the last row whose pages begin at or before this rank
+          while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (p.begin[mid] <= rank) lo = mid; else hi = mid - 1;
+          }
+          p.tables_out[lo * p.stride_out + p.rows[lo].first + (rank - p.begin[lo])] = static_cast<int32_t>(first + i);
+          r = 1;
+        }
+        ++rank;
+      }
+      p.refs_out[first + i] = r;
+    }
+    return;
+  }
+  const int64_t b = blk - p.chunks;
+  const GrowRow r = p.rows[b];
+  for (int64_t j = tid; j < p.max_pages; j += 256) {
+    const bool fresh = want >= 0 && j >= r.first && j < r.first + r.want;
+    if (!fresh) p.tables_out[b * p.stride_out + j] = p.tables[b * p.stride + j];
+  }
+  if (tid == 0) {
+    p.lens_out[b] = want >= 0 ? p.old_len[b] + row_count(p.tokens[b]) : p.lens[b];
+  }
+}
+
+constexpr int kPoolsPerLaunch = 32;
+struct PoolList {
+  uint8_t* base[kPoolsPerLaunch];
+  int64_t entry[kPoolsPerLaunch];  // bytes of one entry, a multiple of 4
+};
+
+// bytes (a multiple of 4) from a to b by a workgroup
+__device__ __forceinline__ void copy_bytes(const uint8_t* a, uint8_t* b, int64_t bytes, int64_t at, int64_t step) {
+  if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0) {
+    const int64_t whole = bytes >> 4;
+    for (int64_t i = at; i < whole; i += step) reinterpret_cast<uint4*>(b)[i] = reinterpret_cast<const uint4*>(a)[i];
+    for (int64_t i = (whole << 2) + at; i < bytes >> 2; i += step)
+      reinterpret_cast<uint32_t*>(b)[i] = reinterpret_cast<const uint32_t*>(a)[i];
+  } else {
+    for (int64_t i = at; i < bytes >> 2; i += step)
+      reinterpret_cast<uint32_t*>(b)[i] = reinterpret_cast<const uint32_t*>(a)[i];
+  }
+}
+
+// Row blockIdx.x's shared last page into its fresh one, a share of it per blockIdx.y; pool blockIdx.z.
+__global__ void __launch_bounds__(256) grow_copy_kernel(const GrowParams p, const PoolList pools, int npools, bool first) {
+  const int64_t b = blockIdx.x;
+  const GrowRow r = p.rows[b];
+  if (r.src < 0 || *p.ok < 0) return;
+  if (first && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicSub(p.refs_out + r.src, 1);
+  if (npools == 0) return;
+  const int64_t dst = p.tables_out[b * p.stride_out + r.first];
+  const int64_t eb = pools.entry[blockIdx.z];
+  uint8_t* const base = pools.base[blockIdx.z];
+  copy_bytes(base + r.src * (p.page * eb), base + dst * (p.page * eb), r.fill * eb,
+             static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.y) * 256);
+}
+
+// ---- fork ---------------------------------------------------------------------------------
+
+struct ForkParams {
+  const int32_t* tables;
+  int64_t stride, B, max_pages;
+  const int64_t* lens;
+  const int32_t* refs;
+  int32_t* refs_out;
+  int64_t P;
+  const int32_t* parents;
+  int64_t R;
+  int page;
+  int32_t* tables_out;
+  int64_t stride_out;
+  int64_t* lens_out;
+  // copies of tables [B, max_pages] and lens [B] for a call whose outputs are its inputs (null: none needed)
+  int32_t* tables_copy;
+  int64_t* lens_copy;
+};
+
+__global__ void __launch_bounds__(256) fork_copy_kernel(const ForkParams p) {
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  if (p.refs_out != p.refs)
+    for (int64_t i = i0; i < p.P; i += step) p.refs_out[i] = p.refs[i];
+  if (p.tables_copy) {
+    for (int64_t i = i0; i < p.B * p.max_pages; i += step)
+      p.tables_copy[i] = p.tables[i / p.max_pages * p.stride + i % p.max_pages];
+    for (int64_t i = i0; i < p.B; i += step) p.lens_copy[i] = p.lens[i];
+  }
+}
+
+__global__ void __launch_bounds__(256) fork_kernel(const ForkParams p) {
+  const int64_t i = blockIdx.x;
+  const int32_t* const t = p.tables_copy ? p.tables_copy : p.tables;
+  const int64_t stride = p.tables_copy ? p.max_pages : p.stride;
+  const int64_t* const lens = p.tables_copy ? p.lens_copy : p.lens;
+  int64_t par = i < p.R ? p.parents[i] : -1;
+  if (par >= p.B) par = -1;
+  int64_t len = par >= 0 ? lens[par] : 0;
+  if (len < 0) len = 0;
+  const int64_t keep = ceil_div64(len, p.page);
+  for (int64_t j = threadIdx.x; j < p.max_pages; j += 256) {
+    const int64_t old = i < p.B ? t[i * stride + j] : -1;
+    int64_t now = par >= 0 && j < keep ? t[par * stride + j] : -1;
+    if (now < 0 || now >= p.P) now = -1;
+    if (i < p.R) p.tables_out[i * p.stride_out + j] = static_cast<int32_t>(now);
+    if (old != now) {
+      if (old >= 0 && old < p.P) atomicSub(p.refs_out + old, 1);
+      if (now >= 0) atomicAdd(p.refs_out + now, 1);
+    }
+  }
+  if (i < p.R && threadIdx.x == 0) p.lens_out[i] = len;
+}
+
+// ---- compact ------------------------------------------------------------------------------
+
+struct CompactParams {
+  const int32_t* tables;
+  int32_t* tables_out;
+  int64_t stride, stride_out, B, max_pages;
+  const int32_t* refs;
+  int32_t* refs_out;
+  int64_t P;
+  int page;
+  // workspace
+  int64_t* base;     // [chunks] used pages before the chunk
+  int64_t* used;     // [2] U, and the moves M
+  int32_t* from;     // [P] page of the k-th move
+  int32_t* to;       // [P]
+  int32_t* from_refs;  // [P]
+  int32_t* rank;     // [P] the move of a page behind U
+  int64_t chunks;
+};
+
+__global__ void __launch_bounds__(256) compact_count_kernel(const CompactParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  int64_t before;
+  const int n = __builtin_popcount(page_bits(p.refs, p.P, blockIdx.x * static_cast<int64_t>(kChunk) + 16 * tid, true));
+  const int64_t total = block_scan(n, before, lds, tid);
+  if (tid == 0) p.base[blockIdx.x] = total;
+}
+
+__global__ void __launch_bounds__(256) compact_plan_kernel(const CompactParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  int64_t used = 0;
+  for (int64_t i = 0; i < p.chunks; i += 256) {
+    const int64_t v = i + tid < p.chunks ? p.base[i + tid] : 0;
+    int64_t before;
+    const int64_t total = block_scan(v, before, lds, tid);
+    if (i + tid < p.chunks) p.base[i + tid] = used + before;
+    used += total;
+  }
+  __syncthreads();
+  // used pages before page U: those of earlier chunks and a part of U's own
+  const int64_t c = used / kChunk;
+  int64_t n = 0;
+  if (c < p.chunks) {
+    const uint32_t m = page_bits(p.refs, p.P, c * kChunk + 16 * tid, true);
+    const int64_t left = used - (c * kChunk + 16 * tid);
+    n = __builtin_popcount(left >= 16 ? m : left <= 0 ? 0u : m & ((1u << left) - 1u));
+  }
+  int64_t unused;
+  const int64_t in_chunk = block_scan(n, unused, lds, tid);
+  if (tid == 0) {
+    p.used[0] = used;
+    p.used[1] = used - (c < p.chunks ? p.base[c] + in_chunk : used);
+  }
+}
+
+__global__ void __launch_bounds__(256) compact_list_kernel(const CompactParams p) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
+  const int64_t U = p.used[0], M = p.used[1];
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kChunk) + 16 * tid;
+  const uint32_t used_bits = page_bits(p.refs, p.P, first, true);
+  int64_t before;
+  block_scan(__builtin_popcount(used_bits), before, lds, tid);
+  int64_t n = p.base[blockIdx.x] + before;  // used pages before this one
+  for (int i = 0; i < 16; ++i) {
+    const int64_t page = first + i;
+    if (page >= p.P) break;
+    const bool used = (used_bits >> i) & 1u;
+    const int32_t r = p.refs[page];
+    if (page < U) {
+      if (!used) p.to[page - n] = static_cast<int32_t>(page);
+      p.refs_out[page] = r;
+    } else {
+      if (used) {
+        const int64_t k = n - (U - M);
+        p.from[k] = static_cast<int32_t>(page);
+        p.from_refs[k] = r;
+        p.rank[page] = static_cast<int32_t>(k);
+      }
+      p.refs_out[page] = used ? 0 : r;
+    }
+    n += used;
+  }
+}
+
+// blockIdx.y == 0: tables and counts; otherwise the moves of pool blockIdx.y - 1
+__global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p, const PoolList pools, bool first) {
+  const int64_t U = p.used[0], M = p.used[1];
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  if (blockIdx.y == 0) {
+    if (!first) return;
+    for (int64_t i = at; i < M; i += step) p.refs_out[p.to[i]] = p.from_refs[i];
+    for (int64_t i = at; i < p.B * p.max_pages; i += step) {
+      const int64_t b = i / p.max_pages, j = i - b * p.max_pages;
+      int32_t v = p.tables[b * p.stride + j];
+      if (v >= U && v < p.P) {
+        // rank[] is written for moved pages only: a page without references, whose word is
+        // whatever was there, is no move's `from`, and a table that names it keeps it
+        const int32_t k = p.rank[v];
+        if (k >= 0 && k < M && p.from[k] == v) v = p.to[k];
+      }
+      p.tables_out[b * p.stride_out + j] = v;
+    }
+    return;
+  }
+  const int64_t eb = pools.entry[blockIdx.y - 1] * p.page;
+  uint8_t* const base = pools.base[blockIdx.y - 1];
+  for (int64_t m = blockIdx.x; m < M; m += gridDim.x)
+    copy_bytes(base + p.from[m] * eb, base + p.to[m] * eb, eb, threadIdx.x, 256);
+}
+
+int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
+
+int64_t grow_bytes(int64_t B, int64_t P) {
+  const int64_t chunks = (P + kChunk - 1) / kChunk;
+  return 8 * (3 * B + chunks + 1) + align16_up(sizeof(GrowRow) * B) + 32;
+}
+int64_t fork_bytes(int64_t B, int64_t max_pages) { return align16_up(4 * B * max_pages) + 8 * B; }
+int64_t compact_bytes(int64_t P) { return 8 * ((P + kChunk - 1) / kChunk + 2) + 16 * P + 32; }
+
+constexpr int64_t kMaxInt = 0x7fffffff;
+
+#define MZK_CHECK_PAGES(name, B, max_pages, P)                                                                     \
+  MZK_CHECK_ARG((B) >= 0 && (B) <= kMaxInt && (max_pages) >= 0 && (max_pages) <= kMaxInt && (P) >= 0 && (P) <= kMaxInt, \
+                name ": bad sizes")
+
+int check_pools(const char* name, const void* const* pools, const int64_t* entry, int n) {
+  MZK_CHECK_ARG(n >= 0 && (n == 0 || (pools && entry)), "%s: null pool list", name);
+  for (int i = 0; i < n; ++i)
+    MZK_CHECK_ARG(pools[i] && entry[i] > 0 && entry[i] % 4 == 0 && (reinterpret_cast<uintptr_t>(pools[i]) & 3u) == 0,
+                  "%s: pool %d needs a 4-byte aligned base and entries of a multiple of 4 bytes", name, i);
+  return MZK_OK;
+}
+
+}  // namespace
+}  // namespace mzk
+
+using namespace mzk;
+
+extern "C" int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_row_stride, const int64_t* cu, int64_t B,
+                                const int32_t* tables, int64_t table_stride, int64_t max_pages, const int64_t* lens,
+                                int fmt, int D, int nope, void* pool, int64_t pages, int page, void* stream) {
+  MZK_CHECK_ARG(T >= 0 && B >= 0, "paged_append: bad sizes");
+  MZK_CHECK_PAGES("paged_append", B, max_pages, pages);
+  MZK_CHECK_ARG(page >= 1, "paged_append: pages of at least one entry");
+  MZK_CHECK_ARG(fmt == 0 || fmt == 1, "paged_append: fmt must be 0 (bf16) or 1 (fp8-b128)");
+  MZK_CHECK_ARG(D >= 8 && D % 8 == 0 && D <= 4096, "paged_append: D must be a multiple of 8 up to 4096, got %d", D);
+  MZK_CHECK_ARG(fmt == 0 || (nope >= 128 && nope % 128 == 0 && nope <= D),
+                "paged_append: fp8 entries need nope, a multiple of 128 up to D (got %d of %d)", nope, D);
+  MZK_CHECK_ARG(x_row_stride >= D && table_stride >= max_pages, "paged_append: strides smaller than the row");
+  MZK_CHECK_ARG(cu || T == B, "paged_append: without cu one token per sequence (%lld tokens, %lld sequences)",
+                (long long)T, (long long)B);
+  if (T == 0 || B == 0) return MZK_OK;
+  MZK_CHECK_ARG(x && tables && lens && pool, "paged_append: null pointer");
+  MZK_CHECK_ARG(aligned16(pool), "paged_append: the pool must be 16-byte aligned");
+  MZK_CHECK_ARG(T <= 4ll * kMaxInt, "paged_append: too many tokens");
+  const AppendParams p{x, x_row_stride, T, cu, B, tables, table_stride, max_pages, lens, static_cast<uint8_t*>(pool),
+                       pages, page, D, fmt ? nope : 0};
+  const bool vec = aligned16(x) && x_row_stride % 8 == 0;
+  MZK_DISPATCH_DT(dtype, launch_append, p, vec, as_stream(stream));
+  MZK_LAUNCH_CHECK("paged_append");
+  return MZK_OK;
+}
+
+extern "C" int mzk_paged_workspace_bytes(int64_t B, int64_t max_pages, int64_t pages, int64_t* bytes) {
+  MZK_CHECK_ARG(bytes != nullptr, "paged_workspace_bytes: null output");
+  MZK_CHECK_PAGES("paged_workspace_bytes", B, max_pages, pages);
+  int64_t n = grow_bytes(B, pages);
+  if (fork_bytes(B, max_pages) > n) n = fork_bytes(B, max_pages);
+  if (compact_bytes(pages) > n) n = compact_bytes(pages);
+  *bytes = align16_up(n);
+  return MZK_OK;
+}
+
+extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages,
+                              const int64_t* lens, const int32_t* refs, int64_t pages, const int64_t* tokens, int page,
+                              void* const* pools, const int64_t* entry_bytes, int npools, int32_t* tables_out,
+                              int64_t table_out_stride, int64_t* lens_out, int32_t* refs_out, int64_t* missing,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  MZK_CHECK_PAGES("paged_grow", B, max_pages, pages);
+  MZK_CHECK_ARG(page >= 1, "paged_grow: pages of at least one entry");
+  MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_grow: strides smaller than the row");
+  if (int rc = check_pools("paged_grow", pools, entry_bytes, npools)) return rc;
+  MZK_CHECK_ARG(tables && lens && refs && tokens && tables_out && lens_out && refs_out && missing, "paged_grow: null pointer");
+  MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= grow_bytes(B, pages),
+                "paged_grow: a 16-byte aligned workspace of %lld bytes is needed", (long long)grow_bytes(B, pages));
+  GrowParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, lens, lens_out, refs, refs_out, pages,
+               tokens, page, missing};
+  p.chunks = (pages + kChunk - 1) / kChunk;
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  p.rows = reinterpret_cast<GrowRow*>(w);
+  w += align16_up(sizeof(GrowRow) * B);
+  p.begin = reinterpret_cast<int64_t*>(w);
+  p.old_len = p.begin + B;
+  p.over = p.old_len + B;
+  p.base = p.over + B;
+  p.ok = p.base + p.chunks;
+  hipStream_t s = as_stream(stream);
+  if (p.chunks + B > 0)
+    grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 255) / 256), 256, 0, s>>>(p);
+  grow_plan_kernel<<<1, 256, 0, s>>>(p);
+  if (p.chunks + B > 0) grow_assign_kernel<<<static_cast<unsigned>(p.chunks + B), 256, 0, s>>>(p);
+  if (B > 0) {
+    int done = 0;
+    do {
+      PoolList l{};
+      const int n = npools - done < kPoolsPerLaunch ? npools - done : kPoolsPerLaunch;
+      for (int i = 0; i < n; ++i) {
+        l.base[i] = static_cast<uint8_t*>(pools[done + i]);
+        l.entry[i] = entry_bytes[done + i];
+      }
+      grow_copy_kernel<<<dim3(static_cast<unsigned>(B), n ? 4 : 1, n ? n : 1), 256, 0, s>>>(p, l, n, done == 0);
+      done += n;
+    } while (done < npools);
+  }
+  MZK_LAUNCH_CHECK("paged_grow");
+  return MZK_OK;
+}
+
+extern "C" int mzk_paged_fork(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages,
+                              const int64_t* lens, const int32_t* refs, int64_t pages, const int32_t* parents,
+                              int64_t rows_out, int page, int32_t* tables_out, int64_t table_out_stride,
+                              int64_t* lens_out, int32_t* refs_out, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  MZK_CHECK_PAGES("paged_fork", B, max_pages, pages);
+  MZK_CHECK_ARG(rows_out >= 0 && rows_out <= kMaxInt && page >= 1, "paged_fork: bad sizes");
+  MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_fork: strides smaller than the row");
+  MZK_CHECK_ARG(tables && lens && refs && parents && tables_out && lens_out && refs_out, "paged_fork: null pointer");
+  ForkParams p{tables, table_stride, B, max_pages, lens, refs, refs_out, pages, parents, rows_out, page, tables_out,
+               table_out_stride, lens_out, nullptr, nullptr};
+  if (tables == tables_out || lens == lens_out) {
+    MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= fork_bytes(B, max_pages),
+                  "paged_fork: in place, a 16-byte aligned workspace of %lld bytes is needed",
+                  (long long)fork_bytes(B, max_pages));
+    p.tables_copy = static_cast<int32_t*>(workspace);
+    p.lens_copy = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(workspace) + align16_up(4 * B * max_pages));
+  }
+  hipStream_t s = as_stream(stream);
+  int64_t n = refs != refs_out ? pages : 0;
+  if (p.tables_copy && B * max_pages > n) n = B * max_pages;
+  if (n > 0) {
+    const int64_t g = (n + 255) / 256;
+    fork_copy_kernel<<<static_cast<unsigned>(g < 2048 ? g : 2048), 256, 0, s>>>(p);
+  }
+  const int64_t rows = B > rows_out ? B : rows_out;
+  if (rows > 0) fork_kernel<<<static_cast<unsigned>(rows), 256, 0, s>>>(p);
+  MZK_LAUNCH_CHECK("paged_fork");
+  return MZK_OK;
+}
+
+extern "C" int mzk_paged_compact(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages,
+                                 const int32_t* refs, int64_t pages, int page, void* const* pools,
+                                 const int64_t* entry_bytes, int npools, int32_t* tables_out, int64_t table_out_stride,
+                                 int32_t* refs_out, void* workspace, int64_t workspace_bytes, void* stream) {
+  MZK_CHECK_PAGES("paged_compact", B, max_pages, pages);
+  MZK_CHECK_ARG(page >= 1, "paged_compact: pages of at least one entry");
+  MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_compact: strides smaller than the row");
+  if (int rc = check_pools("paged_compact", pools, entry_bytes, npools)) return rc;
+  MZK_CHECK_ARG(tables && refs && tables_out && refs_out, "paged_compact: null pointer");
+  MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= compact_bytes(pages),
+                "paged_compact: a 16-byte aligned workspace of %lld bytes is needed", (long long)compact_bytes(pages));
+  CompactParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, refs, refs_out, pages, page};
+  p.chunks = (pages + kChunk - 1) / kChunk;
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  p.base = reinterpret_cast<int64_t*>(w);
+  p.used = p.base + p.chunks;
+  p.from = reinterpret_cast<int32_t*>(p.used + 2);
+  p.to = p.from + pages;
+  p.from_refs = p.to + pages;
+  p.rank = p.from_refs + pages;
+  hipStream_t s = as_stream(stream);
+  if (p.chunks > 0) compact_count_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
+  compact_plan_kernel<<<1, 256, 0, s>>>(p);
+  if (p.chunks > 0) compact_list_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
+  int done = 0;
+  do {
+    PoolList l{};
+    const int n = npools - done < kPoolsPerLaunch ? npools - done : kPoolsPerLaunch;
+    for (int i = 0; i < n; ++i) {
+      l.base[i] = static_cast<uint8_t*>(pools[done + i]);
+      l.entry[i] = entry_bytes[done + i];
+    }
+    compact_move_kernel<<<dim3(1024, 1 + n), 256, 0, s>>>(p, l, done == 0);
+    done += n;
+  } while (done < npools);
+  MZK_LAUNCH_CHECK("paged_compact");
+  return MZK_OK;
+}
