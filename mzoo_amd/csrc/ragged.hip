@@ -7,8 +7,9 @@
 //   positions 0 .. its own, the last `window` of them, or the positions of its list.
 //
 // A unit of work is a block of 64 rows -- a row is a head of a token, the heads of one latent
-// innermost, so 64 rows are 64 heads of a token or all heads of several -- over a share of the
-// sequence's entries.
+// innermost, so 64 rows are 64 heads of a token or all heads of several -- over all of the
+// sequence's entries, or, where there are fewer blocks than compute units, over a share of them;
+// the shares' results are joined by a second launch.
 #include "common.h"
 #include "entries.h"
 
@@ -29,7 +30,7 @@ struct RaggedParams {
   const uint8_t* entries;
   int64_t entry_stride;  // bytes from entry to entry
   const int32_t* tables;
-  int64_t table_stride, max_pages, pages;
+  int64_t table_stride, max_pages, pages;  // max_pages * page and pages * page below 2^31
   int page;
   const int32_t* idx;  // [B, topk] positions (one token per sequence), or null
   int64_t idx_stride;
@@ -38,19 +39,293 @@ struct RaggedParams {
   const float* sinks;
   float scale_log2;
   int rows_per_unit;   // min(64, 32 HG): a unit spans at most 33 tokens
-  int64_t blocks_max;  // units in the grid
+  int64_t blocks_max;  // row blocks at most
+  // splitting: at most `slots` units (0: one unit per block, no joining), shares of at least
+  // min_tiles tiles; a unit of a split sequence leaves its result in the slot of its number
+  int slots, min_tiles;
+  int32_t* plan;       // [B][2] by the first workgroup: the sequence's first unit, its shares
+  float* part_o;       // [slots][64][D]: O / l
+  float* part_ml;      // [slots][64][2]: m in log2 units, l
   uint16_t* out;
   float* lse;          // [T, H]
   int zero_tail;       // rows of no sequence become 0 (else they are left as they are)
 };
 
-// Where a unit's rows are.
+// Where a unit's rows and entries are.
 struct Unit {
-  int64_t b, t0, n;     // sequence, its first packed token, its new tokens
-  int64_t len;          // its tokens in the cache
-  int g;                // latent
-  int64_t r0, r1;       // rows of the sequence and latent: token r / HG, head g HG + r % HG
+  int64_t b, t0;      // sequence, its first packed token
+  int n, len;         // its new tokens, its tokens in the cache
+  int g;              // latent
+  int64_t r0, r1;     // rows of the sequence and latent: token r / HG, head g HG + r % HG
+  int share, shares;  // of the tiles from the first to the last entry that a row sees
+  int slot;
 };
+
+__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Sums over a workgroup of 256 (lds: 4 words).
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_t* lds, int tid) {
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d, 64);
+    if ((tid & 63) >= d) x += y;
+  }
+  if ((tid & 63) == 63) lds[tid >> 6] = x;
+  __syncthreads();
+  int64_t base = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < (tid >> 6)) base += lds[w];
+    total += lds[w];
+  }
+  __syncthreads();
+  before = base + x - v;
+  return total;
+}
+
+// Sequence i's packed tokens a .. z - 1, its row blocks and its tiles.
+__device__ __forceinline__ int64_t sequence(const RaggedParams& p, int64_t i, int64_t& a, int64_t& z, int& tiles) {
+  a = i;
+  z = i + 1;
+  if (p.cu) {
+    a = clamp64(p.cu[i], 0, p.T);
+    z = clamp64(p.cu[i + 1], a, p.T);
+  }
+  int64_t seen = p.lens ? clamp64(p.lens[i], 0, p.max_pages * p.page) : z - a;
+  if (p.idx) seen = seen > 0 ? p.topk : 0;
+  if (seen > p.window + (z - a)) seen = p.window + (z - a);
+  tiles = static_cast<int>((seen + kTile - 1) / kTile);
+  return ((z - a) * p.HG + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
+}
+
+constexpr int kPlanRows = 1024;  // the most sequences that are split
+constexpr int kMaxShares = 256;  // of one sequence
+struct PlanLds {
+  int64_t scan[8];
+  int count[4][64];
+  int blocks[kPlanRows], tiles[kPlanRows];
+};
+
+// The tiles of a share: the least for which the units fit the slots, looked for among 64 values between
+// what an even division gives and what always fits.  Every workgroup finds the same.
+__device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
+  int64_t blocks = 0, work = 0;
+  int most = 1;
+  for (int64_t i = tid; i < p.B; i += 256) {
+    int64_t a, z;
+    int t;
+    const int n = static_cast<int>(sequence(p, i, a, z, t));
+    l.blocks[i] = n;
+    l.tiles[i] = t;
+    blocks += n;
+    work += static_cast<int64_t>(n) * t;
+    most = t > most ? t : most;
+  }
+  int64_t unused;
+  blocks = block_scan(blocks, unused, l.scan, tid);
+  work = block_scan(work, unused, l.scan, tid);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const int o = __shfl_xor(most, d, 64);
+    most = o > most ? o : most;
+  }
+  if ((tid & 63) == 0) l.count[0][tid >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) most = l.count[0][w] > most ? l.count[0][w] : most;
+  __syncthreads();
+  if (blocks >= p.slots) return most;
+  // sum of blocks * ceil(tiles / c) <= work / c + blocks <= slots for c >= work / (slots - blocks)
+  int64_t hi = (work + p.slots - blocks - 1) / (p.slots - blocks), lo = (work + p.slots - 1) / p.slots;
+  if (hi > most) hi = most;
+  if (lo < p.min_tiles) lo = p.min_tiles;
+  if (lo < (most + kMaxShares - 1) / kMaxShares) lo = (most + kMaxShares - 1) / kMaxShares;
+  if (hi <= lo) return static_cast<int>(lo);
+  const int c = static_cast<int>(lo + (hi - lo) * (tid & 63) / 63);
+  const float rc = 1.0f / static_cast<float>(c);
+  int n = 0;
+  for (int i = tid >> 6; i < p.B; i += 4) {
+    const int t = l.tiles[i];
+    int k = static_cast<int>(static_cast<float>(t) * rc);  // ceil(t / c), corrected
+    k += static_cast<int64_t>(k) * c < t;
+    k -= k > 1 && static_cast<int64_t>(k - 1) * c >= t;
+    n += l.blocks[i] * (k > 1 ? k : 1);
+  }
+  l.count[tid >> 6][tid & 63] = n;
+  __syncthreads();
+  const int j = tid & 63;
+  const bool fits = static_cast<int64_t>(l.count[0][j]) + l.count[1][j] + l.count[2][j] + l.count[3][j] <= p.slots || j == 63;
+  const int first = __builtin_ctzll(__ballot(fits));
+  __syncthreads();
+  return static_cast<int>(lo + (hi - lo) * first / 63);
+}
+
+// This workgroup's unit; false: none.  Workgroups go to the 8 XCDs in turn: without shares, two
+// neighbouring blocks (which read the same entries) follow each other on an XCD, and the last
+// blocks, which see the most, come first; with shares, an XCD takes neighbouring units.
+__device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid) {
+  PlanLds& l = *reinterpret_cast<PlanLds*>(smem);
+  const int64_t w = blockIdx.x;
+  const int64_t per_token = (static_cast<int64_t>(p.HG) + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
+  int64_t blk, blocks, k;
+  u.share = 0;
+  u.shares = 1;
+  u.slot = 0;
+  if (p.slots == 0) {
+    k = (w / 16 * 8 + w % 8) * 2 + w / 8 % 2;
+    if (p.cu == nullptr) {
+      u.b = k / per_token;
+      if (u.b >= p.B) return false;
+      blk = k - u.b * per_token;
+      blocks = per_token;
+    } else {
+      int64_t total = 0;
+      for (int64_t i = tid; i < p.B; i += 256) {
+        int64_t a, z;
+        int t;
+        total += sequence(p, i, a, z, t);
+      }
+      int64_t before, base = 0;
+      total = block_scan(total, before, l.scan, tid);
+      if (k >= total) return false;
+      k = total - 1 - k;
+      for (int64_t i = 0;; i += 256) {  // ends: k < total
+        int64_t a, z, v = 0;
+        int t;
+        if (i + tid < p.B) v = sequence(p, i + tid, a, z, t);
+        const int64_t sum = block_scan(v, before, l.scan, tid);
+        if (k >= base + before && k < base + before + v) {
+          l.scan[4] = i + tid;
+          l.scan[5] = k - base - before;
+          l.scan[6] = v;
+        }
+        base += sum;
+        if (k < base) break;
+      }
+      __syncthreads();
+      u.b = l.scan[4];
+      blk = l.scan[5];
+      blocks = l.scan[6];
+    }
+  } else {
+    const int c = share_tiles(p, l, tid);
+    int64_t total = 0, before, base = 0;
+    for (int64_t i = tid; i < p.B; i += 256) total += static_cast<int64_t>(l.blocks[i]) * (l.tiles[i] > c ? (l.tiles[i] + c - 1) / c : 1);
+    total = block_scan(total, before, l.scan, tid);
+    const int64_t per_xcd = (total + 7) / 8;
+    k = w % 8 * per_xcd + w / 8;
+    const bool mine = w / 8 < per_xcd && k < total;
+    if (!mine && w != 0) return false;
+    for (int64_t i = 0; i < p.B; i += 256) {
+      int shares = 1;
+      int64_t v = 0;
+      if (i + tid < p.B) {
+        shares = l.tiles[i + tid] > c ? (l.tiles[i + tid] + c - 1) / c : 1;
+        v = static_cast<int64_t>(l.blocks[i + tid]) * shares;
+      }
+      const int64_t sum = block_scan(v, before, l.scan, tid);
+      if (w == 0 && i + tid < p.B) {
+        p.plan[2 * (i + tid)] = static_cast<int32_t>(base + before);
+        p.plan[2 * (i + tid) + 1] = shares;
+      }
+      if (mine && k >= base + before && k < base + before + v) {
+        l.scan[4] = i + tid;
+        l.scan[5] = k - base - before;
+        l.scan[6] = shares;
+      }
+      base += sum;
+    }
+    __syncthreads();
+    if (!mine) return false;
+    u.b = l.scan[4];
+    blocks = l.blocks[u.b];
+    u.shares = static_cast<int>(l.scan[6]);
+    u.share = static_cast<int>(l.scan[5] / blocks);
+    blk = l.scan[5] - u.share * blocks;
+    u.slot = static_cast<int>(k);
+  }
+  int64_t a, z;
+  int tiles;
+  sequence(p, u.b, a, z, tiles);
+  u.t0 = a;
+  u.n = static_cast<int>(z - a);
+  const int64_t per_latent = blocks / p.G;
+  u.g = static_cast<int>(blk / per_latent);
+  u.r0 = (blk - u.g * per_latent) * p.rows_per_unit;
+  const int64_t rows = static_cast<int64_t>(u.n) * p.HG;
+  u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
+  u.len = u.n;
+  if (p.lens) u.len = static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page));
+  __syncthreads();  // the plan's LDS is free
+  return true;
+}
+
+// Row r of the unit's sequence: its row of q, out and lse.
+__device__ __forceinline__ int64_t row_at(const RaggedParams& p, const Unit& u, int64_t r) {
+  if (p.G == 1) return u.t0 * p.H + r;
+  const int64_t tok = r / p.HG;
+  return (u.t0 + tok) * p.H + u.g * p.HG + (r - tok * p.HG);
+}
+
+// The positions (or places of the list) that tokens tok0 .. tok1 - 1 of the sequence see.
+__device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u, int64_t tok0, int64_t tok1, int& lo, int& hi) {
+  const int64_t shift = static_cast<int64_t>(u.len) - u.n;  // position of the first new token (negative: tokens that see nothing)
+  lo = static_cast<int>(clamp64(shift + tok0 - p.window + 1, 0, u.len));
+  hi = static_cast<int>(clamp64(shift + tok1, 0, u.len));
+  if (p.idx) {
+    lo = 0;
+    hi = u.len > 0 ? p.topk : 0;
+  }
+}
+
+// This unit's share of the tiles that its tokens tok0 .. tok1 - 1 see.
+__device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u, int64_t tok0, int64_t tok1, int& lo, int& hi) {
+  token_range(p, u, tok0, tok1, lo, hi);
+  if (u.shares > 1) {
+    const int tiles = (hi - lo + kTile - 1) / kTile, per = (tiles + u.shares - 1) / u.shares;
+    const int64_t from = lo + static_cast<int64_t>(u.share) * per * kTile;
+    if (from + static_cast<int64_t>(per) * kTile < hi) hi = static_cast<int>(from) + per * kTile;
+    lo = from < hi ? static_cast<int>(from) : hi;
+  }
+}
+
+// The entry at position v of the unit's sequence (or of its list) in a pool; -1: none.
+__device__ __forceinline__ int64_t pool_entry(const RaggedParams& p, const Unit& u, int v) {
+  if (p.idx) {
+    v = p.idx[u.b * p.idx_stride + v];
+    if (v < 0 || v >= u.len) return -1;
+  }
+  const uint32_t at = static_cast<uint32_t>(v) / static_cast<uint32_t>(p.page);
+  const int64_t pid = p.tables[u.b * p.table_stride + at];
+  if (pid < 0 || pid >= p.pages) return -1;
+  return pid * p.page + (static_cast<uint32_t>(v) - at * static_cast<uint32_t>(p.page));
+}
+
+// The address of the entry at position v; null where there is none.
+__device__ __forceinline__ const uint8_t* entry_of(const RaggedParams& p, const Unit& u, int v, int entry_bytes) {
+  if (p.tables == nullptr) return p.entries + (u.t0 + v) * p.entry_stride + static_cast<int64_t>(u.g) * entry_bytes;
+  const int64_t e = pool_entry(p, u, v);
+  return e < 0 ? nullptr : p.entries + e * p.entry_stride;
+}
+
+// A row's result from its maximum, sum and sink: the factor of O^T and the log-sum-exp.
+__device__ __forceinline__ float finish_row(const RaggedParams& p, int head, float m, float l, float& lse) {
+  const bool none = l == 0.0f && m == -__builtin_huge_valf();  // it sees nothing: lse is the sink itself
+  float scale = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  if (p.sinks) {
+    const float sk = p.sinks[head] * kLog2e;
+    const float mm = fmaxf(m, sk);
+    if (mm > -__builtin_huge_valf()) {
+      const float a = m == -__builtin_huge_valf() ? 0.0f : exp2f(m - mm);
+      l = l * a + exp2f(sk - mm);
+      m = mm;
+      scale = a / l;
+    }
+  }
+  lse = !none ? (m + __log2f(l)) * kLn2 : p.sinks ? p.sinks[head] : -__builtin_huge_valf();
+  return scale;
+}
 
 template <int FMT, int D, int NOPE>
 struct RaggedLds {
@@ -59,84 +334,8 @@ struct RaggedLds {
   static constexpr int PMAX = PB + 4096;  // [2][64]
   static constexpr int LSUM = PMAX + 512;
   static constexpr int OKS = LSUM + 512;  // [32] words
-  static constexpr int SCAN = OKS + 128;  // [8] int64
-  static constexpr int LDS = SCAN + 128;
+  static constexpr int LDS = OKS + 128 > static_cast<int>(sizeof(PlanLds)) ? OKS + 128 : static_cast<int>(sizeof(PlanLds));
 };
-
-__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
-
-// The sequence and row block of unit k, by a scan over the sequences' blocks; false: none.
-__device__ bool find_unit(const RaggedParams& p, int64_t k, Unit& u, int64_t* scan, int tid) {
-  int64_t blk, per;
-  if (p.cu == nullptr) {
-    per = (p.HG + p.rows_per_unit - 1) / p.rows_per_unit * static_cast<int64_t>(p.G);
-    u.b = k / per;
-    if (u.b >= p.B) return false;
-    blk = k - u.b * per;
-    u.t0 = u.b;
-    u.n = 1;
-  } else {
-    int64_t base = 0;
-    bool found = false;
-    for (int64_t i = 0; i < p.B && !found; i += 256) {
-      int64_t v = 0, a = 0, z = 0;
-      if (i + tid < p.B) {
-        a = clamp64(p.cu[i + tid], 0, p.T);
-        z = clamp64(p.cu[i + tid + 1], a, p.T);
-        v = ((z - a) * p.HG + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
-      }
-      int64_t x = v;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(x, d, 64);
-        if ((tid & 63) >= d) x += y;
-      }
-      if ((tid & 63) == 63) scan[tid >> 6] = x;
-      __syncthreads();
-      int64_t before = base + x - v, total = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (w < (tid >> 6)) before += scan[w];
-        total += scan[w];
-      }
-      if (v > 0 && k >= before && k < before + v) {
-        scan[4] = i + tid;
-        scan[5] = k - before;
-        scan[6] = a;
-        scan[7] = z - a;
-      }
-      found = k < base + total;
-      base += total;
-      __syncthreads();
-    }
-    if (!found) return false;
-    u.b = scan[4];
-    blk = scan[5];
-    u.t0 = scan[6];
-    u.n = scan[7];
-    per = (u.n * p.HG + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
-  }
-  const int64_t per_latent = per / p.G;
-  u.g = static_cast<int>(blk / per_latent);
-  u.r0 = (blk - u.g * per_latent) * p.rows_per_unit;
-  const int64_t rows = u.n * p.HG;
-  u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
-  u.len = u.n;
-  if (p.lens) u.len = clamp64(p.lens[u.b], 0, p.max_pages * p.page);
-  return true;
-}
-
-// The address of the entry at position v of the unit's sequence (or of its list); null where there is none.
-__device__ __forceinline__ const uint8_t* entry_of(const RaggedParams& p, const Unit& u, int64_t v, int entry_bytes) {
-  if (p.tables == nullptr) return p.entries + (u.t0 + v) * p.entry_stride + static_cast<int64_t>(u.g) * entry_bytes;
-  if (p.idx) {
-    v = p.idx[u.b * p.idx_stride + v];
-    if (v < 0 || v >= u.len) return nullptr;
-  }
-  const int64_t pid = p.tables[u.b * p.table_stride + v / p.page];
-  if (pid < 0 || pid >= p.pages) return nullptr;
-  return p.entries + (pid * p.page + v % p.page) * p.entry_stride;
-}
 
 // A tile of 32 entries at a time: bf16 rows in LDS, S^T by matrix instructions (each wave 16 entries x
 // 32 rows), the softmax's running maximum, P^T through LDS, O^T by matrix instructions (each wave
@@ -157,7 +356,7 @@ ragged_kernel(const RaggedParams p) {
   const int eh = wave & 1, hh = wave >> 1, g = lane >> 4, e16 = lane & 15;
 
   Unit u;
-  if (!find_unit(p, blockIdx.x, u, reinterpret_cast<int64_t*>(smem + M::SCAN), tid)) return;  // uniform
+  if (!find_unit(p, u, smem, tid)) return;  // uniform
 
   // the B operand of S^T: rows 32 hh + 16 b + e16, channels 32 st + 8 g ..
   v8bf qf[KS][2];
@@ -165,21 +364,25 @@ ragged_kernel(const RaggedParams p) {
   for (int b = 0; b < 2; ++b) {
     const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
     const int64_t rc = r < u.r1 ? r : u.r0;
-    const uint16_t* qr = p.q + ((u.t0 + rc / p.HG) * p.H + u.g * p.HG + rc % p.HG) * D;
+    const uint16_t* qr = p.q + row_at(p, u, rc) * D;
 #pragma unroll
     for (int st = 0; st < KS; ++st)
       qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(qr + 32 * st + 8 * g));
   }
 
   const int64_t tok0 = u.r0 / p.HG, tok1 = (u.r1 - 1) / p.HG + 1;
-  const int64_t shift = u.len - u.n;  // position of the sequence's first new token (negative: tokens that see nothing)
+  const int64_t shift = static_cast<int64_t>(u.len) - u.n;
+  int share_lo, share_hi;
+  unit_range(p, u, tok0, tok1, share_lo, share_hi);
   // one pass over all rows; if something in it is not finite, one pass for each token over what it sees
   // itself, since a weight of 0 times an entry hidden from a row would not be 0
   int64_t sub0 = tok0, sub1 = tok1;
   bool strict = false;
   while (true) {
-    int64_t lo = clamp64(shift + sub0 - p.window + 1, 0, u.len), hi = clamp64(shift + sub1, 0, u.len);
-    if (p.idx) { lo = 0; hi = u.len > 0 ? p.topk : 0; }
+    int lo, hi;
+    token_range(p, u, sub0, sub1, lo, hi);
+    lo = lo > share_lo ? lo : share_lo;
+    hi = hi < share_hi ? hi : share_hi;
     int64_t row_lo[2], row_hi[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -198,7 +401,7 @@ ragged_kernel(const RaggedParams p) {
       for (int i = 0; i < NI; ++i) acc[i][hg] = v4f{};
     }
     const int te = tid >> 3, tj = tid & 7;
-    for (int64_t v0 = lo; v0 < hi; v0 += kTile) {
+    for (int v0 = lo; v0 < hi; v0 += kTile) {
       const uint8_t* const e = v0 + te < hi ? entry_of(p, u, v0 + te, L::kEntryBytes) : nullptr;
       for (int q = tj; q < L::kPieces; q += 8) {
         if (e) {
@@ -312,20 +515,20 @@ ragged_kernel(const RaggedParams p) {
       const int64_t r = u.r0 + 16 * hg + e16;
       const int64_t tok = r / p.HG;
       if (r >= u.r1 || tok < sub0 || tok >= sub1) continue;
-      const int head = u.g * p.HG + static_cast<int>(r - tok * p.HG);
-      float m = m4[hg], l = l4[hg], scale = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      const bool none = l == 0.0f && m == -__builtin_huge_valf();  // it sees nothing: lse is the sink itself
-      if (p.sinks) {
-        const float sk = p.sinks[head] * kLog2e;
-        const float mm = fmaxf(m, sk);
-        if (mm > -__builtin_huge_valf()) {
-          const float a = m == -__builtin_huge_valf() ? 0.0f : exp2f(m - mm);
-          l = l * a + exp2f(sk - mm);
-          m = mm;
-          scale = a / l;
-        }
+      if (u.shares > 1) {
+        const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? 1.0f / l4[hg] : 0.0f;
+        float* const o = p.part_o + (static_cast<int64_t>(u.slot) * 64 + 16 * hg + e16) * D;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (wave + 4 * i < NB) *reinterpret_cast<v4f*>(o + 16 * (wave + 4 * i) + 4 * g) = acc[i][hg] * inv;
+        if (wave == hg && g == 0)
+          *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + 16 * hg + e16)) = float2{m4[hg], l4[hg]};
+        continue;
       }
-      uint16_t* const o = p.out + ((u.t0 + tok) * p.H + head) * D;
+      const int64_t at = row_at(p, u, r);
+      float lse;
+      const float scale = finish_row(p, static_cast<int>(at % p.H), m4[hg], l4[hg], lse);
+      uint16_t* const o = p.out + at * D;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int c = 16 * (wave + 4 * i) + 4 * g;
@@ -333,15 +536,98 @@ ragged_kernel(const RaggedParams p) {
           *reinterpret_cast<uint2*>(o + c) = uint2{pack_bf16x2(acc[i][hg][0] * scale, acc[i][hg][1] * scale),
                                                    pack_bf16x2(acc[i][hg][2] * scale, acc[i][hg][3] * scale)};
       }
-      if (wave == hg && g == 0)
-        p.lse[(u.t0 + tok) * p.H + head] = !none      ? (m + __log2f(l)) * kLn2
-                                           : p.sinks ? p.sinks[head]
-                                                     : -__builtin_huge_valf();
+      if (wave == hg && g == 0) p.lse[at] = lse;
     }
     if (!strict || sub1 >= tok1) break;
     ++sub0;
     ++sub1;
     __syncthreads();
+  }
+}
+
+// Joins the shares of a row block: workgroup 4 k + j rows 16 j .. of block k of the split sequences.
+// o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the sink.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
+  __shared__ int64_t scan[8];
+  __shared__ float weight[16][kMaxShares + 1];
+  const int tid = threadIdx.x;
+  const int64_t k = blockIdx.x >> 2;
+  const int r16 = 16 * (blockIdx.x & 3);
+  // the block's sequence, as find_unit without shares
+  int64_t base = 0;
+  bool found = false;
+  for (int64_t i = 0; i < p.B && !found; i += 256) {
+    int64_t a, z, v = 0, before;
+    int t;
+    if (i + tid < p.B) v = sequence(p, i + tid, a, z, t);
+    const int64_t sum = block_scan(v, before, scan, tid);
+    if (k >= base + before && k < base + before + v) {
+      scan[4] = i + tid;
+      scan[5] = k - base - before;
+      scan[6] = v;
+    }
+    base += sum;
+    found = k < base;
+  }
+  __syncthreads();
+  if (!found) return;
+  Unit u;
+  u.b = scan[4];
+  const int64_t blk = scan[5], blocks = scan[6];
+  const int shares = p.plan[2 * u.b + 1];
+  if (shares <= 1) return;
+  int64_t a, z;
+  int t;
+  sequence(p, u.b, a, z, t);
+  u.t0 = a;
+  const int64_t per_latent = blocks / p.G;
+  u.g = static_cast<int>(blk / per_latent);
+  u.r0 = (blk - u.g * per_latent) * p.rows_per_unit;
+  const int64_t rows = (z - a) * p.HG;
+  u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
+  const int64_t slot0 = p.plan[2 * u.b] + blk;
+  // weights: 16 threads a row
+  {
+    const int r = tid >> 4;
+    const int64_t row = u.r0 + r16 + r;
+    const float* const ml = p.part_ml + 2 * (slot0 * 64 + r16 + r);
+    float m = -__builtin_huge_valf(), l = 0.0f;
+    for (int s = tid & 15; s < shares; s += 16) m = fmaxf(m, ml[128 * blocks * s]);
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int s = tid & 15; s < shares; s += 16) {
+      const float2 v = *reinterpret_cast<const float2*>(ml + 128 * blocks * s);
+      // l * 2^(m_s - m): a share that saw nothing has l 0 and m -inf, one with a NaN has l NaN
+      const float w = v.x == -__builtin_huge_valf() && v.y == 0.0f ? 0.0f : v.y * exp2f(v.x - m);
+      weight[r][s] = w;
+      l += w;
+    }
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) l += __shfl_xor(l, d, 64);
+    float lse = 0.0f, scale = 0.0f;
+    if (row < u.r1) {
+      const int64_t at = row_at(p, u, row);
+      scale = finish_row(p, static_cast<int>(at % p.H), m, l, lse);
+      if ((tid & 15) == 0) p.lse[at] = lse;
+    }
+    for (int s = tid & 15; s < shares; s += 16) weight[r][s] *= scale;
+  }
+  __syncthreads();
+  constexpr int PIECES = D / 4;
+  for (int i = tid; i < 16 * PIECES; i += 256) {
+    const int r = i / PIECES, c = 4 * (i - r * PIECES);
+    const int64_t row = u.r0 + r16 + r;
+    if (row >= u.r1) break;  // rows ascend with i
+    const float* const o = p.part_o + (slot0 * 64 + r16 + r) * D + c;
+    v4f sum = v4f{};
+    for (int s = 0; s < shares; ++s) {
+      const float w = weight[r][s];
+      const v4f v = *reinterpret_cast<const v4f*>(o + static_cast<int64_t>(64) * D * blocks * s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(w, v[j], sum[j]);
+    }
+    *reinterpret_cast<uint2*>(p.out + row_at(p, u, row) * D + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
   }
 }
 
@@ -358,7 +644,10 @@ __global__ void __launch_bounds__(256) ragged_tail_kernel(const RaggedParams p) 
 template <int FMT, int D, int NOPE>
 int launch_ragged(const RaggedParams& p, hipStream_t s) {
   using M = RaggedLds<FMT, D, NOPE>;
-  ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(p.blocks_max), 256, M::LDS, s>>>(p);
+  // (find_unit's order takes 16 workgroups at a time)
+  const int64_t grid = p.slots ? p.slots : (p.blocks_max + 15) / 16 * 16;
+  ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
+  if (p.slots) join_kernel<D><<<static_cast<unsigned>(4 * p.blocks_max), 256, 0, s>>>(p);
   if (p.zero_tail && p.cu) ragged_tail_kernel<<<256, 256, 0, s>>>(p);
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;
@@ -392,6 +681,22 @@ int64_t unit_bound(const RaggedParams& p) {
 }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+constexpr int kMinTiles = 4;
+
+// How many units a call is split into: 0 for as many as blocks.  With fewer blocks than twice the 256
+// compute units (a unit fills one), up to 256, or 1024 where the blocks alone fill more than half,
+// so that sequences of different lengths still end together.
+int unit_slots(int64_t blocks, int64_t B) {
+  if (blocks > 512 || B > kPlanRows) return 0;
+  return blocks <= 128 ? 256 : 1024;
+}
+
+int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
+
+int64_t attend_bytes(int64_t blocks, int64_t B, int D) {
+  const int slots = unit_slots(blocks, B);
+  return slots ? align16_up(8 * B) + static_cast<int64_t>(slots) * 64 * 4 * (D + 2) : 0;
+}
 
 }  // namespace
 }  // namespace mzk
@@ -408,6 +713,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                     max_pages <= kMaxInt,
                 "paged_attend: sizes of 2^31 or more");
   MZK_CHECK_ARG(page >= 1, "paged_attend: pages of at least one entry");
+  MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
+                "paged_attend: a sequence and a pool hold less than 2^31 entries");
   MZK_CHECK_ARG(fmt == 0 || fmt == 1, "paged_attend: fmt must be 0 (bf16) or 1 (fp8-b128)");
   MZK_CHECK_ARG(window >= 0 && topk >= 0, "paged_attend: negative window or list");
   MZK_CHECK_ARG(cu || T == B, "paged_attend: without cu one token per sequence (%lld tokens, %lld sequences)",
@@ -446,15 +753,37 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt, "paged_attend: too many rows");
+  MZK_CHECK_ARG(p.blocks_max <= kMaxInt - 16, "paged_attend: too many rows");
+  const int64_t need = attend_bytes(p.blocks_max, B, D);
+  MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attend: workspace needs %lld bytes",
+                (long long)need);
+  // what a sequence can hold, or a token see, in tiles
+  int64_t most = max_pages * page;
+  if (window && window + T < most) most = window + T;
+  if (idx) most = topk;
+  p.min_tiles = kMinTiles;
+  p.slots = (most + kTile - 1) / kTile > kMinTiles ? unit_slots(p.blocks_max, B) : 0;
+  if (p.slots) {
+    p.plan = static_cast<int32_t*>(workspace);
+    p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align16_up(8 * B));
+    p.part_o = p.part_ml + static_cast<int64_t>(p.slots) * 64 * 2;
+  }
   return dispatch_ragged("paged_attend", fmt, nope, p, as_stream(stream));
 }
 
 extern "C" int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t* bytes) {
   MZK_CHECK_ARG(bytes != nullptr, "paged_attend_workspace_bytes: null output");
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0, "paged_attend_workspace_bytes: bad sizes");
-  (void)packed;
-  *bytes = 0;
+  MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536 && D <= 65536, "paged_attend_workspace_bytes: sizes of 2^31 or more");
+  RaggedParams p{};
+  p.T = T;
+  p.HG = H;
+  p.G = 1;
+  p.B = B;
+  p.rows_per_unit = 32 * H < 64 ? 32 * H : 64;
+  const int64_t some = 0;
+  p.cu = packed ? &some : nullptr;  // only whether there is one counts
+  *bytes = attend_bytes(unit_bound(p), B, D);
   return MZK_OK;
 }
 
@@ -489,6 +818,6 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt, "packed_mqa: too many rows");
+  MZK_CHECK_ARG(p.blocks_max <= kMaxInt - 16, "packed_mqa: too many rows");
   return dispatch_ragged("packed_mqa", kFmtBf16, D, p, as_stream(stream));
 }
