@@ -63,6 +63,13 @@ struct Unit {
 
 __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return static_cast<int64_t>(static_cast<uint32_t>(uniform(static_cast<int>(v)))) |
+         static_cast<int64_t>(uniform(static_cast<int>(v >> 32))) << 32;
+}
+
 // Sums over a workgroup of 256 (lds: 4 words).
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_t* lds, int tid) {
   int64_t x = v;
@@ -257,6 +264,16 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
   u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
   u.len = u.n;
   if (p.lens) u.len = static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page));
+  u.b = uniform(u.b);
+  u.t0 = uniform(u.t0);
+  u.n = uniform(u.n);
+  u.len = uniform(u.len);
+  u.g = uniform(u.g);
+  u.r0 = uniform(u.r0);
+  u.r1 = uniform(u.r1);
+  u.share = uniform(u.share);
+  u.shares = uniform(u.shares);
+  u.slot = uniform(u.slot);
   __syncthreads();  // the plan's LDS is free
   return true;
 }
@@ -545,6 +562,8 @@ ragged_kernel(const RaggedParams p) {
   }
 }
 
+#include "ragged_wide.h"
+
 // Joins the shares of a row block: workgroup 4 k + j rows 16 j .. of block k of the split sequences.
 // o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the sink.
 template <int D>
@@ -643,10 +662,29 @@ __global__ void __launch_bounds__(256) ragged_tail_kernel(const RaggedParams p) 
 
 template <int FMT, int D, int NOPE>
 int launch_ragged(const RaggedParams& p, hipStream_t s) {
-  using M = RaggedLds<FMT, D, NOPE>;
   // (find_unit's order takes 16 workgroups at a time)
   const int64_t grid = p.slots ? p.slots : (p.blocks_max + 15) / 16 * 16;
-  ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
+  if constexpr (D >= 512) {
+    using M = WideLds<FMT, D>;
+    auto kern = ragged_wide_kernel<FMT, D, NOPE>;
+    // the dynamic-LDS limit is a per-device function attribute: set once per device
+    static std::atomic<bool> attr_set[kMaxDevices] = {};  // setting it twice is harmless
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
+      set_last_error("ragged attention: no usable current device");
+      return MZK_ELAUNCH;
+    }
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, M::LDS) != hipSuccess) {
+        set_last_error("ragged attention: cannot raise the kernel's LDS limit to %d bytes", M::LDS);
+        return MZK_ELAUNCH;
+      }
+      attr_set[dev].store(true, std::memory_order_release);
+    }
+    kern<<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
+  } else {
+    ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, RaggedLds<FMT, D, NOPE>::LDS, s>>>(p);
+  }
   if (p.slots) join_kernel<D><<<static_cast<unsigned>(4 * p.blocks_max), 256, 0, s>>>(p);
   if (p.zero_tail && p.cu) ragged_tail_kernel<<<256, 256, 0, s>>>(p);
   MZK_LAUNCH_CHECK("ragged attention");
@@ -794,8 +832,8 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536, "packed_mqa: sizes of 2^31 or more");
   MZK_CHECK_ARG(H % G == 0, "packed_mqa: %d heads do not divide into %d latents", H, G);
   MZK_CHECK_ARG(window >= 0, "packed_mqa: negative window");
-  MZK_CHECK_ARG(kv_row_stride >= static_cast<int64_t>(G) * D && kv_row_stride % 8 == 0,
-                "packed_mqa: kv rows must be G * D apart or more, a multiple of 8 elements");
+  MZK_CHECK_ARG(kv_row_stride >= static_cast<int64_t>(G) * D && kv_row_stride % 8 == 0 && kv_row_stride < 1ll << 30,
+                "packed_mqa: kv rows must be G * D apart or more, a multiple of 8 elements below 2^30");
   if (T == 0) return MZK_OK;
   MZK_CHECK_ARG(q && kv && cu && out && lse, "packed_mqa: null pointer");
   MZK_CHECK_ARG(aligned16(q) && aligned16(kv) && aligned16(out), "packed_mqa: q, kv and out must be 16-byte aligned");

@@ -1,0 +1,699 @@
+// The ragged attention kernel for wide latents, D = 512 and 576 (ragged.hip includes this inside its
+// namespace, after the units).
+//
+// One workgroup = one unit: 4 waves, one per SIMD with the whole register file (512 VGPRs per lane),
+// over tiles of 32 entries held as bf16 in LDS.
+//   S^T  wave (eh, hh): entries 16 eh .. + 15 of the tile x rows 32 hh .. + 31 over all channels
+//        (v_mfma_f32_16x16x32_bf16, two row groups per K operand read), so a score is whole in the
+//        lane that has it;
+//   P^T  goes to LDS in bf16 (4 KB a tile, two of them);
+//   O^T  wave w: the 16-channel blocks w, w + 4, .. for all 64 rows, one V^T operand read for four
+//        row groups.
+// One barrier per tile: in iteration u the workgroup runs S(u+1) and PV(u), whose matrix work covers
+// the softmax of u+1, while tile u+2 (8-bit entries, dequantized from registers) or u+3 (bf16
+// entries, loaded straight into LDS) arrives.
+//
+// A tile in LDS is D / 64 columns of 32 rows of 128 bytes: a wave's load instruction (8 rows x 128
+// bytes, a lane 16 of them) fills 1 KB of one column, in lane order as the hardware wants it, from
+// one address per lane and tile.  The 16-byte piece x of row r sits at slot x ^ wide_swz(r).
+//
+// Softmax: the exponent's reference of a row is its maximum over the first tile (0 where it sees
+// none of that): softmax is exact for any reference as long as nothing overflows or underflows.  A
+// weight may then reach 2^(rise of the scores above it): up to kRoomNear the product with a value
+// is within the range of a rescaled softmax; above, the accumulators are looked at after the
+// pass.  Where the sum would overflow, or a row that began at 0 stayed far below, the pass is made
+// again from the true maxima of a pass over the scores alone.  So no tile waits for the other
+// waves' maxima, and O^T is never rescaled.
+//
+// Entries hidden from a row have weight 0, which does not hide a value that is not finite: a unit of
+// several tokens whose result is not finite is computed again one token at a time, each over what it
+// sees itself.
+
+constexpr float kWideRoomNear = 8.0f, kWideRoomAbove = 100.0f, kWideRoomBelow = -40.0f;  // log2 units from the reference
+constexpr float kHidden = -3.0e38f;  // a hidden entry's score: weight 0
+
+// Rows 2 j and 2 j + 1 share a line of banks; rows 16 apart the same slots.  With the bits of j =
+// row / 2 reversed, the 16 rows of a K operand's phase lie on 16 distinct bank quads, and so do the
+// four rows x 32 bytes of a phase of the transposing reads of V^T.
+__device__ __forceinline__ int wide_swz(int row) { return ((row >> 1 & 1) << 2) | ((row >> 2 & 1) << 1) | (row >> 3 & 1); }
+
+template <int FMT, int D>
+struct WideLds {
+  static constexpr bool kDirect = FMT == kFmtBf16;
+  static constexpr int TILE = 64 * D;
+  static constexpr int BUFS = kDirect ? 4 : 3;
+  static constexpr int PB = BUFS * TILE;           // P^T: 2 x [4 row groups][64 lanes] x 16 bytes
+  static constexpr int CT = kDirect ? 40 : 64;     // tiles whose entry codes are laid out at a time (at most 64)
+  static constexpr int TAB = PB + 2 * 4096;        // codes; fetched up to 4 tiles past the last
+  static constexpr int TABN = (CT + 4) * kTile;
+  static constexpr int MASK = TAB + 4 * TABN;      // entries that are there, of each tile
+  static constexpr int PMAX = MASK + 4 * 72;       // [2 eh][64]
+  static constexpr int LSUM = PMAX + 512;          // [2 eh][64]
+  static constexpr int RED = LSUM + 512;
+  static constexpr int LDS = RED + 32;
+  static_assert(LDS <= 160 * 1024 && sizeof(PlanLds) <= PB, "LDS");
+};
+
+// 16 bytes per lane from `at` + 128 J to LDS, for columns J .. N - 1 of a tile: lane l's to byte lds + 4096 J +
+// 16 l.  The wave's base is in m0, and the instruction's offset counts for both addresses.
+template <int J, int N>
+__device__ __forceinline__ void load_columns(gptr_t at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
+               : : "s"(lds + (4096 - 128) * J), "v"(at), "n"(128 * J) : "memory");
+  if constexpr (J + 1 < N) load_columns<J + 1, N>(at, lds);
+}
+
+// 8-bit entries in flight: one thread's pieces of entry tid / 8.
+struct WideRaw {
+  u32x4 v[5];
+  u32x4 s;  // the entry's four block scales
+};
+
+template <int FMT, int D, int NOPE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+ragged_wide_kernel(const RaggedParams p) {
+  using M = WideLds<FMT, D>;
+  constexpr bool kDirect = M::kDirect;
+  constexpr int NT = 256, KS = D / 32, NI = D / 64, COL = 4096;
+  constexpr int EB = Layout<FMT, D, NOPE>::kEntryBytes;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint32_t* const tab = reinterpret_cast<uint32_t*>(smem + M::TAB);
+  uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + M::MASK);
+  float* const pmax = reinterpret_cast<float*>(smem + M::PMAX);
+  float* const lsum = reinterpret_cast<float*>(smem + M::LSUM);
+  int* const redo = reinterpret_cast<int*>(smem + M::RED);
+  int* const high = redo + 1;
+  int* const odd = redo + 2;
+  uint8_t* const pbuf = smem + M::PB;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int eh = wave & 1, hh = wave >> 1;
+  const int g = lane >> 4, e16 = lane & 15;
+
+  Unit u;
+  if (!find_unit(p, u, smem, tid)) return;  // uniform
+
+  // q: the B operand of S^T (rows 32 hh + 16 b + e16, channels 32 st + 8 g ..) through LDS, from
+  // whole lines
+  const int rows = static_cast<int>(u.r1 - u.r0);
+  constexpr int QROW = D / 8, QP = 64 * QROW / NT;
+  u32x4 qraw[QP];
+#pragma unroll
+  for (int k = 0; k < QP; ++k) {
+    const int at = tid + NT * k;
+    const int r = at / QROW;
+    qraw[k] = *reinterpret_cast<const u32x4*>(p.q + row_at(p, u, u.r0 + (r < rows ? r : 0)) * D + 8 * (at - r * QROW));
+  }
+  const int64_t tok0 = u.r0 / p.HG, tok1 = (u.r1 - 1) / p.HG + 1;
+  const int shift = u.len - u.n;
+  int share_lo, share_hi;
+  unit_range(p, u, tok0, tok1, share_lo, share_hi);
+  int tok_b[2];  // the tokens of this lane's rows
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
+    tok_b[b] = static_cast<int>((r < u.r1 ? r : u.r0) / p.HG);
+  }
+  const int win = p.window < 0x7fffffff ? static_cast<int>(p.window) : 0x7fffffff;
+
+  // ---- addresses -------------------------------------------------------------------------
+  const int te = tid >> 3, tj = tid & 7;
+  const uint32_t k_even = static_cast<uint32_t>((16 * eh + e16) * 128 + 16 * (g ^ wide_swz(e16)));
+  const uint32_t k_odd = k_even ^ 64u;
+  const int vrow = 4 * g + (e16 >> 2);
+  const uint32_t v_at = static_cast<uint32_t>(vrow * 128 + 16 * ((2 * wave + ((e16 >> 1) & 1)) ^ wide_swz(vrow)) + 8 * (e16 & 1));
+  // 8-bit entries: this thread's code pieces are pairs of bf16 pieces of columns tj / 4 + 2 k
+  const uint32_t st_at = static_cast<uint32_t>(COL * (tj >> 2) + te * 128 + 16 * ((2 * (tj & 3)) ^ wide_swz(te)));
+  const uint32_t rope_at = static_cast<uint32_t>(COL * 8 + te * 128 + 16 * (tj ^ wide_swz(te)));
+  const uint64_t pool_piece = reinterpret_cast<uint64_t>(p.entries) +
+                              (p.tables ? 0 : static_cast<uint64_t>(u.t0) * p.entry_stride + static_cast<uint64_t>(u.g) * EB) +
+                              16u * (kDirect ? tj ^ wide_swz(te) : tj);
+  const uint32_t entry_stride = static_cast<uint32_t>(p.entry_stride);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem)) + 1024u * wave;
+  const bool paged = p.tables != nullptr;
+
+  auto entry_at = [&](uint32_t code) __attribute__((always_inline)) -> gptr_t {
+    return (gptr_t)(pool_piece + static_cast<uint64_t>(code) * entry_stride);
+  };
+  auto fetch_part = [&](gptr_t e, WideRaw& r, int k) __attribute__((always_inline)) {
+    if (k < 4) r.v[k] = gload<u32x4>(e + 128 * k);
+    if (k == 4) r.v[4] = gload<u32x4>(e + NOPE + 16);
+    if (k == 5) r.s = gload<u32x4>(e - 16 * tj + NOPE);
+  };
+  // part k (of 9) of a fetched tile into LDS: parts 2 q, 2 q + 1 are the halves of code piece q (16
+  // codes: two bf16 pieces), part 8 the rope slice
+  auto store_part = [&](uint8_t* t, const WideRaw& r, int k) __attribute__((always_inline)) {
+    if (k < 8) {
+      const int q = k >> 1;
+      const uint2 codes = k & 1 ? uint2{r.v[q].z, r.v[q].w} : uint2{r.v[q].x, r.v[q].y};
+      *reinterpret_cast<uint4*>(t + ((k & 1 ? st_at ^ 16u : st_at) + 2 * COL * q)) = dequant_fp8x8_bf16(codes, __uint_as_float(r.s[q]));
+    } else {
+      *reinterpret_cast<uint4*>(t + rope_at) = uint4{r.v[4].x, r.v[4].y, r.v[4].z, r.v[4].w};
+    }
+  };
+  auto k_frag = [&](const uint8_t* t, int st) __attribute__((always_inline)) -> v8bf {
+    return __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(t + (st & 1 ? k_odd : k_even) + COL * (st >> 1)));
+  };
+  auto tile_at = [&](int i) __attribute__((always_inline)) -> uint32_t { return static_cast<uint32_t>(i) * M::TILE; };
+
+  float m4[4], m_own[2], l_own[2], m_seen[2];
+  v4f acc[NI][4];
+  v8bf qf[KS][2];
+  v4f s_acc[2];
+  WideRaw raw[2];
+
+  int lo = 0, hi = 0;       // the pass's entries: positions lo .. hi - 1
+  int c0 = 0, nt = 0;       // the chunk at hand: its first entry (from lo), its tiles
+  int row_lo[2], row_span[2];  // of this lane's rows, entries seen, from lo
+  int full_lo = 0, full_hi = 0;  // tiles (from lo) of which every row sees every entry
+  // the entry that a lane fetches for tile t of the chunk: past the end of the range its last one
+  auto code_of = [&](int t) __attribute__((always_inline)) -> uint32_t {
+    if (paged) return tab[t * kTile + te];
+    const int v = c0 + t * kTile + te;
+    return static_cast<uint32_t>(lo + (v < hi - lo ? v : hi - lo - 1));
+  };
+  auto direct = [&](gptr_t e, uint32_t buf) __attribute__((always_inline)) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + buf);
+    load_columns<0, NI>(e, at);
+  };
+  // a whole tile into a buffer, waited for by nobody yet
+  auto bring = [&](int t, uint32_t buf) __attribute__((always_inline)) {
+    const gptr_t e = entry_at(code_of(t));
+    if constexpr (kDirect) {
+      direct(e, buf);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 6; ++k) fetch_part(e, raw[0], k);
+#pragma unroll
+      for (int k = 0; k < 9; ++k) store_part(smem + buf, raw[0], k);
+    }
+  };
+  auto landed = [&]() __attribute__((always_inline)) {
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    lds_barrier();
+  };
+
+  // The entry codes of the chunk's tiles and which entries are there; false: none is.  An empty slot
+  // is fetched as another entry that is there (its weight is 0).
+  int first = 0, last = 0;  // the chunk's first and last tile that hold an entry
+  auto lay_out = [&]() __attribute__((always_inline)) -> bool {
+    const int left = hi - lo - c0;
+    nt = (left < M::CT * kTile ? left + kTile - 1 : M::CT * kTile) / kTile;
+    if (!paged) {
+      nt = (left + kTile - 1) / kTile;
+      first = 0;
+      last = nt - 1;
+      return left > 0;
+    }
+    constexpr uint32_t kEmpty = 0xffffffffu;
+    const int n_tab = (nt + 4) * kTile;
+    for (int e0 = 0; e0 < n_tab; e0 += NT) {
+      const int e = e0 + tid;
+      uint32_t code = kEmpty;
+      if (e < nt * kTile && e < left) {
+        const int64_t at = pool_entry(p, u, lo + c0 + e);
+        if (at >= 0) code = static_cast<uint32_t>(at);
+      }
+      const uint64_t bal = __ballot(code != kEmpty);
+      if (e < n_tab) {
+        tab[e] = code;
+        if ((lane & 31) == 0) masks[e / kTile] = static_cast<uint32_t>(lane ? bal >> 32 : bal);
+      }
+    }
+    lds_barrier();
+    const uint64_t some = __ballot(lane < nt && masks[lane < nt ? lane : 0] != 0u);
+    if (some == 0) return false;
+    first = __builtin_ctzll(some);
+    last = 63 - __builtin_clzll(some);
+    const uint32_t any = tab[first * kTile + __builtin_ctz(masks[first])];
+    for (int e = tid; e < n_tab; e += NT)
+      if (tab[e] == kEmpty) tab[e] = any;
+    lds_barrier();
+    return true;
+  };
+
+  // whether tile t of the chunk is seen whole by every row
+  auto whole = [&](int t) __attribute__((always_inline)) -> bool {
+    const int at = c0 / kTile + t;
+    return at >= full_lo && at < full_hi && (!paged || __builtin_amdgcn_readfirstlane(masks[t]) == 0xffffffffu);
+  };
+  // entry r (of 4) of this lane in tile t, for row group b
+  auto sees = [&](int t, uint32_t bits, int b, int r) __attribute__((always_inline)) -> bool {
+    const int v = c0 + t * kTile + 16 * eh + 4 * g + r;
+    return ((bits >> (16 * eh + 4 * g + r)) & 1u) != 0u && static_cast<uint32_t>(v - row_lo[b]) < static_cast<uint32_t>(row_span[b]);
+  };
+  auto scores = [&](int t, float (&v)[2][4]) __attribute__((always_inline)) {
+    const uint32_t bits = paged ? masks[t] : 0xffffffffu;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[b][r] = sees(t, bits, b, r) ? s_acc[b][r] * p.scale_log2 : -__builtin_huge_valf();
+  };
+  auto s_tile = [&](const uint8_t* kt) __attribute__((always_inline)) {
+    s_acc[0] = s_acc[1] = v4f{};
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
+      const v8bf kf = k_frag(kt, st);
+      s_acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][0], s_acc[0], 0, 0, 0);
+      s_acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][1], s_acc[1], 0, 0, 0);
+    }
+  };
+  auto max4 = [](const float (&v)[4]) __attribute__((always_inline)) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
+  auto row_max = [](float x) __attribute__((always_inline)) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+  };
+  // the rows' maxima over both entry halves into m4 / m_own (one barrier); 0 for a row without one
+  auto agree_max = [&](float t0, float t1) __attribute__((always_inline)) {
+    t0 = row_max(t0);
+    t1 = row_max(t1);
+    if (g == 0) {
+      pmax[eh * 64 + 32 * hh + e16] = t0;
+      pmax[eh * 64 + 32 * hh + 16 + e16] = t1;
+    }
+    lds_barrier();
+    auto known = [](float a, float b) { const float m = fmaxf(a, b); return m == -__builtin_huge_valf() ? 0.0f : m; };
+#pragma unroll
+    for (int hg = 0; hg < 4; ++hg) m4[hg] = known(pmax[16 * hg + e16], pmax[64 + 16 * hg + e16]);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) m_own[b] = known(pmax[32 * hh + 16 * b + e16], pmax[64 + 32 * hh + 16 * b + e16]);
+  };
+  auto put_p = [&](int t, int b, uint2 w) __attribute__((always_inline)) {
+    *reinterpret_cast<uint2*>(pbuf + (t & 1) * 4096 + 2048 * hh + 1024 * b + 16 * lane + 8 * eh) = w;
+  };
+  auto read_v = [&](const uint8_t* vt, int i, v4s (&va)[2]) __attribute__((always_inline)) {
+    const uint8_t* tp = vt + v_at + COL * i;
+    va[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp));
+    va[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp + 2048));
+  };
+
+  // ---- one chunk of the pass: tiles `first` .. `last` ------------------------------------------
+  // begin: the rows' references come from its first tile
+  auto chunk = [&](bool begin) __attribute__((always_inline)) {
+    const int t0 = first, n = last + 1;
+    if constexpr (kDirect) {
+      direct(entry_at(code_of(t0)), tile_at(0));
+      direct(entry_at(code_of(t0 + 1 < n ? t0 + 1 : t0)), tile_at(1));
+      direct(entry_at(code_of(t0 + 2 < n ? t0 + 2 : t0)), tile_at(2));
+      if constexpr (NI > 8) asm volatile("s_waitcnt vmcnt(18)" : : : "memory");
+      else asm volatile("s_waitcnt vmcnt(16)" : : : "memory");
+    } else {
+#pragma unroll
+      for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0)), raw[0], k);
+#pragma unroll
+      for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0 + 1)), raw[1], k);
+#pragma unroll
+      for (int k = 0; k < 9; ++k) store_part(smem, raw[0], k);
+      if (n - t0 > 1) {
+#pragma unroll
+        for (int k = 0; k < 9; ++k) store_part(smem + M::TILE, raw[1], k);
+        const int second = (n - 1 - t0) & 1;  // set 1 is stored first then
+#pragma unroll
+        for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0 + 2 + second)), raw[0], k);
+#pragma unroll
+        for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0 + 3 - second)), raw[1], k);
+      }
+    }
+    lds_barrier();
+    s_tile(smem);
+    {
+      float v[2][4];
+      scores(t0, v);
+      if (begin) agree_max(max4(v[0]), max4(v[1]));
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(v[b][r] - m_own[b]);
+        l_own[b] = l_own[b] + ((w[0] + w[1]) + (w[2] + w[3]));
+        put_p(t0, b, uint2{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])});
+        if (!begin) m_seen[b] = fmaxf(m_seen[b], fmaxf(fmaxf(s_acc[b][0], s_acc[b][1]), fmaxf(s_acc[b][2], s_acc[b][3])));
+      }
+    }
+    uint32_t at_v = 0, at_k = tile_at(1), at_n = tile_at(2), at_w = tile_at(kDirect ? 3 : 2);
+    // One wave per SIMD issues in order, so the iteration is laid out by hand: every LDS operand
+    // is requested several matrix instructions before its use (K six steps, V^T four blocks),
+    // the softmax, the stores and the loads are spread one slice after each matrix instruction,
+    // whose 16 cycles they fill, and the last two blocks of PV(u-1), whose operands are in
+    // registers by then, follow the barrier and cover the first reads of K.
+    constexpr int AH = 6, VH = 4, LATE = 2;
+    v4s va[VH + 1][2];
+    v8bf pf[4];
+    auto pv_block = [&](int i, auto&& fill) __attribute__((always_inline)) {
+      const v4s a = va[i % (VH + 1)][0], b = va[i % (VH + 1)][1];
+      const v8bf vf = __builtin_bit_cast(v8bf, v8s{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+#pragma unroll
+      for (int hg = 0; hg < 4; ++hg) {
+        acc[i][hg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[hg], acc[i][hg], 0, 0, 0);
+        fill(hg);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto read_p = [&](int t, int hg) __attribute__((always_inline)) {
+      pf[hg] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(pbuf + (t & 1) * 4096 + 1024 * hg + 16 * lane));
+    };
+#pragma unroll
+    for (int i = 0; i <= VH; ++i) va[i][0] = va[i][1] = v4s{0, 0, 0, 0};
+#pragma unroll
+    for (int hg = 0; hg < 4; ++hg) pf[hg] = __builtin_bit_cast(v8bf, v4i{0, 0, 0, 0});
+    if constexpr (kDirect) {  // tile t0 + 1
+      if constexpr (NI > 8) asm volatile("s_waitcnt vmcnt(9)" : : : "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
+    }
+    lds_barrier();  // P(t0) complete
+    auto step = [&](int t, WideRaw& r) __attribute__((always_inline)) {
+      // the barrier before: P(t) and tile t+1 complete; tile t-1 is read no more
+      const uint8_t* vt = smem + at_v;
+      const uint8_t* kt = smem + at_k;
+      uint8_t* const wt = smem + at_w;
+      v8bf kf[AH];
+#pragma unroll
+      for (int i = 0; i < AH; ++i) kf[i] = k_frag(kt, i);
+      uint32_t code;
+      if constexpr (kDirect) code = code_of(t + 3 < n ? t + 3 : n - 1);
+      else code = tab[(t + 4) * kTile + te];
+      // hidden entries start from kHidden instead of 0, so that no score needs a test
+      v4f init[2] = {v4f{}, v4f{}};
+      if (!whole(t + 1)) {
+        const uint32_t bits = paged ? masks[t + 1] : 0xffffffffu;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) init[b][k] = sees(t + 1, bits, b, k) ? 0.0f : kHidden;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = NI - LATE; i < NI; ++i) pv_block(i, [](int) {});
+      uint64_t next = 0;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const v8bf cur = kf[st % AH];
+        s_acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur, qf[st][0], st == 0 ? init[0] : s_acc[0], 0, 0, 0);
+        if (st + AH < KS) kf[st % AH] = k_frag(kt, st + AH);
+        __builtin_amdgcn_sched_barrier(0);
+        s_acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur, qf[st][1], st == 0 ? init[1] : s_acc[1], 0, 0, 0);
+        if (st == 2) next = pool_piece + static_cast<uint64_t>(code) * entry_stride;
+        if (st >= 8 && st < 12) read_p(t, st - 8);
+        if (st >= KS - VH - 2 && st < KS - 2) read_v(vt, st - (KS - VH - 2), va[st - (KS - VH - 2)]);
+        if constexpr (!kDirect) {
+          if (st >= KS - 2) store_part(wt, r, 7 + st - (KS - 2));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kDirect) {
+          if (st == 3) {
+            direct((gptr_t)next, at_w);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      const gptr_t from = (gptr_t)next;
+      float v[2][4], pr[2][4];
+      // slice k of what fills the matrix instructions of PV
+      auto slice = [&](int k) __attribute__((always_inline)) {
+        if (k >= 2 && k < 10) {
+          const int b = (k - 2) >> 2, j = (k - 2) & 3;
+          v[b][j] = s_acc[b][j];
+          pr[b][j] = __builtin_fmaf(v[b][j], p.scale_log2, -m_own[b]);
+        } else if (k >= 10 && k < 18) {  // v_exp_f32 directly: results below 2^-126 may flush to 0
+          const int b = (k - 10) >> 2, j = (k - 10) & 3;
+          pr[b][j] = __builtin_amdgcn_exp2f(pr[b][j]);
+        } else if (k == 18 || k == 19) {
+          const int b = k - 18;
+          put_p(t + 1, b, uint2{pack_bf16x2(pr[b][0], pr[b][1]), pack_bf16x2(pr[b][2], pr[b][3])});
+        } else if (k >= 20 && k < 22) {
+          const int b = k - 20;
+          l_own[b] = l_own[b] + ((pr[b][0] + pr[b][1]) + (pr[b][2] + pr[b][3]));
+        } else if (k >= 22 && k < 24) {
+          const int b = k - 22;
+          m_seen[b] = fmaxf(fmaxf(m_seen[b], v[b][0]), fmaxf(v[b][1], fmaxf(v[b][2], v[b][3])));
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < NI - LATE; ++i)
+        pv_block(i, [&](int hg) __attribute__((always_inline)) {
+          if (hg == 0 && i + VH < NI) read_v(vt, i + VH, va[(i + VH) % (VH + 1)]);
+          slice(4 * i + hg);
+          if constexpr (!kDirect) {
+            if (hg == 1) store_part(wt, r, i);
+            // a piece is requested again, for tile t + 4, once all of it is stored
+            if (hg == 3 && (i & 1)) fetch_part(from, r, i >> 1);
+            if (hg >= 2 && i == 6) fetch_part(from, r, hg == 2 ? 3 : 5);
+            if (hg == 3 && i == 0) fetch_part(from, r, 4);
+          }
+        });
+      if constexpr (kDirect) {  // tile t + 2; the loads of t + 3 stay in flight
+        if constexpr (NI > 8) asm volatile("s_waitcnt vmcnt(9)" : : : "memory");
+        else asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
+      }
+      lds_barrier();
+      const uint32_t done = at_v;
+      at_v = at_k;
+      if constexpr (kDirect) {
+        at_k = at_n;
+        at_n = at_w;
+      } else {
+        at_k = at_w;
+      }
+      at_w = done;
+    };
+    int t = t0;
+    if constexpr (kDirect) {
+#pragma unroll 1
+      for (; t + 1 < n; ++t) step(t, raw[0]);
+    } else {
+      // an odd number of steps takes one first: the loop is two steps long (two sets of loads in
+      // flight) with a single exit, or every accumulator would be copied between its ends
+      if ((n - 1 - t0) & 1) step(t++, raw[1]);
+#pragma unroll 1
+      for (; t + 1 < n; t += 2) {
+        step(t, raw[0]);
+        step(t + 1, raw[1]);
+      }
+    }
+    {  // the rest of the last but one, and the last tile
+      const uint8_t* vt = smem + at_v;
+#pragma unroll
+      for (int i = NI - LATE; i < NI; ++i) pv_block(i, [](int) {});
+#pragma unroll
+      for (int hg = 0; hg < 4; ++hg) read_p(n - 1, hg);
+#pragma unroll
+      for (int i = 0; i < VH; ++i) read_v(vt, i, va[i]);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        pv_block(i, [&](int hg) __attribute__((always_inline)) {
+          if (hg == 0 && i + VH < NI) read_v(vt, i + VH, va[(i + VH) % (VH + 1)]);
+        });
+    }
+    landed();  // the LDS is free again
+  };
+
+  // q into its operand's layout
+  {
+    constexpr int QPITCH = 2 * D + 16;  // the pad spreads 16 rows' pieces over the banks
+    static_assert(64 * QPITCH <= M::PB, "q in the tiles' place");
+#pragma unroll
+    for (int k = 0; k < QP; ++k) {
+      const int at = tid + NT * k;
+      const int r = at / QROW;
+      *reinterpret_cast<u32x4*>(smem + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + (32 * hh + 16 * b + e16) * QPITCH + 64 * st + 16 * g));
+    lds_barrier();
+    // the first query fragments live in accumulation registers beside O^T, which the matrix
+    // instructions read directly; left to itself the compiler spills
+#pragma unroll
+    for (int st = 0; st < KS - 6; ++st)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        v4i x = __builtin_bit_cast(v4i, qf[st][b]);
+        asm volatile("" : "+a"(x));
+        qf[st][b] = __builtin_bit_cast(v8bf, x);
+      }
+  }
+
+  // ---- the passes --------------------------------------------------------------------------
+  int64_t sub0 = tok0, sub1 = tok1;
+  bool strict = false;
+  while (true) {
+    token_range(p, u, sub0, sub1, lo, hi);
+    lo = lo > share_lo ? lo : share_lo;
+    hi = hi < share_hi ? hi : share_hi;
+    if (hi < lo) hi = lo;
+    {
+      // what the rows see, from lo; tiles that all of them see whole
+      int most_lo = lo, least_hi = hi;
+      if (!p.idx) {
+        const int64_t a = static_cast<int64_t>(shift) + sub1 - 1 - (static_cast<int64_t>(win) - 1), z = static_cast<int64_t>(shift) + sub0 + 1;
+        most_lo = a > lo ? static_cast<int>(a) : lo;
+        least_hi = z < hi ? static_cast<int>(z) : hi;
+      }
+      full_lo = (most_lo - lo + kTile - 1) / kTile;
+      full_hi = least_hi > lo ? (least_hi - lo) / kTile : 0;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        int64_t a = lo, z = hi;
+        if (!p.idx) {
+          const int64_t pos = static_cast<int64_t>(shift) + tok_b[b];
+          if (pos - win + 1 > a) a = pos - win + 1;
+          if (pos + 1 < z) z = pos + 1;
+        }
+        row_lo[b] = static_cast<int>(a - lo);
+        row_span[b] = z > a ? static_cast<int>(z - a) : 0;
+      }
+    }
+    float l4[4];
+    int e4[4];
+    for (bool given = false;; given = true) {
+      if (tid == 0) *redo = *high = *odd = 0;
+      bool begun = false;
+      if (given) {  // the true maxima of every row: scores only
+        float t0 = -__builtin_huge_valf(), t1 = t0;
+        for (c0 = 0; c0 < hi - lo; c0 += nt * kTile) {
+          if (!lay_out()) continue;
+#pragma unroll 1
+          for (int t = first; t <= last; ++t) {
+            bring(t, 0);
+            landed();
+            s_tile(smem);
+            float v[2][4];
+            scores(t, v);
+            t0 = fmaxf(t0, max4(v[0]));
+            t1 = fmaxf(t1, max4(v[1]));
+            lds_barrier();
+          }
+        }
+        agree_max(t0, t1);
+        lds_barrier();
+        begun = true;
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int hg = 0; hg < 4; ++hg) acc[i][hg] = v4f{};
+      l_own[0] = l_own[1] = 0.0f;
+      m_seen[0] = m_seen[1] = -__builtin_huge_valf();
+      if (!begun) {
+        m_own[0] = m_own[1] = 0.0f;
+#pragma unroll
+        for (int hg = 0; hg < 4; ++hg) m4[hg] = 0.0f;
+      }
+      for (c0 = 0; c0 < hi - lo; c0 += nt * kTile) {
+        if (!lay_out()) continue;
+        chunk(!begun);
+        begun = true;
+      }
+      // each row's sum: its four lanes, then the two entry halves
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        l_own[b] = l_own[b] + __shfl_xor(l_own[b], 16, 64);
+        l_own[b] = l_own[b] + __shfl_xor(l_own[b], 32, 64);
+        if (g == 0) lsum[eh * 64 + 32 * hh + 16 * b + e16] = l_own[b];
+      }
+      lds_barrier();  // redo and high are zero
+      if (!given) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float top = m_seen[b] * p.scale_log2, rise = top - m_own[b];
+          if (rise > kWideRoomNear) *high = 1;
+          if (rise > kWideRoomAbove || (rise < kWideRoomBelow && m_own[b] == 0.0f && m_seen[b] > 0.5f * kHidden)) *redo = 1;
+        }
+      }
+      lds_barrier();
+#pragma unroll
+      for (int hg = 0; hg < 4; ++hg) l4[hg] = lsum[16 * hg + e16] + lsum[64 + 16 * hg + e16];
+      const bool several = !strict && tok1 - tok0 > 1;
+      if (__builtin_expect((!given && *high != 0) || several, 0)) {  // uniform
+        // O^T through the tiles' place, half of it at a time, each lane its own: a few stores and a
+        // short loop
+        float any_bad = 0.0f;  // NaN if an accumulator is not finite
+        v4f* const slot = reinterpret_cast<v4f*>(smem) + tid;
+        static_assert(2 * NI * NT * 16 <= M::PB, "half of O^T in the tiles' place");
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int k = 0; k < 2 * NI; ++k) slot[k * NT] = acc[k >> 1][2 * half + (k & 1)];
+#pragma unroll 1
+          for (int k = 0; k < 2 * NI; ++k) {
+            const v4f x = slot[k * NT];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) any_bad = __builtin_fmaf(x[r], 0.0f, any_bad);
+          }
+        }
+        if (any_bad != 0.0f) {
+          if (!given) *redo = 1;
+          *odd = 1;
+        }
+        lds_barrier();
+      }
+      if (given || *redo == 0) break;  // uniform: set before the barrier above
+      lds_barrier();
+    }
+    if (!strict && tok1 - tok0 > 1 && *odd != 0) {  // uniform
+      strict = true;
+      sub0 = tok0;
+      sub1 = tok0 + 1;
+      lds_barrier();
+      continue;
+    }
+    // (m, l) with l in [1, 2): the reference is not the maximum, so l may be far from 1
+#pragma unroll
+    for (int hg = 0; hg < 4; ++hg) {
+      e4[hg] = l4[hg] > 0.0f && l4[hg] < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(l4[hg]) - 1 : 0;
+      l4[hg] = __builtin_amdgcn_ldexpf(l4[hg], -e4[hg]);
+      m4[hg] = l4[hg] == 0.0f ? -__builtin_huge_valf() : m4[hg] + static_cast<float>(e4[hg]);
+    }
+    // ---- the result: acc[i][hg][r] is row 16 hg + e16, channel 16 (wave + 4 i) + 4 g + r ------------
+    const int keep0 = static_cast<int>((sub0 * p.HG > u.r0 ? sub0 * p.HG : u.r0) - u.r0);
+    const int keep1 = static_cast<int>((sub1 * p.HG < u.r1 ? sub1 * p.HG : u.r1) - u.r0);
+    if (u.shares > 1) {
+#pragma unroll
+      for (int hg = 0; hg < 4; ++hg) {
+        const int r = 16 * hg + e16;
+        if (r >= keep0 && r < keep1) {
+          const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? __builtin_amdgcn_ldexpf(1.0f / l4[hg], -e4[hg]) : 0.0f;
+          float* const o = p.part_o + (static_cast<int64_t>(u.slot) * 64 + r) * D + 16 * wave + 4 * g;
+#pragma unroll
+          for (int i = 0; i < NI; ++i) *reinterpret_cast<v4f*>(o + 64 * i) = acc[i][hg] * inv;
+          if (wave == hg && g == 0)
+            *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + r)) = float2{m4[hg], l4[hg]};
+        }
+      }
+    } else {
+      // through LDS, so that the rows leave in whole lines
+      constexpr int OPITCH = 2 * D + 16;
+#pragma unroll
+      for (int hg = 0; hg < 4; ++hg) {
+        const int r = 16 * hg + e16;
+        if (r >= keep0 && r < keep1) {
+          const int64_t at = row_at(p, u, u.r0 + r);
+          float lse;
+          const float scale = __builtin_amdgcn_ldexpf(finish_row(p, static_cast<int>(at % p.H), m4[hg], l4[hg], lse), -e4[hg]);
+          uint8_t* const orow = smem + r * OPITCH + 32 * wave + 8 * g;
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            *reinterpret_cast<uint2*>(orow + 128 * i) = uint2{pack_bf16x2(acc[i][hg][0] * scale, acc[i][hg][1] * scale),
+                                                              pack_bf16x2(acc[i][hg][2] * scale, acc[i][hg][3] * scale)};
+          if (wave == hg && g == 0) p.lse[at] = lse;
+        }
+      }
+      lds_barrier();
+      for (int at = tid; at < 64 * QROW; at += NT) {
+        const int r = at / QROW;
+        if (r >= keep0 && r < keep1)
+          *reinterpret_cast<u32x4*>(p.out + row_at(p, u, u.r0 + r) * D + 8 * (at - r * QROW)) =
+              *reinterpret_cast<const u32x4*>(smem + r * OPITCH + 16 * (at - r * QROW));
+      }
+    }
+    if (!strict || sub1 >= tok1) break;
+    ++sub0;
+    ++sub1;
+    lds_barrier();
+  }
+}
