@@ -166,7 +166,12 @@ def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int |
     itself, or the last ``window`` tokens of that.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D],
     lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a given ``out``
     and ``lse``."""
-    _lib.require_gpu(q, kv, cu, sinks, out, lse)
+    _lib.require_gpu(q)
+    dev = q.device
+    for x in (kv, cu, sinks, out, lse):
+        if x is not None and x.device != dev:
+            _lib.require_gpu(x)
+            raise ValueError(f"packed: tensors on {dev} and {x.device}")
     if q.dim() != 3 or kv.dim() != 3 or q.dtype != torch.bfloat16 or kv.dtype != torch.bfloat16:
         raise ValueError(f"packed: q [T, H, D] and kv [T, G, D] in bf16 expected, got {q.dtype} {list(q.shape)} and "
                          f"{kv.dtype} {list(kv.shape)}")
@@ -174,30 +179,32 @@ def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int |
     g = kv.shape[1]
     if kv.shape[0] != t or kv.shape[2] != d or g < 1 or h < 1 or h % g:
         raise ValueError(f"packed: kv must be [{t}, G, {d}] with G dividing {h} heads, got {list(kv.shape)}")
-    if cu.dtype != torch.int64 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+    if cu.dtype != torch.int64 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
         raise ValueError(f"packed: cu must be contiguous int64 [B + 1], got {cu.dtype} {list(cu.shape)}")
     if window is not None and (not isinstance(window, int) or window < 1):
         raise ValueError(f"packed: window must be a positive int or None, got {window!r}")
-    if (out is None) != (lse is None):
+    given = out is not None
+    if given != (lse is not None):
         raise ValueError("packed: out and lse go together")
     for name, x, dt, shape in (("sinks", sinks, torch.float32, (h,)), ("out", out, torch.bfloat16, (t, h, d)),
                                ("lse", lse, torch.float32, (t, h))):
-        if x is not None and (x.dtype != dt or not x.is_contiguous() or tuple(x.shape) != shape):
+        if x is not None and (x.dtype != dt or x.shape != shape or not x.is_contiguous()):
             raise ValueError(f"packed: {name} must be a contiguous {dt} tensor of shape {list(shape)}")
-    for x in (kv, cu, sinks, out, lse):
-        if x is not None and x.device != q.device:
-            raise ValueError(f"packed: tensors on {q.device} and {x.device}")
     q = q.contiguous()
-    if kv.stride(2) != 1 or (g > 1 and kv.stride(1) != d) or kv.stride(0) % 8 or kv.stride(0) < g * d or kv.data_ptr() % 16:
+    row, latent, unit = kv.stride()
+    if unit != 1 or (g > 1 and latent != d) or (t > 1 and (row % 8 or row < g * d)) or kv.data_ptr() % 16:
         kv = kv.contiguous()
-    given = out is not None
+        row = g * d
     if not given:
         out = torch.empty_like(q)
-        lse = torch.empty(t, h, dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("mzk_packed_mqa", q.data_ptr(), t, h, d, cu.data_ptr(), cu.numel() - 1, kv.data_ptr(),
-                  kv.stride(0) if t > 1 else g * d, g, window or 0, _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(),
-                  int(not given), _lib.stream_of(q))
+        lse = torch.empty((t, h), dtype=torch.float32, device=dev)
+    args = (q.data_ptr(), t, h, d, cu.data_ptr(), cu.shape[0] - 1, kv.data_ptr(), row if t > 1 else g * d, g, window or 0,
+            _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(), 0 if given else 1, _lib.stream_of(q))
+    if torch.cuda.current_device() == dev.index:
+        _lib.call("mzk_packed_mqa", *args)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call("mzk_packed_mqa", *args)
     return out, lse
 
 

@@ -50,11 +50,25 @@ __device__ __forceinline__ int64_t sequence_of(const int64_t* cu, int64_t B, int
 typedef uint32_t u32x2a4 __attribute__((ext_vector_type(2), aligned(4)));  // entries of 128 + 32 channels are 196 bytes
 
 // One wave per token.  fp8: a lane quantizes 8 neighbouring channels, 16 lanes share a block of 128.
+// The row of x is requested before the chain boundaries -> length -> page that ends in its entry's
+// address (12 prompts of 12.8 K tokens: see the launch).
 template <int DT>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p, bool vec) {
   const int lane = threadIdx.x & 63;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (t >= p.T) return;
+  const int64_t x0 = t * p.x_stride;
+  float v[8];
+  auto load = [&](int c) {
+    float h[4];
+    load4_as_f32<DT>(p.x, x0 + c, vec, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = h[i];
+    load4_as_f32<DT>(p.x, x0 + c + 4, vec, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 + i] = h[i];
+  };
+  if (8 * lane < p.D) load(8 * lane);
   int64_t b = t, pos;
   if (p.cu) {
     b = sequence_of(p.cu, p.B, t, lane);
@@ -68,18 +82,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p, bool 
   if (pid < 0 || pid >= p.P) return;
   const int eb = p.nope ? p.nope + p.nope / 32 + 2 * (p.D - p.nope) : 2 * p.D;
   uint8_t* const e = p.pool + (pid * p.page + pos % p.page) * eb;
-  const int64_t x0 = t * p.x_stride;
   for (int c = 8 * lane; c < p.D; c += 512) {
-    float v[8];
-    {
-      float h[4];
-      load4_as_f32<DT>(p.x, x0 + c, vec, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = h[i];
-      load4_as_f32<DT>(p.x, x0 + c + 4, vec, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 + i] = h[i];
-    }
+    if (c >= 512) load(c);
     if (c < p.nope) {  // nope is a multiple of 128: 16 lanes are in or out together
       const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
       const float s = fp8_scale_from_amax(group_max(nn_max(abs_max4(lo), abs_max4(hi)), 16));
@@ -133,16 +137,50 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_
   return total;
 }
 
-// This thread's 16 pages of a chunk: bit i of the result is set where page first + i is free (used).
-__device__ __forceinline__ uint32_t page_bits(const int32_t* refs, int64_t P, int64_t first, bool used) {
+// This thread's 16 pages of a chunk: their counts (-1 past the last page: neither free nor used).
+__device__ __forceinline__ void load_refs(const int32_t* refs, int64_t P, int64_t first, int32_t (&r)[16]) {
+  if (first + 16 <= P && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int4 v = reinterpret_cast<const int4*>(refs + first)[i];
+      r[4 * i] = v.x; r[4 * i + 1] = v.y; r[4 * i + 2] = v.z; r[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = first + i < P ? refs[first + i] : -1;
+  }
+}
+
+__device__ __forceinline__ void store_refs(int32_t* refs, int64_t P, int64_t first, const int32_t (&r)[16]) {
+  if (first + 16 <= P && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(refs + first)[i] = int4{r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (first + i < P) refs[first + i] = r[i];
+  }
+}
+
+// Bit i is set where page i of these is free (used).
+__device__ __forceinline__ uint32_t page_bits(const int32_t (&r)[16], bool used) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const bool in = first + i < P;
-    const int32_t r = refs[in ? first + i : 0];
-    m |= static_cast<uint32_t>(in && (used ? r > 0 : r == 0)) << i;
-  }
+  for (int i = 0; i < 16; ++i) m |= static_cast<uint32_t>(used ? r[i] > 0 : r[i] == 0) << i;
   return m;
+}
+
+// The sum of v[0 .. n - 1] by a workgroup, and of its first m.
+template <typename T>
+__device__ __forceinline__ int64_t sum_of(const T* v, int64_t step, int64_t n, int64_t m, int64_t& head, int64_t* lds, int tid) {
+  int64_t all = 0, first = 0, unused;
+  for (int64_t i = tid; i < n; i += 256) {
+    const int64_t x = v[i * step];
+    all += x;
+    first += i < m ? x : 0;
+  }
+  head = block_scan(first, unused, lds, tid);
+  return block_scan(all, unused, lds, tid);
 }
 
 // ---- grow ---------------------------------------------------------------------------------
@@ -165,12 +203,12 @@ struct GrowParams {
   int page;
   int64_t* missing;
   // workspace
-  int64_t* begin;   // [B] rank of the row's first fresh page
-  int64_t* old_len; // [B]
   GrowRow* rows;    // [B]
+  int64_t* old_len; // [B]
   int64_t* over;    // [B] pages past the table's width
-  int64_t* base;    // [chunks] free pages of the chunk, then of those before it
-  int64_t* ok;      // [1]
+  int64_t* free_in; // [chunks] free pages of the chunk
+  int64_t* want;    // [1] the pages handed out, -1: none, some lack
+  int32_t* list;    // [P] the page of each rank
   int64_t chunks;
 };
 
@@ -183,9 +221,10 @@ __global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
   const int64_t blk = blockIdx.x;
   if (blk < p.chunks) {
     int64_t before;
-    const int n = __builtin_popcount(page_bits(p.refs, p.P, blk * kChunk + 16 * tid, false));
-    const int64_t total = block_scan(n, before, lds, tid);
-    if (tid == 0) p.base[blk] = total;
+    int32_t r[16];
+    load_refs(p.refs, p.P, blk * kChunk + 16 * tid, r);
+    const int64_t total = block_scan(__builtin_popcount(page_bits(r, false)), before, lds, tid);
+    if (tid == 0) p.free_in[blk] = total;
     return;
   }
   const int64_t b = (blk - p.chunks) * 256 + tid;
@@ -212,70 +251,35 @@ __global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
   p.old_len[b] = len;
 }
 
-__global__ void __launch_bounds__(256) grow_plan_kernel(const GrowParams p) {
-  __shared__ int64_t lds[4];
-  const int tid = threadIdx.x;
-  int64_t free_pages = 0, want = 0, over = 0;
-  for (int64_t i = 0; i < p.chunks; i += 256) {
-    const int64_t v = i + tid < p.chunks ? p.base[i + tid] : 0;
-    int64_t before;
-    const int64_t total = block_scan(v, before, lds, tid);
-    if (i + tid < p.chunks) p.base[i + tid] = free_pages + before;
-    free_pages += total;
-  }
-  for (int64_t i = 0; i < p.B; i += 256) {
-    const int64_t v = i + tid < p.B ? p.rows[i + tid].want : 0;
-    int64_t before, unused;
-    const int64_t total = block_scan(v, before, lds, tid);
-    if (i + tid < p.B) p.begin[i + tid] = want + before;
-    want += total;
-    over += block_scan(i + tid < p.B ? p.over[i + tid] : 0, unused, lds, tid);
-  }
-  if (tid == 0) {
-    const int64_t lack = over + (want > free_pages ? want - free_pages : 0);
-    *p.missing = lack;
-    *p.ok = lack == 0 ? want : -1;
-  }
-}
-
+// A chunk's free pages by rank, and its counts.  Every workgroup adds up the chunks' and the rows' numbers itself.
 __global__ void __launch_bounds__(256) grow_assign_kernel(const GrowParams p) {
   __shared__ int64_t lds[4];
   const int tid = threadIdx.x;
   const int64_t blk = blockIdx.x;
-  const int64_t want = *p.ok;  // -1: nobody gets any
-  if (blk < p.chunks) {
-    const int64_t first = blk * kChunk + 16 * tid;
-    const uint32_t free_bits = page_bits(p.refs, p.P, first, false);
-    int64_t before;
-    block_scan(__builtin_popcount(free_bits), before, lds, tid);
-    int64_t rank = p.base[blk] + before;
-    for (int i = 0; i < 16; ++i) {
-      if (first + i >= p.P) break;
-      int32_t r = p.refs[first + i];
-      if ((free_bits >> i) & 1u) {
-        if (rank < want) {
-          int64_t lo = 0, hi = p.B - 1;  // the last row whose pages begin at or before this rank
-          while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) >> 1;
-            if (p.begin[mid] <= rank) lo = mid; else hi = mid - 1;
-          }
-          p.tables_out[lo * p.stride_out + p.rows[lo].first + (rank - p.begin[lo])] = static_cast<int32_t>(first + i);
-          r = 1;
-        }
-        ++rank;
-      }
-      p.refs_out[first + i] = r;
+  const int64_t first = blk * kChunk + 16 * tid;
+  int32_t r[16];
+  load_refs(p.refs, p.P, first, r);
+  int64_t rank, unused, before;
+  const int64_t free_pages = sum_of(p.free_in, 1, p.chunks, blk, rank, lds, tid);
+  int64_t want = sum_of(&p.rows[0].want, sizeof(GrowRow) / 4, p.B, 0, unused, lds, tid);
+  const int64_t over = sum_of(p.over, 1, p.B, 0, unused, lds, tid);
+  const int64_t lack = over + (want > free_pages ? want - free_pages : 0);
+  if (lack) want = -1;
+  const uint32_t free_bits = page_bits(r, false);
+  block_scan(__builtin_popcount(free_bits), before, lds, tid);
+  rank += before;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (((free_bits >> i) & 1u) && rank < want) {
+      p.list[rank] = static_cast<int32_t>(first + i);
+      r[i] = 1;
     }
-    return;
+    rank += (free_bits >> i) & 1u;
   }
-  const int64_t b = blk - p.chunks;
-  const GrowRow r = p.rows[b];
-  for (int64_t j = tid; j < p.max_pages; j += 256) {
-    const bool fresh = want >= 0 && j >= r.first && j < r.first + r.want;
-    if (!fresh) p.tables_out[b * p.stride_out + j] = p.tables[b * p.stride + j];
-  }
-  if (tid == 0) {
-    p.lens_out[b] = want >= 0 ? p.old_len[b] + row_count(p.tokens[b]) : p.lens[b];
+  store_refs(p.refs_out, p.P, first, r);
+  if (blk == 0 && tid == 0) {
+    *p.missing = lack;
+    *p.want = want;
   }
 }
 
@@ -298,18 +302,37 @@ __device__ __forceinline__ void copy_bytes(const uint8_t* a, uint8_t* b, int64_t
   }
 }
 
-// Row blockIdx.x's shared last page into its fresh one, a share of it per blockIdx.y; pool blockIdx.z.
-__global__ void __launch_bounds__(256) grow_copy_kernel(const GrowParams p, const PoolList pools, int npools, bool first) {
+// Row blockIdx.x: its table, length and count (the first workgroup), and its shared last page into its
+// fresh one, a share of it per blockIdx.y; pool blockIdx.z.
+__global__ void __launch_bounds__(256) grow_row_kernel(const GrowParams p, const PoolList pools, int npools, bool first) {
+  __shared__ int64_t lds[4];
+  const int tid = threadIdx.x;
   const int64_t b = blockIdx.x;
   const GrowRow r = p.rows[b];
-  if (r.src < 0 || *p.ok < 0) return;
-  if (first && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicSub(p.refs_out + r.src, 1);
-  if (npools == 0) return;
-  const int64_t dst = p.tables_out[b * p.stride_out + r.first];
+  const int64_t want = *p.want;
+  const bool lead = first && blockIdx.y == 0 && blockIdx.z == 0;
+  const bool copies = want >= 0 && r.src >= 0;
+  if (!lead && !copies) return;
+  int64_t begin;
+  sum_of(&p.rows[0].want, sizeof(GrowRow) / 4, b, b, begin, lds, tid);
+  if (lead) {
+    const int32_t* const from = p.tables + b * p.stride;
+    int32_t* const to = p.tables_out + b * p.stride_out;
+    for (int64_t j = tid; j < p.max_pages; j += 256) {
+      const bool fresh = want >= 0 && j >= r.first && j < r.first + r.want;
+      to[j] = fresh ? p.list[begin + j - r.first] : from[j];
+    }
+    if (tid == 0) {
+      p.lens_out[b] = want >= 0 ? p.old_len[b] + row_count(p.tokens[b]) : p.lens[b];
+      if (copies) atomicSub(p.refs_out + r.src, 1);
+    }
+  }
+  if (!copies || npools == 0) return;
+  const int64_t dst = p.list[begin];
   const int64_t eb = pools.entry[blockIdx.z];
   uint8_t* const base = pools.base[blockIdx.z];
   copy_bytes(base + r.src * (p.page * eb), base + dst * (p.page * eb), r.fill * eb,
-             static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x, static_cast<int64_t>(gridDim.y) * 256);
+             static_cast<int64_t>(blockIdx.y) * 256 + tid, static_cast<int64_t>(gridDim.y) * 256);
 }
 
 // ---- fork ---------------------------------------------------------------------------------
@@ -377,7 +400,7 @@ struct CompactParams {
   int64_t P;
   int page;
   // workspace
-  int64_t* base;     // [chunks] used pages before the chunk
+  int64_t* used_in;  // [chunks] used pages of the chunk
   int64_t* used;     // [2] U, and the moves M
   int32_t* from;     // [P] page of the k-th move
   int32_t* to;       // [P]
@@ -390,66 +413,47 @@ __global__ void __launch_bounds__(256) compact_count_kernel(const CompactParams 
   __shared__ int64_t lds[4];
   const int tid = threadIdx.x;
   int64_t before;
-  const int n = __builtin_popcount(page_bits(p.refs, p.P, blockIdx.x * static_cast<int64_t>(kChunk) + 16 * tid, true));
-  const int64_t total = block_scan(n, before, lds, tid);
-  if (tid == 0) p.base[blockIdx.x] = total;
+  int32_t r[16];
+  load_refs(p.refs, p.P, blockIdx.x * static_cast<int64_t>(kChunk) + 16 * tid, r);
+  const int64_t total = block_scan(__builtin_popcount(page_bits(r, true)), before, lds, tid);
+  if (tid == 0) p.used_in[blockIdx.x] = total;
 }
 
-__global__ void __launch_bounds__(256) compact_plan_kernel(const CompactParams p) {
-  __shared__ int64_t lds[4];
-  const int tid = threadIdx.x;
-  int64_t used = 0;
-  for (int64_t i = 0; i < p.chunks; i += 256) {
-    const int64_t v = i + tid < p.chunks ? p.base[i + tid] : 0;
-    int64_t before;
-    const int64_t total = block_scan(v, before, lds, tid);
-    if (i + tid < p.chunks) p.base[i + tid] = used + before;
-    used += total;
-  }
-  __syncthreads();
-  // used pages before page U: those of earlier chunks and a part of U's own
-  const int64_t c = used / kChunk;
-  int64_t n = 0;
-  if (c < p.chunks) {
-    const uint32_t m = page_bits(p.refs, p.P, c * kChunk + 16 * tid, true);
-    const int64_t left = used - (c * kChunk + 16 * tid);
-    n = __builtin_popcount(left >= 16 ? m : left <= 0 ? 0u : m & ((1u << left) - 1u));
-  }
-  int64_t unused;
-  const int64_t in_chunk = block_scan(n, unused, lds, tid);
-  if (tid == 0) {
-    p.used[0] = used;
-    p.used[1] = used - (c < p.chunks ? p.base[c] + in_chunk : used);
-  }
-}
-
+// The moves by rank, and the counts without what moves.  The outputs may be the inputs, so a workgroup
+// reads no counts but its own: refs before page U come from the chunks' numbers and its own chunk.
 __global__ void __launch_bounds__(256) compact_list_kernel(const CompactParams p) {
   __shared__ int64_t lds[4];
   const int tid = threadIdx.x;
-  const int64_t U = p.used[0], M = p.used[1];
-  const int64_t first = blockIdx.x * static_cast<int64_t>(kChunk) + 16 * tid;
-  const uint32_t used_bits = page_bits(p.refs, p.P, first, true);
-  int64_t before;
+  const int64_t blk = blockIdx.x;
+  const int64_t first = blk * kChunk + 16 * tid;
+  int32_t r[16];
+  load_refs(p.refs, p.P, first, r);
+  int64_t n, before;
+  const int64_t U = sum_of(p.used_in, 1, p.chunks, blk, n, lds, tid);
+  const uint32_t used_bits = page_bits(r, true);
   block_scan(__builtin_popcount(used_bits), before, lds, tid);
-  int64_t n = p.base[blockIdx.x] + before;  // used pages before this one
+  n += before;  // used pages before this thread's
+  // holes are ranked from the first page, moves from the last: the k-th move is the (M - 1 - k)-th from there
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t page = first + i;
-    if (page >= p.P) break;
     const bool used = (used_bits >> i) & 1u;
-    const int32_t r = p.refs[page];
+    if (page == U) p.used[1] = U - n;
     if (page < U) {
       if (!used) p.to[page - n] = static_cast<int32_t>(page);
-      p.refs_out[page] = r;
-    } else {
-      if (used) {
-        const int64_t k = n - (U - M);
-        p.from[k] = static_cast<int32_t>(page);
-        p.from_refs[k] = r;
-        p.rank[page] = static_cast<int32_t>(k);
-      }
-      p.refs_out[page] = used ? 0 : r;
+    } else if (used) {
+      const int64_t k = U - 1 - n;  // so many used pages come behind it
+      p.from[k] = static_cast<int32_t>(page);
+      p.from_refs[k] = r[i];
+      p.rank[page] = static_cast<int32_t>(k);
+      r[i] = 0;
     }
     n += used;
+  }
+  store_refs(p.refs_out, p.P, first, r);
+  if (tid == 0 && blk == 0) {
+    p.used[0] = U;
+    if (U == p.chunks * kChunk) p.used[1] = 0;  // no page U in any chunk
   }
 }
 
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
   if (blockIdx.y == 0) {
     if (!first) return;
-    for (int64_t i = at; i < M; i += step) p.refs_out[p.to[i]] = p.from_refs[i];
+    for (int64_t i = at; i < M; i += step) p.refs_out[p.to[i]] = p.from_refs[M - 1 - i];
     for (int64_t i = at; i < p.B * p.max_pages; i += step) {
       const int64_t b = i / p.max_pages, j = i - b * p.max_pages;
       int32_t v = p.tables[b * p.stride + j];
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p
         // rank[] is written for moved pages only: a page without references, whose word is
         // whatever was there, is no move's `from`, and a table that names it keeps it
         const int32_t k = p.rank[v];
-        if (k >= 0 && k < M && p.from[k] == v) v = p.to[k];
+        if (k >= 0 && k < M && p.from[k] == v) v = p.to[M - 1 - k];
       }
       p.tables_out[b * p.stride_out + j] = v;
     }
@@ -476,14 +480,14 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p
   const int64_t eb = pools.entry[blockIdx.y - 1] * p.page;
   uint8_t* const base = pools.base[blockIdx.y - 1];
   for (int64_t m = blockIdx.x; m < M; m += gridDim.x)
-    copy_bytes(base + p.from[m] * eb, base + p.to[m] * eb, eb, threadIdx.x, 256);
+    copy_bytes(base + p.from[M - 1 - m] * eb, base + p.to[m] * eb, eb, threadIdx.x, 256);
 }
 
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 int64_t grow_bytes(int64_t B, int64_t P) {
   const int64_t chunks = (P + kChunk - 1) / kChunk;
-  return 8 * (3 * B + chunks + 1) + align16_up(sizeof(GrowRow) * B) + 32;
+  return align16_up(sizeof(GrowRow) * B) + 8 * (2 * B + chunks + 1) + 4 * P + 16;
 }
 int64_t fork_bytes(int64_t B, int64_t max_pages) { return align16_up(4 * B * max_pages) + 8 * B; }
 int64_t compact_bytes(int64_t P) { return 8 * ((P + kChunk - 1) / kChunk + 2) + 16 * P + 32; }
@@ -560,29 +564,26 @@ extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.rows = reinterpret_cast<GrowRow*>(w);
   w += align16_up(sizeof(GrowRow) * B);
-  p.begin = reinterpret_cast<int64_t*>(w);
-  p.old_len = p.begin + B;
+  p.old_len = reinterpret_cast<int64_t*>(w);
   p.over = p.old_len + B;
-  p.base = p.over + B;
-  p.ok = p.base + p.chunks;
+  p.free_in = p.over + B;
+  p.want = p.free_in + p.chunks;
+  p.list = reinterpret_cast<int32_t*>(p.want + 1);
+  if (B == 0 || pages == 0) return MZK_OK;
   hipStream_t s = as_stream(stream);
-  if (p.chunks + B > 0)
-    grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 255) / 256), 256, 0, s>>>(p);
-  grow_plan_kernel<<<1, 256, 0, s>>>(p);
-  if (p.chunks + B > 0) grow_assign_kernel<<<static_cast<unsigned>(p.chunks + B), 256, 0, s>>>(p);
-  if (B > 0) {
-    int done = 0;
-    do {
-      PoolList l{};
-      const int n = npools - done < kPoolsPerLaunch ? npools - done : kPoolsPerLaunch;
-      for (int i = 0; i < n; ++i) {
-        l.base[i] = static_cast<uint8_t*>(pools[done + i]);
-        l.entry[i] = entry_bytes[done + i];
-      }
-      grow_copy_kernel<<<dim3(static_cast<unsigned>(B), n ? 4 : 1, n ? n : 1), 256, 0, s>>>(p, l, n, done == 0);
-      done += n;
-    } while (done < npools);
-  }
+  grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 255) / 256), 256, 0, s>>>(p);
+  grow_assign_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
+  int done = 0;
+  do {
+    PoolList l{};
+    const int n = npools - done < kPoolsPerLaunch ? npools - done : kPoolsPerLaunch;
+    for (int i = 0; i < n; ++i) {
+      l.base[i] = static_cast<uint8_t*>(pools[done + i]);
+      l.entry[i] = entry_bytes[done + i];
+    }
+    grow_row_kernel<<<dim3(static_cast<unsigned>(B), n ? 4 : 1, n ? n : 1), 256, 0, s>>>(p, l, n, done == 0);
+    done += n;
+  } while (done < npools);
   MZK_LAUNCH_CHECK("paged_grow");
   return MZK_OK;
 }
@@ -632,16 +633,16 @@ extern "C" int mzk_paged_compact(const int32_t* tables, int64_t table_stride, in
   CompactParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, refs, refs_out, pages, page};
   p.chunks = (pages + kChunk - 1) / kChunk;
   uint8_t* w = static_cast<uint8_t*>(workspace);
-  p.base = reinterpret_cast<int64_t*>(w);
-  p.used = p.base + p.chunks;
+  p.used_in = reinterpret_cast<int64_t*>(w);
+  p.used = p.used_in + p.chunks;
   p.from = reinterpret_cast<int32_t*>(p.used + 2);
   p.to = p.from + pages;
   p.from_refs = p.to + pages;
   p.rank = p.from_refs + pages;
   hipStream_t s = as_stream(stream);
-  if (p.chunks > 0) compact_count_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
-  compact_plan_kernel<<<1, 256, 0, s>>>(p);
-  if (p.chunks > 0) compact_list_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
+  if (pages == 0) return MZK_OK;
+  compact_count_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
+  compact_list_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
   int done = 0;
   do {
     PoolList l{};

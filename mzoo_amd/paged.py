@@ -27,6 +27,7 @@ layer's.  Packed sequences (``cu``, int64 [B + 1]): rows ``cu[b] .. cu[b + 1] - 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -47,44 +48,59 @@ def new_pool(pages: int, page: int, dim: int, fmt: str = "fp8", *, rope: int = q
     return torch.zeros(pages, page, quant.entry_bytes(dim - rope, rope), dtype=torch.uint8, device=device)
 
 
-def _check(what: str, *tensors) -> None:
-    """(name, tensor, dtype, shape) of contiguous tensors: read through raw pointers, so a wrong dtype or
-    a strided view is rejected, not converted."""
-    for name, t, dt, shape in tensors:
-        if t is None:
-            continue
-        if t.dtype != dt or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
-            raise ValueError(f"{what}: {name} must be a contiguous {dt} tensor"
-                             + (f" of shape {list(shape)}" if shape is not None else "")
-                             + f", got {t.dtype} {list(t.shape)}{'' if t.is_contiguous() else ' (strided)'}")
+def _refuse(what: str, name: str, t: torch.Tensor, dt: torch.dtype, shape=None):
+    """A tensor is read through a raw pointer, so a wrong dtype or a strided view is rejected, not converted."""
+    raise ValueError(f"{what}: {name} must be a contiguous {dt} tensor" + (f" of shape {list(shape)}" if shape is not None else "")
+                     + f", got {t.dtype} {list(t.shape)}{'' if t.is_contiguous() else ' (strided)'}")
 
 
-def _tables(what: str, tables: torch.Tensor, name: str = "tables") -> tuple[int, int, int]:
+def _is(t: torch.Tensor, dt: torch.dtype, shape) -> bool:
+    return t.dtype == dt and t.shape == shape and t.is_contiguous()
+
+
+def _table(what: str, tables: torch.Tensor, name: str = "tables") -> tuple[int, int, int]:
     """(rows, pages per row, row stride) of a table, whose rows may be part of wider ones."""
-    if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1):
-        raise ValueError(f"{what}: {name} must be int32 [B, max_pages] with unit column stride, got {tables.dtype} "
-                         f"{list(tables.shape)}")
+    if tables.dtype != torch.int32 or tables.dim() != 2:
+        raise ValueError(f"{what}: {name} must be int32 [B, max_pages], got {tables.dtype} {list(tables.shape)}")
     b, n = tables.shape
-    return b, n, max(tables.stride(0), n) if b > 1 else n
+    stride, unit = tables.stride()
+    if n > 1 and unit != 1 or b > 1 and stride < n:
+        raise ValueError(f"{what}: {name} must have unit column stride and rows that do not overlap, got strides {(stride, unit)}")
+    return b, n, stride if b > 1 else n
 
 
-def _same_device(what: str, first: torch.Tensor, *rest) -> None:
+def _one_device(what: str, first: torch.Tensor, *rest) -> None:
+    """All tensors on the GPU that holds the first."""
+    _lib.require_gpu(first)
+    dev = first.device
     for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            _lib.require_gpu(t)
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
 
 
 def _pool(what: str, pool: torch.Tensor, dim: int, rope: int) -> tuple[int, int, int, int]:
     """(format, nope, pages, entries per page)."""
-    if pool.dim() != 3 or not pool.is_contiguous() or pool.shape[1] < 1:
-        raise ValueError(f"{what}: the pool must be a contiguous [pages, page, entry] tensor, got {list(pool.shape)}")
-    if pool.dtype == torch.bfloat16 and pool.shape[2] == dim:
-        return FMT_BF16, dim, pool.shape[0], pool.shape[1]
-    nope = dim - rope
-    if pool.dtype == torch.uint8 and nope >= 128 and nope % 128 == 0 and pool.shape[2] == quant.entry_bytes(nope, rope):
-        return FMT_FP8, nope, pool.shape[0], pool.shape[1]
-    raise ValueError(f"{what}: for {dim} channels ({rope} of them rope) the pool must be bf16 [P, page, {dim}] or uint8 "
-                     f"FP8-b128 entries, got {pool.dtype} {list(pool.shape)}")
+    if pool.dim() == 3 and pool.is_contiguous():
+        pages, page, size = pool.shape
+        if page >= 1:
+            if pool.dtype == torch.bfloat16 and size == dim:
+                return FMT_BF16, dim, pages, page
+            nope = dim - rope
+            if pool.dtype == torch.uint8 and nope >= 128 and nope % 128 == 0 and rope >= 0 and size == quant.entry_bytes(nope, rope):
+                return FMT_FP8, nope, pages, page
+    raise ValueError(f"{what}: for {dim} channels ({rope} of them rope) the pool must be contiguous, bf16 [P, page, {dim}] or "
+                     f"uint8 FP8-b128 entries, got {pool.dtype} {list(pool.shape)}")
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """A call on the device of its tensors and its current stream (the last argument of every entry)."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
 
 
 def append(pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, x: torch.Tensor, *,
@@ -93,25 +109,29 @@ def append(pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, x: torc
     token per sequence (T == B), or with ``cu`` packed ones; sequence b's n rows become its last n
     entries, positions ``lens[b] - n .. lens[b] - 1`` (``lens`` counts them already).  Positions
     without a page are skipped.  Returns the pool."""
-    _lib.require_gpu(pool, tables, lens, x, cu)
-    _same_device("append", pool, tables, lens, x, cu)
-    b, width, stride = _tables("append", tables)
+    _one_device("append", pool, tables, lens, x, cu)
+    b, width, stride = _table("append", tables)
     if x.dim() != 2:
         raise ValueError(f"append: x must be [T, D], got {list(x.shape)}")
     t, d = x.shape
     fmt, nope, pages, page = _pool("append", pool, d, rope)
-    _check("append", ("lens", lens, torch.int64, (b,)), ("cu", cu, torch.int64, (b + 1,)))
-    if cu is None and t != b:
-        raise ValueError(f"append: {t} tokens for {b} sequences; packed tokens need cu")
-    if x.stride(1) != 1 or x.stride(0) < d:
+    if not _is(lens, torch.int64, (b,)):
+        _refuse("append", "lens", lens, torch.int64, (b,))
+    if cu is None:
+        if t != b:
+            raise ValueError(f"append: {t} tokens for {b} sequences; packed tokens need cu")
+    elif not _is(cu, torch.int64, (b + 1,)):
+        _refuse("append", "cu", cu, torch.int64, (b + 1,))
+    row, unit = x.stride()
+    if unit != 1 or row < d:
         x = x.contiguous()
-    with torch.cuda.device(pool.device):
-        _lib.call("mzk_paged_append", x.data_ptr(), _lib.dtype_code(x.dtype), t, x.stride(0) if t > 1 else d,
-                  _lib.ptr(cu), b, tables.data_ptr(), stride, width, lens.data_ptr(), fmt, d, nope, pool.data_ptr(),
-                  pages, page, _lib.stream_of(pool))
+        row = d
+    _call(pool.device, "mzk_paged_append", x.data_ptr(), _lib.dtype_code(x.dtype), t, row if t > 1 else d, _lib.ptr(cu), b,
+          tables.data_ptr(), stride, width, lens.data_ptr(), fmt, d, nope, pool.data_ptr(), pages, page)
     return pool
 
 
+@functools.lru_cache(maxsize=1024)
 def attend_workspace_bytes(tokens: int, heads: int, dim: int, batch: int, packed: bool) -> int:
     """What ``attend`` splits long sequences into: the partial results (``mzk_paged_attend_workspace_bytes``)."""
     n = ctypes.c_int64(0)
@@ -132,50 +152,60 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
     [T, H, D], lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a
     given ``out`` and ``lse``.  A token that sees nothing gets 0.  ``workspace``: uint8, of
     ``attend_workspace_bytes``, allocated per call if omitted; calls that overlap need their own."""
-    _lib.require_gpu(q, pool, tables, lens, cu, indices, sinks, workspace, out, lse)
-    _same_device("attend", q, pool, tables, lens, cu, indices, sinks, workspace, out, lse)
+    _one_device("attend", q, pool, tables, lens, cu, indices, sinks, workspace, out, lse)
     if q.dim() != 3 or q.shape[1] < 1:
         raise ValueError(f"attend: q must be [T, H, D], got {list(q.shape)}")
     t, h, d = q.shape
-    b, width, stride = _tables("attend", tables)
+    b, width, stride = _table("attend", tables)
     fmt, nope, pages, page = _pool("attend", pool, d, rope)
-    _check("attend", ("q", q, torch.bfloat16, None), ("lens", lens, torch.int64, (b,)), ("cu", cu, torch.int64, (b + 1,)),
-           ("sinks", sinks, torch.float32, (h,)), ("out", out, torch.bfloat16, (t, h, d)),
-           ("lse", lse, torch.float32, (t, h)), ("workspace", workspace, torch.uint8, None))
-    if cu is None and t != b:
-        raise ValueError(f"attend: {t} tokens for {b} sequences; packed tokens need cu")
-    if (out is None) != (lse is None):
-        raise ValueError("attend: out and lse go together")
+    if q.dtype != torch.bfloat16 or not q.is_contiguous():
+        _refuse("attend", "q", q, torch.bfloat16)
+    if not _is(lens, torch.int64, (b,)):
+        _refuse("attend", "lens", lens, torch.int64, (b,))
+    if cu is None:
+        if t != b:
+            raise ValueError(f"attend: {t} tokens for {b} sequences; packed tokens need cu")
+    elif not _is(cu, torch.int64, (b + 1,)):
+        _refuse("attend", "cu", cu, torch.int64, (b + 1,))
+    if sinks is not None and not _is(sinks, torch.float32, (h,)):
+        _refuse("attend", "sinks", sinks, torch.float32, (h,))
     if window is not None and (not isinstance(window, int) or window < 1):
         raise ValueError(f"attend: window must be a positive int or None, got {window!r}")
     k = istride = 0
     if indices is not None:
         if cu is not None or window is not None:
             raise ValueError("attend: indices go with one token per sequence and no window")
-        rows, k, istride = _tables("attend", indices, "indices")
+        rows, k, istride = _table("attend", indices, "indices")
         if rows != b:
             raise ValueError(f"attend: indices must be [{b}, k], got {list(indices.shape)}")
     given = out is not None
-    if not given:
+    if given != (lse is not None):
+        raise ValueError("attend: out and lse go together")
+    if given:
+        if not _is(out, torch.bfloat16, (t, h, d)):
+            _refuse("attend", "out", out, torch.bfloat16, (t, h, d))
+        if not _is(lse, torch.float32, (t, h)):
+            _refuse("attend", "lse", lse, torch.float32, (t, h))
+    else:
         out = torch.empty_like(q)
-        lse = torch.empty(t, h, dtype=torch.float32, device=q.device)
+        lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
     need = attend_workspace_bytes(t, h, d, b, cu is not None)
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    if need and workspace.numel() < need:
-        raise ValueError(f"attend: the workspace needs {need} bytes, got {workspace.numel()}")
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+            raise ValueError(f"attend: the workspace must be contiguous uint8 of at least {need} bytes")
     if t and not b:  # rows of no sequence
         return (out, lse) if given else (out.zero_(), lse.fill_(float("-inf")))
-    with torch.cuda.device(q.device):
-        _lib.call("mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
-                  tables.data_ptr(), stride, width, lens.data_ptr(), _lib.ptr(indices), istride, k, window or 0,
-                  _lib.ptr(sinks), _lib.ptr(workspace), need, out.data_ptr(), lse.data_ptr(), int(not given),
-                  _lib.stream_of(q))
+    _call(q.device, "mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
+          tables.data_ptr(), stride, width, lens.data_ptr(), _lib.ptr(indices), istride, k, window or 0, _lib.ptr(sinks),
+          _lib.ptr(workspace) if need else None, need, out.data_ptr(), lse.data_ptr(), 0 if given else 1)
     return out, lse
 
 
 # ---- the pages ----------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=1024)
 def workspace_bytes(batch: int, max_pages: int, pages: int) -> int:
     """The workspace of ``grow``, ``fork`` and ``compact``."""
     n = ctypes.c_int64(0)
@@ -183,55 +213,60 @@ def workspace_bytes(batch: int, max_pages: int, pages: int) -> int:
     return n.value
 
 
-def _workspace(what: str, workspace, batch: int, max_pages: int, refs: torch.Tensor) -> tuple[torch.Tensor, int]:
-    need = workspace_bytes(batch, max_pages, refs.numel())
+def _workspace(what: str, workspace, need: int, device) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=refs.device), need
+        return torch.empty(need, dtype=torch.uint8, device=device)
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
         raise ValueError(f"{what}: the workspace must be contiguous uint8 of at least {need} bytes")
-    return workspace, need
+    return workspace
 
 
-def _pool_list(what: str, pools, refs: torch.Tensor, page: int):
-    """The pools as C arrays of base pointers and entry bytes."""
+def _pool_list(what: str, pools, pages: int, page: int):
+    """The pools as C arrays of base pointers and entry bytes, and their number."""
     n = len(pools)
-    base, size = (ctypes.c_void_p * max(n, 1))(), (ctypes.c_int64 * max(n, 1))()
+    if n == 0:
+        return None, None, 0
+    base, size = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
     for i, t in enumerate(pools):
-        if t.dim() < 2 or not t.is_contiguous() or tuple(t.shape[:2]) != (refs.numel(), page):
-            raise ValueError(f"{what}: pool {i} must be contiguous [{refs.numel()}, {page}, ...], got {list(t.shape)}")
-        size[i] = t[0, 0].numel() * t.element_size() if t.numel() else 4
+        if t.dim() < 2 or not t.is_contiguous() or t.shape[:2] != (pages, page) or t.numel() == 0:
+            raise ValueError(f"{what}: pool {i} must be contiguous [{pages}, {page}, ...], got {list(t.shape)}")
+        size[i] = t.stride(1) * t.element_size()
         if size[i] % 4:
             raise ValueError(f"{what}: pool {i} has entries of {size[i]} bytes, not a multiple of 4")
-        base[i] = t.data_ptr() if t.numel() else None
-    return base, size, n if refs.numel() else 0
+        base[i] = t.data_ptr()
+    return base, size, n
 
 
-def _state(what: str, tables, lens, refs, page: int, pools=()) -> tuple[int, int, int]:
-    _lib.require_gpu(tables, lens, refs, *pools)
-    _same_device(what, tables, lens, refs, *pools)
-    b, width, stride = _tables(what, tables)
-    _check(what, ("lens", lens, torch.int64, (b,)), ("refs", refs, torch.int32, None))
-    if refs.dim() != 1 or page < 1:
-        raise ValueError(f"{what}: refs must be [pages] and page at least 1")
-    return b, width, stride
+def _book(what: str, tables, lens, refs) -> tuple[int, int, int, int]:
+    """(sequences, pages per table row, row stride, pages) of a cache's tables, lengths and counts."""
+    b, width, stride = _table(what, tables)
+    if lens is not None and not _is(lens, torch.int64, (b,)):
+        _refuse(what, "lens", lens, torch.int64, (b,))
+    if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous():
+        _refuse(what, "refs", refs, torch.int32, ("pages",))
+    if b == 0 or width == 0 or refs.shape[0] == 0:
+        raise ValueError(f"{what}: a pool of no pages, or tables of no rows or width")
+    return b, width, stride, refs.shape[0]
 
 
 def _outs(what: str, out, rows: int, width: int, tables, refs, with_lens: bool):
-    """(tables, lens or None, refs) to write, new ones unless given."""
+    """(tables, lens or None, refs, table stride) to write, new ones unless given."""
     if out is None:
-        new = (torch.empty(rows, width, dtype=torch.int32, device=tables.device),
-               torch.empty(rows, dtype=torch.int64, device=tables.device) if with_lens else None, torch.empty_like(refs))
-        return (*new, width)
+        dev = tables.device
+        return (torch.empty((rows, width), dtype=torch.int32, device=dev),
+                torch.empty(rows, dtype=torch.int64, device=dev) if with_lens else None, torch.empty_like(refs), width)
     got = tuple(out)
     if len(got) != 2 + with_lens:
         raise ValueError(f"{what}: out must be ({'tables, lens, refs' if with_lens else 'tables, refs'})")
     ot, ol, orf = got if with_lens else (got[0], None, got[1])
-    _lib.require_gpu(*got)
-    _same_device(what, tables, *got)
-    r, w, stride = _tables(what, ot, "out tables")
+    _one_device(what, tables, *got)
+    r, w, stride = _table(what, ot, "out tables")
     if (r, w) != (rows, width):
         raise ValueError(f"{what}: out tables must be [{rows}, {width}], got {list(ot.shape)}")
-    _check(what, ("out lens", ol, torch.int64, (rows,)), ("out refs", orf, torch.int32, tuple(refs.shape)))
+    if with_lens and not _is(ol, torch.int64, (rows,)):
+        _refuse(what, "out lens", ol, torch.int64, (rows,))
+    if not _is(orf, torch.int32, refs.shape):
+        _refuse(what, "out refs", orf, torch.int32, refs.shape)
     return ot, ol, orf, stride
 
 
@@ -243,26 +278,23 @@ def grow(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, tokens: t
     refs, missing): ``missing`` int64 [1] is 0, or the pages that lack, and then the rest is
     unchanged.  ``out=(tables, lens, refs)``, which may be the inputs themselves, is written instead
     of new tensors."""
-    b, width, stride = _state("grow", tables, lens, refs, page, pools)
-    _lib.require_gpu(tokens, missing, workspace)
-    _same_device("grow", tables, tokens, missing, workspace)
-    _check("grow", ("tokens", tokens, torch.int64, (b,)), ("missing", missing, torch.int64, (1,)))
-    ot, ol, orf, ostride = _outs("grow", out, b, width, tables, refs, True)
-    base, size, n = _pool_list("grow", pools, refs, page)
-    ws, need = _workspace("grow", workspace, b, width, refs)
+    _one_device("grow", tables, lens, refs, tokens, missing, workspace, *pools)
+    b, width, stride, pages = _book("grow", tables, lens, refs)
+    if not _is(tokens, torch.int64, (b,)):
+        _refuse("grow", "tokens", tokens, torch.int64, (b,))
+    if page < 1:
+        raise ValueError(f"grow: page must be at least 1, got {page}")
     if missing is None:
         missing = torch.empty(1, dtype=torch.int64, device=refs.device)
-    if b == 0:
-        missing.zero_()
-        if orf is not refs:
-            orf.copy_(refs)
-        return ot, ol, orf, missing
-    if refs.numel() == 0 or width == 0:
-        raise ValueError("grow: a pool of no pages, or tables of no width")
-    with torch.cuda.device(refs.device):
-        _lib.call("mzk_paged_grow", tables.data_ptr(), stride, b, width, lens.data_ptr(), refs.data_ptr(), refs.numel(),
-                  tokens.data_ptr(), page, base, size, n, ot.data_ptr(), ostride, ol.data_ptr(), orf.data_ptr(),
-                  missing.data_ptr(), ws.data_ptr(), need, _lib.stream_of(refs))
+    elif not _is(missing, torch.int64, (1,)):
+        _refuse("grow", "missing", missing, torch.int64, (1,))
+    base, size, n = _pool_list("grow", pools, pages, page)
+    ot, ol, orf, ostride = _outs("grow", out, b, width, tables, refs, True)
+    need = workspace_bytes(b, width, pages)
+    ws = _workspace("grow", workspace, need, refs.device)
+    _call(refs.device, "mzk_paged_grow", tables.data_ptr(), stride, b, width, lens.data_ptr(), refs.data_ptr(), pages,
+          tokens.data_ptr(), page, base, size, n, ot.data_ptr(), ostride, ol.data_ptr(), orf.data_ptr(), missing.data_ptr(),
+          ws.data_ptr(), need)
     return ot, ol, orf, missing
 
 
@@ -272,25 +304,20 @@ def fork(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: 
     (int32 [R]; -1: it is empty), and the present ones hold theirs no longer.  Covers beams (any
     parent, any number of times), repeated prompts (R > B), sequences that end (-1).  Returns (tables
     [R, max_pages], lens [R], refs); ``out`` as in ``grow`` (the inputs themselves if R == B)."""
-    b, width, stride = _state("fork", tables, lens, refs, page)
-    _lib.require_gpu(parents, workspace)
-    _same_device("fork", tables, parents, workspace)
-    if parents.dim() != 1:
-        raise ValueError(f"fork: parents must be [R], got {list(parents.shape)}")
-    _check("fork", ("parents", parents, torch.int32, None))
-    r = parents.shape[0]
+    _one_device("fork", tables, lens, refs, parents, workspace)
+    b, width, stride, pages = _book("fork", tables, lens, refs)
+    r = parents.shape[0] if parents.dim() == 1 else 0
+    if r < 1 or parents.dtype != torch.int32 or not parents.is_contiguous():
+        _refuse("fork", "parents", parents, torch.int32, ("R",))
+    if page < 1:
+        raise ValueError(f"fork: page must be at least 1, got {page}")
     ot, ol, orf, ostride = _outs("fork", out, r, width, tables, refs, True)
-    ws = need = None
+    ws, need = None, 0
     if out is not None:
-        ws, need = _workspace("fork", workspace, b, width, refs)
-    if refs.numel() == 0 or width == 0 or max(b, r) == 0:
-        raise ValueError("fork: a pool of no pages, or tables of no rows or width")
-    # an empty tensor has no address; nothing of it is read
-    some = refs.data_ptr()
-    with torch.cuda.device(refs.device):
-        _lib.call("mzk_paged_fork", tables.data_ptr() or some, stride, b, width, lens.data_ptr() or some, refs.data_ptr(),
-                  refs.numel(), parents.data_ptr() or some, r, page, ot.data_ptr() or some, ostride, ol.data_ptr() or some,
-                  orf.data_ptr(), _lib.ptr(ws), need or 0, _lib.stream_of(refs))
+        need = workspace_bytes(b, width, pages)
+        ws = _workspace("fork", workspace, need, refs.device)
+    _call(refs.device, "mzk_paged_fork", tables.data_ptr(), stride, b, width, lens.data_ptr(), refs.data_ptr(), pages,
+          parents.data_ptr(), r, page, ot.data_ptr(), ostride, ol.data_ptr(), orf.data_ptr(), _lib.ptr(ws), need)
     return ot, ol, orf
 
 
@@ -298,19 +325,13 @@ def compact(tables: torch.Tensor, refs: torch.Tensor, *, pools=(), out=None, wor
     """The used pages moved to the front of the pools ([P, page, ...]): of U used ones, those behind
     page U - 1, in order, into the free ones before it.  Returns (tables, refs); ``out=(tables, refs)``
     may be the inputs."""
-    _lib.require_gpu(tables, refs, workspace, *pools)
-    _same_device("compact", tables, refs, workspace, *pools)
-    b, width, stride = _tables("compact", tables)
-    _check("compact", ("refs", refs, torch.int32, None))
-    if refs.dim() != 1:
-        raise ValueError("compact: refs must be [pages]")
+    _one_device("compact", tables, refs, workspace, *pools)
+    b, width, stride, pages = _book("compact", tables, None, refs)
     page = pools[0].shape[1] if pools and pools[0].dim() >= 2 else 1
+    base, size, n = _pool_list("compact", pools, pages, page)
     ot, _, orf, ostride = _outs("compact", out, b, width, tables, refs, False)
-    base, size, n = _pool_list("compact", pools, refs, page)
-    ws, need = _workspace("compact", workspace, b, width, refs)
-    if refs.numel() == 0 or width == 0 or b == 0:
-        raise ValueError("compact: a pool of no pages, or tables of no rows or width")
-    with torch.cuda.device(refs.device):
-        _lib.call("mzk_paged_compact", tables.data_ptr(), stride, b, width, refs.data_ptr(), refs.numel(), page, base, size,
-                  n, ot.data_ptr(), ostride, orf.data_ptr(), ws.data_ptr(), need, _lib.stream_of(refs))
+    need = workspace_bytes(b, width, pages)
+    ws = _workspace("compact", workspace, need, refs.device)
+    _call(refs.device, "mzk_paged_compact", tables.data_ptr(), stride, b, width, refs.data_ptr(), pages, page, base, size, n,
+          ot.data_ptr(), ostride, orf.data_ptr(), ws.data_ptr(), need)
     return ot, orf
