@@ -43,12 +43,19 @@ struct RaggedParams {
   // splitting: at most `slots` units (0: one unit per block, no joining), shares of at least
   // min_tiles tiles; a unit of a split sequence leaves its result in the slot of its number
   int slots, min_tiles;
-  int32_t* plan;       // [B][2] by the first workgroup: the sequence's first unit, its shares
+  struct JoinRow* joins;  // [blocks], by each block's first share
+  int32_t* blocks_out;    // the blocks, by the first workgroup
   float* part_o;       // [slots][64][D]: O / l
   float* part_ml;      // [slots][64][2]: m in log2 units, l
   uint16_t* out;
   float* lse;          // [T, H]
   int zero_tail;       // rows of no sequence become 0 (else they are left as they are)
+};
+
+// What the joining launch knows of a row block.
+struct JoinRow {
+  int64_t row0;  // its first row of out and lse
+  int32_t rows, shares, slot0, step;  // share s is in slot slot0 + s * step
 };
 
 // Where a unit's rows and entries are.
@@ -114,8 +121,44 @@ struct PlanLds {
   int blocks[kPlanRows], tiles[kPlanRows];
 };
 
-// The tiles of a share: the least for which the units fit the slots, looked for among 64 values between
-// what an even division gives and what always fits.  Every workgroup finds the same.
+// ceil(t / c), at least 1, from an approximate quotient
+__device__ __forceinline__ int shares_of(int t, int c, float rc) {
+  int k = static_cast<int>(static_cast<float>(t) * rc);
+  k += static_cast<int64_t>(k) * c < t;
+  k -= k > 1 && static_cast<int64_t>(k - 1) * c >= t;
+  return k > 1 ? k : 1;
+}
+
+// The tiles of a share lie between what an even division gives and what always fits: the sum of
+// blocks * ceil(tiles / c) <= work / c + blocks <= slots for c >= work / (slots - blocks).
+__device__ __forceinline__ void share_bounds(const RaggedParams& p, int64_t blocks, int64_t work, int most, int64_t& lo, int64_t& hi) {
+  hi = (work + p.slots - blocks - 1) / (p.slots - blocks);
+  lo = (work + p.slots - 1) / p.slots;
+  if (hi > most) hi = most;
+  if (lo < p.min_tiles) lo = p.min_tiles;
+  if (lo < (most + kMaxShares - 1) / kMaxShares) lo = (most + kMaxShares - 1) / kMaxShares;
+  if (hi < lo) hi = lo;
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+// sum over the lanes before this one
+__device__ __forceinline__ int wave_before(int v, int lane) {
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  return x - v;
+}
+
+// The tiles of a share: the least for which the units fit the slots, of 64 values between the bounds.
+// Every workgroup finds the same.
 __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
   int64_t blocks = 0, work = 0;
   int most = 1;
@@ -129,7 +172,7 @@ __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
     work += static_cast<int64_t>(n) * t;
     most = t > most ? t : most;
   }
-  int64_t unused;
+  int64_t unused, lo, hi;
   blocks = block_scan(blocks, unused, l.scan, tid);
   work = block_scan(work, unused, l.scan, tid);
 #pragma unroll
@@ -142,23 +185,11 @@ __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) most = l.count[0][w] > most ? l.count[0][w] : most;
   __syncthreads();
-  if (blocks >= p.slots) return most;
-  // sum of blocks * ceil(tiles / c) <= work / c + blocks <= slots for c >= work / (slots - blocks)
-  int64_t hi = (work + p.slots - blocks - 1) / (p.slots - blocks), lo = (work + p.slots - 1) / p.slots;
-  if (hi > most) hi = most;
-  if (lo < p.min_tiles) lo = p.min_tiles;
-  if (lo < (most + kMaxShares - 1) / kMaxShares) lo = (most + kMaxShares - 1) / kMaxShares;
-  if (hi <= lo) return static_cast<int>(lo);
+  share_bounds(p, blocks, work, most, lo, hi);
   const int c = static_cast<int>(lo + (hi - lo) * (tid & 63) / 63);
   const float rc = 1.0f / static_cast<float>(c);
   int n = 0;
-  for (int i = tid >> 6; i < p.B; i += 4) {
-    const int t = l.tiles[i];
-    int k = static_cast<int>(static_cast<float>(t) * rc);  // ceil(t / c), corrected
-    k += static_cast<int64_t>(k) * c < t;
-    k -= k > 1 && static_cast<int64_t>(k - 1) * c >= t;
-    n += l.blocks[i] * (k > 1 ? k : 1);
-  }
+  for (int i = tid >> 6; i < p.B; i += 4) n += l.blocks[i] * shares_of(l.tiles[i], c, rc);
   l.count[tid >> 6][tid & 63] = n;
   __syncthreads();
   const int j = tid & 63;
@@ -171,14 +202,18 @@ __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
 // This workgroup's unit; false: none.  Workgroups go to the 8 XCDs in turn: without shares, two
 // neighbouring blocks (which read the same entries) follow each other on an XCD, and the last
 // blocks, which see the most, come first; with shares, an XCD takes neighbouring units.
+// Up to 64 sequences every wave finds it alone, a lane per sequence: through LDS and barriers, as for
+// more, it took 5.4 of the 33 us of a split call's attention launch.
 __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid) {
   PlanLds& l = *reinterpret_cast<PlanLds*>(smem);
+  const int lane = tid & 63;
   const int64_t w = blockIdx.x;
   const int64_t per_token = (static_cast<int64_t>(p.HG) + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
-  int64_t blk, blocks, k;
+  int64_t blk, blocks, k, ordinal = 0;
   u.share = 0;
   u.shares = 1;
   u.slot = 0;
+  const bool small = p.B <= 64;
   if (p.slots == 0) {
     k = (w / 16 * 8 + w % 8) * 2 + w / 8 % 2;
     if (p.cu == nullptr) {
@@ -186,6 +221,18 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
       if (u.b >= p.B) return false;
       blk = k - u.b * per_token;
       blocks = per_token;
+    } else if (small) {
+      int64_t a, z;
+      int t;
+      const int v = lane < p.B ? static_cast<int>(sequence(p, lane, a, z, t)) : 0;  // below blocks_max
+      const int before = wave_before(v, lane);
+      const int total = __builtin_amdgcn_readlane(before + v, 63);
+      if (k >= total) return false;
+      k = total - 1 - k;
+      const int at = __builtin_ctzll(__ballot(k >= before && k < before + v));
+      u.b = at;
+      blk = k - __builtin_amdgcn_readlane(before, at);
+      blocks = __builtin_amdgcn_readlane(v, at);
     } else {
       int64_t total = 0;
       for (int64_t i = tid; i < p.B; i += 256) {
@@ -215,10 +262,45 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
       blk = l.scan[5];
       blocks = l.scan[6];
     }
+  } else if (small) {
+    int64_t a, z, lo, hi;
+    int t = 0, v = 0;
+    if (lane < p.B) v = static_cast<int>(sequence(p, lane, a, z, t));
+    int most = t;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      const int o = __shfl_xor(most, d, 64);
+      most = o > most ? o : most;
+    }
+    if (most < 1) most = 1;
+    share_bounds(p, wave_sum(v), wave_sum(static_cast<int64_t>(v) * t), most, lo, hi);
+    int c = static_cast<int>(lo + (hi - lo) * lane / 63);
+    if (hi > lo) {
+      const float rc = 1.0f / static_cast<float>(c);
+      int n = 0;
+      for (int i = 0; i < p.B; ++i) n += __builtin_amdgcn_readlane(v, i) * shares_of(__builtin_amdgcn_readlane(t, i), c, rc);
+      c = __builtin_amdgcn_readlane(c, __builtin_ctzll(__ballot(n <= p.slots || lane == 63)));
+    }
+    const int shares = shares_of(t, c, 1.0f / static_cast<float>(c));
+    const int units = v * shares, before = wave_before(units, lane), blocks_before = wave_before(v, lane);
+    const int total = __builtin_amdgcn_readlane(before + units, 63);
+    const int per_xcd = (total + 7) / 8;
+    k = w % 8 * per_xcd + w / 8;
+    if (w == 0 && tid == 63) *p.blocks_out = blocks_before + v;
+    if (w / 8 >= per_xcd || k >= total) return false;
+    const int at = __builtin_ctzll(__ballot(k >= before && k < before + units));
+    u.b = at;
+    blocks = __builtin_amdgcn_readlane(v, at);
+    u.shares = __builtin_amdgcn_readlane(shares, at);
+    const int in = static_cast<int>(k) - __builtin_amdgcn_readlane(before, at);
+    u.share = in / static_cast<int>(blocks);
+    blk = in - u.share * blocks;
+    ordinal = __builtin_amdgcn_readlane(blocks_before, at) + blk;
   } else {
     const int c = share_tiles(p, l, tid);
-    int64_t total = 0, before, base = 0;
-    for (int64_t i = tid; i < p.B; i += 256) total += static_cast<int64_t>(l.blocks[i]) * (l.tiles[i] > c ? (l.tiles[i] + c - 1) / c : 1);
+    const float rc = 1.0f / static_cast<float>(c);
+    int64_t total = 0, before, base = 0, blocks_base = 0;
+    for (int64_t i = tid; i < p.B; i += 256) total += static_cast<int64_t>(l.blocks[i]) * shares_of(l.tiles[i], c, rc);
     total = block_scan(total, before, l.scan, tid);
     const int64_t per_xcd = (total + 7) / 8;
     k = w % 8 * per_xcd + w / 8;
@@ -226,23 +308,23 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     if (!mine && w != 0) return false;
     for (int64_t i = 0; i < p.B; i += 256) {
       int shares = 1;
-      int64_t v = 0;
+      int64_t n = 0, blocks_before;
       if (i + tid < p.B) {
-        shares = l.tiles[i + tid] > c ? (l.tiles[i + tid] + c - 1) / c : 1;
-        v = static_cast<int64_t>(l.blocks[i + tid]) * shares;
+        shares = shares_of(l.tiles[i + tid], c, rc);
+        n = l.blocks[i + tid];
       }
-      const int64_t sum = block_scan(v, before, l.scan, tid);
-      if (w == 0 && i + tid < p.B) {
-        p.plan[2 * (i + tid)] = static_cast<int32_t>(base + before);
-        p.plan[2 * (i + tid) + 1] = shares;
-      }
-      if (mine && k >= base + before && k < base + before + v) {
+      const int64_t sum = block_scan(n * shares, before, l.scan, tid);
+      const int64_t blocks_sum = block_scan(n, blocks_before, l.scan, tid);
+      if (mine && k >= base + before && k < base + before + n * shares) {
         l.scan[4] = i + tid;
         l.scan[5] = k - base - before;
         l.scan[6] = shares;
+        l.scan[7] = blocks_base + blocks_before;
       }
       base += sum;
+      blocks_base += blocks_sum;
     }
+    if (w == 0 && tid == 0) *p.blocks_out = static_cast<int32_t>(blocks_base);
     __syncthreads();
     if (!mine) return false;
     u.b = l.scan[4];
@@ -250,32 +332,38 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     u.shares = static_cast<int>(l.scan[6]);
     u.share = static_cast<int>(l.scan[5] / blocks);
     blk = l.scan[5] - u.share * blocks;
-    u.slot = static_cast<int>(k);
+    ordinal = l.scan[7] + blk;
   }
   int64_t a, z;
   int tiles;
+  u.b = uniform(u.b);
   sequence(p, u.b, a, z, tiles);
-  u.t0 = a;
-  u.n = static_cast<int>(z - a);
+  u.t0 = uniform(a);
+  u.n = uniform(static_cast<int>(z - a));
   const int64_t per_latent = blocks / p.G;
-  u.g = static_cast<int>(blk / per_latent);
-  u.r0 = (blk - u.g * per_latent) * p.rows_per_unit;
+  u.g = uniform(static_cast<int>(blk / per_latent));
+  u.r0 = uniform((blk - u.g * per_latent) * p.rows_per_unit);
   const int64_t rows = static_cast<int64_t>(u.n) * p.HG;
   u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
   u.len = u.n;
-  if (p.lens) u.len = static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page));
-  u.b = uniform(u.b);
-  u.t0 = uniform(u.t0);
-  u.n = uniform(u.n);
-  u.len = uniform(u.len);
-  u.g = uniform(u.g);
-  u.r0 = uniform(u.r0);
-  u.r1 = uniform(u.r1);
+  if (p.lens) u.len = uniform(static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page)));
   u.share = uniform(u.share);
   u.shares = uniform(u.shares);
-  u.slot = uniform(u.slot);
-  __syncthreads();  // the plan's LDS is free
+  u.slot = uniform(static_cast<int>(k));
+  if (p.slots && u.share == 0 && tid == 0)
+    p.joins[ordinal] = JoinRow{u.t0 * p.H + u.r0, static_cast<int32_t>(u.r1 - u.r0), u.shares, u.slot, static_cast<int32_t>(blocks)};
+  if (!small) __syncthreads();  // the plan's LDS is free
   return true;
+}
+
+// Rows behind the last sequence, shared out over the workgroups: 0, and a log-sum-exp of -inf.
+__device__ __forceinline__ void zero_rows(const RaggedParams& p, int tid) {
+  if (!p.zero_tail || !p.cu) return;
+  const int64_t end = clamp64(p.cu[p.B], 0, p.T) * p.H;
+  for (int64_t r = end + blockIdx.x; r < p.T * p.H; r += gridDim.x) {
+    for (int i = tid; i < p.D / 2; i += 256) reinterpret_cast<uint32_t*>(p.out + r * p.D)[i] = 0;
+    if (tid == 0) p.lse[r] = -__builtin_huge_valf();
+  }
 }
 
 // Row r of the unit's sequence: its row of q, out and lse.
@@ -373,6 +461,7 @@ ragged_kernel(const RaggedParams p) {
   const int eh = wave & 1, hh = wave >> 1, g = lane >> 4, e16 = lane & 15;
 
   Unit u;
+  zero_rows(p, tid);
   if (!find_unit(p, u, smem, tid)) return;  // uniform
 
   // the B operand of S^T: rows 32 hh + 16 b + e16, channels 32 st + 8 g ..
@@ -564,100 +653,73 @@ ragged_kernel(const RaggedParams p) {
 
 #include "ragged_wide.h"
 
-// Joins the shares of a row block: workgroup 4 k + j rows 16 j .. of block k of the split sequences.
+// Joins the shares of a row block's rows, ROWS of them a workgroup, 4 channels a thread.
 // o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the sink.
+// Bound by latency for a few rows (record, then maxima and sums, then the shares' rows, all
+// requested together) and by the memory for many.
+template <int D>
+struct JoinShape {
+  static constexpr int PIECES = D / 4;
+  static constexpr int ROWS = 256 / PIECES;                       // a workgroup's rows
+  static constexpr int THREADS = (ROWS * PIECES + 63) / 64 * 64;  // (one row of 576 channels in 192 threads)
+};
+
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
-  __shared__ int64_t scan[8];
-  __shared__ float weight[16][kMaxShares + 1];
+  using J = JoinShape<D>;
+  constexpr int PIECES = J::PIECES, ROWS = J::ROWS, PER = (64 + ROWS - 1) / ROWS;
+  __shared__ float weight[ROWS][kMaxShares];
   const int tid = threadIdx.x;
-  const int64_t k = blockIdx.x >> 2;
-  const int r16 = 16 * (blockIdx.x & 3);
-  // the block's sequence, as find_unit without shares
-  int64_t base = 0;
-  bool found = false;
-  for (int64_t i = 0; i < p.B && !found; i += 256) {
-    int64_t a, z, v = 0, before;
-    int t;
-    if (i + tid < p.B) v = sequence(p, i + tid, a, z, t);
-    const int64_t sum = block_scan(v, before, scan, tid);
-    if (k >= base + before && k < base + before + v) {
-      scan[4] = i + tid;
-      scan[5] = k - base - before;
-      scan[6] = v;
-    }
-    base += sum;
-    found = k < base;
-  }
-  __syncthreads();
-  if (!found) return;
-  Unit u;
-  u.b = scan[4];
-  const int64_t blk = scan[5], blocks = scan[6];
-  const int shares = p.plan[2 * u.b + 1];
-  if (shares <= 1) return;
-  int64_t a, z;
-  int t;
-  sequence(p, u.b, a, z, t);
-  u.t0 = a;
-  const int64_t per_latent = blocks / p.G;
-  u.g = static_cast<int>(blk / per_latent);
-  u.r0 = (blk - u.g * per_latent) * p.rows_per_unit;
-  const int64_t rows = (z - a) * p.HG;
-  u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
-  const int64_t slot0 = p.plan[2 * u.b] + blk;
-  // weights: 16 threads a row
-  {
-    const int r = tid >> 4;
-    const int64_t row = u.r0 + r16 + r;
-    const float* const ml = p.part_ml + 2 * (slot0 * 64 + r16 + r);
-    float m = -__builtin_huge_valf(), l = 0.0f;
-    for (int s = tid & 15; s < shares; s += 16) m = fmaxf(m, ml[128 * blocks * s]);
+  const int k = blockIdx.x / PER, r0 = (blockIdx.x - k * PER) * ROWS;
+  if (k >= *p.blocks_out) return;
+  const JoinRow j = p.joins[k];
+  if (j.shares <= 1 || r0 >= j.rows) return;
+  {  // weights: 16 threads a row
+    static_assert(ROWS * 16 <= 256 && J::THREADS >= ROWS * 16, "weights");
+    const int r = tid >> 4, row = r0 + r;
+    if (r < ROWS && row < j.rows) {
+      const float* const ml = p.part_ml + 2 * (static_cast<int64_t>(j.slot0) * 64 + row);
+      const int64_t step = 128ll * j.step;
+      float m = -__builtin_huge_valf(), l = 0.0f;
+      for (int s = tid & 15; s < j.shares; s += 16) m = fmaxf(m, ml[step * s]);
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    for (int s = tid & 15; s < shares; s += 16) {
-      const float2 v = *reinterpret_cast<const float2*>(ml + 128 * blocks * s);
-      // l * 2^(m_s - m): a share that saw nothing has l 0 and m -inf, one with a NaN has l NaN
-      const float w = v.x == -__builtin_huge_valf() && v.y == 0.0f ? 0.0f : v.y * exp2f(v.x - m);
-      weight[r][s] = w;
-      l += w;
-    }
+      for (int d = 8; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+      for (int s = tid & 15; s < j.shares; s += 16) {
+        const float2 v = *reinterpret_cast<const float2*>(ml + step * s);
+        // a share that saw nothing has l 0 and m -inf, one with a NaN has l NaN
+        const float w = v.x == -__builtin_huge_valf() && v.y == 0.0f ? 0.0f : v.y * exp2f(v.x - m);
+        weight[r][s] = w;
+        l += w;
+      }
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) l += __shfl_xor(l, d, 64);
-    float lse = 0.0f, scale = 0.0f;
-    if (row < u.r1) {
-      const int64_t at = row_at(p, u, row);
-      scale = finish_row(p, static_cast<int>(at % p.H), m, l, lse);
+      for (int d = 8; d >= 1; d >>= 1) l += __shfl_xor(l, d, 64);
+      const int64_t at = j.row0 + row;
+      float lse;
+      const float scale = finish_row(p, static_cast<int>(at % p.H), m, l, lse);
       if ((tid & 15) == 0) p.lse[at] = lse;
+      for (int s = tid & 15; s < j.shares; s += 16) weight[r][s] *= scale;
     }
-    for (int s = tid & 15; s < shares; s += 16) weight[r][s] *= scale;
   }
   __syncthreads();
-  constexpr int PIECES = D / 4;
-  for (int i = tid; i < 16 * PIECES; i += 256) {
-    const int r = i / PIECES, c = 4 * (i - r * PIECES);
-    const int64_t row = u.r0 + r16 + r;
-    if (row >= u.r1) break;  // rows ascend with i
-    const float* const o = p.part_o + (slot0 * 64 + r16 + r) * D + c;
-    v4f sum = v4f{};
-    for (int s = 0; s < shares; ++s) {
-      const float w = weight[r][s];
-      const v4f v = *reinterpret_cast<const v4f*>(o + static_cast<int64_t>(64) * D * blocks * s);
+  const int r = tid / PIECES, c = 4 * (tid - r * PIECES), row = r0 + r;
+  if (r >= ROWS || row >= j.rows) return;
+  const float* const o = p.part_o + (static_cast<int64_t>(j.slot0) * 64 + row) * D + c;
+  const int64_t step = 64ll * D * j.step;
+  v4f sum = v4f{};
+  constexpr int AHEAD = 8;
+  for (int s0 = 0; s0 < j.shares; s0 += AHEAD) {
+    v4f v[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(w, v[j], sum[j]);
-    }
-    *reinterpret_cast<uint2*>(p.out + row_at(p, u, row) * D + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
+    for (int s = 0; s < AHEAD; ++s) v[s] = *reinterpret_cast<const v4f*>(o + step * (s0 + s < j.shares ? s0 + s : s0));
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s)
+      if (s0 + s < j.shares) {
+        const float w = weight[r][s0 + s];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[s][i], sum[i]);
+      }
   }
-}
-
-// Rows behind the last sequence: 0, and a log-sum-exp of -inf.
-__global__ void __launch_bounds__(256) ragged_tail_kernel(const RaggedParams p) {
-  const int64_t end = clamp64(p.cu[p.B], 0, p.T);
-  const int64_t rows = (p.T - end) * p.H;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
-  uint32_t* const o = reinterpret_cast<uint32_t*>(p.out + end * p.H * p.D);
-  for (int64_t i = at; i < rows * (p.D / 2); i += step) o[i] = 0;
-  for (int64_t i = at; i < rows; i += step) p.lse[end * p.H + i] = -__builtin_huge_valf();
+  *reinterpret_cast<uint2*>(p.out + (j.row0 + row) * D + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
 }
 
 template <int FMT, int D, int NOPE>
@@ -685,8 +747,10 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   } else {
     ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, RaggedLds<FMT, D, NOPE>::LDS, s>>>(p);
   }
-  if (p.slots) join_kernel<D><<<static_cast<unsigned>(4 * p.blocks_max), 256, 0, s>>>(p);
-  if (p.zero_tail && p.cu) ragged_tail_kernel<<<256, 256, 0, s>>>(p);
+  if (p.slots) {
+    using J = JoinShape<D>;
+    join_kernel<D><<<static_cast<unsigned>((64 + J::ROWS - 1) / J::ROWS * p.blocks_max), J::THREADS, 0, s>>>(p);
+  }
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;
 }
@@ -733,7 +797,7 @@ int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 int64_t attend_bytes(int64_t blocks, int64_t B, int D) {
   const int slots = unit_slots(blocks, B);
-  return slots ? align16_up(8 * B) + static_cast<int64_t>(slots) * 64 * 4 * (D + 2) : 0;
+  return slots ? 16 + align16_up(static_cast<int64_t>(sizeof(JoinRow)) * blocks) + static_cast<int64_t>(slots) * 64 * 4 * (D + 2) : 0;
 }
 
 }  // namespace
@@ -802,8 +866,10 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.min_tiles = kMinTiles;
   p.slots = (most + kTile - 1) / kTile > kMinTiles ? unit_slots(p.blocks_max, B) : 0;
   if (p.slots) {
-    p.plan = static_cast<int32_t*>(workspace);
-    p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align16_up(8 * B));
+    p.blocks_out = static_cast<int32_t*>(workspace);
+    p.joins = reinterpret_cast<JoinRow*>(static_cast<uint8_t*>(workspace) + 16);
+    p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 16 +
+                                         align16_up(static_cast<int64_t>(sizeof(JoinRow)) * p.blocks_max));
     p.part_o = p.part_ml + static_cast<int64_t>(p.slots) * 64 * 2;
   }
   return dispatch_ragged("paged_attend", fmt, nope, p, as_stream(stream));

@@ -93,6 +93,7 @@ ragged_wide_kernel(const RaggedParams p) {
   const int g = lane >> 4, e16 = lane & 15;
 
   Unit u;
+  zero_rows(p, tid);
   if (!find_unit(p, u, smem, tid)) return;  // uniform
 
   // q: the B operand of S^T (rows 32 hh + 16 b + e16, channels 32 st + 8 g ..) through LDS, from
