@@ -101,11 +101,20 @@ ragged_wide_kernel(const RaggedParams p) {
   const int rows = static_cast<int>(u.r1 - u.r0);
   constexpr int QROW = D / 8, QP = 64 * QROW / NT;
   u32x4 qraw[QP];
+  if (p.G == 1) {  // one run of rows
+    const u32x4* const qb = reinterpret_cast<const u32x4*>(p.q + (u.t0 * p.H + u.r0) * D);
 #pragma unroll
-  for (int k = 0; k < QP; ++k) {
-    const int at = tid + NT * k;
-    const int r = at / QROW;
-    qraw[k] = *reinterpret_cast<const u32x4*>(p.q + row_at(p, u, u.r0 + (r < rows ? r : 0)) * D + 8 * (at - r * QROW));
+    for (int k = 0; k < QP; ++k) {
+      const int at = tid + NT * k;
+      qraw[k] = qb[at < rows * QROW ? at : 0];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < QP; ++k) {
+      const int at = tid + NT * k;
+      const int r = at / QROW;
+      qraw[k] = *reinterpret_cast<const u32x4*>(p.q + row_at(p, u, u.r0 + (r < rows ? r : 0)) * D + 8 * (at - r * QROW));
+    }
   }
   const int64_t tok0 = u.r0 / p.HG, tok1 = (u.r1 - 1) / p.HG + 1;
   const int shift = u.len - u.n;
@@ -117,7 +126,7 @@ ragged_wide_kernel(const RaggedParams p) {
     const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
     tok_b[b] = static_cast<int>((r < u.r1 ? r : u.r0) / p.HG);
   }
-  const int win = p.window < 0x7fffffff ? static_cast<int>(p.window) : 0x7fffffff;
+  const int64_t win = p.window < 0x7fffffff ? p.window : 0x7fffffff;
 
   // ---- addresses -------------------------------------------------------------------------
   const int te = tid >> 3, tj = tid & 7;
@@ -290,21 +299,29 @@ ragged_wide_kernel(const RaggedParams p) {
     va[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp + 2048));
   };
 
-  // ---- one chunk of the pass: tiles `first` .. `last` ------------------------------------------
+  // the chunk's first two tiles requested
+  auto ask = [&]() __attribute__((always_inline)) {
+    const gptr_t a = entry_at(code_of(first)), b = entry_at(code_of(first < last ? first + 1 : first));
+    if constexpr (kDirect) {
+      direct(a, tile_at(0));
+      direct(b, tile_at(1));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 6; ++k) fetch_part(a, raw[0], k);
+#pragma unroll
+      for (int k = 0; k < 6; ++k) fetch_part(b, raw[1], k);
+    }
+  };
+
+  // ---- one chunk of the pass: tiles `first` .. `last`, the first two asked for ------------------------------------------
   // begin: the rows' references come from its first tile
   auto chunk = [&](bool begin) __attribute__((always_inline)) {
     const int t0 = first, n = last + 1;
     if constexpr (kDirect) {
-      direct(entry_at(code_of(t0)), tile_at(0));
-      direct(entry_at(code_of(t0 + 1 < n ? t0 + 1 : t0)), tile_at(1));
       direct(entry_at(code_of(t0 + 2 < n ? t0 + 2 : t0)), tile_at(2));
       if constexpr (NI > 8) asm volatile("s_waitcnt vmcnt(18)" : : : "memory");
       else asm volatile("s_waitcnt vmcnt(16)" : : : "memory");
     } else {
-#pragma unroll
-      for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0)), raw[0], k);
-#pragma unroll
-      for (int k = 0; k < 6; ++k) fetch_part(entry_at(code_of(t0 + 1)), raw[1], k);
 #pragma unroll
       for (int k = 0; k < 9; ++k) store_part(smem, raw[0], k);
       if (n - t0 > 1) {
@@ -490,22 +507,56 @@ ragged_wide_kernel(const RaggedParams p) {
     landed();  // the LDS is free again
   };
 
-  // q into its operand's layout
+  // the entries that tokens sub0 .. sub1 - 1 see of this unit's share, and what the rows see of them
+  int64_t sub0 = tok0, sub1 = tok1;
+  auto set_range = [&]() __attribute__((always_inline)) {
+    token_range(p, u, sub0, sub1, lo, hi);
+    lo = lo > share_lo ? lo : share_lo;
+    hi = hi < share_hi ? hi : share_hi;
+    if (hi < lo) hi = lo;
+    int most_lo = lo, least_hi = hi;
+    if (!p.idx) {
+      const int64_t a = static_cast<int64_t>(shift) + sub1 - win, z = static_cast<int64_t>(shift) + sub0 + 1;
+      most_lo = a > lo ? static_cast<int>(a) : lo;
+      least_hi = z < hi ? static_cast<int>(z) : hi;
+    }
+    full_lo = (most_lo - lo + kTile - 1) / kTile;
+    full_hi = least_hi > lo ? (least_hi - lo) / kTile : 0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      int64_t a = lo, z = hi;
+      if (!p.idx) {
+        const int64_t pos = static_cast<int64_t>(shift) + tok_b[b];
+        if (pos - win + 1 > a) a = pos - win + 1;
+        if (pos + 1 < z) z = pos + 1;
+      }
+      row_lo[b] = static_cast<int>(a - lo);
+      row_span[b] = z > a ? static_cast<int>(z - a) : 0;
+    }
+  };
+
+  // The first chunk is laid out and its first tiles requested while q arrives; then q goes into its
+  // operand's layout through the LDS behind those tiles.  (One after the other this took 17 us of a
+  // split call over 4096 entries.)
+  set_range();
+  const bool none = !(lo < hi && lay_out());  // uniform
+  if (!none) ask();
   {
     constexpr int QPITCH = 2 * D + 16;  // the pad spreads 16 rows' pieces over the banks
-    static_assert(64 * QPITCH <= M::PB, "q in the tiles' place");
+    constexpr int QB = M::PB + 2 * 4096 - 64 * QPITCH;
+    static_assert(QB >= (kDirect ? 2 * M::TILE : 0), "q behind the first tiles");
 #pragma unroll
     for (int k = 0; k < QP; ++k) {
       const int at = tid + NT * k;
       const int r = at / QROW;
-      *reinterpret_cast<u32x4*>(smem + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
+      *reinterpret_cast<u32x4*>(smem + QB + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
     }
     lds_barrier();
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + (32 * hh + 16 * b + e16) * QPITCH + 64 * st + 16 * g));
+        qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + QB + (32 * hh + 16 * b + e16) * QPITCH + 64 * st + 16 * g));
     lds_barrier();
     // the first query fragments live in accumulation registers beside O^T, which the matrix
     // instructions read directly; left to itself the compiler spills
@@ -520,35 +571,9 @@ ragged_wide_kernel(const RaggedParams p) {
   }
 
   // ---- the passes --------------------------------------------------------------------------
-  int64_t sub0 = tok0, sub1 = tok1;
-  bool strict = false;
+  bool strict = false, at_start = true;
   while (true) {
-    token_range(p, u, sub0, sub1, lo, hi);
-    lo = lo > share_lo ? lo : share_lo;
-    hi = hi < share_hi ? hi : share_hi;
-    if (hi < lo) hi = lo;
-    {
-      // what the rows see, from lo; tiles that all of them see whole
-      int most_lo = lo, least_hi = hi;
-      if (!p.idx) {
-        const int64_t a = static_cast<int64_t>(shift) + sub1 - 1 - (static_cast<int64_t>(win) - 1), z = static_cast<int64_t>(shift) + sub0 + 1;
-        most_lo = a > lo ? static_cast<int>(a) : lo;
-        least_hi = z < hi ? static_cast<int>(z) : hi;
-      }
-      full_lo = (most_lo - lo + kTile - 1) / kTile;
-      full_hi = least_hi > lo ? (least_hi - lo) / kTile : 0;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        int64_t a = lo, z = hi;
-        if (!p.idx) {
-          const int64_t pos = static_cast<int64_t>(shift) + tok_b[b];
-          if (pos - win + 1 > a) a = pos - win + 1;
-          if (pos + 1 < z) z = pos + 1;
-        }
-        row_lo[b] = static_cast<int>(a - lo);
-        row_span[b] = z > a ? static_cast<int>(z - a) : 0;
-      }
-    }
+    if (!at_start) set_range();
     float l4[4];
     int e4[4];
     for (bool given = false;; given = true) {
@@ -586,10 +611,13 @@ ragged_wide_kernel(const RaggedParams p) {
         for (int hg = 0; hg < 4; ++hg) m4[hg] = 0.0f;
       }
       for (c0 = 0; c0 < hi - lo; c0 += nt * kTile) {
-        if (!lay_out()) continue;
+        const bool ready = at_start && c0 == 0;
+        if (ready ? none : !lay_out()) continue;
+        if (!ready) ask();
         chunk(!begun);
         begun = true;
       }
+      at_start = false;
       // each row's sum: its four lanes, then the two entry halves
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
