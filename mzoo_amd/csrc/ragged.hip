@@ -18,6 +18,22 @@ namespace {
 
 constexpr int64_t kNoWindow = 1ll << 62;
 
+// Division of n < 2^31 by a constant of the call: floor(n m / 2^32) + n, shifted, with m = floor(2^32 (2^s -
+// d) / d) + 1 and 2^s >= d.  Three instructions; what is executed once runs from a cold instruction
+// cache, where a 64-bit division is half a microsecond.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> s);
+  }
+};
+FastDiv fast_div(uint32_t d) {
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  return FastDiv{d, static_cast<uint32_t>(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+
 struct RaggedParams {
   const uint16_t* q;  // [T, H, D] bf16
   int64_t T;
@@ -38,14 +54,15 @@ struct RaggedParams {
   int64_t window;
   const float* sinks;
   float scale_log2;
-  int rows_per_unit;   // min(64, 32 HG): a unit spans at most 33 tokens
+  FastDiv by_heads, by_page, by_blocks;  // HG, page, the row blocks of one token
+  int unit_shift;      // log2 of a unit's rows: 32 for one head, else 64, so a unit spans at most 33 tokens
   int64_t blocks_max;  // row blocks at most
   // splitting: at most `slots` units (0: one unit per block, no joining), shares of at least
   // min_tiles tiles; a unit of a split sequence leaves its result in the slot of its number
   int slots, min_tiles;
   struct JoinRow* joins;  // [blocks], by each block's first share
   int32_t* blocks_out;    // the blocks, by the first workgroup
-  float* part_o;       // [slots][64][D]: O / l
+  float* part_o;       // [slots][D / 16][64][16]: O / l, a store instruction of the attention kernel 1 KB of it
   float* part_ml;      // [slots][64][2]: m in log2 units, l
   uint16_t* out;
   float* lse;          // [T, H]
@@ -60,10 +77,10 @@ struct JoinRow {
 
 // Where a unit's rows and entries are.
 struct Unit {
-  int64_t b, t0;      // sequence, its first packed token
+  int b, t0;          // sequence, its first packed token
   int n, len;         // its new tokens, its tokens in the cache
   int g;              // latent
-  int64_t r0, r1;     // rows of the sequence and latent: token r / HG, head g HG + r % HG
+  int r0, r1;         // rows of the sequence and latent: token r / HG, head g HG + r % HG
   int share, shares;  // of the tiles from the first to the last entry that a row sees
   int slot;
 };
@@ -98,19 +115,20 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& before, int64_
   return total;
 }
 
-// Sequence i's packed tokens a .. z - 1, its row blocks and its tiles.
-__device__ __forceinline__ int64_t sequence(const RaggedParams& p, int64_t i, int64_t& a, int64_t& z, int& tiles) {
+// Sequence i's packed tokens a .. z - 1, its row blocks of one latent and its tiles.
+__device__ __forceinline__ int sequence(const RaggedParams& p, int i, int& a, int& z, int& tiles) {
   a = i;
   z = i + 1;
   if (p.cu) {
-    a = clamp64(p.cu[i], 0, p.T);
-    z = clamp64(p.cu[i + 1], a, p.T);
+    a = static_cast<int>(clamp64(p.cu[i], 0, p.T));
+    z = static_cast<int>(clamp64(p.cu[i + 1], a, p.T));
   }
-  int64_t seen = p.lens ? clamp64(p.lens[i], 0, p.max_pages * p.page) : z - a;
+  int seen = z - a;
+  if (p.lens) seen = static_cast<int>(clamp64(p.lens[i], 0, p.max_pages * p.page));
   if (p.idx) seen = seen > 0 ? p.topk : 0;
-  if (seen > p.window + (z - a)) seen = p.window + (z - a);
-  tiles = static_cast<int>((seen + kTile - 1) / kTile);
-  return ((z - a) * p.HG + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
+  if (seen > p.window + (z - a)) seen = static_cast<int>(p.window) + (z - a);
+  tiles = (seen + kTile - 1) / kTile;
+  return ((z - a) * p.HG + (1 << p.unit_shift) - 1) >> p.unit_shift;
 }
 
 constexpr int kPlanRows = 1024;  // the most sequences that are split
@@ -131,19 +149,28 @@ __device__ __forceinline__ int shares_of(int t, int c, float rc) {
 
 // The tiles of a share lie between what an even division gives and what always fits: the sum of
 // blocks * ceil(tiles / c) <= work / c + blocks <= slots for c >= work / (slots - blocks).
-__device__ __forceinline__ void share_bounds(const RaggedParams& p, int64_t blocks, int64_t work, int most, int64_t& lo, int64_t& hi) {
-  hi = (work + p.slots - blocks - 1) / (p.slots - blocks);
-  lo = (work + p.slots - 1) / p.slots;
+__device__ __forceinline__ void share_bounds(const RaggedParams& p, int blocks, float work, int most, int& lo, int& hi) {
+  hi = static_cast<int>(work / static_cast<float>(p.slots - blocks) * 1.00001f) + 2;
+  lo = static_cast<int>(work / static_cast<float>(p.slots));
   if (hi > most) hi = most;
   if (lo < p.min_tiles) lo = p.min_tiles;
   if (lo < (most + kMaxShares - 1) / kMaxShares) lo = (most + kMaxShares - 1) / kMaxShares;
   if (hi < lo) hi = lo;
 }
+__device__ __forceinline__ int share_candidate(int lo, int hi, int j) { return lo + static_cast<uint32_t>(hi - lo) * static_cast<uint32_t>(j) / 63u; }
 
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_most(int v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const int o = __shfl_xor(v, d, 64);
+    v = o > v ? o : v;
+  }
   return v;
 }
 // sum over the lanes before this one
@@ -158,45 +185,50 @@ __device__ __forceinline__ int wave_before(int v, int lane) {
 }
 
 // The tiles of a share: the least for which the units fit the slots, of 64 values between the bounds.
-// Every workgroup finds the same.
+// Every workgroup finds the same.  (G == 1 where there are shares.)
 __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
-  int64_t blocks = 0, work = 0;
-  int most = 1;
-  for (int64_t i = tid; i < p.B; i += 256) {
-    int64_t a, z;
-    int t;
-    const int n = static_cast<int>(sequence(p, i, a, z, t));
+  int blocks = 0, most = 1;
+  float work = 0.0f;
+  for (int i = tid; i < p.B; i += 256) {
+    int a, z, t;
+    const int n = sequence(p, i, a, z, t);
     l.blocks[i] = n;
     l.tiles[i] = t;
     blocks += n;
-    work += static_cast<int64_t>(n) * t;
+    work += static_cast<float>(n) * static_cast<float>(t);
     most = t > most ? t : most;
   }
-  int64_t unused, lo, hi;
-  blocks = block_scan(blocks, unused, l.scan, tid);
-  work = block_scan(work, unused, l.scan, tid);
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    const int o = __shfl_xor(most, d, 64);
-    most = o > most ? o : most;
+  blocks = wave_sum(blocks);
+  work = wave_sum(work);
+  most = wave_most(most);
+  if ((tid & 63) == 0) {
+    l.count[0][tid >> 6] = most;
+    l.count[1][tid >> 6] = blocks;
+    l.count[2][tid >> 6] = __float_as_int(work);
   }
-  if ((tid & 63) == 0) l.count[0][tid >> 6] = most;
   __syncthreads();
+  blocks = 0;
+  work = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) most = l.count[0][w] > most ? l.count[0][w] : most;
+  for (int w = 0; w < 4; ++w) {
+    most = l.count[0][w] > most ? l.count[0][w] : most;
+    blocks += l.count[1][w];
+    work += __int_as_float(l.count[2][w]);
+  }
   __syncthreads();
+  int lo, hi;
   share_bounds(p, blocks, work, most, lo, hi);
-  const int c = static_cast<int>(lo + (hi - lo) * (tid & 63) / 63);
+  const int c = share_candidate(lo, hi, tid & 63);
   const float rc = 1.0f / static_cast<float>(c);
   int n = 0;
   for (int i = tid >> 6; i < p.B; i += 4) n += l.blocks[i] * shares_of(l.tiles[i], c, rc);
   l.count[tid >> 6][tid & 63] = n;
   __syncthreads();
   const int j = tid & 63;
-  const bool fits = static_cast<int64_t>(l.count[0][j]) + l.count[1][j] + l.count[2][j] + l.count[3][j] <= p.slots || j == 63;
+  const bool fits = l.count[0][j] + l.count[1][j] + l.count[2][j] + l.count[3][j] <= p.slots || j == 63;
   const int first = __builtin_ctzll(__ballot(fits));
   __syncthreads();
-  return static_cast<int>(lo + (hi - lo) * first / 63);
+  return share_candidate(lo, hi, first);
 }
 
 // This workgroup's unit; false: none.  Workgroups go to the 8 XCDs in turn: without shares, two
@@ -207,24 +239,20 @@ __device__ int share_tiles(const RaggedParams& p, PlanLds& l, int tid) {
 __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid) {
   PlanLds& l = *reinterpret_cast<PlanLds*>(smem);
   const int lane = tid & 63;
-  const int64_t w = blockIdx.x;
-  const int64_t per_token = (static_cast<int64_t>(p.HG) + p.rows_per_unit - 1) / p.rows_per_unit * p.G;
-  int64_t blk, blocks, k, ordinal = 0;
+  const int w = static_cast<int>(blockIdx.x);
+  int blk, blocks, k, ordinal = 0, a, z, t = 0;  // blocks: of one latent
   u.share = 0;
   u.shares = 1;
-  u.slot = 0;
   const bool small = p.B <= 64;
   if (p.slots == 0) {
-    k = (w / 16 * 8 + w % 8) * 2 + w / 8 % 2;
+    k = ((w >> 4) * 8 + (w & 7)) * 2 + (w >> 3 & 1);
     if (p.cu == nullptr) {
-      u.b = k / per_token;
+      u.b = p.by_blocks(k);
       if (u.b >= p.B) return false;
-      blk = k - u.b * per_token;
-      blocks = per_token;
+      blk = k - u.b * static_cast<int>(p.by_blocks.d);
+      blocks = (p.HG + 63) >> 6;
     } else if (small) {
-      int64_t a, z;
-      int t;
-      const int v = lane < p.B ? static_cast<int>(sequence(p, lane, a, z, t)) : 0;  // below blocks_max
+      const int v = lane < p.B ? sequence(p, lane, a, z, t) * p.G : 0;  // in all below blocks_max
       const int before = wave_before(v, lane);
       const int total = __builtin_amdgcn_readlane(before + v, 63);
       if (k >= total) return false;
@@ -232,22 +260,16 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
       const int at = __builtin_ctzll(__ballot(k >= before && k < before + v));
       u.b = at;
       blk = k - __builtin_amdgcn_readlane(before, at);
-      blocks = __builtin_amdgcn_readlane(v, at);
+      blocks = __builtin_amdgcn_readlane(v, at) / p.G;
     } else {
       int64_t total = 0;
-      for (int64_t i = tid; i < p.B; i += 256) {
-        int64_t a, z;
-        int t;
-        total += sequence(p, i, a, z, t);
-      }
+      for (int i = tid; i < p.B; i += 256) total += sequence(p, i, a, z, t) * p.G;
       int64_t before, base = 0;
       total = block_scan(total, before, l.scan, tid);
       if (k >= total) return false;
-      k = total - 1 - k;
-      for (int64_t i = 0;; i += 256) {  // ends: k < total
-        int64_t a, z, v = 0;
-        int t;
-        if (i + tid < p.B) v = sequence(p, i + tid, a, z, t);
+      k = static_cast<int>(total) - 1 - k;
+      for (int i = 0;; i += 256) {  // ends: k < total
+        const int64_t v = i + tid < p.B ? sequence(p, i + tid, a, z, t) * p.G : 0;
         const int64_t sum = block_scan(v, before, l.scan, tid);
         if (k >= base + before && k < base + before + v) {
           l.scan[4] = i + tid;
@@ -258,24 +280,18 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
         if (k < base) break;
       }
       __syncthreads();
-      u.b = l.scan[4];
-      blk = l.scan[5];
-      blocks = l.scan[6];
+      u.b = static_cast<int>(l.scan[4]);
+      blk = static_cast<int>(l.scan[5]);
+      blocks = static_cast<int>(l.scan[6]) / p.G;
     }
   } else if (small) {
-    int64_t a, z, lo, hi;
-    int t = 0, v = 0;
-    if (lane < p.B) v = static_cast<int>(sequence(p, lane, a, z, t));
-    int most = t;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const int o = __shfl_xor(most, d, 64);
-      most = o > most ? o : most;
-    }
-    if (most < 1) most = 1;
-    share_bounds(p, wave_sum(v), wave_sum(static_cast<int64_t>(v) * t), most, lo, hi);
-    int c = static_cast<int>(lo + (hi - lo) * lane / 63);
+    int v = 0, lo, hi;
+    if (lane < p.B) v = sequence(p, lane, a, z, t);
+    const int most = wave_most(t);
+    share_bounds(p, wave_sum(v), wave_sum(static_cast<float>(v) * static_cast<float>(t)), most > 1 ? most : 1, lo, hi);
+    int c = lo;
     if (hi > lo) {
+      c = share_candidate(lo, hi, lane);
       const float rc = 1.0f / static_cast<float>(c);
       int n = 0;
       for (int i = 0; i < p.B; ++i) n += __builtin_amdgcn_readlane(v, i) * shares_of(__builtin_amdgcn_readlane(t, i), c, rc);
@@ -285,28 +301,28 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     const int units = v * shares, before = wave_before(units, lane), blocks_before = wave_before(v, lane);
     const int total = __builtin_amdgcn_readlane(before + units, 63);
     const int per_xcd = (total + 7) / 8;
-    k = w % 8 * per_xcd + w / 8;
+    k = (w & 7) * per_xcd + (w >> 3);
     if (w == 0 && tid == 63) *p.blocks_out = blocks_before + v;
-    if (w / 8 >= per_xcd || k >= total) return false;
+    if ((w >> 3) >= per_xcd || k >= total) return false;
     const int at = __builtin_ctzll(__ballot(k >= before && k < before + units));
     u.b = at;
     blocks = __builtin_amdgcn_readlane(v, at);
     u.shares = __builtin_amdgcn_readlane(shares, at);
-    const int in = static_cast<int>(k) - __builtin_amdgcn_readlane(before, at);
-    u.share = in / static_cast<int>(blocks);
+    const int in = k - __builtin_amdgcn_readlane(before, at);
+    u.share = in / blocks;
     blk = in - u.share * blocks;
     ordinal = __builtin_amdgcn_readlane(blocks_before, at) + blk;
   } else {
     const int c = share_tiles(p, l, tid);
     const float rc = 1.0f / static_cast<float>(c);
     int64_t total = 0, before, base = 0, blocks_base = 0;
-    for (int64_t i = tid; i < p.B; i += 256) total += static_cast<int64_t>(l.blocks[i]) * shares_of(l.tiles[i], c, rc);
+    for (int i = tid; i < p.B; i += 256) total += l.blocks[i] * shares_of(l.tiles[i], c, rc);
     total = block_scan(total, before, l.scan, tid);
-    const int64_t per_xcd = (total + 7) / 8;
-    k = w % 8 * per_xcd + w / 8;
-    const bool mine = w / 8 < per_xcd && k < total;
+    const int per_xcd = static_cast<int>((total + 7) / 8);
+    k = (w & 7) * per_xcd + (w >> 3);
+    const bool mine = (w >> 3) < per_xcd && k < total;
     if (!mine && w != 0) return false;
-    for (int64_t i = 0; i < p.B; i += 256) {
+    for (int i = 0; i < p.B; i += 256) {
       int shares = 1;
       int64_t n = 0, blocks_before;
       if (i + tid < p.B) {
@@ -327,31 +343,27 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     if (w == 0 && tid == 0) *p.blocks_out = static_cast<int32_t>(blocks_base);
     __syncthreads();
     if (!mine) return false;
-    u.b = l.scan[4];
+    u.b = static_cast<int>(l.scan[4]);
     blocks = l.blocks[u.b];
     u.shares = static_cast<int>(l.scan[6]);
-    u.share = static_cast<int>(l.scan[5] / blocks);
-    blk = l.scan[5] - u.share * blocks;
-    ordinal = l.scan[7] + blk;
+    u.share = static_cast<int>(l.scan[5]) / blocks;
+    blk = static_cast<int>(l.scan[5]) - u.share * blocks;
+    ordinal = static_cast<int>(l.scan[7]) + blk;
   }
-  int64_t a, z;
-  int tiles;
   u.b = uniform(u.b);
-  sequence(p, u.b, a, z, tiles);
+  sequence(p, u.b, a, z, t);
   u.t0 = uniform(a);
-  u.n = uniform(static_cast<int>(z - a));
-  const int64_t per_latent = blocks / p.G;
-  u.g = uniform(static_cast<int>(blk / per_latent));
-  u.r0 = uniform((blk - u.g * per_latent) * p.rows_per_unit);
-  const int64_t rows = static_cast<int64_t>(u.n) * p.HG;
-  u.r1 = u.r0 + p.rows_per_unit < rows ? u.r0 + p.rows_per_unit : rows;
+  u.n = uniform(z - a);
+  u.g = p.G == 1 ? 0 : uniform(blk / blocks);
+  u.r0 = uniform((blk - u.g * blocks) << p.unit_shift);
+  u.r1 = u.r0 + (1 << p.unit_shift) < u.n * p.HG ? u.r0 + (1 << p.unit_shift) : u.n * p.HG;
   u.len = u.n;
   if (p.lens) u.len = uniform(static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page)));
   u.share = uniform(u.share);
   u.shares = uniform(u.shares);
-  u.slot = uniform(static_cast<int>(k));
+  u.slot = uniform(k);
   if (p.slots && u.share == 0 && tid == 0)
-    p.joins[ordinal] = JoinRow{u.t0 * p.H + u.r0, static_cast<int32_t>(u.r1 - u.r0), u.shares, u.slot, static_cast<int32_t>(blocks)};
+    p.joins[ordinal] = JoinRow{static_cast<int64_t>(u.t0) * p.H + u.r0, u.r1 - u.r0, u.shares, u.slot, blocks};
   if (!small) __syncthreads();  // the plan's LDS is free
   return true;
 }
@@ -366,15 +378,15 @@ __device__ __forceinline__ void zero_rows(const RaggedParams& p, int tid) {
   }
 }
 
-// Row r of the unit's sequence: its row of q, out and lse.
-__device__ __forceinline__ int64_t row_at(const RaggedParams& p, const Unit& u, int64_t r) {
-  if (p.G == 1) return u.t0 * p.H + r;
-  const int64_t tok = r / p.HG;
-  return (u.t0 + tok) * p.H + u.g * p.HG + (r - tok * p.HG);
+// Row r of the unit's sequence: its row of q, out and lse, and its head.
+__device__ __forceinline__ int row_at(const RaggedParams& p, const Unit& u, int r, int& head) {
+  const int tok = p.by_heads(r);
+  head = u.g * p.HG + (r - tok * p.HG);
+  return (u.t0 + tok) * p.H + head;
 }
 
 // The positions (or places of the list) that tokens tok0 .. tok1 - 1 of the sequence see.
-__device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u, int64_t tok0, int64_t tok1, int& lo, int& hi) {
+__device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u, int tok0, int tok1, int& lo, int& hi) {
   const int64_t shift = static_cast<int64_t>(u.len) - u.n;  // position of the first new token (negative: tokens that see nothing)
   lo = static_cast<int>(clamp64(shift + tok0 - p.window + 1, 0, u.len));
   hi = static_cast<int>(clamp64(shift + tok1, 0, u.len));
@@ -385,7 +397,7 @@ __device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u
 }
 
 // This unit's share of the tiles that its tokens tok0 .. tok1 - 1 see.
-__device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u, int64_t tok0, int64_t tok1, int& lo, int& hi) {
+__device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u, int tok0, int tok1, int& lo, int& hi) {
   token_range(p, u, tok0, tok1, lo, hi);
   if (u.shares > 1) {
     const int tiles = (hi - lo + kTile - 1) / kTile, per = (tiles + u.shares - 1) / u.shares;
@@ -396,20 +408,21 @@ __device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u,
 }
 
 // The entry at position v of the unit's sequence (or of its list) in a pool; -1: none.
-__device__ __forceinline__ int64_t pool_entry(const RaggedParams& p, const Unit& u, int v) {
+__device__ __forceinline__ int pool_entry(const RaggedParams& p, const Unit& u, int v) {
   if (p.idx) {
     v = p.idx[u.b * p.idx_stride + v];
     if (v < 0 || v >= u.len) return -1;
   }
-  const uint32_t at = static_cast<uint32_t>(v) / static_cast<uint32_t>(p.page);
-  const int64_t pid = p.tables[u.b * p.table_stride + at];
+  const int at = p.by_page(v);
+  const int pid = p.tables[u.b * p.table_stride + at];
   if (pid < 0 || pid >= p.pages) return -1;
-  return pid * p.page + (static_cast<uint32_t>(v) - at * static_cast<uint32_t>(p.page));
+  return pid * p.page + (v - at * p.page);
 }
 
 // The address of the entry at position v; null where there is none.
 __device__ __forceinline__ const uint8_t* entry_of(const RaggedParams& p, const Unit& u, int v, int entry_bytes) {
-  if (p.tables == nullptr) return p.entries + (u.t0 + v) * p.entry_stride + static_cast<int64_t>(u.g) * entry_bytes;
+  if (p.tables == nullptr)
+    return p.entries + (static_cast<int64_t>(u.t0) + v) * p.entry_stride + static_cast<int64_t>(u.g) * entry_bytes;
   const int64_t e = pool_entry(p, u, v);
   return e < 0 ? nullptr : p.entries + e * p.entry_stride;
 }
@@ -468,21 +481,21 @@ ragged_kernel(const RaggedParams p) {
   v8bf qf[KS][2];
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
-    const int64_t rc = r < u.r1 ? r : u.r0;
-    const uint16_t* qr = p.q + row_at(p, u, rc) * D;
+    const int r = u.r0 + 32 * hh + 16 * b + e16;
+    int head;
+    const uint16_t* qr = p.q + static_cast<int64_t>(row_at(p, u, r < u.r1 ? r : u.r0, head)) * D;
 #pragma unroll
     for (int st = 0; st < KS; ++st)
       qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(qr + 32 * st + 8 * g));
   }
 
-  const int64_t tok0 = u.r0 / p.HG, tok1 = (u.r1 - 1) / p.HG + 1;
+  const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
   const int64_t shift = static_cast<int64_t>(u.len) - u.n;
   int share_lo, share_hi;
   unit_range(p, u, tok0, tok1, share_lo, share_hi);
   // one pass over all rows; if something in it is not finite, one pass for each token over what it sees
   // itself, since a weight of 0 times an entry hidden from a row would not be 0
-  int64_t sub0 = tok0, sub1 = tok1;
+  int sub0 = tok0, sub1 = tok1;
   bool strict = false;
   while (true) {
     int lo, hi;
@@ -492,8 +505,8 @@ ragged_kernel(const RaggedParams p) {
     int64_t row_lo[2], row_hi[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
-      const int64_t pos = shift + (r < u.r1 ? r : u.r0) / p.HG;
+      const int r = u.r0 + 32 * hh + 16 * b + e16;
+      const int64_t pos = shift + p.by_heads(r < u.r1 ? r : u.r0);
       row_lo[b] = p.idx ? 0 : pos - p.window + 1;
       row_hi[b] = p.idx ? hi : pos + 1;
     }
@@ -618,22 +631,23 @@ ragged_kernel(const RaggedParams p) {
     }
 #pragma unroll
     for (int hg = 0; hg < 4; ++hg) {
-      const int64_t r = u.r0 + 16 * hg + e16;
-      const int64_t tok = r / p.HG;
+      const int r = u.r0 + 16 * hg + e16;
+      const int tok = p.by_heads(r);
       if (r >= u.r1 || tok < sub0 || tok >= sub1) continue;
       if (u.shares > 1) {
         const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? 1.0f / l4[hg] : 0.0f;
-        float* const o = p.part_o + (static_cast<int64_t>(u.slot) * 64 + 16 * hg + e16) * D;
+        float* const o = p.part_o + static_cast<int64_t>(u.slot) * 64 * D + 16 * (16 * hg + e16) + 4 * g;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-          if (wave + 4 * i < NB) *reinterpret_cast<v4f*>(o + 16 * (wave + 4 * i) + 4 * g) = acc[i][hg] * inv;
+          if (wave + 4 * i < NB) *reinterpret_cast<v4f*>(o + 1024 * (wave + 4 * i)) = acc[i][hg] * inv;
         if (wave == hg && g == 0)
           *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + 16 * hg + e16)) = float2{m4[hg], l4[hg]};
         continue;
       }
-      const int64_t at = row_at(p, u, r);
+      int head;
+      const int64_t at = row_at(p, u, r, head);
       float lse;
-      const float scale = finish_row(p, static_cast<int>(at % p.H), m4[hg], l4[hg], lse);
+      const float scale = finish_row(p, head, m4[hg], l4[hg], lse);
       uint16_t* const o = p.out + at * D;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -653,37 +667,29 @@ ragged_kernel(const RaggedParams p) {
 
 #include "ragged_wide.h"
 
-// Joins the shares of a row block's rows, ROWS of them a workgroup, 4 channels a thread.
-// o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the sink.
-// Bound by latency for a few rows (record, then maxima and sums, then the shares' rows, all
+// Joins the shares of 16 rows of a row block: o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the
+// sink.  A wave takes one 16-channel block, so that a load instruction covers 1 KB of a share.
+// Bound by latency for a few rows (record, then maxima and sums, then the shares' rows, eight of them
 // requested together) and by the memory for many.
 template <int D>
-struct JoinShape {
-  static constexpr int PIECES = D / 4;
-  static constexpr int ROWS = 256 / PIECES;                       // a workgroup's rows
-  static constexpr int THREADS = (ROWS * PIECES + 63) / 64 * 64;  // (one row of 576 channels in 192 threads)
-};
-
-template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
-  using J = JoinShape<D>;
-  constexpr int PIECES = J::PIECES, ROWS = J::ROWS, PER = (64 + ROWS - 1) / ROWS;
-  __shared__ float weight[ROWS][kMaxShares];
+  constexpr int NB = D / 16;
+  __shared__ float weight[16][kMaxShares + 1];
   const int tid = threadIdx.x;
-  const int k = blockIdx.x / PER, r0 = (blockIdx.x - k * PER) * ROWS;
+  const int k = blockIdx.x >> 2, r0 = 16 * (blockIdx.x & 3);
   if (k >= *p.blocks_out) return;
   const JoinRow j = p.joins[k];
   if (j.shares <= 1 || r0 >= j.rows) return;
   {  // weights: 16 threads a row
-    static_assert(ROWS * 16 <= 256 && J::THREADS >= ROWS * 16, "weights");
     const int r = tid >> 4, row = r0 + r;
-    if (r < ROWS && row < j.rows) {
-      const float* const ml = p.part_ml + 2 * (static_cast<int64_t>(j.slot0) * 64 + row);
-      const int64_t step = 128ll * j.step;
-      float m = -__builtin_huge_valf(), l = 0.0f;
+    const float* const ml = p.part_ml + 2 * (static_cast<int64_t>(j.slot0) * 64 + row);
+    const int64_t step = 128ll * j.step;
+    float m = -__builtin_huge_valf(), l = 0.0f;
+    if (row < j.rows)
       for (int s = tid & 15; s < j.shares; s += 16) m = fmaxf(m, ml[step * s]);
 #pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int d = 8; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (row < j.rows)
       for (int s = tid & 15; s < j.shares; s += 16) {
         const float2 v = *reinterpret_cast<const float2*>(ml + step * s);
         // a share that saw nothing has l 0 and m -inf, one with a NaN has l NaN
@@ -692,18 +698,19 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
         l += w;
       }
 #pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) l += __shfl_xor(l, d, 64);
+    for (int d = 8; d >= 1; d >>= 1) l += __shfl_xor(l, d, 64);
+    if (row < j.rows) {
       const int64_t at = j.row0 + row;
       float lse;
       const float scale = finish_row(p, static_cast<int>(at % p.H), m, l, lse);
-      if ((tid & 15) == 0) p.lse[at] = lse;
+      if ((tid & 15) == 0 && blockIdx.y == 0) p.lse[at] = lse;
       for (int s = tid & 15; s < j.shares; s += 16) weight[r][s] *= scale;
     }
   }
   __syncthreads();
-  const int r = tid / PIECES, c = 4 * (tid - r * PIECES), row = r0 + r;
-  if (r >= ROWS || row >= j.rows) return;
-  const float* const o = p.part_o + (static_cast<int64_t>(j.slot0) * 64 + row) * D + c;
+  const int r = (tid & 63) >> 2, c = 4 * (tid & 3), row = r0 + r, blk = 4 * blockIdx.y + (tid >> 6);
+  if (row >= j.rows || blk >= NB) return;
+  const float* const o = p.part_o + (static_cast<int64_t>(j.slot0) * NB + blk) * 1024 + 16 * row + c;
   const int64_t step = 64ll * D * j.step;
   v4f sum = v4f{};
   constexpr int AHEAD = 8;
@@ -719,7 +726,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
         for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[s][i], sum[i]);
       }
   }
-  *reinterpret_cast<uint2*>(p.out + (j.row0 + row) * D + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
+  *reinterpret_cast<uint2*>(p.out + (j.row0 + row) * D + 16 * blk + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
 }
 
 template <int FMT, int D, int NOPE>
@@ -747,10 +754,7 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   } else {
     ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, RaggedLds<FMT, D, NOPE>::LDS, s>>>(p);
   }
-  if (p.slots) {
-    using J = JoinShape<D>;
-    join_kernel<D><<<static_cast<unsigned>((64 + J::ROWS - 1) / J::ROWS * p.blocks_max), J::THREADS, 0, s>>>(p);
-  }
+  if (p.slots) join_kernel<D><<<dim3(static_cast<unsigned>(4 * p.blocks_max), (D / 16 + 3) / 4), 256, 0, s>>>(p);
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;
 }
@@ -776,10 +780,14 @@ int dispatch_ragged(const char* name, int fmt, int nope, const RaggedParams& p, 
   }
 }
 
-// Units of rows_per_unit rows in the grid: at most this many, whatever the lengths are.
-int64_t unit_bound(const RaggedParams& p) {
-  const int64_t per = (static_cast<int64_t>(p.HG) + p.rows_per_unit - 1) / p.rows_per_unit;
-  return p.cu == nullptr ? p.B * p.G * per : (p.T * p.HG / p.rows_per_unit + (p.B < p.T ? p.B : p.T)) * p.G;
+// The divisions and the row blocks of a call: at most blocks_max, whatever the lengths are.
+void set_units(RaggedParams& p) {
+  p.unit_shift = p.HG == 1 ? 5 : 6;
+  const int64_t per = (static_cast<int64_t>(p.HG) + (1 << p.unit_shift) - 1) >> p.unit_shift;
+  p.blocks_max = p.cu == nullptr ? p.B * p.G * per : ((p.T * p.HG >> p.unit_shift) + (p.B < p.T ? p.B : p.T)) * p.G;
+  p.by_heads = fast_div(static_cast<uint32_t>(p.HG));
+  p.by_page = fast_div(static_cast<uint32_t>(p.page < 1 ? 1 : p.page));
+  p.by_blocks = fast_div(static_cast<uint32_t>(p.G * per));
 }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
@@ -850,12 +858,11 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.window = window ? window : kNoWindow;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
-  p.rows_per_unit = 32 * p.HG < 64 ? 32 * p.HG : 64;
-  p.blocks_max = unit_bound(p);
+  set_units(p);
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt - 16, "paged_attend: too many rows");
+  MZK_CHECK_ARG(p.blocks_max <= kMaxInt / 64 && T * H <= kMaxInt - 64, "paged_attend: too many rows");
   const int64_t need = attend_bytes(p.blocks_max, B, D);
   MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attend: workspace needs %lld bytes",
                 (long long)need);
@@ -884,10 +891,10 @@ extern "C" int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int pac
   p.HG = H;
   p.G = 1;
   p.B = B;
-  p.rows_per_unit = 32 * H < 64 ? 32 * H : 64;
   const int64_t some = 0;
   p.cu = packed ? &some : nullptr;  // only whether there is one counts
-  *bytes = attend_bytes(unit_bound(p), B, D);
+  set_units(p);
+  *bytes = attend_bytes(p.blocks_max, B, D);
   return MZK_OK;
 }
 
@@ -917,11 +924,10 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   p.window = window ? window : kNoWindow;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
-  p.rows_per_unit = 32 * p.HG < 64 ? 32 * p.HG : 64;
-  p.blocks_max = unit_bound(p);
+  set_units(p);
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt - 16, "packed_mqa: too many rows");
+  MZK_CHECK_ARG(p.blocks_max <= kMaxInt / 64 && T * H <= kMaxInt - 64, "packed_mqa: too many rows");
   return dispatch_ragged("packed_mqa", kFmtBf16, D, p, as_stream(stream));
 }

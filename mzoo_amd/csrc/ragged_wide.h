@@ -98,33 +98,32 @@ ragged_wide_kernel(const RaggedParams p) {
 
   // q: the B operand of S^T (rows 32 hh + 16 b + e16, channels 32 st + 8 g ..) through LDS, from
   // whole lines
-  const int rows = static_cast<int>(u.r1 - u.r0);
+  const int rows = u.r1 - u.r0;
   constexpr int QROW = D / 8, QP = 64 * QROW / NT;
   u32x4 qraw[QP];
-  if (p.G == 1) {  // one run of rows
-    const u32x4* const qb = reinterpret_cast<const u32x4*>(p.q + (u.t0 * p.H + u.r0) * D);
+  if (p.G == 1 && rows == 64) {  // one run of rows
+    const u32x4* const qb = reinterpret_cast<const u32x4*>(p.q + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
 #pragma unroll
-    for (int k = 0; k < QP; ++k) {
-      const int at = tid + NT * k;
-      qraw[k] = qb[at < rows * QROW ? at : 0];
-    }
+    for (int k = 0; k < QP; ++k) qraw[k] = (qb + NT * k)[tid];
   } else {
 #pragma unroll
     for (int k = 0; k < QP; ++k) {
       const int at = tid + NT * k;
       const int r = at / QROW;
-      qraw[k] = *reinterpret_cast<const u32x4*>(p.q + row_at(p, u, u.r0 + (r < rows ? r : 0)) * D + 8 * (at - r * QROW));
+      int head;
+      qraw[k] = *reinterpret_cast<const u32x4*>(
+          p.q + static_cast<int64_t>(row_at(p, u, u.r0 + (r < rows ? r : 0), head)) * D + 8 * (at - r * QROW));
     }
   }
-  const int64_t tok0 = u.r0 / p.HG, tok1 = (u.r1 - 1) / p.HG + 1;
+  const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
   const int shift = u.len - u.n;
   int share_lo, share_hi;
   unit_range(p, u, tok0, tok1, share_lo, share_hi);
   int tok_b[2];  // the tokens of this lane's rows
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const int64_t r = u.r0 + 32 * hh + 16 * b + e16;
-    tok_b[b] = static_cast<int>((r < u.r1 ? r : u.r0) / p.HG);
+    const int r = u.r0 + 32 * hh + 16 * b + e16;
+    tok_b[b] = p.by_heads(r < u.r1 ? r : u.r0);
   }
   const int64_t win = p.window < 0x7fffffff ? p.window : 0x7fffffff;
 
@@ -223,8 +222,7 @@ ragged_wide_kernel(const RaggedParams p) {
       const int e = e0 + tid;
       uint32_t code = kEmpty;
       if (e < nt * kTile && e < left) {
-        const int64_t at = pool_entry(p, u, lo + c0 + e);
-        if (at >= 0) code = static_cast<uint32_t>(at);
+        code = static_cast<uint32_t>(pool_entry(p, u, lo + c0 + e));  // -1: kEmpty
       }
       const uint64_t bal = __ballot(code != kEmpty);
       if (e < n_tab) {
@@ -508,7 +506,7 @@ ragged_wide_kernel(const RaggedParams p) {
   };
 
   // the entries that tokens sub0 .. sub1 - 1 see of this unit's share, and what the rows see of them
-  int64_t sub0 = tok0, sub1 = tok1;
+  int sub0 = tok0, sub1 = tok1;
   auto set_range = [&]() __attribute__((always_inline)) {
     token_range(p, u, sub0, sub1, lo, hi);
     lo = lo > share_lo ? lo : share_lo;
@@ -678,18 +676,21 @@ ragged_wide_kernel(const RaggedParams p) {
       l4[hg] = __builtin_amdgcn_ldexpf(l4[hg], -e4[hg]);
       m4[hg] = l4[hg] == 0.0f ? -__builtin_huge_valf() : m4[hg] + static_cast<float>(e4[hg]);
     }
+    // (an address that depends on nothing in the passes would be computed before them, and kept in memory)
+    int col = e16;
+    asm volatile("" : "+v"(col));
     // ---- the result: acc[i][hg][r] is row 16 hg + e16, channel 16 (wave + 4 i) + 4 g + r ------------
-    const int keep0 = static_cast<int>((sub0 * p.HG > u.r0 ? sub0 * p.HG : u.r0) - u.r0);
-    const int keep1 = static_cast<int>((sub1 * p.HG < u.r1 ? sub1 * p.HG : u.r1) - u.r0);
+    const int keep0 = (sub0 * p.HG > u.r0 ? sub0 * p.HG : u.r0) - u.r0;
+    const int keep1 = (sub1 * p.HG < u.r1 ? sub1 * p.HG : u.r1) - u.r0;
     if (u.shares > 1) {
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) {
-        const int r = 16 * hg + e16;
+        const int r = 16 * hg + col;
         if (r >= keep0 && r < keep1) {
           const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? __builtin_amdgcn_ldexpf(1.0f / l4[hg], -e4[hg]) : 0.0f;
-          float* const o = p.part_o + (static_cast<int64_t>(u.slot) * 64 + r) * D + 16 * wave + 4 * g;
+          float* o = p.part_o + static_cast<int64_t>(u.slot) * 64 * D + 1024 * wave + 16 * r + 4 * g;
 #pragma unroll
-          for (int i = 0; i < NI; ++i) *reinterpret_cast<v4f*>(o + 64 * i) = acc[i][hg] * inv;
+          for (int i = 0; i < NI; ++i, o += 4096) *reinterpret_cast<v4f*>(o) = acc[i][hg] * inv;
           if (wave == hg && g == 0)
             *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + r)) = float2{m4[hg], l4[hg]};
         }
@@ -699,11 +700,12 @@ ragged_wide_kernel(const RaggedParams p) {
       constexpr int OPITCH = 2 * D + 16;
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) {
-        const int r = 16 * hg + e16;
+        const int r = 16 * hg + col;
         if (r >= keep0 && r < keep1) {
-          const int64_t at = row_at(p, u, u.r0 + r);
+          int head;
+          const int at = row_at(p, u, u.r0 + r, head);
           float lse;
-          const float scale = __builtin_amdgcn_ldexpf(finish_row(p, static_cast<int>(at % p.H), m4[hg], l4[hg], lse), -e4[hg]);
+          const float scale = __builtin_amdgcn_ldexpf(finish_row(p, head, m4[hg], l4[hg], lse), -e4[hg]);
           uint8_t* const orow = smem + r * OPITCH + 32 * wave + 8 * g;
 #pragma unroll
           for (int i = 0; i < NI; ++i)
@@ -713,10 +715,12 @@ ragged_wide_kernel(const RaggedParams p) {
         }
       }
       lds_barrier();
+#pragma unroll 1
       for (int at = tid; at < 64 * QROW; at += NT) {
         const int r = at / QROW;
+        int head;
         if (r >= keep0 && r < keep1)
-          *reinterpret_cast<u32x4*>(p.out + row_at(p, u, u.r0 + r) * D + 8 * (at - r * QROW)) =
+          *reinterpret_cast<u32x4*>(p.out + static_cast<int64_t>(row_at(p, u, u.r0 + r, head)) * D + 8 * (at - r * QROW)) =
               *reinterpret_cast<const u32x4*>(smem + r * OPITCH + 16 * (at - r * QROW));
       }
     }
