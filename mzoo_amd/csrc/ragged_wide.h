@@ -635,8 +635,7 @@ ragged_wide_kernel(const RaggedParams p) {
       lds_barrier();
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) l4[hg] = lsum[16 * hg + e16] + lsum[64 + 16 * hg + e16];
-      const bool several = !strict && tok1 - tok0 > 1;
-      if (__builtin_expect((!given && *high != 0) || several, 0)) {  // uniform
+      if (__builtin_expect(!given && *high != 0, 0)) {  // uniform
         // O^T through the tiles' place, half of it at a time, each lane its own: a few stores and a
         // short loop
         float any_bad = 0.0f;  // NaN if an accumulator is not finite
@@ -653,21 +652,11 @@ ragged_wide_kernel(const RaggedParams p) {
             for (int r = 0; r < 4; ++r) any_bad = __builtin_fmaf(x[r], 0.0f, any_bad);
           }
         }
-        if (any_bad != 0.0f) {
-          if (!given) *redo = 1;
-          *odd = 1;
-        }
+        if (any_bad != 0.0f) *redo = 1;
         lds_barrier();
       }
       if (given || *redo == 0) break;  // uniform: set before the barrier above
       lds_barrier();
-    }
-    if (!strict && tok1 - tok0 > 1 && *odd != 0) {  // uniform
-      strict = true;
-      sub0 = tok0;
-      sub1 = tok0 + 1;
-      lds_barrier();
-      continue;
     }
     // (m, l) with l in [1, 2): the reference is not the maximum, so l may be far from 1
 #pragma unroll
@@ -680,6 +669,9 @@ ragged_wide_kernel(const RaggedParams p) {
     int col = e16;
     asm volatile("" : "+v"(col));
     // ---- the result: acc[i][hg][r] is row 16 hg + e16, channel 16 (wave + 4 i) + 4 g + r ------------
+    // A unit of several tokens whose result is not finite is looked at again, token by token: its rows
+    // are written here and once more then.
+    float bad = 0.0f;  // NaN if a result is not finite
     const int keep0 = (sub0 * p.HG > u.r0 ? sub0 * p.HG : u.r0) - u.r0;
     const int keep1 = (sub1 * p.HG < u.r1 ? sub1 * p.HG : u.r1) - u.r0;
     if (u.shares > 1) {
@@ -690,11 +682,18 @@ ragged_wide_kernel(const RaggedParams p) {
           const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? __builtin_amdgcn_ldexpf(1.0f / l4[hg], -e4[hg]) : 0.0f;
           float* o = p.part_o + static_cast<int64_t>(u.slot) * 64 * D + 1024 * wave + 16 * r + 4 * g;
 #pragma unroll
-          for (int i = 0; i < NI; ++i, o += 4096) *reinterpret_cast<v4f*>(o) = acc[i][hg] * inv;
+          for (int i = 0; i < NI; ++i, o += 4096) {
+            const v4f x = acc[i][hg] * inv;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bad = __builtin_fmaf(x[c], 0.0f, bad);
+            *reinterpret_cast<v4f*>(o) = x;
+          }
           if (wave == hg && g == 0)
             *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + r)) = float2{m4[hg], l4[hg]};
         }
       }
+      if (bad != 0.0f) *odd = 1;
+      lds_barrier();
     } else {
       // through LDS, so that the rows leave in whole lines
       constexpr int OPITCH = 2 * D + 16;
@@ -708,21 +707,43 @@ ragged_wide_kernel(const RaggedParams p) {
           const float scale = __builtin_amdgcn_ldexpf(finish_row(p, head, m4[hg], l4[hg], lse), -e4[hg]);
           uint8_t* const orow = smem + r * OPITCH + 32 * wave + 8 * g;
 #pragma unroll
-          for (int i = 0; i < NI; ++i)
-            *reinterpret_cast<uint2*>(orow + 128 * i) = uint2{pack_bf16x2(acc[i][hg][0] * scale, acc[i][hg][1] * scale),
-                                                              pack_bf16x2(acc[i][hg][2] * scale, acc[i][hg][3] * scale)};
+          for (int i = 0; i < NI; ++i) {
+            const v4f x = acc[i][hg] * scale;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bad = __builtin_fmaf(x[c], 0.0f, bad);
+            *reinterpret_cast<uint2*>(orow + 128 * i) = uint2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+          }
           if (wave == hg && g == 0) p.lse[at] = lse;
         }
       }
+      if (bad != 0.0f) *odd = 1;
       lds_barrier();
+      if (p.G == 1 && keep0 == 0 && keep1 == 64) {  // one run of rows
+        u32x4* const ob = reinterpret_cast<u32x4*>(p.out + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
+        int mine = tid;
+        asm volatile("" : "+v"(mine));
+#pragma unroll
+        for (int k = 0; k < QP; ++k) {
+          const int at = mine + NT * k;
+          (ob + NT * k)[mine] = *reinterpret_cast<const u32x4*>(smem + 16 * at + (OPITCH - 2 * D) * (at / QROW));
+        }
+      } else {
 #pragma unroll 1
-      for (int at = tid; at < 64 * QROW; at += NT) {
-        const int r = at / QROW;
-        int head;
-        if (r >= keep0 && r < keep1)
-          *reinterpret_cast<u32x4*>(p.out + static_cast<int64_t>(row_at(p, u, u.r0 + r, head)) * D + 8 * (at - r * QROW)) =
-              *reinterpret_cast<const u32x4*>(smem + r * OPITCH + 16 * (at - r * QROW));
+        for (int at = tid; at < 64 * QROW; at += NT) {
+          const int r = at / QROW;
+          int head;
+          if (r >= keep0 && r < keep1)
+            *reinterpret_cast<u32x4*>(p.out + static_cast<int64_t>(row_at(p, u, u.r0 + r, head)) * D + 8 * (at - r * QROW)) =
+                *reinterpret_cast<const u32x4*>(smem + r * OPITCH + 16 * (at - r * QROW));
+        }
       }
+    }
+    if (!strict && tok1 - tok0 > 1 && *odd != 0) {  // uniform: set before the barrier above
+      strict = true;
+      sub0 = tok0;
+      sub1 = tok0 + 1;
+      lds_barrier();
+      continue;
     }
     if (!strict || sub1 >= tok1) break;
     ++sub0;
