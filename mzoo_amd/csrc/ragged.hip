@@ -10,6 +10,8 @@
 // innermost, so 64 rows are 64 heads of a token or all heads of several -- over all of the
 // sequence's entries, or, where there are fewer blocks than compute units, over a share of them;
 // the shares' results are joined by a second launch.
+#include <type_traits>
+
 #include "common.h"
 #include "entries.h"
 
@@ -419,14 +421,6 @@ __device__ __forceinline__ int pool_entry(const RaggedParams& p, const Unit& u, 
   return pid * p.page + (v - at * p.page);
 }
 
-// The address of the entry at position v; null where there is none.
-__device__ __forceinline__ const uint8_t* entry_of(const RaggedParams& p, const Unit& u, int v, int entry_bytes) {
-  if (p.tables == nullptr)
-    return p.entries + (static_cast<int64_t>(u.t0) + v) * p.entry_stride + static_cast<int64_t>(u.g) * entry_bytes;
-  const int64_t e = pool_entry(p, u, v);
-  return e < 0 ? nullptr : p.entries + e * p.entry_stride;
-}
-
 // A row's result from its maximum, sum and sink: the factor of O^T and the log-sum-exp.
 __device__ __forceinline__ float finish_row(const RaggedParams& p, int head, float m, float l, float& lse) {
   const bool none = l == 0.0f && m == -__builtin_huge_valf();  // it sees nothing: lse is the sink itself
@@ -445,227 +439,11 @@ __device__ __forceinline__ float finish_row(const RaggedParams& p, int head, flo
   return scale;
 }
 
-template <int FMT, int D, int NOPE>
-struct RaggedLds {
-  static constexpr int PITCH = 2 * D + 16;
-  static constexpr int PB = kTile * PITCH;
-  static constexpr int PMAX = PB + 4096;  // [2][64]
-  static constexpr int LSUM = PMAX + 512;
-  static constexpr int OKS = LSUM + 512;  // [32] words
-  static constexpr int LDS = OKS + 128 > static_cast<int>(sizeof(PlanLds)) ? OKS + 128 : static_cast<int>(sizeof(PlanLds));
-};
-
-// A tile of 32 entries at a time: bf16 rows in LDS, S^T by matrix instructions (each wave 16 entries x
-// 32 rows), the softmax's running maximum, P^T through LDS, O^T by matrix instructions (each wave
-// every fourth block of 16 channels x 64 rows).  Entries that are not there are rows of zeros.
-template <int FMT, int D, int NOPE>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
-ragged_kernel(const RaggedParams p) {
-  using M = RaggedLds<FMT, D, NOPE>;
-  using L = Layout<FMT, D, NOPE>;
-  constexpr int KS = D / 32, NB = D / 16, NI = (NB + 3) / 4;
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t* const pbuf = smem + M::PB;
-  float* const pmax = reinterpret_cast<float*>(smem + M::PMAX);
-  float* const lsum = reinterpret_cast<float*>(smem + M::LSUM);
-  int* const oks = reinterpret_cast<int*>(smem + M::OKS);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int eh = wave & 1, hh = wave >> 1, g = lane >> 4, e16 = lane & 15;
-
-  Unit u;
-  zero_rows(p, tid);
-  if (!find_unit(p, u, smem, tid)) return;  // uniform
-
-  // the B operand of S^T: rows 32 hh + 16 b + e16, channels 32 st + 8 g ..
-  v8bf qf[KS][2];
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int r = u.r0 + 32 * hh + 16 * b + e16;
-    int head;
-    const uint16_t* qr = p.q + static_cast<int64_t>(row_at(p, u, r < u.r1 ? r : u.r0, head)) * D;
-#pragma unroll
-    for (int st = 0; st < KS; ++st)
-      qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(qr + 32 * st + 8 * g));
-  }
-
-  const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
-  const int64_t shift = static_cast<int64_t>(u.len) - u.n;
-  int share_lo, share_hi;
-  unit_range(p, u, tok0, tok1, share_lo, share_hi);
-  // one pass over all rows; if something in it is not finite, one pass for each token over what it sees
-  // itself, since a weight of 0 times an entry hidden from a row would not be 0
-  int sub0 = tok0, sub1 = tok1;
-  bool strict = false;
-  while (true) {
-    int lo, hi;
-    token_range(p, u, sub0, sub1, lo, hi);
-    lo = lo > share_lo ? lo : share_lo;
-    hi = hi < share_hi ? hi : share_hi;
-    int64_t row_lo[2], row_hi[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int r = u.r0 + 32 * hh + 16 * b + e16;
-      const int64_t pos = shift + p.by_heads(r < u.r1 ? r : u.r0);
-      row_lo[b] = p.idx ? 0 : pos - p.window + 1;
-      row_hi[b] = p.idx ? hi : pos + 1;
-    }
-    float m_own[2] = {-__builtin_huge_valf(), -__builtin_huge_valf()}, l_own[2] = {0.0f, 0.0f};
-    float m4[4];
-    v4f acc[NI][4];
-#pragma unroll
-    for (int hg = 0; hg < 4; ++hg) {
-      m4[hg] = -__builtin_huge_valf();
-#pragma unroll
-      for (int i = 0; i < NI; ++i) acc[i][hg] = v4f{};
-    }
-    const int te = tid >> 3, tj = tid & 7;
-    for (int v0 = lo; v0 < hi; v0 += kTile) {
-      const uint8_t* const e = v0 + te < hi ? entry_of(p, u, v0 + te, L::kEntryBytes) : nullptr;
-      for (int q = tj; q < L::kPieces; q += 8) {
-        if (e) {
-          store_piece<FMT, D, NOPE>(smem + te * M::PITCH, fetch_piece<FMT, D, NOPE>((gptr_t)e, q), q);
-        } else {
-          Piece z{};
-          store_piece<FMT, D, NOPE>(smem + te * M::PITCH, z, q);
-        }
-      }
-      if (tj == 0) oks[te] = e != nullptr;
-      __syncthreads();
-      v4f s[2] = {v4f{}, v4f{}};
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const v8bf kf = __builtin_bit_cast(
-            v8bf, *reinterpret_cast<const v4i*>(smem + (16 * eh + e16) * M::PITCH + 64 * st + 16 * g));
-        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][0], s[0], 0, 0, 0);
-        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][1], s[1], 0, 0, 0);
-      }
-      float v[2][4], t[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        t[b] = -__builtin_huge_valf();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int at = 16 * eh + 4 * g + r;
-          const bool in = oks[at] != 0 && v0 + at >= row_lo[b] && v0 + at < row_hi[b];
-          v[b][r] = in ? s[b][r] * p.scale_log2 : -__builtin_huge_valf();
-          t[b] = fmaxf(t[b], v[b][r]);
-        }
-        t[b] = fmaxf(t[b], __shfl_xor(t[b], 16, 64));
-        t[b] = fmaxf(t[b], __shfl_xor(t[b], 32, 64));
-        if (g == 0) pmax[eh * 64 + 32 * hh + 16 * b + e16] = t[b];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int hg = 0; hg < 4; ++hg) {
-        const float mn = fmaxf(m4[hg], fmaxf(pmax[16 * hg + e16], pmax[64 + 16 * hg + e16]));
-        const float a = m4[hg] == -__builtin_huge_valf() ? 0.0f : exp2f(m4[hg] - mn);
-        m4[hg] = mn;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][hg][r] *= a;
-      }
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int row = 32 * hh + 16 * b + e16;
-        const float mn = fmaxf(m_own[b], fmaxf(pmax[row], pmax[64 + row]));
-        const float a = m_own[b] == -__builtin_huge_valf() ? 0.0f : exp2f(m_own[b] - mn);
-        m_own[b] = mn;
-        const float ref = mn == -__builtin_huge_valf() ? 0.0f : mn;
-        float w[4], sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          w[r] = exp2f(v[b][r] - ref);
-          sum += w[r];
-        }
-        l_own[b] = l_own[b] * a + sum;
-        *reinterpret_cast<uint2*>(pbuf + 2048 * hh + 1024 * b + 16 * lane + 8 * eh) =
-            uint2{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
-      }
-      __syncthreads();
-#pragma unroll
-      for (int hg = 0; hg < 4; ++hg) {
-        const v8bf pf = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(pbuf + 1024 * hg + 16 * lane));
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          if (wave + 4 * i < NB) {
-            const uint8_t* tp = smem + (4 * g + (e16 >> 2)) * M::PITCH + 32 * (wave + 4 * i) + 8 * (e16 & 3);
-            const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp));
-            const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp + 16 * M::PITCH));
-            const v8bf vf = __builtin_bit_cast(v8bf, v8s{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
-            acc[i][hg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, acc[i][hg], 0, 0, 0);
-          }
-        }
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      l_own[b] += __shfl_xor(l_own[b], 16, 64);
-      l_own[b] += __shfl_xor(l_own[b], 32, 64);
-      if (g == 0) lsum[eh * 64 + 32 * hh + 16 * b + e16] = l_own[b];
-    }
-    if (tid == 0) oks[0] = 0;
-    __syncthreads();
-    float l4[4];
-    float bad = 0.0f;
-#pragma unroll
-    for (int hg = 0; hg < 4; ++hg) {
-      l4[hg] = lsum[16 * hg + e16] + lsum[64 + 16 * hg + e16];
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(acc[i][hg][r], 0.0f, bad);
-    }
-    if (!strict && tok1 - tok0 > 1) {
-      if (bad != 0.0f) oks[0] = 1;
-      __syncthreads();
-      if (oks[0]) {  // uniform
-        strict = true;
-        sub0 = tok0;
-        sub1 = tok0 + 1;
-        __syncthreads();
-        continue;
-      }
-    }
-#pragma unroll
-    for (int hg = 0; hg < 4; ++hg) {
-      const int r = u.r0 + 16 * hg + e16;
-      const int tok = p.by_heads(r);
-      if (r >= u.r1 || tok < sub0 || tok >= sub1) continue;
-      if (u.shares > 1) {
-        const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? 1.0f / l4[hg] : 0.0f;
-        float* const o = p.part_o + static_cast<int64_t>(u.slot) * 64 * D + 16 * (16 * hg + e16) + 4 * g;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (wave + 4 * i < NB) *reinterpret_cast<v4f*>(o + 1024 * (wave + 4 * i)) = acc[i][hg] * inv;
-        if (wave == hg && g == 0)
-          *reinterpret_cast<float2*>(p.part_ml + 2 * (static_cast<int64_t>(u.slot) * 64 + 16 * hg + e16)) = float2{m4[hg], l4[hg]};
-        continue;
-      }
-      int head;
-      const int64_t at = row_at(p, u, r, head);
-      float lse;
-      const float scale = finish_row(p, head, m4[hg], l4[hg], lse);
-      uint16_t* const o = p.out + at * D;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = 16 * (wave + 4 * i) + 4 * g;
-        if (wave + 4 * i < NB)
-          *reinterpret_cast<uint2*>(o + c) = uint2{pack_bf16x2(acc[i][hg][0] * scale, acc[i][hg][1] * scale),
-                                                   pack_bf16x2(acc[i][hg][2] * scale, acc[i][hg][3] * scale)};
-      }
-      if (wave == hg && g == 0) p.lse[at] = lse;
-    }
-    if (!strict || sub1 >= tok1) break;
-    ++sub0;
-    ++sub1;
-    __syncthreads();
-  }
-}
+constexpr float kRoomHigh = 8.0f, kRoomAbove = 100.0f, kRoomBelow = -40.0f;  // log2 units from a row's reference
+constexpr float kHidden = -3.0e38f;  // a hidden entry's score: weight 0
 
 #include "ragged_wide.h"
+#include "ragged_narrow.h"
 
 // Joins the shares of 16 rows of a row block: o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the
 // sink.  A wave takes one 16-channel block, so that a load instruction covers 1 KB of a share.
@@ -733,27 +511,25 @@ template <int FMT, int D, int NOPE>
 int launch_ragged(const RaggedParams& p, hipStream_t s) {
   // (find_unit's order takes 16 workgroups at a time)
   const int64_t grid = p.slots ? p.slots : (p.blocks_max + 15) / 16 * 16;
-  if constexpr (D >= 512) {
-    using M = WideLds<FMT, D>;
-    auto kern = ragged_wide_kernel<FMT, D, NOPE>;
-    // the dynamic-LDS limit is a per-device function attribute: set once per device
-    static std::atomic<bool> attr_set[kMaxDevices] = {};  // setting it twice is harmless
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
-      set_last_error("ragged attention: no usable current device");
+  using M = std::conditional_t<(D > 256), WideLds<FMT, D>, NarrowLds<FMT, D>>;
+  void (*kern)(const RaggedParams);
+  if constexpr (D > 256) kern = ragged_wide_kernel<FMT, D, NOPE>;
+  else kern = ragged_narrow_kernel<FMT, D, NOPE>;
+  // the dynamic-LDS limit is a per-device function attribute: set once per device
+  static std::atomic<bool> attr_set[kMaxDevices] = {};  // setting it twice is harmless
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
+    set_last_error("ragged attention: no usable current device");
+    return MZK_ELAUNCH;
+  }
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, M::LDS) != hipSuccess) {
+      set_last_error("ragged attention: cannot raise the kernel's LDS limit to %d bytes", M::LDS);
       return MZK_ELAUNCH;
     }
-    if (!attr_set[dev].load(std::memory_order_acquire)) {
-      if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, M::LDS) != hipSuccess) {
-        set_last_error("ragged attention: cannot raise the kernel's LDS limit to %d bytes", M::LDS);
-        return MZK_ELAUNCH;
-      }
-      attr_set[dev].store(true, std::memory_order_release);
-    }
-    kern<<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
-  } else {
-    ragged_kernel<FMT, D, NOPE><<<static_cast<unsigned>(grid), 256, RaggedLds<FMT, D, NOPE>::LDS, s>>>(p);
+    attr_set[dev].store(true, std::memory_order_release);
   }
+  kern<<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
   if (p.slots) join_kernel<D><<<dim3(static_cast<unsigned>(4 * p.blocks_max), (D / 16 + 3) / 4), 256, 0, s>>>(p);
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;

@@ -19,7 +19,7 @@
 //
 // Softmax: the exponent's reference of a row is its maximum over the first tile (0 where it sees
 // none of that): softmax is exact for any reference as long as nothing overflows or underflows.  A
-// weight may then reach 2^(rise of the scores above it): up to kRoomNear the product with a value
+// weight may then reach 2^(rise of the scores above it): up to kRoomHigh the product with a value
 // is within the range of a rescaled softmax; above, the accumulators are looked at after the
 // pass.  Where the sum would overflow, or a row that began at 0 stayed far below, the pass is made
 // again from the true maxima of a pass over the scores alone.  So no tile waits for the other
@@ -28,9 +28,6 @@
 // Entries hidden from a row have weight 0, which does not hide a value that is not finite: a unit of
 // several tokens whose result is not finite is computed again one token at a time, each over what it
 // sees itself.
-
-constexpr float kWideRoomNear = 8.0f, kWideRoomAbove = 100.0f, kWideRoomBelow = -40.0f;  // log2 units from the reference
-constexpr float kHidden = -3.0e38f;  // a hidden entry's score: weight 0
 
 // Rows 2 j and 2 j + 1 share a line of banks; rows 16 apart the same slots.  With the bits of j =
 // row / 2 reversed, the 16 rows of a K operand's phase lie on 16 distinct bank quads, and so do the
@@ -628,8 +625,8 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const float top = m_seen[b] * p.scale_log2, rise = top - m_own[b];
-          if (rise > kWideRoomNear) *high = 1;
-          if (rise > kWideRoomAbove || (rise < kWideRoomBelow && m_own[b] == 0.0f && m_seen[b] > 0.5f * kHidden)) *redo = 1;
+          if (rise > kRoomHigh) *high = 1;
+          if (rise > kRoomAbove || (rise < kRoomBelow && m_own[b] == 0.0f && m_seen[b] > 0.5f * kHidden)) *redo = 1;
         }
       }
       lds_barrier();
