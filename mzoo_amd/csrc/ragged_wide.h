@@ -51,12 +51,16 @@ struct WideLds {
   static_assert(LDS <= 160 * 1024 && sizeof(PlanLds) <= PB, "LDS");
 };
 
-// 16 bytes per lane from `at` + 128 J to LDS, for columns J .. N - 1 of a tile: lane l's to byte lds + 4096 J +
-// 16 l.  The wave's base is in m0, and the instruction's offset counts for both addresses.
+// 16 bytes per lane from `at` + 128 J to LDS, column J of a tile: lane l's to byte lds + 4096 J + 16 l.  The
+// wave's base is in m0, and the instruction's offset counts for both addresses.
+template <int J>
+__device__ __forceinline__ void load_column(gptr_t at, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
+               : : "s"(lds), "v"(at), "n"(128 * J), "n"((4096 - 128) * J) : "memory", "scc");
+}
 template <int J, int N>
 __device__ __forceinline__ void load_columns(gptr_t at, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
-               : : "s"(lds + (4096 - 128) * J), "v"(at), "n"(128 * J) : "memory");
+  load_column<J>(at, lds);
   if constexpr (J + 1 < N) load_columns<J + 1, N>(at, lds);
 }
 
@@ -400,6 +404,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
       for (int i = NI - LATE; i < NI; ++i) pv_block(i, [](int) {});
       uint64_t next = 0;
+      uint32_t to = 0;
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
         const v8bf cur = kf[st % AH];
@@ -414,9 +419,19 @@ ragged_wide_kernel(const RaggedParams p) {
           if (st >= KS - 2) store_part(wt, r, 7 + st - (KS - 2));
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (kDirect) {
-          if (st == 3) {
-            direct((gptr_t)next, at_w);
+        if constexpr (kDirect) {  // one of tile t + 3's loads
+          if (st == 2) to = __builtin_amdgcn_readfirstlane(lds0 + at_w);
+          if (st >= 3 && st < 3 + NI) {
+            const gptr_t e = (gptr_t)next;
+            if (st == 3) load_column<0>(e, to);
+            if (st == 4) load_column<1>(e, to);
+            if (st == 5) load_column<2>(e, to);
+            if (st == 6) load_column<3>(e, to);
+            if (st == 7) load_column<4>(e, to);
+            if (st == 8) load_column<5>(e, to);
+            if (st == 9) load_column<6>(e, to);
+            if (st == 10) load_column<7>(e, to);
+            if (NI > 8 && st == 11) load_column<(NI > 8 ? 8 : 0)>(e, to);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
