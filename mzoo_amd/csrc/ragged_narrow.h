@@ -12,20 +12,25 @@
 // registers, at most 80 KB).  bf16 entries are loaded straight into LDS, D / 32 instructions a wave and tile; 8-bit
 // ones pass through registers.
 //
-// The 16-byte piece x of a tile's row r sits at slot x ^ narrow_swz(r) of the row.
+// A tile in LDS is D / 32 columns of 64 rows of 64 bytes: a wave's load instruction (16 rows x 64 bytes, a
+// lane 16 of them) fills 1 KB of one column from one address per lane and tile, and an MFMA step of S^T
+// reads one column.  The 16-byte piece x of row r sits at slot x ^ narrow_swz(r) of its 64 bytes.
 //
 // Softmax and hidden entries as in ragged_wide.h: a fixed reference from the first tile, a second pass
 // from the true maxima where that does not hold, and token by token where a result is not finite.
 
 constexpr int kTile64 = 64;
 
-// Rows of D channels are 2 D bytes, a line of banks is 256: what is the same in all of the 16 rows of a K
-// operand's phase, and of the four rows of a V^T operand's, is told apart by the swizzle.
-template <int D>
-__device__ __forceinline__ int narrow_swz(int row) {
-  if constexpr (D == 64) return ((row >> 1 & 1) << 2) | ((row >> 2 & 1) << 1) | (row >> 3 & 1);
-  else if constexpr (D % 128 == 0) return ((row & 3) << 2) | (row >> 2 & 3);
-  else return row >> 2 & 3;  // 96, 160
+// Four rows are a line of banks, so the rows of a phase that meet in one are told apart: 16 rows of a K
+// operand's piece, four rows x 32 bytes of V^T.
+__device__ __forceinline__ int narrow_swz(int row) { return row >> 2 & 3; }
+
+// 16 bytes per lane from `at` + 64 J to LDS, column J of a tile (see load_column in ragged_wide.h)
+template <int J, int N>
+__device__ __forceinline__ void load_narrow(gptr_t at, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
+               : : "s"(lds), "v"(at), "n"(64 * J), "n"((4096 - 64) * J) : "memory", "scc");
+  if constexpr (J + 1 < N) load_narrow<J + 1, N>(at, lds);
 }
 
 template <int FMT, int D>
@@ -48,8 +53,7 @@ template <int FMT, int D, int NOPE>
 __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(const RaggedParams p) {
   using M = NarrowLds<FMT, D>;
   using L = Layout<FMT, D, NOPE>;
-  constexpr int NT = 256, KS = D / 32, NB = D / 16, NI = (NB + 3) / 4, ROW = 2 * D, PPR = D / 8;
-  constexpr int LD = D / 32;                                // load instructions of a wave and tile
+  constexpr int NT = 256, KS = D / 32, NB = D / 16, NI = (NB + 3) / 4, COL = 4096;
   constexpr int PPT = (L::kPieces + 3) / 4;                 // 8-bit entries: pieces of a thread
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* const tab = reinterpret_cast<uint32_t*>(smem + M::TAB);
@@ -90,21 +94,15 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   const uint64_t first_entry = reinterpret_cast<uint64_t>(p.entries) +
                                (paged ? 0 : static_cast<uint64_t>(u.t0) * p.entry_stride + static_cast<uint64_t>(u.g) * L::kEntryBytes);
   const uint32_t entry_stride = static_cast<uint32_t>(p.entry_stride);
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem)) + 1024u * LD * wave;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)smem)) + 1024u * wave;
 
   // addresses within a tile
-  const int krow = 16 * wave + e16;
-  const uint32_t k_at = static_cast<uint32_t>(krow * ROW);
-  const int kx = narrow_swz<D>(krow);
+  const uint32_t k_at = static_cast<uint32_t>((16 * wave + e16) * 64 + 16 * (g ^ narrow_swz(e16)));
   const int vrow = 4 * g + (e16 >> 2);
-  const int vx = narrow_swz<D>(vrow);  // the same 16 rows on
-  int ld_row[LD], ld_piece[LD];        // this lane's 16 bytes of each load instruction
-#pragma unroll
-  for (int j = 0; j < LD; ++j) {
-    const int s = 64 * j + lane;
-    ld_row[j] = 16 * wave + s / PPR;
-    ld_piece[j] = 16 * ((s % PPR) ^ narrow_swz<D>(ld_row[j]));
-  }
+  const uint32_t v_at = static_cast<uint32_t>(COL * (wave >> 1) + vrow * 64 + 16 * ((2 * (wave & 1) + ((e16 >> 1) & 1)) ^ narrow_swz(vrow)) +
+                                              8 * (e16 & 1));
+  const int ld_row = M::kDirect ? 16 * wave + (lane >> 2) : tid >> 2;  // the entry this lane fetches
+  const uint64_t piece = first_entry + (M::kDirect ? 16u * ((lane & 3) ^ narrow_swz(ld_row)) : 0u);
 
   int lo = 0, hi = 0, c0 = 0, nt = 0;
   int sub0 = tok0, sub1 = tok1;
@@ -183,15 +181,10 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   Piece raw[M::kDirect ? 1 : PPT];
   // tile t requested: straight into its buffer, or into registers
   auto ask = [&](int t) __attribute__((always_inline)) {
+    const gptr_t e = (gptr_t)(piece + static_cast<uint64_t>(code_of(t, ld_row)) * entry_stride);
     if constexpr (M::kDirect) {
-      const uint32_t buf = __builtin_amdgcn_readfirstlane(lds0 + (t & 1) * M::TILE);
-#pragma unroll
-      for (int j = 0; j < LD; ++j) {
-        const gptr_t e = (gptr_t)(first_entry + static_cast<uint64_t>(code_of(t, ld_row[j])) * entry_stride + static_cast<uint32_t>(ld_piece[j]));
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(buf + 1024 * j), "v"(e) : "memory");
-      }
+      load_narrow<0, KS>(e, __builtin_amdgcn_readfirstlane(lds0 + (t & 1) * M::TILE));
     } else {
-      const gptr_t e = (gptr_t)(first_entry + static_cast<uint64_t>(code_of(t, tid >> 2)) * entry_stride);
 #pragma unroll
       for (int j = 0; j < PPT; ++j) {
         const int q = (tid & 3) + 4 * j;
@@ -204,16 +197,18 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
     if constexpr (M::kDirect) {
       asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     } else {
-      const int row = tid >> 2, x = narrow_swz<D>(row);
-      uint8_t* const at = smem + (t & 1) * M::TILE + row * ROW;
+      const int x = narrow_swz(ld_row);
+      uint8_t* const at = smem + (t & 1) * M::TILE + ld_row * 64;
 #pragma unroll
       for (int j = 0; j < PPT; ++j) {
         const int q = (tid & 3) + 4 * j;
-        if (q < L::kCodePieces) {
-          *reinterpret_cast<uint4*>(at + 16 * ((2 * q) ^ x)) = dequant_fp8x8_bf16(uint2{raw[j].v.x, raw[j].v.y}, raw[j].s);
-          *reinterpret_cast<uint4*>(at + 16 * ((2 * q + 1) ^ x)) = dequant_fp8x8_bf16(uint2{raw[j].v.z, raw[j].v.w}, raw[j].s);
+        if (q < L::kCodePieces) {  // 16 codes: two bf16 pieces
+          uint8_t* const c = at + COL * (q >> 1);
+          *reinterpret_cast<uint4*>(c + 16 * ((2 * (q & 1)) ^ x)) = dequant_fp8x8_bf16(uint2{raw[j].v.x, raw[j].v.y}, raw[j].s);
+          *reinterpret_cast<uint4*>(c + 16 * ((2 * (q & 1) + 1) ^ x)) = dequant_fp8x8_bf16(uint2{raw[j].v.z, raw[j].v.w}, raw[j].s);
         } else if (q < L::kPieces) {
-          *reinterpret_cast<uint4*>(at + 16 * ((NOPE / 8 + q - L::kCodePieces) ^ x)) = uint4{raw[j].v.x, raw[j].v.y, raw[j].v.z, raw[j].v.w};
+          const int i = NOPE / 8 + q - L::kCodePieces;
+          *reinterpret_cast<uint4*>(at + COL * (i >> 2) + 16 * ((i & 3) ^ x)) = uint4{raw[j].v.x, raw[j].v.y, raw[j].v.z, raw[j].v.w};
         }
       }
     }
@@ -224,7 +219,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
     v4f s[4] = {v4f{}, v4f{}, v4f{}, v4f{}};
 #pragma unroll
     for (int st = 0; st < KS; ++st) {
-      const v8bf kf = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(kt + 16 * ((4 * st + g) ^ kx)));
+      const v8bf kf = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(kt + COL * st));
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) s[hg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][hg], s[hg], 0, 0, 0);
     }
@@ -335,7 +330,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
                 uint2{pack_bf16x2(v[hg][0], v[hg][1]), pack_bf16x2(v[hg][2], v[hg][3])};
           }
           lds_barrier();  // the weights of tile t are there
-          const uint8_t* const vt = smem + (t & 1) * M::TILE + vrow * ROW + 8 * (e16 & 1);
+          const uint8_t* const vt = smem + (t & 1) * M::TILE + v_at;
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
             v8bf pf[4];
@@ -345,9 +340,9 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
 #pragma unroll
             for (int i = 0; i < NI; ++i)
               if (wave + 4 * i < NB) {  // uniform
-                const uint8_t* const tp = vt + 32 * ROW * ks + 16 * ((2 * (wave + 4 * i) + ((e16 >> 1) & 1)) ^ vx);
+                const uint8_t* const tp = vt + 2 * COL * i + 2048 * ks;
                 const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp));
-                const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp + 16 * ROW));
+                const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_v4s(tp + 1024));
                 const v8bf vf = __builtin_bit_cast(v8bf, v8s{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 #pragma unroll
                 for (int hg = 0; hg < 4; ++hg) acc[i][hg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[hg], acc[i][hg], 0, 0, 0);
