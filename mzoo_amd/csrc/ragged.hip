@@ -18,7 +18,7 @@
 namespace mzk {
 namespace {
 
-constexpr int64_t kNoWindow = 1ll << 62;
+constexpr int kNoWindow = 1 << 30;  // also the most tokens of a call, so that no position overflows
 
 // Division of n < 2^31 by a constant of the call: floor(n m / 2^32) + n, shifted, with m = floor(2^32 (2^s -
 // d) / d) + 1 and 2^s >= d.  Three instructions; what is executed once runs from a cold instruction
@@ -53,7 +53,7 @@ struct RaggedParams {
   const int32_t* idx;  // [B, topk] positions (one token per sequence), or null
   int64_t idx_stride;
   int topk;
-  int64_t window;
+  int window;
   const float* sinks;
   float scale_log2;
   FastDiv by_heads, by_page, by_blocks;  // HG, page, the row blocks of one token
@@ -87,6 +87,7 @@ struct Unit {
   int slot;
 };
 
+__device__ __forceinline__ int clamp32(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // A value that is the same in every lane, in scalar registers.
@@ -128,7 +129,7 @@ __device__ __forceinline__ int sequence(const RaggedParams& p, int i, int& a, in
   int seen = z - a;
   if (p.lens) seen = static_cast<int>(clamp64(p.lens[i], 0, p.max_pages * p.page));
   if (p.idx) seen = seen > 0 ? p.topk : 0;
-  if (seen > p.window + (z - a)) seen = static_cast<int>(p.window) + (z - a);
+  if (seen > p.window + (z - a)) seen = p.window + (z - a);
   tiles = (seen + kTile - 1) / kTile;
   return ((z - a) * p.HG + (1 << p.unit_shift) - 1) >> p.unit_shift;
 }
@@ -389,9 +390,9 @@ __device__ __forceinline__ int row_at(const RaggedParams& p, const Unit& u, int 
 
 // The positions (or places of the list) that tokens tok0 .. tok1 - 1 of the sequence see.
 __device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u, int tok0, int tok1, int& lo, int& hi) {
-  const int64_t shift = static_cast<int64_t>(u.len) - u.n;  // position of the first new token (negative: tokens that see nothing)
-  lo = static_cast<int>(clamp64(shift + tok0 - p.window + 1, 0, u.len));
-  hi = static_cast<int>(clamp64(shift + tok1, 0, u.len));
+  const int shift = u.len - u.n;  // position of the first new token (negative: tokens that see nothing)
+  lo = clamp32(shift + tok0 - p.window + 1, 0, u.len);
+  hi = clamp32(shift + tok1, 0, u.len);
   if (p.idx) {
     lo = 0;
     hi = u.len > 0 ? p.topk : 0;
@@ -404,7 +405,7 @@ __device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u,
   if (u.shares > 1) {
     const int tiles = (hi - lo + kTile - 1) / kTile, per = (tiles + u.shares - 1) / u.shares;
     const int64_t from = lo + static_cast<int64_t>(u.share) * per * kTile;
-    if (from + static_cast<int64_t>(per) * kTile < hi) hi = static_cast<int>(from) + per * kTile;
+    if (from + per * kTile < hi) hi = static_cast<int>(from) + per * kTile;
     lo = from < hi ? static_cast<int>(from) : hi;
   }
 }
@@ -421,21 +422,18 @@ __device__ __forceinline__ int pool_entry(const RaggedParams& p, const Unit& u, 
   return pid * p.page + (v - at * p.page);
 }
 
-// A row's result from its maximum, sum and sink: the factor of O^T and the log-sum-exp.
-__device__ __forceinline__ float finish_row(const RaggedParams& p, int head, float m, float l, float& lse) {
+// A row's result from its maximum, sum and sink (-inf: none): the factor of O^T and the log-sum-exp.
+__device__ __forceinline__ float finish_row(float m, float l, float sink, float& lse) {
   const bool none = l == 0.0f && m == -__builtin_huge_valf();  // it sees nothing: lse is the sink itself
   float scale = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  if (p.sinks) {
-    const float sk = p.sinks[head] * kLog2e;
-    const float mm = fmaxf(m, sk);
-    if (mm > -__builtin_huge_valf()) {
-      const float a = m == -__builtin_huge_valf() ? 0.0f : exp2f(m - mm);
-      l = l * a + exp2f(sk - mm);
-      m = mm;
-      scale = a / l;
-    }
+  const float sk = sink * kLog2e, mm = fmaxf(m, sk);
+  if (sk != -__builtin_huge_valf()) {
+    const float a = m == -__builtin_huge_valf() ? 0.0f : exp2f(m - mm);
+    l = l * a + exp2f(sk - mm);
+    m = mm;
+    scale = a / l;
   }
-  lse = !none ? (m + __log2f(l)) * kLn2 : p.sinks ? p.sinks[head] : -__builtin_huge_valf();
+  lse = none ? sink : (m + __log2f(l)) * kLn2;
   return scale;
 }
 
@@ -480,7 +478,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
     if (row < j.rows) {
       const int64_t at = j.row0 + row;
       float lse;
-      const float scale = finish_row(p, static_cast<int>(at % p.H), m, l, lse);
+      const float scale = finish_row(m, l, p.sinks ? p.sinks[at % p.H] : -__builtin_huge_valf(), lse);
       if ((tid & 15) == 0 && blockIdx.y == 0) p.lse[at] = lse;
       for (int s = tid & 15; s < j.shares; s += 16) weight[r][s] *= scale;
     }
@@ -595,9 +593,9 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                                 int topk, int64_t window, const float* sinks, void* workspace, int64_t workspace_bytes,
                                 void* out, float* lse, int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0, "paged_attend: bad sizes");
-  MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536 && pages >= 0 && pages <= kMaxInt && max_pages >= 0 &&
+  MZK_CHECK_ARG(T <= kNoWindow && B <= kMaxInt && H <= 65536 && pages >= 0 && pages <= kMaxInt && max_pages >= 0 &&
                     max_pages <= kMaxInt,
-                "paged_attend: sizes of 2^31 or more");
+                "paged_attend: more than 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(page >= 1, "paged_attend: pages of at least one entry");
   MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
                 "paged_attend: a sequence and a pool hold less than 2^31 entries");
@@ -631,7 +629,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.idx = idx;
   p.idx_stride = idx_row_stride;
   p.topk = topk;
-  p.window = window ? window : kNoWindow;
+  p.window = window && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);
@@ -678,7 +676,7 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
                               int64_t kv_row_stride, int G, int64_t window, const float* sinks, void* out, float* lse,
                               int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && G >= 1, "packed_mqa: bad sizes");
-  MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536, "packed_mqa: sizes of 2^31 or more");
+  MZK_CHECK_ARG(T <= kNoWindow && B <= kMaxInt && H <= 65536, "packed_mqa: more than 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(H % G == 0, "packed_mqa: %d heads do not divide into %d latents", H, G);
   MZK_CHECK_ARG(window >= 0, "packed_mqa: negative window");
   MZK_CHECK_ARG(kv_row_stride >= static_cast<int64_t>(G) * D && kv_row_stride % 8 == 0 && kv_row_stride < 1ll << 30,
@@ -697,7 +695,7 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   p.B = B;
   p.entries = static_cast<const uint8_t*>(kv);
   p.entry_stride = 2 * kv_row_stride;
-  p.window = window ? window : kNoWindow;
+  p.window = window && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);

@@ -72,24 +72,10 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   zero_rows(p, tid);
   if (!find_unit(p, u, smem, tid)) return;  // uniform
 
-  // the B operand of S^T: rows 16 hg + e16, channels 32 st + 8 g ..
-  v8bf qf[KS][4];
-  int tok_h[4];
-#pragma unroll
-  for (int hg = 0; hg < 4; ++hg) {
-    const int r = u.r0 + 16 * hg + e16;
-    const int rc = r < u.r1 ? r : u.r0;
-    int head;
-    const uint16_t* const qr = p.q + static_cast<int64_t>(row_at(p, u, rc, head)) * D + 8 * g;
-#pragma unroll
-    for (int st = 0; st < KS; ++st) qf[st][hg] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(qr + 32 * st));
-    tok_h[hg] = p.by_heads(rc);
-  }
   const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
   const int shift = u.len - u.n;
   int share_lo, share_hi;
   unit_range(p, u, tok0, tok1, share_lo, share_hi);
-  const int64_t win = p.window < 0x7fffffff ? p.window : 0x7fffffff;
   const bool paged = p.tables != nullptr;
   const uint64_t first_entry = reinterpret_cast<uint64_t>(p.entries) +
                                (paged ? 0 : static_cast<uint64_t>(u.t0) * p.entry_stride + static_cast<uint64_t>(u.g) * L::kEntryBytes);
@@ -106,7 +92,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
 
   int lo = 0, hi = 0, c0 = 0, nt = 0;
   int sub0 = tok0, sub1 = tok1;
-  int row_lo[4], row_span[4];
+  int row_lo[4], row_span[4], tok_h[4];
   int full_lo = 0, full_hi = 0;
   auto set_range = [&]() __attribute__((always_inline)) {
     token_range(p, u, sub0, sub1, lo, hi);
@@ -115,22 +101,23 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
     if (hi < lo) hi = lo;
     int most_lo = lo, least_hi = hi;
     if (!p.idx) {
-      const int64_t a = static_cast<int64_t>(shift) + sub1 - win, z = static_cast<int64_t>(shift) + sub0 + 1;
-      most_lo = a > lo ? static_cast<int>(a) : lo;
-      least_hi = z < hi ? static_cast<int>(z) : hi;
+      most_lo = clamp32(shift + sub1 - p.window, lo, 0x7fffffff - kTile64);
+      least_hi = shift + sub0 + 1 < hi ? shift + sub0 + 1 : hi;
     }
     full_lo = (most_lo - lo + kTile64 - 1) / kTile64;
     full_hi = least_hi > lo ? (least_hi - lo) / kTile64 : 0;
+  };
+  auto set_rows = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int hg = 0; hg < 4; ++hg) {
-      int64_t a = lo, z = hi;
+      int a = lo, z = hi;
       if (!p.idx) {
-        const int64_t pos = static_cast<int64_t>(shift) + tok_h[hg];
-        if (pos - win + 1 > a) a = pos - win + 1;
+        const int pos = shift + tok_h[hg];
+        if (pos - p.window + 1 > a) a = pos - p.window + 1;
         if (pos + 1 < z) z = pos + 1;
       }
-      row_lo[hg] = static_cast<int>(a - lo);
-      row_span[hg] = z > a ? static_cast<int>(z - a) : 0;
+      row_lo[hg] = a - lo;
+      row_span[hg] = z > a ? z - a : 0;
     }
   };
 
@@ -213,6 +200,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
       }
     }
   };
+  v8bf qf[KS][4];
   // this lane's scaled scores of tile t, -inf where hidden
   auto scores = [&](int t, float (&v)[4][4]) __attribute__((always_inline)) {
     const uint8_t* const kt = smem + (t & 1) * M::TILE + k_at;
@@ -266,9 +254,28 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
     }
   };
 
-  bool strict = false;
+  // The first tile is requested before q (the B operand of S^T: rows 16 hg + e16, channels 32 st + 8 g ..)
+  // and what the rows see of it is worked out.
+  set_range();
+  const bool none = !(lo < hi && lay_out());  // uniform
+  if (!none) ask(0);
+  float sink4[4];
+#pragma unroll
+  for (int hg = 0; hg < 4; ++hg) {
+    const int r = u.r0 + 16 * hg + e16;
+    const int rc = r < u.r1 ? r : u.r0;
+    int head;
+    const uint16_t* const qr = p.q + static_cast<int64_t>(row_at(p, u, rc, head)) * D + 8 * g;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) qf[st][hg] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(qr + 32 * st));
+    sink4[hg] = p.sinks ? p.sinks[head] : -__builtin_huge_valf();
+    tok_h[hg] = p.by_heads(rc);
+  }
+
+  bool strict = false, at_start = true;
   while (true) {
-    set_range();
+    if (!at_start) set_range();
+    set_rows();
     float l4[4];
     int e4[4];
     for (bool given = false;; given = true) {
@@ -303,8 +310,9 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
         if (!begun) m4[hg] = 0.0f;
       }
       for (c0 = 0; c0 < hi - lo; c0 += nt * kTile64) {
-        if (!lay_out()) continue;
-        ask(0);
+        const bool ready = at_start && c0 == 0;
+        if (ready ? none : !lay_out()) continue;
+        if (!ready) ask(0);
 #pragma unroll 1
         for (int t = 0; t < nt; ++t) {
           arrive(t);
@@ -351,6 +359,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
         }
         lds_barrier();  // the LDS is free again
       }
+      at_start = false;
       // each row's sum: its four lanes, then the four waves
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) {
@@ -358,8 +367,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
         l_own[hg] = l_own[hg] + __shfl_xor(l_own[hg], 32, 64);
         if (g == 0) lsum[64 * wave + 16 * hg + e16] = l_own[hg];
       }
-      lds_barrier();  // redo and high are zero
-      if (!given) {
+      if (!given) {  // (zero before the barriers of the pass; without an entry nothing is set)
 #pragma unroll
         for (int hg = 0; hg < 4; ++hg) {
           const float rise = m_seen[hg] - m4[hg];
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
         int head;
         const int at = row_at(p, u, u.r0 + r, head);
         float lse;
-        const float scale = __builtin_amdgcn_ldexpf(finish_row(p, head, m4[hg], l4[hg], lse), -e4[hg]);
+        const float scale = __builtin_amdgcn_ldexpf(finish_row(m4[hg], l4[hg], sink4[hg], lse), -e4[hg]);
         uint16_t* const o = p.out + static_cast<int64_t>(at) * D + 16 * wave + 4 * g;
 #pragma unroll
         for (int i = 0; i < NI; ++i)

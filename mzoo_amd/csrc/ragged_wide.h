@@ -46,7 +46,8 @@ struct WideLds {
   static constexpr int MASK = TAB + 4 * TABN;      // entries that are there, of each tile
   static constexpr int PMAX = MASK + 4 * 72;       // [2 eh][64]
   static constexpr int LSUM = PMAX + 512;          // [2 eh][64]
-  static constexpr int RED = LSUM + 512;
+  static constexpr int SINK = LSUM + 512;          // [64]
+  static constexpr int RED = SINK + 256;
   static constexpr int LDS = RED + 32;
   static_assert(LDS <= 160 * 1024 && sizeof(PlanLds) <= PB, "LDS");
 };
@@ -82,6 +83,7 @@ ragged_wide_kernel(const RaggedParams p) {
   uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + M::MASK);
   float* const pmax = reinterpret_cast<float*>(smem + M::PMAX);
   float* const lsum = reinterpret_cast<float*>(smem + M::LSUM);
+  float* const sinks = reinterpret_cast<float*>(smem + M::SINK);
   int* const redo = reinterpret_cast<int*>(smem + M::RED);
   int* const high = redo + 1;
   int* const odd = redo + 2;
@@ -126,7 +128,12 @@ ragged_wide_kernel(const RaggedParams p) {
     const int r = u.r0 + 32 * hh + 16 * b + e16;
     tok_b[b] = p.by_heads(r < u.r1 ? r : u.r0);
   }
-  const int64_t win = p.window < 0x7fffffff ? p.window : 0x7fffffff;
+  float sink = -__builtin_huge_valf();  // of row tid, kept in LDS for the end
+  if (p.sinks && tid < 64) {
+    int head;
+    row_at(p, u, tid < rows ? u.r0 + tid : u.r0, head);
+    sink = p.sinks[head];
+  }
 
   // ---- addresses -------------------------------------------------------------------------
   const int te = tid >> 3, tj = tid & 7;
@@ -526,22 +533,21 @@ ragged_wide_kernel(const RaggedParams p) {
     if (hi < lo) hi = lo;
     int most_lo = lo, least_hi = hi;
     if (!p.idx) {
-      const int64_t a = static_cast<int64_t>(shift) + sub1 - win, z = static_cast<int64_t>(shift) + sub0 + 1;
-      most_lo = a > lo ? static_cast<int>(a) : lo;
-      least_hi = z < hi ? static_cast<int>(z) : hi;
+      most_lo = clamp32(shift + sub1 - p.window, lo, 0x7fffffff - kTile);
+      least_hi = shift + sub0 + 1 < hi ? shift + sub0 + 1 : hi;
     }
     full_lo = (most_lo - lo + kTile - 1) / kTile;
     full_hi = least_hi > lo ? (least_hi - lo) / kTile : 0;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      int64_t a = lo, z = hi;
+      int a = lo, z = hi;
       if (!p.idx) {
-        const int64_t pos = static_cast<int64_t>(shift) + tok_b[b];
-        if (pos - win + 1 > a) a = pos - win + 1;
+        const int pos = shift + tok_b[b];
+        if (pos - p.window + 1 > a) a = pos - p.window + 1;
         if (pos + 1 < z) z = pos + 1;
       }
-      row_lo[b] = static_cast<int>(a - lo);
-      row_span[b] = z > a ? static_cast<int>(z - a) : 0;
+      row_lo[b] = a - lo;
+      row_span[b] = z > a ? z - a : 0;
     }
   };
 
@@ -561,6 +567,7 @@ ragged_wide_kernel(const RaggedParams p) {
       const int r = at / QROW;
       *reinterpret_cast<u32x4*>(smem + QB + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
     }
+    if (tid < 64) sinks[tid] = sink;
     lds_barrier();
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -635,8 +642,7 @@ ragged_wide_kernel(const RaggedParams p) {
         l_own[b] = l_own[b] + __shfl_xor(l_own[b], 32, 64);
         if (g == 0) lsum[eh * 64 + 32 * hh + 16 * b + e16] = l_own[b];
       }
-      lds_barrier();  // redo and high are zero
-      if (!given) {
+      if (!given) {  // (zero before the barriers of the pass; without an entry nothing is set)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const float top = m_seen[b] * p.scale_log2, rise = top - m_own[b];
@@ -716,7 +722,7 @@ ragged_wide_kernel(const RaggedParams p) {
           int head;
           const int at = row_at(p, u, u.r0 + r, head);
           float lse;
-          const float scale = __builtin_amdgcn_ldexpf(finish_row(p, head, m4[hg], l4[hg], lse), -e4[hg]);
+          const float scale = __builtin_amdgcn_ldexpf(finish_row(m4[hg], l4[hg], sinks[r], lse), -e4[hg]);
           uint8_t* const orow = smem + r * OPITCH + 32 * wave + 8 * g;
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
