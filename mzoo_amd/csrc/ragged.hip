@@ -511,21 +511,22 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   const int64_t grid = p.slots ? p.slots : (p.blocks_max + 15) / 16 * 16;
   using M = std::conditional_t<(D > 256), WideLds<FMT, D>, NarrowLds<FMT, D>>;
   void (*kern)(const RaggedParams);
-  if constexpr (D > 256) kern = ragged_wide_kernel<FMT, D, NOPE>;
+  if constexpr (D > 256) kern = p.cu == nullptr && p.H <= 16 ? ragged_wide_kernel<FMT, D, NOPE, true> : ragged_wide_kernel<FMT, D, NOPE, false>;
   else kern = ragged_narrow_kernel<FMT, D, NOPE>;
   // the dynamic-LDS limit is a per-device function attribute: set once per device
-  static std::atomic<bool> attr_set[kMaxDevices] = {};  // setting it twice is harmless
+  static std::atomic<bool> attr_set[2][kMaxDevices] = {};  // setting it twice is harmless
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
     set_last_error("ragged attention: no usable current device");
     return MZK_ELAUNCH;
   }
-  if (!attr_set[dev].load(std::memory_order_acquire)) {
+  const int which = D > 256 && p.cu == nullptr && p.H <= 16;
+  if (!attr_set[which][dev].load(std::memory_order_acquire)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, M::LDS) != hipSuccess) {
       set_last_error("ragged attention: cannot raise the kernel's LDS limit to %d bytes", M::LDS);
       return MZK_ELAUNCH;
     }
-    attr_set[dev].store(true, std::memory_order_release);
+    attr_set[which][dev].store(true, std::memory_order_release);
   }
   kern<<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
   if (p.slots) join_kernel<D><<<dim3(static_cast<unsigned>(4 * p.blocks_max), (D / 16 + 3) / 4), 256, 0, s>>>(p);
@@ -565,7 +566,11 @@ void set_units(RaggedParams& p) {
 }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+// Shares of at least 4 tiles (one sequence of 4096: 29 us); no shares where a token cannot see more than
+// 12 tiles, since the joining launch is 6 to 7 us (10 sequences x 128 heads over 8 tiles: 23.2 us with, 19.9
+// without; 2 sequences over 17: 22.1 with, 29.0 without).
 constexpr int kMinTiles = 4;
+constexpr int kWholeTiles = 12;
 
 // How many units a call is split into: 0 for as many as blocks.  With fewer blocks than twice the 256
 // compute units (a unit fills one), up to 256, or 1024 where the blocks alone fill more than half,
@@ -645,7 +650,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   if (window && window + T < most) most = window + T;
   if (idx) most = topk;
   p.min_tiles = kMinTiles;
-  p.slots = (most + kTile - 1) / kTile > kMinTiles ? unit_slots(p.blocks_max, B) : 0;
+  p.slots = (most + kTile - 1) / kTile > kWholeTiles ? unit_slots(p.blocks_max, B) : 0;
   if (p.slots) {
     p.blocks_out = static_cast<int32_t*>(workspace);
     p.joins = reinterpret_cast<JoinRow*>(static_cast<uint8_t*>(workspace) + 16);

@@ -13,6 +13,10 @@
 // the softmax of u+1, while tile u+2 (8-bit entries, dequantized from registers) or u+3 (bf16
 // entries, loaded straight into LDS) arrives.
 //
+// Up to 16 rows (FEW: one new token of up to 16 heads): one row group instead of four, the waves of hh = 1
+// repeating the scores of hh = 0.  The matrix work falls to a quarter, and the clock need not: 32
+// sequences of up to 32k x 16 heads, 8-bit entries, 154 -> 123 us.
+//
 // A tile in LDS is D / 64 columns of 32 rows of 128 bytes: a wave's load instruction (8 rows x 128
 // bytes, a lane 16 of them) fills 1 KB of one column, in lane order as the hardware wants it, from
 // one address per lane and tile.  The 16-byte piece x of row r sits at slot x ^ wide_swz(r).
@@ -71,12 +75,14 @@ struct WideRaw {
   u32x4 s;  // the entry's four block scales
 };
 
-template <int FMT, int D, int NOPE>
+template <int FMT, int D, int NOPE, bool FEW>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 ragged_wide_kernel(const RaggedParams p) {
   using M = WideLds<FMT, D>;
   constexpr bool kDirect = M::kDirect;
   constexpr int NT = 256, KS = D / 32, NI = D / 64, COL = 4096;
+  // row groups of 16: of the unit, and of a wave's scores (FEW: both halves of the waves have the same)
+  constexpr int RG = FEW ? 1 : 4, SB = FEW ? 1 : 2, ROWS = 16 * RG;
   constexpr int EB = Layout<FMT, D, NOPE>::kEntryBytes;
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* const tab = reinterpret_cast<uint32_t*>(smem + M::TAB);
@@ -92,7 +98,7 @@ ragged_wide_kernel(const RaggedParams p) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int eh = wave & 1, hh = wave >> 1;
+  const int eh = wave & 1, hh = FEW ? 0 : wave >> 1;
   const int g = lane >> 4, e16 = lane & 15;
 
   Unit u;
@@ -102,9 +108,9 @@ ragged_wide_kernel(const RaggedParams p) {
   // q: the B operand of S^T (rows 32 hh + 16 b + e16, channels 32 st + 8 g ..) through LDS, from
   // whole lines
   const int rows = u.r1 - u.r0;
-  constexpr int QROW = D / 8, QP = 64 * QROW / NT;
+  constexpr int QROW = D / 8, QP = (ROWS * QROW + NT - 1) / NT;
   u32x4 qraw[QP];
-  if (p.G == 1 && rows == 64) {  // one run of rows
+  if (!FEW && p.G == 1 && rows == 64) {  // one run of rows
     const u32x4* const qb = reinterpret_cast<const u32x4*>(p.q + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
 #pragma unroll
     for (int k = 0; k < QP; ++k) qraw[k] = (qb + NT * k)[tid];
@@ -112,7 +118,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
     for (int k = 0; k < QP; ++k) {
       const int at = tid + NT * k;
-      const int r = at / QROW;
+      const int r = at / QROW;  // (beyond the unit's rows: its first)
       int head;
       qraw[k] = *reinterpret_cast<const u32x4*>(
           p.q + static_cast<int64_t>(row_at(p, u, u.r0 + (r < rows ? r : 0), head)) * D + 8 * (at - r * QROW));
@@ -122,9 +128,9 @@ ragged_wide_kernel(const RaggedParams p) {
   const int shift = u.len - u.n;
   int share_lo, share_hi;
   unit_range(p, u, tok0, tok1, share_lo, share_hi);
-  int tok_b[2];  // the tokens of this lane's rows
+  int tok_b[SB];  // the tokens of this lane's rows
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int b = 0; b < SB; ++b) {
     const int r = u.r0 + 32 * hh + 16 * b + e16;
     tok_b[b] = p.by_heads(r < u.r1 ? r : u.r0);
   }
@@ -175,15 +181,15 @@ ragged_wide_kernel(const RaggedParams p) {
   };
   auto tile_at = [&](int i) __attribute__((always_inline)) -> uint32_t { return static_cast<uint32_t>(i) * M::TILE; };
 
-  float m4[4], m_own[2], l_own[2], m_seen[2];
-  v4f acc[NI][4];
-  v8bf qf[KS][2];
-  v4f s_acc[2];
+  float m4[RG], m_own[SB], l_own[SB], m_seen[SB];
+  v4f acc[NI][RG];
+  v8bf qf[KS][SB];
+  v4f s_acc[SB];
   WideRaw raw[2];
 
   int lo = 0, hi = 0;       // the pass's entries: positions lo .. hi - 1
   int c0 = 0, nt = 0;       // the chunk at hand: its first entry (from lo), its tiles
-  int row_lo[2], row_span[2];  // of this lane's rows, entries seen, from lo
+  int row_lo[SB], row_span[SB];  // of this lane's rows, entries seen, from lo
   int full_lo = 0, full_hi = 0;  // tiles (from lo) of which every row sees every entry
   // the entry that a lane fetches for tile t of the chunk: past the end of the range its last one
   auto code_of = [&](int t) __attribute__((always_inline)) -> uint32_t {
@@ -260,20 +266,21 @@ ragged_wide_kernel(const RaggedParams p) {
     const int v = c0 + t * kTile + 16 * eh + 4 * g + r;
     return ((bits >> (16 * eh + 4 * g + r)) & 1u) != 0u && static_cast<uint32_t>(v - row_lo[b]) < static_cast<uint32_t>(row_span[b]);
   };
-  auto scores = [&](int t, float (&v)[2][4]) __attribute__((always_inline)) {
+  auto scores = [&](int t, float (&v)[SB][4]) __attribute__((always_inline)) {
     const uint32_t bits = paged ? masks[t] : 0xffffffffu;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < SB; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[b][r] = sees(t, bits, b, r) ? s_acc[b][r] * p.scale_log2 : -__builtin_huge_valf();
   };
   auto s_tile = [&](const uint8_t* kt) __attribute__((always_inline)) {
-    s_acc[0] = s_acc[1] = v4f{};
+#pragma unroll
+    for (int b = 0; b < SB; ++b) s_acc[b] = v4f{};
 #pragma unroll
     for (int st = 0; st < KS; ++st) {
       const v8bf kf = k_frag(kt, st);
-      s_acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][0], s_acc[0], 0, 0, 0);
-      s_acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][1], s_acc[1], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < SB; ++b) s_acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st][b], s_acc[b], 0, 0, 0);
     }
   };
   auto max4 = [](const float (&v)[4]) __attribute__((always_inline)) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
@@ -282,19 +289,18 @@ ragged_wide_kernel(const RaggedParams p) {
     return fmaxf(x, __shfl_xor(x, 32, 64));
   };
   // the rows' maxima over both entry halves into m4 / m_own (one barrier); 0 for a row without one
-  auto agree_max = [&](float t0, float t1) __attribute__((always_inline)) {
-    t0 = row_max(t0);
-    t1 = row_max(t1);
-    if (g == 0) {
-      pmax[eh * 64 + 32 * hh + e16] = t0;
-      pmax[eh * 64 + 32 * hh + 16 + e16] = t1;
+  auto agree_max = [&](float (&t)[SB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < SB; ++b) {
+      t[b] = row_max(t[b]);
+      if (g == 0) pmax[eh * 64 + 32 * hh + 16 * b + e16] = t[b];
     }
     lds_barrier();
     auto known = [](float a, float b) { const float m = fmaxf(a, b); return m == -__builtin_huge_valf() ? 0.0f : m; };
 #pragma unroll
-    for (int hg = 0; hg < 4; ++hg) m4[hg] = known(pmax[16 * hg + e16], pmax[64 + 16 * hg + e16]);
+    for (int hg = 0; hg < RG; ++hg) m4[hg] = known(pmax[16 * hg + e16], pmax[64 + 16 * hg + e16]);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) m_own[b] = known(pmax[32 * hh + 16 * b + e16], pmax[64 + 32 * hh + 16 * b + e16]);
+    for (int b = 0; b < SB; ++b) m_own[b] = known(pmax[32 * hh + 16 * b + e16], pmax[64 + 32 * hh + 16 * b + e16]);
   };
   auto put_p = [&](int t, int b, uint2 w) __attribute__((always_inline)) {
     *reinterpret_cast<uint2*>(pbuf + (t & 1) * 4096 + 2048 * hh + 1024 * b + 16 * lane + 8 * eh) = w;
@@ -343,11 +349,16 @@ ragged_wide_kernel(const RaggedParams p) {
     lds_barrier();
     s_tile(smem);
     {
-      float v[2][4];
+      float v[SB][4];
       scores(t0, v);
-      if (begin) agree_max(max4(v[0]), max4(v[1]));
+      if (begin) {
+        float top[SB];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < SB; ++b) top[b] = max4(v[b]);
+        agree_max(top);
+      }
+#pragma unroll
+      for (int b = 0; b < SB; ++b) {
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(v[b][r] - m_own[b]);
@@ -364,13 +375,13 @@ ragged_wide_kernel(const RaggedParams p) {
     // registers by then, follow the barrier and cover the first reads of K.
     constexpr int AH = 6, VH = 4, LATE = 2;
     v4s va[VH + 1][2];
-    v8bf pf[4];
+    v8bf pf[RG];
     auto pv_block = [&](int i, auto&& fill) __attribute__((always_inline)) {
       const v4s a = va[i % (VH + 1)][0], b = va[i % (VH + 1)][1];
       const v8bf vf = __builtin_bit_cast(v8bf, v8s{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 #pragma unroll
       for (int hg = 0; hg < 4; ++hg) {
-        acc[i][hg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[hg], acc[i][hg], 0, 0, 0);
+        if (hg < RG) acc[i][hg < RG ? hg : 0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[hg < RG ? hg : 0], acc[i][hg < RG ? hg : 0], 0, 0, 0);
         fill(hg);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -381,7 +392,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
     for (int i = 0; i <= VH; ++i) va[i][0] = va[i][1] = v4s{0, 0, 0, 0};
 #pragma unroll
-    for (int hg = 0; hg < 4; ++hg) pf[hg] = __builtin_bit_cast(v8bf, v4i{0, 0, 0, 0});
+    for (int hg = 0; hg < RG; ++hg) pf[hg] = __builtin_bit_cast(v8bf, v4i{0, 0, 0, 0});
     if constexpr (kDirect) {  // tile t0 + 1
       if constexpr (NI > 8) asm volatile("s_waitcnt vmcnt(9)" : : : "memory");
       else asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
@@ -399,11 +410,13 @@ ragged_wide_kernel(const RaggedParams p) {
       if constexpr (kDirect) code = code_of(t + 3 < n ? t + 3 : n - 1);
       else code = tab[(t + 4) * kTile + te];
       // hidden entries start from kHidden instead of 0, so that no score needs a test
-      v4f init[2] = {v4f{}, v4f{}};
+      v4f init[SB];
+#pragma unroll
+      for (int b = 0; b < SB; ++b) init[b] = v4f{};
       if (!whole(t + 1)) {
         const uint32_t bits = paged ? masks[t + 1] : 0xffffffffu;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < SB; ++b)
 #pragma unroll
           for (int k = 0; k < 4; ++k) init[b][k] = sees(t + 1, bits, b, k) ? 0.0f : kHidden;
       }
@@ -418,9 +431,9 @@ ragged_wide_kernel(const RaggedParams p) {
         s_acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur, qf[st][0], st == 0 ? init[0] : s_acc[0], 0, 0, 0);
         if (st + AH < KS) kf[st % AH] = k_frag(kt, st + AH);
         __builtin_amdgcn_sched_barrier(0);
-        s_acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur, qf[st][1], st == 0 ? init[1] : s_acc[1], 0, 0, 0);
+        if constexpr (SB > 1) s_acc[SB - 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur, qf[st][SB - 1], st == 0 ? init[SB - 1] : s_acc[SB - 1], 0, 0, 0);
         if (st == 2) next = pool_piece + static_cast<uint64_t>(code) * entry_stride;
-        if (st >= 8 && st < 12) read_p(t, st - 8);
+        if (st >= 8 && st < 8 + RG) read_p(t, st - 8);
         if (st >= KS - VH - 2 && st < KS - 2) read_v(vt, st - (KS - VH - 2), va[st - (KS - VH - 2)]);
         if constexpr (!kDirect) {
           if (st >= KS - 2) store_part(wt, r, 7 + st - (KS - 2));
@@ -444,24 +457,29 @@ ragged_wide_kernel(const RaggedParams p) {
         }
       }
       const gptr_t from = (gptr_t)next;
-      float v[2][4], pr[2][4];
+      float v[SB][4], pr[SB][4];
       // slice k of what fills the matrix instructions of PV
       auto slice = [&](int k) __attribute__((always_inline)) {
         if (k >= 2 && k < 10) {
           const int b = (k - 2) >> 2, j = (k - 2) & 3;
+          if (b >= SB) return;
           v[b][j] = s_acc[b][j];
           pr[b][j] = __builtin_fmaf(v[b][j], p.scale_log2, -m_own[b]);
         } else if (k >= 10 && k < 18) {  // v_exp_f32 directly: results below 2^-126 may flush to 0
           const int b = (k - 10) >> 2, j = (k - 10) & 3;
+          if (b >= SB) return;
           pr[b][j] = __builtin_amdgcn_exp2f(pr[b][j]);
         } else if (k == 18 || k == 19) {
           const int b = k - 18;
+          if (b >= SB) return;
           put_p(t + 1, b, uint2{pack_bf16x2(pr[b][0], pr[b][1]), pack_bf16x2(pr[b][2], pr[b][3])});
         } else if (k >= 20 && k < 22) {
           const int b = k - 20;
+          if (b >= SB) return;
           l_own[b] = l_own[b] + ((pr[b][0] + pr[b][1]) + (pr[b][2] + pr[b][3]));
         } else if (k >= 22 && k < 24) {
           const int b = k - 22;
+          if (b >= SB) return;
           m_seen[b] = fmaxf(fmaxf(m_seen[b], v[b][0]), fmaxf(v[b][1], fmaxf(v[b][2], v[b][3])));
         }
       };
@@ -512,7 +530,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
       for (int i = NI - LATE; i < NI; ++i) pv_block(i, [](int) {});
 #pragma unroll
-      for (int hg = 0; hg < 4; ++hg) read_p(n - 1, hg);
+      for (int hg = 0; hg < RG; ++hg) read_p(n - 1, hg);
 #pragma unroll
       for (int i = 0; i < VH; ++i) read_v(vt, i, va[i]);
 #pragma unroll
@@ -539,7 +557,7 @@ ragged_wide_kernel(const RaggedParams p) {
     full_lo = (most_lo - lo + kTile - 1) / kTile;
     full_hi = least_hi > lo ? (least_hi - lo) / kTile : 0;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < SB; ++b) {
       int a = lo, z = hi;
       if (!p.idx) {
         const int pos = shift + tok_b[b];
@@ -559,18 +577,19 @@ ragged_wide_kernel(const RaggedParams p) {
   if (!none) ask();
   {
     constexpr int QPITCH = 2 * D + 16;  // the pad spreads 16 rows' pieces over the banks
-    constexpr int QB = M::PB + 2 * 4096 - 64 * QPITCH;
+    constexpr int QB = M::PB + 2 * 4096 - ROWS * QPITCH;
     static_assert(QB >= (kDirect ? 2 * M::TILE : 0), "q behind the first tiles");
 #pragma unroll
     for (int k = 0; k < QP; ++k) {
       const int at = tid + NT * k;
       const int r = at / QROW;
-      *reinterpret_cast<u32x4*>(smem + QB + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
+      if (ROWS * QROW % NT == 0 || at < ROWS * QROW)
+        *reinterpret_cast<u32x4*>(smem + QB + r * QPITCH + 16 * (at - r * QROW)) = qraw[k];
     }
     if (tid < 64) sinks[tid] = sink;
     lds_barrier();
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < SB; ++b)
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + QB + (32 * hh + 16 * b + e16) * QPITCH + 64 * st + 16 * g));
@@ -580,7 +599,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
     for (int st = 0; st < KS - 6; ++st)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < SB; ++b) {
         v4i x = __builtin_bit_cast(v4i, qf[st][b]);
         asm volatile("" : "+a"(x));
         qf[st][b] = __builtin_bit_cast(v8bf, x);
@@ -591,13 +610,15 @@ ragged_wide_kernel(const RaggedParams p) {
   bool strict = false, at_start = true;
   while (true) {
     if (!at_start) set_range();
-    float l4[4];
-    int e4[4];
+    float l4[RG];
+    int e4[RG];
     for (bool given = false;; given = true) {
       if (tid == 0) *redo = *high = *odd = 0;
       bool begun = false;
       if (given) {  // the true maxima of every row: scores only
-        float t0 = -__builtin_huge_valf(), t1 = t0;
+        float top[SB];
+#pragma unroll
+        for (int b = 0; b < SB; ++b) top[b] = -__builtin_huge_valf();
         for (c0 = 0; c0 < hi - lo; c0 += nt * kTile) {
           if (!lay_out()) continue;
 #pragma unroll 1
@@ -605,27 +626,30 @@ ragged_wide_kernel(const RaggedParams p) {
             bring(t, 0);
             landed();
             s_tile(smem);
-            float v[2][4];
+            float v[SB][4];
             scores(t, v);
-            t0 = fmaxf(t0, max4(v[0]));
-            t1 = fmaxf(t1, max4(v[1]));
+#pragma unroll
+            for (int b = 0; b < SB; ++b) top[b] = fmaxf(top[b], max4(v[b]));
             lds_barrier();
           }
         }
-        agree_max(t0, t1);
+        agree_max(top);
         lds_barrier();
         begun = true;
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int hg = 0; hg < 4; ++hg) acc[i][hg] = v4f{};
-      l_own[0] = l_own[1] = 0.0f;
-      m_seen[0] = m_seen[1] = -__builtin_huge_valf();
-      if (!begun) {
-        m_own[0] = m_own[1] = 0.0f;
+        for (int hg = 0; hg < RG; ++hg) acc[i][hg] = v4f{};
 #pragma unroll
-        for (int hg = 0; hg < 4; ++hg) m4[hg] = 0.0f;
+      for (int b = 0; b < SB; ++b) {
+        l_own[b] = 0.0f;
+        m_seen[b] = -__builtin_huge_valf();
+        if (!begun) m_own[b] = 0.0f;
+      }
+      if (!begun) {
+#pragma unroll
+        for (int hg = 0; hg < RG; ++hg) m4[hg] = 0.0f;
       }
       for (c0 = 0; c0 < hi - lo; c0 += nt * kTile) {
         const bool ready = at_start && c0 == 0;
@@ -637,14 +661,14 @@ ragged_wide_kernel(const RaggedParams p) {
       at_start = false;
       // each row's sum: its four lanes, then the two entry halves
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < SB; ++b) {
         l_own[b] = l_own[b] + __shfl_xor(l_own[b], 16, 64);
         l_own[b] = l_own[b] + __shfl_xor(l_own[b], 32, 64);
         if (g == 0) lsum[eh * 64 + 32 * hh + 16 * b + e16] = l_own[b];
       }
       if (!given) {  // (zero before the barriers of the pass; without an entry nothing is set)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < SB; ++b) {
           const float top = m_seen[b] * p.scale_log2, rise = top - m_own[b];
           if (rise > kRoomHigh) *high = 1;
           if (rise > kRoomAbove || (rise < kRoomBelow && m_own[b] == 0.0f && m_seen[b] > 0.5f * kHidden)) *redo = 1;
@@ -652,7 +676,7 @@ ragged_wide_kernel(const RaggedParams p) {
       }
       lds_barrier();
 #pragma unroll
-      for (int hg = 0; hg < 4; ++hg) l4[hg] = lsum[16 * hg + e16] + lsum[64 + 16 * hg + e16];
+      for (int hg = 0; hg < RG; ++hg) l4[hg] = lsum[16 * hg + e16] + lsum[64 + 16 * hg + e16];
       if (__builtin_expect(!given && *high != 0, 0)) {  // uniform
         // O^T through the tiles' place, half of it at a time, each lane its own: a few stores and a
         // short loop
@@ -660,11 +684,12 @@ ragged_wide_kernel(const RaggedParams p) {
         v4f* const slot = reinterpret_cast<v4f*>(smem) + tid;
         static_assert(2 * NI * NT * 16 <= M::PB, "half of O^T in the tiles' place");
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int h0 = 0; h0 < RG; h0 += 2) {
+          constexpr int W = RG < 2 ? RG : 2;  // row groups at a time
 #pragma unroll
-          for (int k = 0; k < 2 * NI; ++k) slot[k * NT] = acc[k >> 1][2 * half + (k & 1)];
+          for (int k = 0; k < W * NI; ++k) slot[k * NT] = acc[k / W][h0 + k % W];
 #pragma unroll 1
-          for (int k = 0; k < 2 * NI; ++k) {
+          for (int k = 0; k < W * NI; ++k) {
             const v4f x = slot[k * NT];
 #pragma unroll
             for (int r = 0; r < 4; ++r) any_bad = __builtin_fmaf(x[r], 0.0f, any_bad);
@@ -678,7 +703,7 @@ ragged_wide_kernel(const RaggedParams p) {
     }
     // (m, l) with l in [1, 2): the reference is not the maximum, so l may be far from 1
 #pragma unroll
-    for (int hg = 0; hg < 4; ++hg) {
+    for (int hg = 0; hg < RG; ++hg) {
       e4[hg] = l4[hg] > 0.0f && l4[hg] < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(l4[hg]) - 1 : 0;
       l4[hg] = __builtin_amdgcn_ldexpf(l4[hg], -e4[hg]);
       m4[hg] = l4[hg] == 0.0f ? -__builtin_huge_valf() : m4[hg] + static_cast<float>(e4[hg]);
@@ -694,7 +719,7 @@ ragged_wide_kernel(const RaggedParams p) {
     const int keep1 = (sub1 * p.HG < u.r1 ? sub1 * p.HG : u.r1) - u.r0;
     if (u.shares > 1) {
 #pragma unroll
-      for (int hg = 0; hg < 4; ++hg) {
+      for (int hg = 0; hg < RG; ++hg) {
         const int r = 16 * hg + col;
         if (r >= keep0 && r < keep1) {
           const float inv = l4[hg] > 0.0f || l4[hg] != l4[hg] ? __builtin_amdgcn_ldexpf(1.0f / l4[hg], -e4[hg]) : 0.0f;
@@ -716,7 +741,7 @@ ragged_wide_kernel(const RaggedParams p) {
       // through LDS, so that the rows leave in whole lines
       constexpr int OPITCH = 2 * D + 16;
 #pragma unroll
-      for (int hg = 0; hg < 4; ++hg) {
+      for (int hg = 0; hg < RG; ++hg) {
         const int r = 16 * hg + col;
         if (r >= keep0 && r < keep1) {
           int head;
@@ -736,7 +761,7 @@ ragged_wide_kernel(const RaggedParams p) {
       }
       if (bad != 0.0f) *odd = 1;
       lds_barrier();
-      if (p.G == 1 && keep0 == 0 && keep1 == 64) {  // one run of rows
+      if (!FEW && p.G == 1 && keep0 == 0 && keep1 == 64) {  // one run of rows
         u32x4* const ob = reinterpret_cast<u32x4*>(p.out + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
         int mine = tid;
         asm volatile("" : "+v"(mine));
@@ -747,7 +772,7 @@ ragged_wide_kernel(const RaggedParams p) {
         }
       } else {
 #pragma unroll 1
-        for (int at = tid; at < 64 * QROW; at += NT) {
+        for (int at = tid; at < ROWS * QROW; at += NT) {
           const int r = at / QROW;
           int head;
           if (r >= keep0 && r < keep1)
