@@ -493,9 +493,10 @@ int64_t fork_bytes(int64_t B, int64_t max_pages) { return align16_up(4 * B * max
 int64_t compact_bytes(int64_t P) { return 8 * ((P + kChunk - 1) / kChunk + 2) + 16 * P + 32; }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+constexpr int64_t kMaxRows = (1 << 24) - 1;  // a workgroup each: a launch has less than 2^32 threads
 
 #define MZK_CHECK_PAGES(name, B, max_pages, P)                                                                     \
-  MZK_CHECK_ARG((B) >= 0 && (B) <= kMaxInt && (max_pages) >= 0 && (max_pages) <= kMaxInt && (P) >= 0 && (P) <= kMaxInt, \
+  MZK_CHECK_ARG((B) >= 0 && (B) <= kMaxRows && (max_pages) >= 0 && (max_pages) <= kMaxInt && (P) >= 0 && (P) <= kMaxInt, \
                 name ": bad sizes")
 
 int check_pools(const char* name, const void* const* pools, const int64_t* entry, int n) {
@@ -527,7 +528,7 @@ extern "C" int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_r
   if (T == 0 || B == 0) return MZK_OK;
   MZK_CHECK_ARG(x && tables && lens && pool, "paged_append: null pointer");
   MZK_CHECK_ARG(aligned16(pool), "paged_append: the pool must be 16-byte aligned");
-  MZK_CHECK_ARG(T <= 4ll * kMaxInt, "paged_append: too many tokens");
+  MZK_CHECK_ARG(T <= 4 * kMaxRows, "paged_append: too many tokens");
   const AppendParams p{x, x_row_stride, T, cu, B, tables, table_stride, max_pages, lens, static_cast<uint8_t*>(pool),
                        pages, page, D, fmt ? nope : 0};
   const bool vec = aligned16(x) && x_row_stride % 8 == 0;
@@ -552,7 +553,7 @@ extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64
                               int64_t table_out_stride, int64_t* lens_out, int32_t* refs_out, int64_t* missing,
                               void* workspace, int64_t workspace_bytes, void* stream) {
   MZK_CHECK_PAGES("paged_grow", B, max_pages, pages);
-  MZK_CHECK_ARG(page >= 1, "paged_grow: pages of at least one entry");
+  MZK_CHECK_ARG(B >= 1 && pages >= 1 && page >= 1, "paged_grow: at least one sequence, and one page of one entry");
   MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_grow: strides smaller than the row");
   if (int rc = check_pools("paged_grow", pools, entry_bytes, npools)) return rc;
   MZK_CHECK_ARG(tables && lens && refs && tokens && tables_out && lens_out && refs_out && missing, "paged_grow: null pointer");
@@ -569,7 +570,6 @@ extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64
   p.free_in = p.over + B;
   p.want = p.free_in + p.chunks;
   p.list = reinterpret_cast<int32_t*>(p.want + 1);
-  if (B == 0 || pages == 0) return MZK_OK;
   hipStream_t s = as_stream(stream);
   grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 255) / 256), 256, 0, s>>>(p);
   grow_assign_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
@@ -594,7 +594,7 @@ extern "C" int mzk_paged_fork(const int32_t* tables, int64_t table_stride, int64
                               int64_t* lens_out, int32_t* refs_out, void* workspace, int64_t workspace_bytes,
                               void* stream) {
   MZK_CHECK_PAGES("paged_fork", B, max_pages, pages);
-  MZK_CHECK_ARG(rows_out >= 0 && rows_out <= kMaxInt && page >= 1, "paged_fork: bad sizes");
+  MZK_CHECK_ARG(rows_out >= 0 && rows_out <= kMaxRows && page >= 1, "paged_fork: bad sizes");
   MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_fork: strides smaller than the row");
   MZK_CHECK_ARG(tables && lens && refs && parents && tables_out && lens_out && refs_out, "paged_fork: null pointer");
   ForkParams p{tables, table_stride, B, max_pages, lens, refs, refs_out, pages, parents, rows_out, page, tables_out,

@@ -18,7 +18,7 @@
 namespace mzk {
 namespace {
 
-constexpr int kNoWindow = 1 << 30;  // also the most tokens of a call, so that no position overflows
+constexpr int kNoWindow = 1 << 30;  // a call has fewer tokens, so that no position overflows
 
 // Division of n < 2^31 by a constant of the call: floor(n m / 2^32) + n, shifted, with m = floor(2^32 (2^s -
 // d) / d) + 1 and 2^s >= d.  Three instructions; what is executed once runs from a cold instruction
@@ -303,10 +303,12 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     const int shares = shares_of(t, c, 1.0f / static_cast<float>(c));
     const int units = v * shares, before = wave_before(units, lane), blocks_before = wave_before(v, lane);
     const int total = __builtin_amdgcn_readlane(before + units, 63);
+    const int in_all = __builtin_amdgcn_readlane(blocks_before + v, 63);
+    const bool fits = total <= p.slots && in_all <= p.blocks_max;  // not where cu does not ascend
     const int per_xcd = (total + 7) / 8;
     k = (w & 7) * per_xcd + (w >> 3);
-    if (w == 0 && tid == 63) *p.blocks_out = blocks_before + v;
-    if ((w >> 3) >= per_xcd || k >= total) return false;
+    if (w == 0 && tid == 63) *p.blocks_out = fits ? in_all : 0;
+    if (!fits || (w >> 3) >= per_xcd || k >= total) return false;
     const int at = __builtin_ctzll(__ballot(k >= before && k < before + units));
     u.b = at;
     blocks = __builtin_amdgcn_readlane(v, at);
@@ -323,7 +325,7 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
     total = block_scan(total, before, l.scan, tid);
     const int per_xcd = static_cast<int>((total + 7) / 8);
     k = (w & 7) * per_xcd + (w >> 3);
-    const bool mine = (w >> 3) < per_xcd && k < total;
+    const bool mine = (w >> 3) < per_xcd && k < total && total <= p.slots;
     if (!mine && w != 0) return false;
     for (int i = 0; i < p.B; i += 256) {
       int shares = 1;
@@ -343,9 +345,10 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
       base += sum;
       blocks_base += blocks_sum;
     }
-    if (w == 0 && tid == 0) *p.blocks_out = static_cast<int32_t>(blocks_base);
+    const bool fits = total <= p.slots && blocks_base <= p.blocks_max;  // not where cu does not ascend
+    if (w == 0 && tid == 0) *p.blocks_out = fits ? static_cast<int32_t>(blocks_base) : 0;
     __syncthreads();
-    if (!mine) return false;
+    if (!mine || !fits) return false;
     u.b = static_cast<int>(l.scan[4]);
     blocks = l.blocks[u.b];
     u.shares = static_cast<int>(l.scan[6]);
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
 template <int FMT, int D, int NOPE>
 int launch_ragged(const RaggedParams& p, hipStream_t s) {
   // (find_unit's order takes 16 workgroups at a time)
-  const int64_t grid = p.slots ? p.slots : (p.blocks_max + 15) / 16 * 16;
+  const int64_t grid = p.slots ? p.slots : p.blocks_max / 16 * 16 + 16;
   using M = std::conditional_t<(D > 256), WideLds<FMT, D>, NarrowLds<FMT, D>>;
   void (*kern)(const RaggedParams);
   if constexpr (D > 256) kern = p.cu == nullptr && p.H <= 16 ? ragged_wide_kernel<FMT, D, NOPE, true> : ragged_wide_kernel<FMT, D, NOPE, false>;
@@ -566,6 +569,7 @@ void set_units(RaggedParams& p) {
 }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+constexpr int64_t kMaxBlocks = (1 << 24) - 16;  // a launch has less than 2^32 threads
 // Shares of at least 4 tiles (one sequence of 4096: 29 us); no shares where a token cannot see more than
 // 12 tiles, since the joining launch is 6 to 7 us (10 sequences x 128 heads over 8 tiles: 23.2 us with, 19.9
 // without; 2 sequences over 17: 22.1 with, 29.0 without).
@@ -598,9 +602,9 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                                 int topk, int64_t window, const float* sinks, void* workspace, int64_t workspace_bytes,
                                 void* out, float* lse, int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0, "paged_attend: bad sizes");
-  MZK_CHECK_ARG(T <= kNoWindow && B <= kMaxInt && H <= 65536 && pages >= 0 && pages <= kMaxInt && max_pages >= 0 &&
+  MZK_CHECK_ARG(T < kNoWindow && B <= kMaxInt && H <= 65536 && pages >= 0 && pages <= kMaxInt && max_pages >= 0 &&
                     max_pages <= kMaxInt,
-                "paged_attend: more than 2^30 tokens, or sizes of 2^31");
+                "paged_attend: 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(page >= 1, "paged_attend: pages of at least one entry");
   MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
                 "paged_attend: a sequence and a pool hold less than 2^31 entries");
@@ -611,8 +615,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   MZK_CHECK_ARG(!idx || (cu == nullptr && window == 0 && idx_row_stride >= topk),
                 "paged_attend: a list of entries takes one token per sequence and no window, rows of at least topk");
   MZK_CHECK_ARG(table_stride >= max_pages, "paged_attend: table rows shorter than max_pages");
-  if (T == 0 || B == 0) return MZK_OK;
-  MZK_CHECK_ARG(q && pool && tables && lens && out && lse, "paged_attend: null pointer");
+  if (T == 0) return MZK_OK;
+  MZK_CHECK_ARG(q && out && lse && (B == 0 || (pool && tables && lens)), "paged_attend: null pointer");
   MZK_CHECK_ARG(aligned16(q) && aligned16(pool) && aligned16(out) && aligned16(workspace),
                 "paged_attend: q, pool, workspace and out must be 16-byte aligned");
   RaggedParams p{};
@@ -641,16 +645,16 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt / 64 && T * H <= kMaxInt - 64, "paged_attend: too many rows");
+  MZK_CHECK_ARG(p.blocks_max < kMaxBlocks && T * H <= kMaxInt - 64, "paged_attend: too many rows");
   const int64_t need = attend_bytes(p.blocks_max, B, D);
   MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attend: workspace needs %lld bytes",
                 (long long)need);
   // what a sequence can hold, or a token see, in tiles
   int64_t most = max_pages * page;
-  if (window && window + T < most) most = window + T;
+  if (p.window + T < most) most = p.window + T;
   if (idx) most = topk;
   p.min_tiles = kMinTiles;
-  p.slots = (most + kTile - 1) / kTile > kWholeTiles ? unit_slots(p.blocks_max, B) : 0;
+  p.slots = B && (most + kTile - 1) / kTile > kWholeTiles ? unit_slots(p.blocks_max, B) : 0;
   if (p.slots) {
     p.blocks_out = static_cast<int32_t*>(workspace);
     p.joins = reinterpret_cast<JoinRow*>(static_cast<uint8_t*>(workspace) + 16);
@@ -681,7 +685,7 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
                               int64_t kv_row_stride, int G, int64_t window, const float* sinks, void* out, float* lse,
                               int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && G >= 1, "packed_mqa: bad sizes");
-  MZK_CHECK_ARG(T <= kNoWindow && B <= kMaxInt && H <= 65536, "packed_mqa: more than 2^30 tokens, or sizes of 2^31");
+  MZK_CHECK_ARG(T < kNoWindow && B <= kMaxInt && H <= 65536, "packed_mqa: 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(H % G == 0, "packed_mqa: %d heads do not divide into %d latents", H, G);
   MZK_CHECK_ARG(window >= 0, "packed_mqa: negative window");
   MZK_CHECK_ARG(kv_row_stride >= static_cast<int64_t>(G) * D && kv_row_stride % 8 == 0 && kv_row_stride < 1ll << 30,
@@ -707,6 +711,6 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.zero_tail = zero_tail;
-  MZK_CHECK_ARG(p.blocks_max <= kMaxInt / 64 && T * H <= kMaxInt - 64, "packed_mqa: too many rows");
+  MZK_CHECK_ARG(p.blocks_max < kMaxBlocks && T * H <= kMaxInt - 64, "packed_mqa: too many rows");
   return dispatch_ragged("packed_mqa", kFmtBf16, D, p, as_stream(stream));
 }

@@ -136,3 +136,16 @@ def test_packed_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_nothing(dev):
+    """No tokens, no sequences, sequences of no tokens."""
+    q = torch.randn(70, 8, 160, device=dev).bfloat16()
+    for t, cu in ((0, [0]), (0, [0, 0, 0]), (3, [0]), (70, [0]), (70, [0, 0, 0])):
+        o, lse = csa2_attn.packed(q[:t], q[:t, :2].contiguous(), torch.tensor(cu, device=dev))
+        assert o.shape == (t, 8, 160) and bool((o == 0).all()) and bool((lse == float("-inf")).all())
+    cu = torch.tensor([0, 30, 70], device=dev)
+    want = csa2_attn.packed(q, q[:, :2].contiguous(), cu)
+    for window in (40, 2 ** 30, 2 ** 62, 2 ** 64 + 1):
+        got = csa2_attn.packed(q, q[:, :2].contiguous(), cu, window=window)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

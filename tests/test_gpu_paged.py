@@ -315,6 +315,115 @@ def test_attend_padded_batch_and_other_stream(dev):
         assert bool((a[1] == 0).all()) and bool((b[3] == float("-inf")).all())
 
 
+@pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (512, "bf16")])
+@pytest.mark.parametrize("heads", [1, 2, 15, 16, 17])
+def test_attend_few_heads(dev, dim, fmt, heads):
+    """One token of few heads: whole, split and joined, behind a window."""
+    _check_attend(dev, [1, 0, 31, 32, 33, 370], 1, heads, dim, fmt, 16, None, heads)
+    _check_attend(dev, [6000, 1, 900], 1, heads, dim, fmt, 64, None, heads + 1, sinks=heads % 2 == 0)
+    _check_attend(dev, [600, 3, 900], 1, heads, dim, fmt, 24, 500, heads + 2)
+
+
+@pytest.mark.parametrize("heads,dim,fmt", [(4, 576, "fp8"), (128, 576, "fp8"), (16, 160, "bf16")])
+def test_attend_many_sequences(dev, heads, dim, fmt):
+    """More sequences than lanes: their units found together, split where one of them is long."""
+    g = _gen(heads)
+    lens = torch.randint(0, 90, (70,), generator=g).tolist()
+    lens[40] = 4000
+    _check_attend(dev, lens, 1, heads, dim, fmt, 32, None, heads)
+    new = torch.randint(0, 4, (70,), generator=g).tolist()
+    _check_attend(dev, lens, [min(a, b) for a, b in zip(new, lens)], heads, dim, fmt, 32, None, heads + 1)
+    _check_attend(dev, [n % 9 + 1 for n in range(1100)], 1, min(heads, 8), dim, fmt, 8, None, heads + 2)  # too many to split
+    _check_attend(dev, [n % 9 + 2 for n in range(1100)], [n % 3 for n in range(1100)], min(heads, 8), dim, fmt, 8, None, heads + 3)
+
+
+@pytest.mark.parametrize("heads,new", [(16, None), (64, None), (16, [5, 2]), (1, [40, 2])])
+@pytest.mark.parametrize("dim", [576, 160])
+def test_attend_unseen_entries_of_shares(dev, dim, heads, new):
+    """An entry that is not finite, in one share of a long sequence: the tokens that see it, and no other."""
+    lens, page = [3000, 40], 64
+    pool, tables, n64, _, _ = _setup(dev, lens, page, dim, "bf16", 25)
+    t, flat = tables.cpu(), pool.view(-1, dim)
+    count = new or [1, 1]
+    flat[_of(t, 0, 3000, page)[2998 if new else 2100], 5] = float("nan")   # the second last token's, or an old one
+    q = torch.randn(sum(count), heads, dim, generator=_gen(26)).bfloat16().to(dev)
+    cu = torch.tensor([0, count[0], sum(count)], device=dev)
+    o, lse = paged.attend(q, pool, tables, n64, cu=cu if new else None)
+    for b in range(2):
+        for i in range(count[b]):
+            pos, at = lens[b] - count[b] + i, int(cu[b]) + i
+            if b == 0 and pos >= (2998 if new else 2100):
+                assert not bool(torch.isfinite(o[at]).all(-1).any())
+                continue
+            e = flat[_of(t, b, pos + 1, page)].double()
+            seen = torch.ones(1, pos + 1, dtype=torch.bool, device=dev)
+            R.check(o[at:at + 1], lse[at:at + 1], R.attend(q[at:at + 1], e, seen, None), f"{b} {i}")
+
+
+@pytest.mark.parametrize("heads", [8, 64])
+@pytest.mark.parametrize("scale", [30.0, 1e4])
+@pytest.mark.parametrize("down", [False, True])
+def test_attend_wide_scores_of_shares(dev, heads, scale, down):
+    """As test_attend_wide_scores, for few heads too, rising or falling, split and whole."""
+    lens, page = [3000, 300], 64
+    for dim in (576, 160):
+        pool, tables, n64, x, cu = _setup(dev, lens, page, dim, "bf16", 33)
+        q = torch.randn(2, heads, dim, generator=_gen(34)).bfloat16().to(dev)
+        flat, t = pool.view(-1, dim), tables.cpu()
+        for b, n in enumerate(lens):
+            ramp = torch.linspace(-scale, scale, n, device=dev)[:, None]
+            flat[_of(t, b, n, page)] = ((-ramp if down else ramp) * q[b, 3].float()[None, :] / 24.0).bfloat16()
+        for last in (n64, n64.clamp(max=300)):
+            for tab in (tables, tables[:, :5].contiguous()):
+                o, lse = paged.attend(q, pool, tab, last)
+                for b in range(2):
+                    n = min(int(last[b]), tab.shape[1] * page)
+                    e = flat[_of(t, b, n, page)].double()
+                    R.check(o[b:b + 1], lse[b:b + 1], R.attend(q[b:b + 1], e, torch.ones(1, n, dtype=torch.bool, device=dev), None), f"{b}")
+
+
+def test_attend_nothing(dev):
+    """No tokens; no sequences; a window wider than anything; tokens that no sequence holds."""
+    pool, tables, n64, _, _ = _setup(dev, [50, 70], 16, 576, "fp8", 53)
+    q = torch.randn(5, 40, 576, generator=_gen(54)).bfloat16().to(dev)
+    o, lse = paged.attend(q[:0], pool, tables, n64, cu=torch.tensor([0, 0, 0], device=dev))
+    assert o.shape == (0, 40, 576) and lse.shape == (0, 40)
+    for none in (paged.attend(q, pool, tables[:0], n64[:0], cu=torch.tensor([0], device=dev)),
+                 paged.attend(q, pool, tables, n64, cu=torch.tensor([0, 0, 0], device=dev))):
+        assert bool((none[0] == 0).all()) and bool((none[1] == float("-inf")).all())
+    cu = torch.tensor([0, 2, 5], device=dev)
+    want = paged.attend(q, pool, tables, n64, cu=cu)
+    for window in (70, 2 ** 30, 2 ** 62, 2 ** 64 + 1):
+        got = paged.attend(q, pool, tables, n64, cu=cu, window=window)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_attend_shares_in_a_graph(dev):
+    """A captured call over split sequences, replayed with other lengths, tables and queries, and with
+    eager calls of the same workspace between the replays."""
+    lens, page, heads = [5000, 40, 2500], 32, 16
+    pool, tables, n64, _, _ = _setup(dev, lens, page, 576, "fp8", 63)
+    q = torch.randn(3, heads, 576, generator=_gen(64)).bfloat16().to(dev)
+    ws = torch.empty(paged.attend_workspace_bytes(3, heads, 576, 3, False), dtype=torch.uint8, device=dev)
+    out, lse = torch.empty_like(q), torch.empty(3, heads, device=dev)
+    s_q, s_t, s_n = q.clone(), tables.clone(), n64.clone()
+    paged.attend(s_q, pool, s_t, s_n, workspace=ws, out=out, lse=lse)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.attend(s_q, pool, s_t, s_n, workspace=ws, out=out, lse=lse)
+    for i, order in enumerate(([0, 1, 2], [2, 0, 1], [1, 1, 0], [0, 2, 2])):
+        s_t.copy_(tables[order])
+        s_n.copy_((n64[order] - 7 * i).clamp(min=0))
+        s_q.copy_(q.roll(i, 1))
+        want = paged.attend(s_q, pool, s_t, s_n)
+        paged.attend(q, pool, tables, n64, workspace=ws)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
 # ---- the pages ----------------------------------------------------------------------------
 
 def _grow_ref(tables, lens, refs, new, page, pool):
@@ -452,6 +561,27 @@ def test_compact(dev, batch, page, pages, most, inplace):
     dp = pool.to(dev)
     got = paged.compact(*d, pools=[dp], out=d if inplace else None)
     assert torch.equal(got[0].cpu(), want_t) and torch.equal(got[1].cpu(), want_r) and torch.equal(dp.cpu(), want_p)
+
+
+def test_grow_and_compact_many_pools(dev):
+    """More pools than one launch takes, of different entries."""
+    tables, lens, refs = _book(4, 12, 16, 400, 100, 9)
+    new = torch.randint(0, 20, (12,), generator=_gen(5))
+    pools = [torch.randint(0, 256, (400, 16, 4 * (1 + i % 5)), generator=_gen(i)).byte() for i in range(35)]
+    want = [_grow_ref(tables, lens, refs, new, 16, p) for p in pools]
+    assert want[0][3] == 0
+    dp = [p.to(dev) for p in pools]
+    got = paged.grow(*[t.to(dev) for t in (tables, lens, refs)], new.to(dev), 16, pools=dp)
+    for a, w in zip(dp, want):
+        assert torch.equal(a.cpu(), w[4])
+    moved = paged.compact(got[0], got[2], pools=dp)
+    t, m = got[0].cpu(), moved[0].cpu()
+    for b in range(12):
+        for j in range(-(-int(got[1][b]) // 16)):
+            for a, w in zip(dp, want):
+                assert torch.equal(a[int(m[b, j])].cpu(), w[4][int(t[b, j])])
+    used = int((moved[1] > 0).sum())
+    assert bool((moved[1][:used] > 0).all()) and used == int((got[2] > 0).sum())
 
 
 # ---- together -----------------------------------------------------------------------------

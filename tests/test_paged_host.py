@@ -142,3 +142,24 @@ def test_entry_points_check_their_arguments():
     co = [p, 8, 4, 8, p, 100, 16, None, None, 0, p, 8, p, p, 1 << 20, None]
     refuse("mzk_paged_compact", co[:14] + [16] + co[15:], "workspace")
     refuse("mzk_paged_compact", co[:9] + [1] + co[10:], "pool list")
+
+
+def test_sizes_past_a_launch_are_refused():
+    lib = _lib.load()
+    p = ctypes.c_void_p(256)
+
+    def refuse(name, args, text):
+        assert getattr(lib, name)(*args) < 0
+        assert text in lib.mzk_last_error().decode(), lib.mzk_last_error()
+
+    refuse("mzk_paged_attend", [p, 1 << 30, 1, 576, p, 4, 1, 512, p, 16, 64, p, 8, 8, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None], "tokens")
+    refuse("mzk_paged_attend", [p, 1 << 24, 128, 576, None, 1 << 24, 1, 512, p, 16, 64, p, 8, 8, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None],
+           "too many rows")
+    refuse("mzk_paged_attend", [p, 4, 8, 576, None, 4, 1, 512, p, 1 << 26, 64, p, 8, 8, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None], "less than 2^31")
+    refuse("mzk_packed_mqa", [p, 1 << 30, 1, 576, p, 3, p, 576, 1, 0, None, p, p, 0, None], "tokens")
+    refuse("mzk_packed_mqa", [p, 1 << 29, 1, 64, p, 3, p, 64, 1, 0, None, p, p, 0, None], "too many rows")
+    refuse("mzk_paged_append", [p, 1, 1 << 27, 576, p, 4, p, 8, 8, p, 1, 576, 512, p, 16, 64, None], "too many tokens")
+    refuse("mzk_paged_grow", [p, 8, 1 << 24, 8, p, p, 100, p, 16, None, None, 0, p, 8, p, p, p, p, 1 << 40, None], "bad sizes")
+    refuse("mzk_paged_grow", [p, 8, 0, 8, p, p, 100, p, 16, None, None, 0, p, 8, p, p, p, p, 1 << 40, None], "at least one sequence")
+    refuse("mzk_paged_fork", [p, 8, 4, 8, p, p, 100, p, 1 << 24, 16, p, 8, p, p, p, 1 << 40, None], "bad sizes")
+    assert lib.mzk_paged_attend(p, 0, 128, 576, None, 0, 1, 512, p, 16, 64, p, 8, 8, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None) == 0
