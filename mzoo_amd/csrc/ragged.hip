@@ -447,10 +447,11 @@ constexpr float kHidden = -3.0e38f;  // a hidden entry's score: weight 0
 #include "ragged_narrow.h"
 
 // Joins the shares of 16 rows of a row block: o = sum_s w_s O_s / sum_s w_s with w_s = l_s 2^(m_s - m), and the
-// sink.  A wave takes one 16-channel block, so that a load instruction covers 1 KB of a share.
+// sink.  A wave takes one 16-channel block, so that a load instruction covers 1 KB of a share; SPLIT: the
+// four waves of a workgroup take a quarter of one's shares each.
 // Bound by latency for a few rows (record, then maxima and sums, then the shares' rows, eight of them
 // requested together) and by the memory for many.
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
   constexpr int NB = D / 16;
   __shared__ float weight[16][kMaxShares + 1];
@@ -487,23 +488,34 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
     }
   }
   __syncthreads();
-  const int r = (tid & 63) >> 2, c = 4 * (tid & 3), row = r0 + r, blk = 4 * blockIdx.y + (tid >> 6);
-  if (row >= j.rows || blk >= NB) return;
-  const float* const o = p.part_o + (static_cast<int64_t>(j.slot0) * NB + blk) * 1024 + 16 * row + c;
+  const int wave = tid >> 6, r = (tid & 63) >> 2, c = 4 * (tid & 3), row = r0 + r;
+  const int blk = SPLIT ? static_cast<int>(blockIdx.y) : 4 * static_cast<int>(blockIdx.y) + wave;
+  if (!SPLIT && (row >= j.rows || blk >= NB)) return;
+  const float* const o = p.part_o + (static_cast<int64_t>(j.slot0) * NB + blk) * 1024 + 16 * (row < j.rows ? row : r0) + c;
   const int64_t step = 64ll * D * j.step;
   v4f sum = v4f{};
   constexpr int AHEAD = 8;
-  for (int s0 = 0; s0 < j.shares; s0 += AHEAD) {
+  const int per = SPLIT ? (j.shares + 3) / 4 : j.shares;
+  const int from = SPLIT ? per * wave : 0, to = from + per < j.shares ? from + per : j.shares;
+  for (int s0 = from; s0 < to; s0 += AHEAD) {
     v4f v[AHEAD];
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) v[s] = *reinterpret_cast<const v4f*>(o + step * (s0 + s < j.shares ? s0 + s : s0));
+    for (int s = 0; s < AHEAD; ++s) v[s] = *reinterpret_cast<const v4f*>(o + step * (s0 + s < to ? s0 + s : s0));
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s)
-      if (s0 + s < j.shares) {
+      if (s0 + s < to) {
         const float w = weight[r][s0 + s];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[s][i], sum[i]);
       }
+  }
+  if constexpr (SPLIT) {
+    __shared__ v4f part[3][64];
+    if (wave > 0) part[wave - 1][tid & 63] = sum;
+    __syncthreads();
+    if (wave > 0 || row >= j.rows) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) sum = sum + part[w][tid];
   }
   *reinterpret_cast<uint2*>(p.out + (j.row0 + row) * D + 16 * blk + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
 }
@@ -532,7 +544,13 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
     attr_set[which][dev].store(true, std::memory_order_release);
   }
   kern<<<static_cast<unsigned>(grid), 256, M::LDS, s>>>(p);
-  if (p.slots) join_kernel<D><<<dim3(static_cast<unsigned>(4 * p.blocks_max), (D / 16 + 3) / 4), 256, 0, s>>>(p);
+  if (p.slots) {
+    const unsigned x = static_cast<unsigned>(4 * p.blocks_max);
+    // one sequence of up to 32768 x 128 heads, 2 blocks of 128 shares: 44 us, 50 with a wave per channel block; 200
+    // blocks: 209 us, 179
+    if (p.slots >= 16 * p.blocks_max) join_kernel<D, true><<<dim3(x, D / 16), 256, 0, s>>>(p);
+    else join_kernel<D, false><<<dim3(x, (D / 16 + 3) / 4), 256, 0, s>>>(p);
+  }
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;
 }
@@ -570,24 +588,29 @@ void set_units(RaggedParams& p) {
 
 constexpr int64_t kMaxInt = 0x7fffffff;
 constexpr int64_t kMaxBlocks = (1 << 24) - 16;  // a launch has less than 2^32 threads
-// Shares of at least 4 tiles (one sequence of 4096: 29 us); no shares where a token cannot see more than
-// 12 tiles, since the joining launch is 6 to 7 us (10 sequences x 128 heads over 8 tiles: 23.2 us with, 19.9
-// without; 2 sequences over 17: 22.1 with, 29.0 without).
+// Shares of at least 4 tiles (one sequence of 4096: 28 us).
 constexpr int kMinTiles = 4;
-constexpr int kWholeTiles = 12;
 
-// How many units a call is split into: 0 for as many as blocks.  With fewer blocks than twice the 256
-// compute units (a unit fills one), up to 256, or 1024 where the blocks alone fill more than half,
-// so that sequences of different lengths still end together.
-int unit_slots(int64_t blocks, int64_t B) {
+// The most units a call is split into.  A unit fills a compute unit (two of them at D <= 160), so one
+// round of them, or two where the blocks alone fill more than half a round (and any number of blocks
+// past two rounds stays whole): 100 sequences of up to 20000 x 128 heads, 200 blocks, take 697 us whole,
+// 457 as 512 units and 475 as 1024; 400 blocks of up to 16000 entries 977, 924 and 769.
+int unit_slots(int64_t blocks, int64_t B, int D) {
   if (blocks > 512 || B > kPlanRows) return 0;
-  return blocks <= 128 ? 256 : 1024;
+  if (blocks <= 128) return D <= 160 ? 512 : 256;
+  return blocks <= 256 ? 512 : 1024;
 }
+
+// Whether a call is split in whose longest sequence a token may see so many tiles.  The joining launch
+// and the second start of a compute unit cost some 7 and 15 us.  10 sequences x 128 heads over 8 tiles take
+// 19.9 us whole and 23.2 split, 2 over 17 tiles 29.0 and 22.1; 140 blocks over 31 tiles 49 and 75, over 94
+// tiles 115 and 102; 500 blocks over 125 tiles 290 and 317.
+bool splits(int64_t tiles, int64_t blocks) { return tiles > 12 && tiles > blocks / 2; }
 
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 int64_t attend_bytes(int64_t blocks, int64_t B, int D) {
-  const int slots = unit_slots(blocks, B);
+  const int slots = unit_slots(blocks, B, D);
   return slots ? 16 + align16_up(static_cast<int64_t>(sizeof(JoinRow)) * blocks) + static_cast<int64_t>(slots) * 64 * 4 * (D + 2) : 0;
 }
 
@@ -654,7 +677,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   if (p.window + T < most) most = p.window + T;
   if (idx) most = topk;
   p.min_tiles = kMinTiles;
-  p.slots = B && (most + kTile - 1) / kTile > kWholeTiles ? unit_slots(p.blocks_max, B) : 0;
+  p.slots = B && splits((most + kTile - 1) / kTile, p.blocks_max) ? unit_slots(p.blocks_max, B, D) : 0;
   if (p.slots) {
     p.blocks_out = static_cast<int32_t*>(workspace);
     p.joins = reinterpret_cast<JoinRow*>(static_cast<uint8_t*>(workspace) + 16);

@@ -337,6 +337,15 @@ def test_attend_many_sequences(dev, heads, dim, fmt):
     _check_attend(dev, [n % 9 + 2 for n in range(1100)], [n % 3 for n in range(1100)], min(heads, 8), dim, fmt, 8, None, heads + 3)
 
 
+@pytest.mark.parametrize("blocks", [128, 129, 256, 257, 512, 513])
+@pytest.mark.parametrize("dim", [576, 64])
+def test_attend_splits_by_blocks(dev, blocks, dim):
+    """Either side of the numbers of blocks at which a call is split otherwise, one sequence long enough for it."""
+    lens = [n % 5 for n in range(blocks)]
+    lens[blocks // 3] = 16 * blocks + 40
+    _check_attend(dev, lens, 1, 3, dim, "bf16", 16, None, blocks)
+
+
 @pytest.mark.parametrize("heads,new", [(16, None), (64, None), (16, [5, 2]), (1, [40, 2])])
 @pytest.mark.parametrize("dim", [576, 160])
 def test_attend_unseen_entries_of_shares(dev, dim, heads, new):
