@@ -8,8 +8,8 @@
 //
 // A unit of work is a block of 64 rows -- a row is a head of a token, the heads of one latent
 // innermost, so 64 rows are 64 heads of a token or all heads of several -- over all of the
-// sequence's entries, or, where there are fewer blocks than compute units, over a share of them;
-// the shares' results are joined by a second launch.
+// sequence's entries, or, where the blocks alone would leave compute units idle, over a share of
+// them; the shares' results are joined by a second launch (unit_slots, splits).
 #include <type_traits>
 
 #include "common.h"
@@ -450,7 +450,7 @@ constexpr float kHidden = -3.0e38f;  // a hidden entry's score: weight 0
 // sink.  A wave takes one 16-channel block, so that a load instruction covers 1 KB of a share; SPLIT: the
 // four waves of a workgroup take a quarter of one's shares each.
 // Bound by latency for a few rows (record, then maxima and sums, then the shares' rows, eight of them
-// requested together) and by the memory for many.
+// requested together; 6 us) and by the memory for many (64 blocks of four shares of 576 channels, 38 MB: 12 us).
 template <int D, bool SPLIT>
 __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
   constexpr int NB = D / 16;

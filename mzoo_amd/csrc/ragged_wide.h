@@ -17,6 +17,12 @@
 // repeating the scores of hh = 0.  The matrix work falls to a quarter, and the clock need not: 32
 // sequences of up to 32k x 16 heads, 8-bit entries, 154 -> 123 us.
 //
+// What bounds it: the matrix units, shared with one wave's issue of everything else.  8192 tokens x 128 heads of 576
+// channels, causal, take 8.3 to 9.2 ms (1190 to 1080 TFLOP/s, by the clock the device holds); 32 sequences of up
+// to 32768 x 128 heads, 8-bit, 238 us (850 TFLOP/s: shares of unequal length, a start of 15 us); one of
+// 4096 21 us, a chain: unit 3, q and tables 5, tiles 5, results 4.  Behind a window of 128, 16 heads,
+// 23.7 K tokens take 420 us: q 4, tiles 6, results 3 of a unit's 18 us, one after the other.
+//
 // A tile in LDS is D / 64 columns of 32 rows of 128 bytes: a wave's load instruction (8 rows x 128
 // bytes, a lane 16 of them) fills 1 KB of one column, in lane order as the hardware wants it, from
 // one address per lane and tile.  The 16-byte piece x of row r sits at slot x ^ wide_swz(r).

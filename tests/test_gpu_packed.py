@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from mzoo_amd import csa2_attn
+from mzoo_amd import csa2_attn, paged
+from oracle import quant as OQ
 from tests import ragged_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +150,58 @@ def test_nothing(dev):
     for window in (40, 2 ** 30, 2 ** 62, 2 ** 64 + 1):
         got = csa2_attn.packed(q, q[:, :2].contiguous(), cu, window=window)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (160, "bf16")])
+def test_prompts_then_steps(dev, dim, fmt):
+    """As a server runs them: pages for prompts of different lengths, their attention packed, and from the
+    pages in two chunks; then steps of one token, one sequence ending and another forked on the way."""
+    page, pages, heads, rope = 16, 90, 24, 64 if dim == 576 else 32
+    g = torch.Generator().manual_seed(dim)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)
+    lens = [50, 1, 33, 80]
+    pool = paged.new_pool(pages, page, dim, fmt, rope=rope, device=dev)
+    tables = torch.full((4, 12), -1, dtype=torch.int32, device=dev)
+    n, refs = torch.zeros(4, dtype=torch.int64, device=dev), torch.zeros(pages, dtype=torch.int32, device=dev)
+    state, sinks = (tables, n, refs), torch.randn(heads, generator=g).to(dev)
+    hist = [rnd(k, dim) for k in lens]
+    q = [rnd(k, heads, dim) for k in lens]
+
+    def values(x):  # what a page gives back of x
+        if fmt == "bf16" or len(x) == 0:
+            return x.double()
+        return torch.from_numpy(OQ.unpack_latent_fp8_b128(OQ.pack_latent_fp8_b128(x.float().cpu().numpy(), dim - rope), dim - rope, rope)).to(dev)
+
+    def see(o, lse, qs, x, first, sink, what):
+        if len(qs) == 0:
+            return
+        seen = torch.arange(x.shape[0], device=dev)[None, :] <= first + torch.arange(qs.shape[0], device=dev)[:, None]
+        R.check(o, lse, R.attend(qs, x.double(), seen, sink), what)
+
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), device=dev)
+    o, lse = csa2_attn.packed(torch.cat(q), torch.cat(hist)[:, None], cu, sinks=sinks)
+    for b in range(4):
+        see(o[cu[b]:cu[b + 1]], lse[cu[b]:cu[b + 1]], q[b], hist[b], 0, sinks, f"prompt {b}")
+    half = [k // 2 for k in lens]
+    for lo, hi in ((lambda b: 0, lambda b: half[b]), (lambda b: half[b], lambda b: lens[b])):
+        new = [hi(b) - lo(b) for b in range(4)]
+        c = torch.tensor(np.concatenate([[0], np.cumsum(new)]), device=dev)
+        assert int(paged.grow(*state, torch.tensor(new, device=dev), page, pools=[pool], out=state)[3]) == 0
+        paged.append(pool, tables, n, torch.cat([hist[b][lo(b):hi(b)] for b in range(4)]), cu=c, rope=rope)
+        o, lse = paged.attend(torch.cat([q[b][lo(b):hi(b)] for b in range(4)]), pool, tables, n, cu=c, sinks=sinks, rope=rope)
+        for b in range(4):
+            see(o[c[b]:c[b + 1]], lse[c[b]:c[b + 1]], q[b][lo(b):hi(b)], values(hist[b][:hi(b)]), lo(b), sinks, f"chunk {b}")
+    ones = torch.ones(4, dtype=torch.int64, device=dev)
+    for i in range(6):
+        if i == 3:  # sequence 1 ends, its row goes on from sequence 3
+            paged.fork(*state, torch.tensor([0, 3, 2, 3], dtype=torch.int32, device=dev), page, out=state)
+            hist[1] = hist[3]
+        kv, qs = rnd(4, dim), rnd(4, heads, dim)
+        assert int(paged.grow(*state, ones, page, pools=[pool], out=state)[3]) == 0
+        paged.append(pool, tables, n, kv, rope=rope)
+        o, lse = paged.attend(qs, pool, tables, n, sinks=sinks, rope=rope)
+        for b in range(4):
+            hist[b] = torch.cat([hist[b], kv[b:b + 1]])
+            see(o[b:b + 1], lse[b:b + 1], qs[b:b + 1], values(hist[b]), hist[b].shape[0] - 1, sinks, f"step {i} {b}")
+    used = -(-n // page)  # rows 1 and 3 share their whole pages of the fork
+    assert int((refs > 0).sum()) == int(used.sum()) - 83 // page
