@@ -526,16 +526,20 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   const int64_t grid = p.slots ? p.slots : p.blocks_max / 16 * 16 + 16;
   using M = std::conditional_t<(D > 256), WideLds<FMT, D>, NarrowLds<FMT, D>>;
   void (*kern)(const RaggedParams);
-  if constexpr (D > 256) kern = p.cu == nullptr && p.H <= 16 ? ragged_wide_kernel<FMT, D, NOPE, true> : ragged_wide_kernel<FMT, D, NOPE, false>;
-  else kern = ragged_narrow_kernel<FMT, D, NOPE>;
+  int which = 0;
+  if constexpr (D > 256) {
+    which = p.cu || p.H > 32 ? 0 : p.H > 16 ? 1 : 2;
+    kern = which == 0 ? ragged_wide_kernel<FMT, D, NOPE, 4> : which == 1 ? ragged_wide_kernel<FMT, D, NOPE, 2> : ragged_wide_kernel<FMT, D, NOPE, 1>;
+  } else {
+    kern = ragged_narrow_kernel<FMT, D, NOPE>;
+  }
   // the dynamic-LDS limit is a per-device function attribute: set once per device
-  static std::atomic<bool> attr_set[2][kMaxDevices] = {};  // setting it twice is harmless
+  static std::atomic<bool> attr_set[3][kMaxDevices] = {};  // setting it twice is harmless
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
     set_last_error("ragged attention: no usable current device");
     return MZK_ELAUNCH;
   }
-  const int which = D > 256 && p.cu == nullptr && p.H <= 16;
   if (!attr_set[which][dev].load(std::memory_order_acquire)) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, M::LDS) != hipSuccess) {
       set_last_error("ragged attention: cannot raise the kernel's LDS limit to %d bytes", M::LDS);

@@ -13,9 +13,9 @@
 // the softmax of u+1, while tile u+2 (8-bit entries, dequantized from registers) or u+3 (bf16
 // entries, loaded straight into LDS) arrives.
 //
-// Up to 16 rows (FEW: one new token of up to 16 heads): one row group instead of four, the waves of hh = 1
-// repeating the scores of hh = 0.  The matrix work falls to a quarter, and the clock need not: 32
-// sequences of up to 32k x 16 heads, 8-bit entries, 154 -> 123 us.
+// RG: the unit's row groups of 16, 4, or for one new token of up to 16 or 32 heads 1 or 2 (1: the waves of
+// hh = 1 repeat the scores of hh = 0).  The matrix work falls with them, and the device's clock need not: 32
+// sequences of up to 32k, 8-bit entries, 154 -> 120 us with 16 heads, 158 -> 132 with 32.
 //
 // What bounds it: the matrix units, shared with one wave's issue of everything else.  8192 tokens x 128 heads of 576
 // channels, causal, take 8.3 to 9.2 ms (1190 to 1080 TFLOP/s, by the clock the device holds); 32 sequences of up
@@ -81,14 +81,13 @@ struct WideRaw {
   u32x4 s;  // the entry's four block scales
 };
 
-template <int FMT, int D, int NOPE, bool FEW>
+template <int FMT, int D, int NOPE, int RG>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 ragged_wide_kernel(const RaggedParams p) {
   using M = WideLds<FMT, D>;
   constexpr bool kDirect = M::kDirect;
   constexpr int NT = 256, KS = D / 32, NI = D / 64, COL = 4096;
-  // row groups of 16: of the unit, and of a wave's scores (FEW: both halves of the waves have the same)
-  constexpr int RG = FEW ? 1 : 4, SB = FEW ? 1 : 2, ROWS = 16 * RG;
+  constexpr int SB = RG == 4 ? 2 : 1, ROWS = 16 * RG;  // row groups of a wave's scores; rows
   constexpr int EB = Layout<FMT, D, NOPE>::kEntryBytes;
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* const tab = reinterpret_cast<uint32_t*>(smem + M::TAB);
@@ -104,7 +103,7 @@ ragged_wide_kernel(const RaggedParams p) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int eh = wave & 1, hh = FEW ? 0 : wave >> 1;
+  const int eh = wave & 1, hh = RG == 1 ? 0 : wave >> 1;
   const int g = lane >> 4, e16 = lane & 15;
 
   Unit u;
@@ -116,7 +115,7 @@ ragged_wide_kernel(const RaggedParams p) {
   const int rows = u.r1 - u.r0;
   constexpr int QROW = D / 8, QP = (ROWS * QROW + NT - 1) / NT;
   u32x4 qraw[QP];
-  if (!FEW && p.G == 1 && rows == 64) {  // one run of rows
+  if (RG == 4 && p.G == 1 && rows == 64) {  // one run of rows
     const u32x4* const qb = reinterpret_cast<const u32x4*>(p.q + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
 #pragma unroll
     for (int k = 0; k < QP; ++k) qraw[k] = (qb + NT * k)[tid];
@@ -137,7 +136,7 @@ ragged_wide_kernel(const RaggedParams p) {
   int tok_b[SB];  // the tokens of this lane's rows
 #pragma unroll
   for (int b = 0; b < SB; ++b) {
-    const int r = u.r0 + 32 * hh + 16 * b + e16;
+    const int r = u.r0 + 16 * (SB * hh + b) + e16;
     tok_b[b] = p.by_heads(r < u.r1 ? r : u.r0);
   }
   float sink = -__builtin_huge_valf();  // of row tid, kept in LDS for the end
@@ -299,17 +298,17 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
     for (int b = 0; b < SB; ++b) {
       t[b] = row_max(t[b]);
-      if (g == 0) pmax[eh * 64 + 32 * hh + 16 * b + e16] = t[b];
+      if (g == 0) pmax[eh * 64 + 16 * (SB * hh + b) + e16] = t[b];
     }
     lds_barrier();
     auto known = [](float a, float b) { const float m = fmaxf(a, b); return m == -__builtin_huge_valf() ? 0.0f : m; };
 #pragma unroll
     for (int hg = 0; hg < RG; ++hg) m4[hg] = known(pmax[16 * hg + e16], pmax[64 + 16 * hg + e16]);
 #pragma unroll
-    for (int b = 0; b < SB; ++b) m_own[b] = known(pmax[32 * hh + 16 * b + e16], pmax[64 + 32 * hh + 16 * b + e16]);
+    for (int b = 0; b < SB; ++b) m_own[b] = known(pmax[16 * (SB * hh + b) + e16], pmax[64 + 16 * (SB * hh + b) + e16]);
   };
   auto put_p = [&](int t, int b, uint2 w) __attribute__((always_inline)) {
-    *reinterpret_cast<uint2*>(pbuf + (t & 1) * 4096 + 2048 * hh + 1024 * b + 16 * lane + 8 * eh) = w;
+    *reinterpret_cast<uint2*>(pbuf + (t & 1) * 4096 + 1024 * (SB * hh + b) + 16 * lane + 8 * eh) = w;
   };
   auto read_v = [&](const uint8_t* vt, int i, v4s (&va)[2]) __attribute__((always_inline)) {
     const uint8_t* tp = vt + v_at + COL * i;
@@ -598,7 +597,7 @@ ragged_wide_kernel(const RaggedParams p) {
     for (int b = 0; b < SB; ++b)
 #pragma unroll
       for (int st = 0; st < KS; ++st)
-        qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + QB + (32 * hh + 16 * b + e16) * QPITCH + 64 * st + 16 * g));
+        qf[st][b] = __builtin_bit_cast(v8bf, *reinterpret_cast<const v4i*>(smem + QB + (16 * (SB * hh + b) + e16) * QPITCH + 64 * st + 16 * g));
     lds_barrier();
     // the first query fragments live in accumulation registers beside O^T, which the matrix
     // instructions read directly; left to itself the compiler spills
@@ -623,7 +622,7 @@ ragged_wide_kernel(const RaggedParams p) {
   for (int k = 0; k < LINES; ++k) hint[k] = 0;
   auto look_ahead = [&]() __attribute__((always_inline)) {
     const int64_t row = static_cast<int64_t>(u.t0) * p.H + u.r0 - 256 * 64;
-    if (FEW || !p.cu || p.slots || p.G != 1 || row < 0 || hi - lo > 32 * kTile) return;
+    if (RG < 4 || !p.cu || p.slots || p.G != 1 || row < 0 || hi - lo > 32 * kTile) return;
     int line = tid;
     asm volatile("" : "+v"(line));
     const uint8_t* const at = reinterpret_cast<const uint8_t*>(p.q + row * D);
@@ -690,7 +689,7 @@ ragged_wide_kernel(const RaggedParams p) {
       for (int b = 0; b < SB; ++b) {
         l_own[b] = l_own[b] + __shfl_xor(l_own[b], 16, 64);
         l_own[b] = l_own[b] + __shfl_xor(l_own[b], 32, 64);
-        if (g == 0) lsum[eh * 64 + 32 * hh + 16 * b + e16] = l_own[b];
+        if (g == 0) lsum[eh * 64 + 16 * (SB * hh + b) + e16] = l_own[b];
       }
       if (!given) {  // (zero before the barriers of the pass; without an entry nothing is set)
 #pragma unroll
@@ -789,7 +788,7 @@ ragged_wide_kernel(const RaggedParams p) {
 #pragma unroll
       for (int k = 0; k < LINES; ++k) asm volatile("" : : "v"(hint[k]));
       lds_barrier();
-      if (!FEW && p.G == 1 && keep0 == 0 && keep1 == 64) {  // one run of rows
+      if (RG == 4 && p.G == 1 && keep0 == 0 && keep1 == 64) {  // one run of rows
         u32x4* const ob = reinterpret_cast<u32x4*>(p.out + (static_cast<int64_t>(u.t0) * p.H + u.r0) * D);
         int mine = tid;
         asm volatile("" : "+v"(mine));

@@ -316,7 +316,7 @@ def test_attend_padded_batch_and_other_stream(dev):
 
 
 @pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (512, "bf16")])
-@pytest.mark.parametrize("heads", [1, 2, 15, 16, 17])
+@pytest.mark.parametrize("heads", [1, 2, 15, 16, 17, 31, 32, 33])
 def test_attend_few_heads(dev, dim, fmt, heads):
     """One token of few heads: whole, split and joined, behind a window."""
     _check_attend(dev, [1, 0, 31, 32, 33, 370], 1, heads, dim, fmt, 16, None, heads)
@@ -346,7 +346,7 @@ def test_attend_splits_by_blocks(dev, blocks, dim):
     _check_attend(dev, lens, 1, 3, dim, "bf16", 16, None, blocks)
 
 
-@pytest.mark.parametrize("heads,new", [(16, None), (64, None), (16, [5, 2]), (1, [40, 2])])
+@pytest.mark.parametrize("heads,new", [(16, None), (20, None), (64, None), (16, [5, 2]), (1, [40, 2])])
 @pytest.mark.parametrize("dim", [576, 160])
 def test_attend_unseen_entries_of_shares(dev, dim, heads, new):
     """An entry that is not finite, in one share of a long sequence: the tokens that see it, and no other."""
@@ -369,7 +369,7 @@ def test_attend_unseen_entries_of_shares(dev, dim, heads, new):
             R.check(o[at:at + 1], lse[at:at + 1], R.attend(q[at:at + 1], e, seen, None), f"{b} {i}")
 
 
-@pytest.mark.parametrize("heads", [8, 64])
+@pytest.mark.parametrize("heads", [8, 24, 64])
 @pytest.mark.parametrize("scale", [30.0, 1e4])
 @pytest.mark.parametrize("down", [False, True])
 def test_attend_wide_scores_of_shares(dev, heads, scale, down):
