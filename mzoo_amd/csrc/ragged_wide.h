@@ -251,7 +251,10 @@ ragged_wide_kernel(const RaggedParams p) {
     }
     lds_barrier();
     const uint64_t some = __ballot(lane < nt && masks[lane < nt ? lane : 0] != 0u);
-    if (some == 0) return false;
+    if (some == 0) {
+      lds_barrier();  // the next chunk's codes come here
+      return false;
+    }
     first = __builtin_ctzll(some);
     last = 63 - __builtin_clzll(some);
     const uint32_t any = tab[first * kTile + __builtin_ctz(masks[first])];

@@ -337,6 +337,25 @@ def test_attend_many_sequences(dev, heads, dim, fmt):
     _check_attend(dev, [n % 9 + 2 for n in range(1100)], [n % 3 for n in range(1100)], min(heads, 8), dim, fmt, 8, None, heads + 3)
 
 
+@pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (160, "bf16")])
+@pytest.mark.parametrize("heads", [3, 40])
+def test_attend_long_runs_of_no_page(dev, dim, fmt, heads):
+    """Chunks of entry codes of which none is there, before, between and behind others, in one unit (so many
+    sequences are not split)."""
+    page, lens = 64, [9000, 8000] + [1] * 520
+    pool, tables, n64, _, _ = _setup(dev, lens, page, dim, fmt, 14)
+    tables[0, :70] = -1
+    tables[0, 75:130] = -1
+    tables[1, 2:] = -1
+    q = torch.randn(522, heads, dim, generator=_gen(15)).bfloat16().to(dev)
+    o, lse = paged.attend(q, pool, tables, n64, rope=ROPE[dim])
+    vals, t = _entries(pool, dim).to(dev), tables.cpu()
+    for b in (0, 1, 2, 521):
+        at = [a for p, a in enumerate(_of(t, b, lens[b], page)) if int(t[b, p // page]) >= 0]
+        seen = torch.ones(1, len(at), dtype=torch.bool, device=dev)
+        R.check(o[b:b + 1], lse[b:b + 1], R.attend(q[b:b + 1], vals[at], seen, None), f"sequence {b}")
+
+
 @pytest.mark.parametrize("blocks", [128, 129, 256, 257, 512, 513])
 @pytest.mark.parametrize("dim", [576, 64])
 def test_attend_splits_by_blocks(dev, blocks, dim):
