@@ -199,7 +199,7 @@ def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int |
         out = torch.empty_like(q)
         lse = torch.empty((t, h), dtype=torch.float32, device=dev)
     args = (q.data_ptr(), t, h, d, cu.data_ptr(), cu.shape[0] - 1, kv.data_ptr(), row if t > 1 else g * d, g, min(window or 0, 1 << 30),
-            _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(), 0 if given else 1, _lib.stream_of(q))
+            _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(), 0 if given else 1, _lib.raw_stream(dev))
     if torch.cuda.current_device() == dev.index:
         _lib.call("mzk_packed_mqa", *args)
     else:

@@ -95,7 +95,7 @@ def _pool(what: str, pool: torch.Tensor, dim: int, rope: int) -> tuple[int, int,
 
 def _call(device: torch.device, name: str, *args) -> None:
     """A call on the device of its tensors and its current stream (the last argument of every entry)."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)  # 0.1 us; as a Stream object 1.9 of append's 8
+    stream = _lib.raw_stream(device)
     if torch.cuda.current_device() == device.index:
         _lib.call(name, *args, stream)
     else:
