@@ -607,10 +607,12 @@ int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_row_stride, 
 int mzk_paged_workspace_bytes(int64_t B, int64_t max_pages, int64_t pages, int64_t* bytes);
 
 /* Room for tokens[b] (int64, >= 0) more tokens of each sequence: the lowest free pages, in the order
- * of the sequences, and lens + tokens.  A partly filled last page that others hold too (refs > 1) is
- * replaced by a fresh one, and its filled entries are copied in each of the npools pools (host
- * arrays of base pointers and of bytes per entry, a multiple of 4).  Either every sequence gets its pages or none
- * does: *missing (int64 on the device) is 0, or the pages that lack, and then nothing changes.
+ * of the sequences, and lens + tokens.  Where a row names pages behind its tokens (after lens was lowered,
+ * as for refused drafted tokens), those that it alone holds (refs 1) are used first, and the others among
+ * the entries that are needed are replaced, their counts one less.  A partly filled last page that others hold too
+ * (refs > 1) is replaced by a fresh one, for each of its holders that grows, and its filled entries are copied in each of
+ * the npools pools (host arrays of base pointers and of bytes per entry, a multiple of 4).  Either every
+ * sequence gets its pages or none does: *missing (int64 on the device) is 0, or the pages that lack, and then nothing changes.
  * The outputs may be the inputs. */
 int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages, const int64_t* lens,
                    const int32_t* refs, int64_t pages, const int64_t* tokens, int page, void* const* pools,

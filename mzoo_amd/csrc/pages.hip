@@ -6,8 +6,9 @@
 // decode loop grows its sequences without the host.
 //
 //   append   token i of the n new ones of sequence b -> position len_b - n + i
-//   grow     pages for n_b more tokens each: the lowest free pages, in the order of the sequences;
-//            a partly filled last page that others hold too is replaced by a copy; all or none
+//   grow     pages for n_b more tokens each: those that a row holds behind its tokens and nobody else
+//            does, then the lowest free pages, in the order of the sequences; a partly filled last
+//            page that others hold too is replaced by a copy; all or none
 //   fork     sequence i goes on from the tokens of sequence parents[i]
 //   compact  of U used pages, the k-th behind page U moves to the k-th free one before it
 //
@@ -187,8 +188,9 @@ __device__ __forceinline__ int64_t sum_of(const T* v, int64_t step, int64_t n, i
 // ---- grow ---------------------------------------------------------------------------------
 
 struct GrowRow {
-  int32_t first, want;  // the fresh table entries: first .. first + want - 1
-  int32_t src, fill;    // the page whose first `fill` entries the first fresh page begins with (-1: none)
+  int32_t first, end, want;  // want of the table entries first .. end - 1 get a fresh page
+  int32_t src, fill;         // the page whose first `fill` entries the first fresh page begins with (-1: none)
+  int32_t base;              // -1: all of them do; else they are told by kept[], whose first bit is entry `base`
 };
 
 struct GrowParams {
@@ -209,8 +211,10 @@ struct GrowParams {
   int64_t* over;    // [B] pages past the table's width
   int64_t* free_in; // [chunks] free pages of the chunk
   int64_t* want;    // [1] the pages handed out, -1: none, some lack
+  uint64_t* kept;   // [B][words] entries behind the row's tokens whose pages it alone holds: they stay
+  uint64_t* given;  // [B][words] entries whose pages others hold too: they get fresh ones, and count one less
   int32_t* list;    // [P] the page of each rank
-  int64_t chunks;
+  int64_t chunks, words;
 };
 
 // A count from the device, within what sums of two cannot overflow.
@@ -228,26 +232,51 @@ __global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
     if (tid == 0) p.free_in[blk] = total;
     return;
   }
-  const int64_t b = (blk - p.chunks) * 256 + tid;
+  // A wave per row, a lane per entry.  After refused tokens a row names pages behind the ones that
+  // its tokens fill; written over, they would be nobody's and never free again.
+  const int64_t b = (blk - p.chunks) * 4 + (tid >> 6);
+  const int lane = tid & 63;
   if (b >= p.B) return;
   const int64_t len = row_count(p.lens[b]), n = row_count(p.tokens[b]);
   const int64_t held = ceil_div64(len, p.page), end = ceil_div64(len + n, p.page);
-  GrowRow r{0, 0, -1, 0};
-  p.over[b] = n > 0 && end > p.max_pages ? end - p.max_pages : 0;
+  GrowRow r{0, 0, 0, -1, 0, -1};
   if (n > 0 && end <= p.max_pages) {
     const int64_t fill = len % p.page;
-    int64_t first = held;
-    if (fill != 0) {
-      const int64_t pid = p.tables[b * p.stride + held - 1];
-      if (pid >= 0 && pid < p.P && p.refs[pid] > 1) {
-        r.src = static_cast<int32_t>(pid);
-        r.fill = static_cast<int32_t>(fill);
-        --first;
+    const int64_t base = fill != 0 ? held - 1 : held;  // the partly filled last page, too
+    int64_t first = base;
+    int kept = 0;
+    bool some = false;
+    for (int64_t j0 = base; j0 < end; j0 += 64) {
+      const int64_t j = j0 + lane;
+      const int32_t pid = j < end ? p.tables[b * p.stride + j] : -1;
+      const int32_t refs = pid >= 0 && pid < p.P ? p.refs[pid] : 0;
+      const bool last = fill != 0 && j == base;
+      const uint64_t keep = __ballot(last ? refs <= 1 : refs == 1), give = __ballot(!last && refs > 1);
+      if (lane == 0) {
+        const int64_t word = b * p.words + (j0 - base) / 64;
+        p.kept[word] = keep;
+        p.given[word] = give;
       }
+      kept += __builtin_popcountll(keep);
+      uint64_t behind = keep | give;
+      if (fill != 0 && j0 == base) {
+        if (keep & 1u) {
+          first = held;
+        } else {
+          r.src = __builtin_amdgcn_readfirstlane(pid);
+          r.fill = static_cast<int32_t>(fill);
+        }
+        behind &= ~1ull;
+      }
+      some |= behind != 0;
     }
     r.first = static_cast<int32_t>(first);
-    r.want = static_cast<int32_t>(end - first);
+    r.end = static_cast<int32_t>(end);
+    r.want = static_cast<int32_t>(end - base) - kept;
+    if (some) r.base = static_cast<int32_t>(base);
   }
+  if (lane != 0) return;
+  p.over[b] = n > 0 && end > p.max_pages ? end - p.max_pages : 0;
   p.rows[b] = r;
   p.old_len[b] = len;
 }
@@ -323,8 +352,22 @@ __global__ void __launch_bounds__(256) grow_row_kernel(const GrowParams p, const
     const int32_t* const from = p.tables + b * p.stride;
     int32_t* const to = p.tables_out + b * p.stride_out;
     for (int64_t j = tid; j < p.max_pages; j += 256) {
-      const bool fresh = want >= 0 && j >= r.first && j < r.first + r.want;
-      to[j] = fresh ? p.list[begin + j - r.first] : from[j];
+      int32_t page = from[j];
+      if (want >= 0 && j >= r.first && j < r.end) {
+        int64_t rank = j - r.first;
+        bool fresh = true;
+        if (r.base >= 0) {  // behind the entries that stay
+          const uint64_t* const kept = p.kept + b * p.words;
+          const int64_t at = j - r.base, word = at >> 6;
+          const uint64_t bit = 1ull << (at & 63);
+          rank = at - __builtin_popcountll(kept[word] & (bit - 1));
+          for (int64_t w = 0; w < word; ++w) rank -= __builtin_popcountll(kept[w]);
+          fresh = (kept[word] & bit) == 0;
+          if (p.given[b * p.words + word] & bit) atomicSub(p.refs_out + page, 1);
+        }
+        if (fresh) page = p.list[begin + rank];
+      }
+      to[j] = page;
     }
     if (tid == 0) {
       p.lens_out[b] = want >= 0 ? p.old_len[b] + row_count(p.tokens[b]) : p.lens[b];
@@ -494,9 +537,9 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p
 
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
-int64_t grow_bytes(int64_t B, int64_t P) {
-  const int64_t chunks = (P + kChunk - 1) / kChunk;
-  return align16_up(sizeof(GrowRow) * B) + 8 * (2 * B + chunks + 1) + 4 * P + 16;
+int64_t grow_bytes(int64_t B, int64_t max_pages, int64_t P) {
+  const int64_t chunks = (P + kChunk - 1) / kChunk, words = (max_pages + 63) / 64;
+  return align16_up(sizeof(GrowRow) * B) + 8 * (2 * B + chunks + 1 + 2 * B * words) + 4 * P + 16;
 }
 int64_t fork_bytes(int64_t B, int64_t max_pages) { return align16_up(4 * B * max_pages) + 8 * B; }
 int64_t compact_bytes(int64_t P) { return 8 * ((P + kChunk - 1) / kChunk + 2) + 16 * P + 32; }
@@ -549,7 +592,7 @@ extern "C" int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_r
 extern "C" int mzk_paged_workspace_bytes(int64_t B, int64_t max_pages, int64_t pages, int64_t* bytes) {
   MZK_CHECK_ARG(bytes != nullptr, "paged_workspace_bytes: null output");
   MZK_CHECK_PAGES("paged_workspace_bytes", B, max_pages, pages);
-  int64_t n = grow_bytes(B, pages);
+  int64_t n = grow_bytes(B, max_pages, pages);
   if (fork_bytes(B, max_pages) > n) n = fork_bytes(B, max_pages);
   if (compact_bytes(pages) > n) n = compact_bytes(pages);
   *bytes = align16_up(n);
@@ -566,11 +609,12 @@ extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64
   MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_grow: strides smaller than the row");
   if (int rc = check_pools("paged_grow", pools, entry_bytes, npools)) return rc;
   MZK_CHECK_ARG(tables && lens && refs && tokens && tables_out && lens_out && refs_out && missing, "paged_grow: null pointer");
-  MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= grow_bytes(B, pages),
-                "paged_grow: a 16-byte aligned workspace of %lld bytes is needed", (long long)grow_bytes(B, pages));
+  MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= grow_bytes(B, max_pages, pages),
+                "paged_grow: a 16-byte aligned workspace of %lld bytes is needed", (long long)grow_bytes(B, max_pages, pages));
   GrowParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, lens, lens_out, refs, refs_out, pages,
                tokens, page, missing};
   p.chunks = (pages + kChunk - 1) / kChunk;
+  p.words = (max_pages + 63) / 64;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.rows = reinterpret_cast<GrowRow*>(w);
   w += align16_up(sizeof(GrowRow) * B);
@@ -578,9 +622,11 @@ extern "C" int mzk_paged_grow(const int32_t* tables, int64_t table_stride, int64
   p.over = p.old_len + B;
   p.free_in = p.over + B;
   p.want = p.free_in + p.chunks;
-  p.list = reinterpret_cast<int32_t*>(p.want + 1);
+  p.kept = reinterpret_cast<uint64_t*>(p.want + 1);
+  p.given = p.kept + B * p.words;
+  p.list = reinterpret_cast<int32_t*>(p.given + B * p.words);
   hipStream_t s = as_stream(stream);
-  grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 255) / 256), 256, 0, s>>>(p);
+  grow_count_kernel<<<static_cast<unsigned>(p.chunks + (B + 3) / 4), 256, 0, s>>>(p);
   grow_assign_kernel<<<static_cast<unsigned>(p.chunks), 256, 0, s>>>(p);
   int done = 0;
   do {

@@ -272,10 +272,14 @@ def grow(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, tokens: t
          out=None, missing: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """Room for ``tokens`` int64 [B] more tokens of each sequence: the lowest free pages, in the order
     of the sequences.  A partly filled last page that others hold too is replaced by a copy, in every
-    one of ``pools`` ([P, page, ...]).  Either every sequence gets its pages or none does.  Returns (tables, lens + tokens,
-    refs, missing): ``missing`` int64 [1] is 0, or the pages that lack, and then the rest is
-    unchanged.  ``out=(tables, lens, refs)``, which may be the inputs themselves, is written instead
-    of new tensors."""
+    one of ``pools`` ([P, page, ...]), for each of its holders that grows.  Either every sequence gets its pages or none
+    does.  Returns (tables, lens + tokens, refs, missing): ``missing`` int64 [1] is 0, or the pages that lack, and then
+    the rest is unchanged.  ``out=(tables, lens, refs)``, which may be the inputs themselves, is written
+    instead of new tensors.
+
+    ``lens`` may be lowered between calls, as for drafted tokens that were refused: the pages behind a
+    sequence's tokens stay its own, and the next ``grow`` uses them first (those that others hold too
+    it gives up); ``fork`` of a sequence to itself gives them back."""
     _one_device("grow", tables, lens, refs, tokens, missing, workspace, *pools)
     b, width, stride, pages = _book("grow", tables, lens, refs)
     if not _is(tokens, torch.int64, (b,)):

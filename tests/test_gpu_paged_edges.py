@@ -1,0 +1,122 @@
+"""GPU: the paged cache at its edges, against plain restatements."""
+
+import pytest
+import torch
+
+from mzoo_amd import paged
+from tests.test_gpu_paged import _gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- grow: pages behind the tokens --------------------------------------------------------------
+
+def _counts(tables, pages):
+    return torch.bincount(tables[tables >= 0].long().cpu(), minlength=pages).int()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_grow_after_refused_tokens(dev, inplace):
+    """Four drafted tokens a step that cross a page's end, all refused again: the row keeps its second page."""
+    page, pages = 16, 6
+    tables = torch.full((2, 4), -1, dtype=torch.int32, device=dev)
+    tables[0, 0] = 0
+    lens = torch.tensor([14, 0], device=dev)
+    refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+    refs[0] = 1
+    pool = torch.randn(pages, page, 4, device=dev)
+    four = torch.tensor([4, 0], device=dev)
+    for _ in range(6):
+        state = (tables, lens, refs)
+        tables, lens, refs, missing = paged.grow(*state, four, page, pools=[pool], out=state if inplace else None)
+        assert int(missing) == 0 and lens.tolist() == [18, 0]
+        assert tables.tolist() == [[0, 1, -1, -1], [-1] * 4]
+        assert torch.equal(refs.cpu(), _counts(tables, pages))
+        lens = lens - torch.tensor([4, 0], device=dev)
+
+
+def _grow_kept(tables, lens, refs, new, page, pool):
+    """grow where rows may hold pages behind their tokens: a row's own ones are used first, those that others
+    hold too are given up."""
+    tables, lens, refs, pool = tables.clone(), lens.clone(), refs.clone(), pool.clone()
+    pages, width = refs.numel(), tables.shape[1]
+    free = [p for p in range(pages) if refs[p] == 0]
+    plan, over = [], 0
+    for b, n in enumerate(new.tolist()):
+        held, end = -(-int(lens[b]) // page), -(-(int(lens[b]) + n) // page)
+        fresh, gone, copy = [], [], None
+        if n > 0 and end > width:
+            over += end - width
+        elif n > 0:
+            if int(lens[b]) % page:
+                p = int(tables[b, held - 1])
+                if 0 <= p < pages and refs[p] > 1:
+                    fresh, gone, copy = [held - 1], [p], p
+            for j in range(held, end):
+                p = int(tables[b, j])
+                count = int(refs[p]) if 0 <= p < pages else 0
+                if count != 1:
+                    fresh.append(j)
+                if count > 1:
+                    gone.append(p)
+        plan.append((fresh, gone, copy))
+    lack = over + max(0, sum(len(f) for f, _, _ in plan) - len(free))
+    if lack:
+        return tables, lens, refs, lack, pool
+    for b, (fresh, gone, copy) in enumerate(plan):
+        for i, j in enumerate(fresh):
+            p = free.pop(0)
+            tables[b, j], refs[p] = p, 1
+            if i == 0 and copy is not None:
+                pool[p, :int(lens[b]) % page] = pool[copy, :int(lens[b]) % page]
+        for p in gone:
+            refs[p] -= 1
+    return tables, lens + new, refs, 0, pool
+
+
+def _rolled_back(seed, batch, page, pages, most, spare):
+    """Consistent rows of which many hold pages behind their tokens, some of them shared."""
+    g = _gen(seed)
+    width = -(-most // page) + 4
+    perm = torch.randperm(pages - spare, generator=g).tolist()
+    tables = torch.full((batch, width), -1, dtype=torch.int32)
+    lens = torch.randint(0, most + 1, (batch,), generator=g)
+    for b in range(batch):
+        if b and b % 3 == 0:
+            tables[b], lens[b] = tables[b - 1], lens[b - 1]
+        else:
+            for j in range(-(-int(lens[b]) // page)):
+                tables[b, j] = perm.pop()
+    for b in range(0, batch, 2):
+        lens[b] = int(torch.randint(0, int(lens[b]) + 1, (1,), generator=g))
+        held = -(-int(lens[b]) // page)
+        if b % 4 == 0 and held + 2 < width and tables[b, held] >= 0:
+            tables[b, held + 1] = -1              # a hole among them
+    return tables, lens, _counts(tables, pages)
+
+
+@pytest.mark.parametrize("batch,page,most", [(2, 16, 60), (9, 1, 300), (40, 4, 1500), (150, 16, 900)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_grow_uses_the_pages_that_a_row_holds(dev, batch, page, most, inplace):
+    pages = batch * (-(-most // page)) + 40
+    tables, lens, refs = _rolled_back(batch + page, batch, page, pages, most, 30)
+    new = torch.randint(0, most // 2, (batch,), generator=_gen(3)) * torch.randint(0, 2, (batch,), generator=_gen(4))
+    new = torch.minimum(new, tables.shape[1] * page - lens)
+    pool = torch.randn(pages, page, 4, generator=_gen(5))
+    want = _grow_kept(tables, lens, refs, new, page, pool)
+    assert want[3] == 0 and torch.equal(want[2], _counts(want[0], pages))
+    d, dp = [t.to(dev) for t in (tables, lens, refs)], pool.to(dev)
+    got = paged.grow(*d, new.to(dev), page, pools=[dp], out=d if inplace else None)
+    assert int(got[3]) == 0
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a.cpu(), b)
+    assert torch.equal(dp.cpu(), want[4])
+
+
+def test_grow_needs_no_free_page_for_a_row_that_holds_one(dev):
+    tables = torch.tensor([[2, 0, -1], [1, 3, -1]], dtype=torch.int32, device=dev)
+    lens, refs = torch.tensor([6, 16], device=dev), torch.ones(4, dtype=torch.int32, device=dev)
+    got = paged.grow(tables, lens, refs, torch.tensor([6, 0], device=dev), 8)
+    assert int(got[3]) == 0 and torch.equal(got[0], tables) and got[1].tolist() == [12, 16] and torch.equal(got[2], refs)
+    got = paged.grow(tables, lens, refs, torch.tensor([12, 1], device=dev), 8)      # two pages lack
+    assert int(got[3]) == 2 and torch.equal(got[0], tables) and torch.equal(got[1], lens) and torch.equal(got[2], refs)
