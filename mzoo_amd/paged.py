@@ -148,7 +148,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
     q bf16 [T, H, D]: one token per sequence, or with ``cu`` the last ``cu[b + 1] - cu[b]`` of each (drafted
     tokens, a chunk of a prompt), each at its own position and causal.  A token sees its sequence up
     to itself, the last ``window`` positions of that, or -- one token per sequence -- the positions
-    ``indices`` int32 [B, k] lists (outside the sequence: empty).  ``sinks`` fp32 [H].  Returns (o bf16
+    ``indices`` int32 [B, k] lists (outside the sequence: empty; k 0: none).  ``sinks`` fp32 [H].  Returns (o bf16
     [T, H, D], lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a
     given ``out`` and ``lse``.  A token that sees nothing gets 0.  ``workspace``: uint8, of
     ``attend_workspace_bytes``, allocated per call if omitted; calls that overlap need their own."""
@@ -171,13 +171,15 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
         _refuse("attend", "sinks", sinks, torch.float32, (h,))
     if window is not None and (not isinstance(window, int) or window < 1):
         raise ValueError(f"attend: window must be a positive int or None, got {window!r}")
-    k = istride = 0
+    k = istride = idx = 0
     if indices is not None:
         if cu is not None or window is not None:
             raise ValueError("attend: indices go with one token per sequence and no window")
         rows, k, istride = _table("attend", indices, "indices")
         if rows != b:
             raise ValueError(f"attend: indices must be [{b}, k], got {list(indices.shape)}")
+        # a list of no positions has no address either, and none means no list: any other that is never read
+        idx = indices.data_ptr() or lens.data_ptr()
     given = out is not None
     if given != (lse is not None):
         raise ValueError("attend: out and lse go together")
@@ -196,7 +198,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
         elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"attend: the workspace must be contiguous uint8 of at least {need} bytes")
     _call(q.device, "mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
-          tables.data_ptr(), stride, width, lens.data_ptr(), _lib.ptr(indices), istride, k, min(window or 0, 1 << 30), _lib.ptr(sinks),
+          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, min(window or 0, 1 << 30), _lib.ptr(sinks),
           _lib.ptr(workspace) if need else None, need, out.data_ptr(), lse.data_ptr(), 0 if given else 1)
     return out, lse
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from mzoo_amd import paged
-from tests.test_gpu_paged import _gen
+from tests.test_gpu_paged import ROPE, _gen, _setup
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,19 @@ def test_grow_needs_no_free_page_for_a_row_that_holds_one(dev):
     assert int(got[3]) == 0 and torch.equal(got[0], tables) and got[1].tolist() == [12, 16] and torch.equal(got[2], refs)
     got = paged.grow(tables, lens, refs, torch.tensor([12, 1], device=dev), 8)      # two pages lack
     assert int(got[3]) == 2 and torch.equal(got[0], tables) and torch.equal(got[1], lens) and torch.equal(got[2], refs)
+
+
+# ---- attend -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (160, "bf16")])
+@pytest.mark.parametrize("lens", [[50, 1, 0], [5000, 40, 0]])
+def test_attend_empty_list(dev, dim, fmt, lens):
+    """A list of no positions: every token sees nothing."""
+    pool, tables, n64, _, _ = _setup(dev, lens, 16, dim, fmt, 81)
+    q = torch.randn(3, 24, dim, generator=_gen(82)).bfloat16().to(dev)
+    sinks = torch.randn(24, generator=_gen(83)).to(dev)
+    for idx in (torch.empty(3, 0, dtype=torch.int32, device=dev), torch.zeros(3, 7, dtype=torch.int32, device=dev)[:, :0]):
+        o, lse = paged.attend(q, pool, tables, n64, indices=idx, sinks=sinks, rope=ROPE[dim])
+        assert bool((o == 0).all()) and torch.equal(lse, sinks.expand(3, 24))
+        o, lse = paged.attend(q, pool, tables, n64, indices=idx, rope=ROPE[dim])
+        assert bool((o == 0).all()) and bool((lse == float("-inf")).all())

@@ -163,3 +163,20 @@ def test_sizes_past_a_launch_are_refused():
     refuse("mzk_paged_grow", [p, 8, 0, 8, p, p, 100, p, 16, None, None, 0, p, 8, p, p, p, p, 1 << 40, None], "at least one sequence")
     refuse("mzk_paged_fork", [p, 8, 4, 8, p, p, 100, p, 1 << 24, 16, p, 8, p, p, p, 1 << 40, None], "bad sizes")
     assert lib.mzk_paged_attend(p, 0, 128, 576, None, 0, 1, 512, p, 16, 64, p, 8, 8, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None) == 0
+
+
+def test_attend_hands_over_an_empty_list(monkeypatch):
+    """A list of no positions is a list: its pointer, which an empty tensor lacks, is not null."""
+    got = {}
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(paged, "attend_workspace_bytes", lambda *a: 0)
+    monkeypatch.setattr(paged, "_call", lambda dev, name, *args: got.update(args=args))
+    t, n, _ = _state()
+    pool = paged.new_pool(8, 16, 576, device="cpu")
+    q = torch.zeros(2, 8, 576, dtype=torch.bfloat16)
+    for idx, k in ((torch.empty(2, 0, dtype=torch.int32), 0), (torch.zeros(2, 3, dtype=torch.int32)[:, :0], 0),
+                   (torch.zeros(2, 3, dtype=torch.int32), 3)):
+        paged.attend(q, pool, t, n, indices=idx)
+        assert got["args"][15] and got["args"][17] == k
+    paged.attend(q, pool, t, n)
+    assert not got["args"][15]
