@@ -589,8 +589,9 @@ int mzk_sparse_mqa_noalloc(const void* q, int64_t B, int64_t S, int H, int D, in
  * table_stride) names its pages in order, -1 where there is none; its tokens are the first
  * lens[b] (int64) entries.  refs[p] (int32) counts the table entries that name page p and whatever
  * else holds it; a page of refs 0 is free.  Table entries outside [0, pages) name no page: nothing
- * is read or written there.  Packed sequences: cu int64 [B + 1], ascending from 0; sequence b's
- * tokens are rows cu[b] .. cu[b + 1] - 1.  Everything is read on the device, so calls can be captured.
+ * is read or written there (so tables without columns or a pool without pages may be null, in _append and
+ * _attend).  Packed sequences: cu int64 [B + 1], ascending from 0; sequence b's tokens are rows cu[b] ..
+ * cu[b + 1] - 1.  Everything is read on the device, so calls can be captured.
  * --------------------------------------------------------------------------------- */
 
 /* Entries of new tokens, the cache write of DeepseekV41CSACache.update (owlet1/cache.py:84-94) into

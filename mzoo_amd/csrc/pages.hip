@@ -578,9 +578,10 @@ extern "C" int mzk_paged_append(const void* x, int dtype, int64_t T, int64_t x_r
   MZK_CHECK_ARG(cu || T == B, "paged_append: without cu one token per sequence (%lld tokens, %lld sequences)",
                 (long long)T, (long long)B);
   if (T == 0 || B == 0) return MZK_OK;
-  MZK_CHECK_ARG(x && tables && lens && pool, "paged_append: null pointer");
+  MZK_CHECK_ARG(x && lens && (tables || max_pages == 0) && (pool || pages == 0), "paged_append: null pointer");
   MZK_CHECK_ARG(aligned16(pool), "paged_append: the pool must be 16-byte aligned");
   MZK_CHECK_ARG(T <= 4 * kMaxRows, "paged_append: too many tokens");
+  if (max_pages == 0 || pages == 0) return MZK_OK;  // every position is on no page
   const AppendParams p{x, x_row_stride, T, cu, B, tables, table_stride, max_pages, lens, static_cast<uint8_t*>(pool),
                        pages, page, D, fmt ? nope : 0};
   const bool vec = aligned16(x) && x_row_stride % 8 == 0;

@@ -643,7 +643,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                 "paged_attend: a list of entries takes one token per sequence and no window, rows of at least topk");
   MZK_CHECK_ARG(table_stride >= max_pages, "paged_attend: table rows shorter than max_pages");
   if (T == 0) return MZK_OK;
-  MZK_CHECK_ARG(q && out && lse && (B == 0 || (pool && tables && lens)), "paged_attend: null pointer");
+  MZK_CHECK_ARG(q && out && lse && (B == 0 || (lens && (pool || pages == 0) && (tables || max_pages == 0))),
+                "paged_attend: null pointer");
   MZK_CHECK_ARG(aligned16(q) && aligned16(pool) && aligned16(out) && aligned16(workspace),
                 "paged_attend: q, pool, workspace and out must be 16-byte aligned");
   RaggedParams p{};
@@ -657,7 +658,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.lens = lens;
   p.entries = static_cast<const uint8_t*>(pool);
   p.entry_stride = fmt ? nope + nope / 32 + 2 * (D - nope) : 2 * D;
-  p.tables = tables;
+  // (null would mean packed entries; a table without columns is never read)
+  p.tables = max_pages ? tables : reinterpret_cast<const int32_t*>(lens);
   p.table_stride = table_stride;
   p.max_pages = max_pages;
   p.pages = pages;

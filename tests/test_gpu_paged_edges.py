@@ -136,3 +136,21 @@ def test_attend_empty_list(dev, dim, fmt, lens):
         assert bool((o == 0).all()) and torch.equal(lse, sinks.expand(3, 24))
         o, lse = paged.attend(q, pool, tables, n64, indices=idx, rope=ROPE[dim])
         assert bool((o == 0).all()) and bool((lse == float("-inf")).all())
+
+
+def test_no_pages_and_no_columns(dev):
+    """A pool of no pages, or tables of no columns: nothing is written, and tokens see nothing."""
+    q = torch.randn(2, 8, 576, generator=_gen(84)).bfloat16().to(dev)
+    x, sinks = q[:, 0].contiguous(), torch.randn(8, generator=_gen(85)).to(dev)
+    lens = torch.tensor([3, 40], device=dev)
+    some = paged.new_pool(4, 16, 576, device=dev)
+    cu = torch.tensor([0, 1, 2], device=dev)
+    for pool, tables in ((some, torch.empty(2, 0, dtype=torch.int32, device=dev)),
+                         (paged.new_pool(0, 16, 576, device=dev), torch.zeros(2, 3, dtype=torch.int32, device=dev))):
+        for c in (None, cu):
+            paged.append(pool, tables, lens, x, cu=c)
+            o, lse = paged.attend(q, pool, tables, lens, cu=c, sinks=sinks)
+            assert bool((o == 0).all()) and torch.equal(lse, sinks.expand(2, 8))
+        o, lse = paged.attend(q, pool, tables, lens, indices=torch.zeros(2, 5, dtype=torch.int32, device=dev))
+        assert bool((o == 0).all()) and bool((lse == float("-inf")).all())
+    assert bool((some == 0).all())
