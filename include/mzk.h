@@ -643,7 +643,7 @@ int mzk_paged_compact(const int32_t* tables, int64_t table_stride, int64_t B, in
  *   each.  Token i of n is at position lens[b] - n + i and sees the positions up to its own, the last
  *   `window` of them (0: all), or, with idx (int32 [B, idx_row_stride], one token per sequence, window
  *   0), the positions idx[b, :topk] (outside [0, lens[b]): empty; topk 0: none) -- an indexer's selection.
- *   Positions on no page are empty; a token that sees nothing gets 0, and the sink (or -inf) as lse.
+ *   Positions on no page, those past the table among them, are empty; a token that sees nothing gets 0, and the sink (or -inf) as lse.
  *   fmt 0: bf16 entries (D 64, 96, 128, 160, 256, 512, 576), 1: FP8-b128 (512 + 64, 128 + 32).
  *   out [T, H, D] bf16, lse [T, H] fp32; rows behind the last sequence are left as they are, or, with
  *   zero_tail, become 0 (lse -inf).

@@ -18,6 +18,7 @@
 namespace mzk {
 namespace {
 
+constexpr int64_t kMaxInt = 0x7fffffff;
 constexpr int kNoWindow = 1 << 30;  // a call has fewer tokens, so that no position overflows
 
 // Division of n < 2^31 by a constant of the call: floor(n m / 2^32) + n, shifted, with m = floor(2^32 (2^s -
@@ -54,6 +55,7 @@ struct RaggedParams {
   int64_t idx_stride;
   int topk;
   int window;
+  int64_t past;  // lengths past a table's entries that are told apart: the window; without one -1
   const float* sinks;
   float scale_log2;
   FastDiv by_heads, by_page, by_blocks;  // HG, page, the row blocks of one token
@@ -80,7 +82,8 @@ struct JoinRow {
 // Where a unit's rows and entries are.
 struct Unit {
   int b, t0;          // sequence, its first packed token
-  int n, len;         // its new tokens, its tokens in the cache
+  int n, len;         // its new tokens, its tokens in all
+  int room;           // those of them that its pages may hold: the table ends there
   int g;              // latent
   int r0, r1;         // rows of the sequence and latent: token r / HG, head g HG + r % HG
   int share, shares;  // of the tiles from the first to the last entry that a row sees
@@ -363,8 +366,15 @@ __device__ bool find_unit(const RaggedParams& p, Unit& u, uint8_t* smem, int tid
   u.g = p.G == 1 ? 0 : uniform(blk / blocks);
   u.r0 = uniform((blk - u.g * blocks) << p.unit_shift);
   u.r1 = u.r0 + (1 << p.unit_shift) < u.n * p.HG ? u.r0 + (1 << p.unit_shift) : u.n * p.HG;
-  u.len = u.n;
-  if (p.lens) u.len = uniform(static_cast<int>(clamp64(p.lens[u.b], 0, p.max_pages * p.page)));
+  u.len = u.room = u.n;
+  if (p.lens) {
+    // A sequence may be longer than its table.  From `most` on its new tokens see what they see there:
+    // nothing behind their window, or all that the table holds.
+    const int64_t len = p.lens[u.b], room = p.max_pages * p.page;
+    const int64_t most = room + u.n + p.past < kMaxInt - 64 ? room + u.n + p.past : kMaxInt - 64;
+    u.room = uniform(static_cast<int>(clamp64(len, 0, room)));
+    u.len = uniform(static_cast<int>(clamp64(len, 0, most)));
+  }
   u.share = uniform(u.share);
   u.shares = uniform(u.shares);
   u.slot = uniform(k);
@@ -394,11 +404,11 @@ __device__ __forceinline__ int row_at(const RaggedParams& p, const Unit& u, int 
 // The positions (or places of the list) that tokens tok0 .. tok1 - 1 of the sequence see.
 __device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u, int tok0, int tok1, int& lo, int& hi) {
   const int shift = u.len - u.n;  // position of the first new token (negative: tokens that see nothing)
-  lo = clamp32(shift + tok0 - p.window + 1, 0, u.len);
-  hi = clamp32(shift + tok1, 0, u.len);
+  lo = clamp32(shift + tok0 - p.window + 1, 0, u.room);
+  hi = clamp32(shift + tok1, 0, u.room);
   if (p.idx) {
     lo = 0;
-    hi = u.len > 0 ? p.topk : 0;
+    hi = u.room > 0 ? p.topk : 0;
   }
 }
 
@@ -417,7 +427,7 @@ __device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u,
 __device__ __forceinline__ int pool_entry(const RaggedParams& p, const Unit& u, int v) {
   if (p.idx) {
     v = p.idx[u.b * p.idx_stride + v];
-    if (v < 0 || v >= u.len) return -1;
+    if (v < 0 || v >= u.room) return -1;
   }
   const int at = p.by_page(v);
   const int pid = p.tables[u.b * p.table_stride + at];
@@ -590,7 +600,6 @@ void set_units(RaggedParams& p) {
   p.by_blocks = fast_div(static_cast<uint32_t>(p.G * per));
 }
 
-constexpr int64_t kMaxInt = 0x7fffffff;
 constexpr int64_t kMaxBlocks = (1 << 24) - 16;  // a launch has less than 2^32 threads
 // Shares of at least 4 tiles (one sequence of 4096: 28 us).
 constexpr int kMinTiles = 4;
@@ -668,6 +677,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.idx_stride = idx_row_stride;
   p.topk = topk;
   p.window = window && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
+  p.past = p.window < kNoWindow ? p.window : -1;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);

@@ -150,7 +150,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
     to itself, the last ``window`` positions of that, or -- one token per sequence -- the positions
     ``indices`` int32 [B, k] lists (outside the sequence: empty; k 0: none).  ``sinks`` fp32 [H].  Returns (o bf16
     [T, H, D], lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a
-    given ``out`` and ``lse``.  A token that sees nothing gets 0.  ``workspace``: uint8, of
+    given ``out`` and ``lse``.  Positions on no page or past the table are empty; a token that sees nothing gets 0.  ``workspace``: uint8, of
     ``attend_workspace_bytes``, allocated per call if omitted; calls that overlap need their own."""
     _one_device("attend", q, pool, tables, lens, cu, indices, sinks, workspace, out, lse)
     if q.dim() != 3 or q.shape[1] < 1:

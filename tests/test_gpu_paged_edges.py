@@ -1,10 +1,12 @@
 """GPU: the paged cache at its edges, against plain restatements."""
 
+import numpy as np
 import pytest
 import torch
 
 from mzoo_amd import paged
-from tests.test_gpu_paged import ROPE, _gen, _setup
+from tests import ragged_ref as R
+from tests.test_gpu_paged import ROPE, _entries, _gen, _of, _setup
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +156,44 @@ def test_no_pages_and_no_columns(dev):
         o, lse = paged.attend(q, pool, tables, lens, indices=torch.zeros(2, 5, dtype=torch.int32, device=dev))
         assert bool((o == 0).all()) and bool((lse == float("-inf")).all())
     assert bool((some == 0).all())
+
+
+@pytest.mark.parametrize("dim,fmt", [(576, "fp8"), (576, "bf16"), (160, "fp8"), (160, "bf16")])
+@pytest.mark.parametrize("window", [None, 1, 4, 100])
+@pytest.mark.parametrize("width", [5, 100])
+def test_attend_past_the_table(dev, dim, fmt, window, width):
+    """Sequences longer than their table: a token stays at its own position, and the entries past the
+    table are on no page."""
+    page = 16
+    room = width * page
+    lens = [room + 5, room, room - 1, room + 3, room + 130, room + 40, 20]
+    pool, tables, n64, _, _ = _setup(dev, lens, page, dim, fmt, width)
+    vals, t = _entries(pool, dim).to(dev), tables.cpu()
+    sinks = torch.randn(16, generator=_gen(86)).to(dev)
+    for new in (None, [4, 2, 3, 4, 1, 70, 20]):
+        count = new or [1] * len(lens)
+        q = torch.randn(sum(count), 16, dim, generator=_gen(87)).bfloat16().to(dev)
+        cu = torch.tensor(np.concatenate([[0], np.cumsum(count)]), device=dev)
+        o, lse = paged.attend(q, pool, tables[:, :width], n64, cu=cu if new else None, window=window, sinks=sinks, rope=ROPE[dim])
+        for b, (n, end) in enumerate(zip(count, lens)):
+            a, e = int(cu[b]), vals[_of(t, b, min(end, room), page)]
+            pos, col = (end - n + torch.arange(n))[:, None], torch.arange(min(end, room))[None, :]
+            seen = (col <= pos) & (col > pos - (window or 1 << 40))
+            R.check(o[a:a + n], lse[a:a + n], R.attend(q[a:a + n], e, seen.to(dev), sinks), f"sequence {b} of {n}")
+
+
+@pytest.mark.parametrize("dim", [576, 64])
+@pytest.mark.parametrize("window", [None, 3])
+def test_attend_lengths_past_any_table(dev, dim, window):
+    """Lengths beyond 32 bits, over a table of 64 entries."""
+    pool, tables, _, _, _ = _setup(dev, [64, 64, 64], 16, dim, "bf16", 91)
+    q = torch.randn(6, 8, dim, generator=_gen(92)).bfloat16().to(dev)
+    cu = torch.tensor([0, 2, 4, 6], device=dev)
+    vals, t = _entries(pool, dim).to(dev), tables.cpu()
+    for far in ([2 ** 31, 2 ** 33 + 5, 2 ** 62], [66, 2 ** 31 - 1, 2 ** 32 + 64]):
+        o, lse = paged.attend(q, pool, tables, torch.tensor(far, device=dev), cu=cu, window=window)
+        for b in range(3):
+            pos, col = (far[b] - 2 + torch.arange(2))[:, None], torch.arange(64)[None, :]
+            seen = (col > pos - (window or 1 << 63)) if window else torch.ones(2, 64, dtype=torch.bool)
+            R.check(o[2 * b:2 * b + 2], lse[2 * b:2 * b + 2],
+                    R.attend(q[2 * b:2 * b + 2], vals[_of(t, b, 64, 16)], seen.to(dev), None), f"{far[b]}")
