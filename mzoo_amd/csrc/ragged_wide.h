@@ -372,7 +372,7 @@ ragged_wide_kernel(const RaggedParams p) {
         for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(v[b][r] - m_own[b]);
         l_own[b] = l_own[b] + ((w[0] + w[1]) + (w[2] + w[3]));
         put_p(t0, b, uint2{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])});
-        if (!begin) m_seen[b] = fmaxf(m_seen[b], fmaxf(fmaxf(s_acc[b][0], s_acc[b][1]), fmaxf(s_acc[b][2], s_acc[b][3])));
+        if (!begin) m_seen[b] = fmaxf(m_seen[b], max4(v[b]) / p.scale_log2);  // (this tile's s_acc has the hidden entries too)
       }
     }
     uint32_t at_v = 0, at_k = tile_at(1), at_n = tile_at(2), at_w = tile_at(kDirect ? 3 : 2);

@@ -197,3 +197,37 @@ def test_attend_lengths_past_any_table(dev, dim, window):
             seen = (col > pos - (window or 1 << 63)) if window else torch.ones(2, 64, dtype=torch.bool)
             R.check(o[2 * b:2 * b + 2], lse[2 * b:2 * b + 2],
                     R.attend(q[2 * b:2 * b + 2], vals[_of(t, b, 64, 16)], seen.to(dev), None), f"{far[b]}")
+
+
+@pytest.mark.parametrize("dim,fmt,chunk", [(576, "bf16", 1280), (512, "bf16", 1280), (576, "fp8", 2048), (160, "bf16", 512)])
+def test_attend_hidden_entries_of_a_later_chunk(dev, dim, fmt, chunk):
+    """32 tokens in one unit (so many sequences are not split) behind a window that ends in the first tile of a
+    second chunk of entries.  Of the unit's first tile only the first token's entry is there, so the
+    others' exponents start from 0; the entries that tokens 1 to 3 see score -200, the later ones of
+    that last tile, hidden from them, 0."""
+    n, window, first = 32, chunk, 64
+    end = first + window + n - 1
+    lens = [end] + [1] * 520
+    pool, tables, n64, _, _ = _setup(dev, lens, 1, dim, fmt, 95, poison=False)
+    g = _gen(96)
+    base = torch.zeros(dim)
+    base[:16] = 4.0                                              # in 8-bit entries these channels are exact
+    ends = torch.randn(end, dim, generator=g) * 0.25
+    ends[:, :16] = 0.0
+    ends[:first + window + 3] -= 200.0 * dim ** 0.5 / (base @ base) * base
+    ends[first, :16] = 0.0
+    sub = tables[:1].clone()
+    paged.append(pool, sub, n64[:1], ends.bfloat16().to(dev), cu=torch.tensor([0, end], device=dev), rope=ROPE.get(dim, 64))
+    tables[0, first + 1:first + 32] = -1
+    q = torch.zeros(n + 520, 1, dim)
+    q[:n, 0] = base
+    q[n:] = torch.randn(520, 1, dim, generator=g)
+    q = q.bfloat16().to(dev)
+    cu = torch.tensor([0] + list(range(n, n + 521)), device=dev)
+    o, lse = paged.attend(q, pool, tables, n64, cu=cu, window=window, rope=ROPE.get(dim, 64))
+    vals, t = _entries(pool, dim).to(dev), tables.cpu()
+    there = (t[0] >= 0)[:end]
+    pos, col = (end - n + torch.arange(n))[:, None], torch.arange(end)[None, :]
+    seen = (col <= pos) & (col > pos - window) & there[None, :]
+    at = t[0, :end].clamp(min=0).long()
+    R.check(o[:n], lse[:n], R.attend(q[:n], vals[at.to(dev)], seen.to(dev), None), "the window's sequence")
