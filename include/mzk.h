@@ -647,6 +647,7 @@ int mzk_paged_compact(const int32_t* tables, int64_t table_stride, int64_t B, in
  *   fmt 0: bf16 entries (D 64, 96, 128, 160, 256, 512, 576), 1: FP8-b128 (512 + 64, 128 + 32).
  *   out [T, H, D] bf16, lse [T, H] fp32; rows behind the last sequence are left as they are, or, with
  *   zero_tail, become 0 (lse -inf).
+ *   A sequence and a pool hold less than 2^31 entries, a sequence twice the new tokens (with cu, T) less.
  *   workspace: mzk_paged_attend_workspace_bytes (16-byte aligned, no initialization). */
 int mzk_paged_attend(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, int fmt, int nope,
                      const void* pool, int64_t pages, int page, const int32_t* tables, int64_t table_stride,

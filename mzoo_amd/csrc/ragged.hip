@@ -19,7 +19,7 @@ namespace mzk {
 namespace {
 
 constexpr int64_t kMaxInt = 0x7fffffff;
-constexpr int kNoWindow = 1 << 30;  // a call has fewer tokens, so that no position overflows
+constexpr int kNoWindow = 1 << 30;  // packed prompts without a window: a call has fewer tokens
 
 // Division of n < 2^31 by a constant of the call: floor(n m / 2^32) + n, shifted, with m = floor(2^32 (2^s -
 // d) / d) + 1 and 2^s >= d.  Three instructions; what is executed once runs from a cold instruction
@@ -132,7 +132,7 @@ __device__ __forceinline__ int sequence(const RaggedParams& p, int i, int& a, in
   int seen = z - a;
   if (p.lens) seen = static_cast<int>(clamp64(p.lens[i], 0, p.max_pages * p.page));
   if (p.idx) seen = seen > 0 ? p.topk : 0;
-  if (seen > p.window + (z - a)) seen = p.window + (z - a);
+  if (seen - (z - a) > p.window) seen = p.window + (z - a);
   tiles = (seen + kTile - 1) / kTile;
   return ((z - a) * p.HG + (1 << p.unit_shift) - 1) >> p.unit_shift;
 }
@@ -642,8 +642,11 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                     max_pages <= kMaxInt,
                 "paged_attend: 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(page >= 1, "paged_attend: pages of at least one entry");
-  MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
-                "paged_attend: a sequence and a pool hold less than 2^31 entries");
+  // A call without a window has one of 2^31 - most_new, with which the position of no new token, as low as
+  // -most_new, overflows; it cuts no sequence, as the last of them is at most at max_pages * page + most_new - 2.
+  const int64_t most_new = cu ? T : 1;
+  MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 - 2 * (T ? most_new - 1 : 0) && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
+                "paged_attend: a sequence and a pool hold less than 2^31 entries, a sequence twice the new tokens less");
   MZK_CHECK_ARG(fmt == 0 || fmt == 1, "paged_attend: fmt must be 0 (bf16) or 1 (fp8-b128)");
   MZK_CHECK_ARG(window >= 0 && topk >= 0, "paged_attend: negative window or list");
   MZK_CHECK_ARG(cu || T == B, "paged_attend: without cu one token per sequence (%lld tokens, %lld sequences)",
@@ -676,8 +679,9 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.idx = idx;
   p.idx_stride = idx_row_stride;
   p.topk = topk;
-  p.window = window && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
-  p.past = p.window < kNoWindow ? p.window : -1;
+  const bool windowed = window && window < (1ll << 31) - most_new;
+  p.window = static_cast<int>(windowed ? window : (1ll << 31) - most_new);
+  p.past = windowed ? p.window : -1;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);

@@ -198,7 +198,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
         elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"attend: the workspace must be contiguous uint8 of at least {need} bytes")
     _call(q.device, "mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
-          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, min(window or 0, 1 << 30), _lib.ptr(sinks),
+          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, min(window or 0, (1 << 63) - 1), _lib.ptr(sinks),
           _lib.ptr(workspace) if need else None, need, out.data_ptr(), lse.data_ptr(), 0 if given else 1)
     return out, lse
 

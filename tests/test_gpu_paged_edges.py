@@ -231,3 +231,31 @@ def test_attend_hidden_entries_of_a_later_chunk(dev, dim, fmt, chunk):
     seen = (col <= pos) & (col > pos - window) & there[None, :]
     at = t[0, :end].clamp(min=0).long()
     R.check(o[:n], lse[:n], R.attend(q[:n], vals[at.to(dev)], seen.to(dev), None), "the window's sequence")
+
+
+def test_attend_more_than_2_30_entries(dev):
+    """A sequence of 2^30 + 65536 entries (its table names two pages again and again) without a window: its first
+    entry, the only one whose score is not 0, counts."""
+    page, dim, heads = 65536, 64, 2
+    width = (1 << 30) // page + 1
+    n = width * page
+    pool = torch.zeros(2, page, dim, dtype=torch.bfloat16, device=dev)
+    q = torch.zeros(1, heads, dim, dtype=torch.bfloat16, device=dev)
+    q[:, :, 0] = 8.0
+    pool[0, 0, 0], pool[0, 0, 1] = 20.75, 3.0                    # score 8 * 20.75 / 8, about log(n)
+    tables = torch.ones(1, width, dtype=torch.int32, device=dev)
+    tables[0, 0] = 0
+    weight = np.exp(20.75) / (np.exp(20.75) + n - 1)
+    want = torch.tensor([20.75 * weight, 3.0 * weight], dtype=torch.float64)
+    lens = torch.tensor([n], device=dev)
+    for window in (None, n, n - 1):
+        o, lse = paged.attend(q, pool, tables, lens, window=window)
+        if window == n - 1:                                      # all but the first
+            assert bool((o == 0).all()) and bool(((lse.double() - np.log(n - 1)).abs() < 2.0 ** -10).all())
+            continue
+        # the shares without the first entry sum ones, exactly; its own adds 2^22 weights of 2^-30, 2^-8 of the sum, in
+        # lanes of 2^18 terms, off by 2^-6 of that; exponent, join and logarithm 2^-16; the result's rounding 2^-8
+        err = (o[0, :, :2].double().cpu() - want).abs()
+        assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want).all()), o[0, 0, :2]
+        assert bool((o[0, :, 2:] == 0).all())
+        assert bool(((lse.double() - np.log(np.exp(20.75) + n - 1)).abs() < 2.0 ** -10).all())

@@ -180,3 +180,14 @@ def test_attend_hands_over_an_empty_list(monkeypatch):
         assert got["args"][15] and got["args"][17] == k
     paged.attend(q, pool, t, n)
     assert not got["args"][15]
+
+
+def test_room_for_the_new_tokens_positions():
+    """Several tokens of a sequence over a table of nearly 2^31 entries would pass 32 bits: refused."""
+    lib = _lib.load()
+    p = ctypes.c_void_p(256)
+    att = [p, 100, 8, 576, p, 4, 1, 512, p, 16, 1, p, 0x7fffffff - 64 - 197, 0x7fffffff - 64 - 197, p, None, 0, 0, 0, None, p, 1 << 40, p, p, 0, None]
+    assert lib.mzk_paged_attend(*att) < 0
+    assert b"twice the new tokens" in lib.mzk_last_error()
+    assert lib.mzk_paged_attend(*att[:12], 0x7fffffff, 0x7fffffff - 63, *att[14:]) < 0
+    assert b"less than 2^31" in lib.mzk_last_error()
