@@ -217,6 +217,8 @@ struct GrowParams {
   int64_t chunks, words;
 };
 
+constexpr int64_t kMostOver = 1ll << 38;  // of a row's pages past its table: 2^24 rows stay below 2^63
+
 // A count from the device, within what sums of two cannot overflow.
 __device__ __forceinline__ int64_t row_count(int64_t n) { return n < 0 ? 0 : n < (1ll << 60) ? n : 1ll << 60; }
 
@@ -276,7 +278,8 @@ __global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
     if (some) r.base = static_cast<int32_t>(base);
   }
   if (lane != 0) return;
-  p.over[b] = n > 0 && end > p.max_pages ? end - p.max_pages : 0;
+  const int64_t over = n > 0 && end > p.max_pages ? end - p.max_pages : 0;
+  p.over[b] = over < kMostOver ? over : kMostOver;
   p.rows[b] = r;
   p.old_len[b] = len;
 }

@@ -259,3 +259,15 @@ def test_attend_more_than_2_30_entries(dev):
         assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want).all()), o[0, 0, :2]
         assert bool((o[0, :, 2:] == 0).all())
         assert bool(((lse.double() - np.log(np.exp(20.75) + n - 1)).abs() < 2.0 ** -10).all())
+
+
+def test_grow_counts_past_any_table(dev):
+    """Numbers of tokens whose pages' sum passes 64 bits: they lack, and nothing changes."""
+    rows = 16
+    tables = torch.full((rows, 4), -1, dtype=torch.int32, device=dev)
+    lens, refs = torch.zeros(rows, dtype=torch.int64, device=dev), torch.zeros(100, dtype=torch.int32, device=dev)
+    for n in (2 ** 60, 2 ** 62, 2 ** 63 - 1):
+        got = paged.grow(tables, lens, refs, torch.full((rows,), n, device=dev), 1)
+        assert int(got[3]) > 0
+        for a, b in zip(got[:3], (tables, lens, refs)):
+            assert torch.equal(a, b)
