@@ -667,7 +667,10 @@ extern "C" int mzk_paged_fork(const int32_t* tables, int64_t table_stride, int64
   }
   hipStream_t s = as_stream(stream);
   int64_t n = refs != refs_out ? pages : 0;
-  if (p.tables_copy && B * max_pages > n) n = B * max_pages;
+  if (p.tables_copy) {  // (the lengths, too, of tables without columns)
+    const int64_t copied = max_pages ? B * max_pages : B;
+    if (copied > n) n = copied;
+  }
   if (n > 0) {
     const int64_t g = (n + 255) / 256;
     fork_copy_kernel<<<static_cast<unsigned>(g < 2048 ? g : 2048), 256, 0, s>>>(p);

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from mzoo_amd import paged
+from mzoo_amd import _lib, paged
 from tests import ragged_ref as R
 from tests.test_gpu_paged import ROPE, _entries, _gen, _of, _setup
 
@@ -271,3 +271,17 @@ def test_grow_counts_past_any_table(dev):
         assert int(got[3]) > 0
         for a, b in zip(got[:3], (tables, lens, refs)):
             assert torch.equal(a, b)
+
+
+# ---- fork ---------------------------------------------------------------------------------------
+
+
+def test_fork_in_place_of_tables_without_columns(dev):
+    """The C entry takes tables of no width; lengths alone change places."""
+    lens, refs = torch.tensor([5, 7, 9], device=dev), torch.zeros(4, dtype=torch.int32, device=dev)
+    parents = torch.tensor([1, -1, 0], dtype=torch.int32, device=dev)
+    some = torch.zeros(4, dtype=torch.int32, device=dev)
+    ws = torch.full((256,), 0x55, dtype=torch.uint8, device=dev)
+    _lib.call("mzk_paged_fork", some.data_ptr(), 0, 3, 0, lens.data_ptr(), refs.data_ptr(), 4, parents.data_ptr(), 3, 16,
+              some.data_ptr(), 0, lens.data_ptr(), refs.data_ptr(), ws.data_ptr(), 256, _lib.raw_stream(lens.device))
+    assert lens.tolist() == [7, 0, 5]
