@@ -638,6 +638,13 @@ int mzk_paged_compact(const int32_t* tables, int64_t table_stride, int64_t B, in
                       int32_t* tables_out, int64_t table_out_stride, int32_t* refs_out, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
+/* The same, with moved (int32 [pages], or NULL): where each page's entries are now, for whatever else
+ * than the tables holds pages (refs counts it, and its pages move as any other's). */
+int mzk_paged_compact_map(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages, const int32_t* refs,
+                          int64_t pages, int page, void* const* pools, const int64_t* entry_bytes, int npools,
+                          int32_t* tables_out, int64_t table_out_stride, int32_t* refs_out, int32_t* moved,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Attention of new tokens over their sequences' pages, K == V, scale D^-0.5, sinks as mzk_sparse_mqa.
  *   q [T, H, D] bf16: one token per sequence (cu NULL, T == B), or the last cu[b+1] - cu[b] tokens of
  *   each.  Token i of n is at position lens[b] - n + i and sees the positions up to its own, the last

@@ -93,6 +93,7 @@ _SIGS = {
     "mzk_paged_grow": [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P, _I32, _P, _I64, _P, _P, _P, _P, _I64, _P],
     "mzk_paged_fork": [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P, _I64, _P, _P, _P, _I64, _P],
     "mzk_paged_compact": [_P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P, _P, _I64, _P],
+    "mzk_paged_compact_map": [_P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _I64, _P, _P, _P, _I64, _P],
     "mzk_paged_attend": [_P, _I64, _I32, _I32, _P, _I64, _I32, _I32, _P, _I64, _I32, _P, _I64, _I64, _P, _P, _I64, _I32,
                          _I64, _P, _P, _I64, _P, _P, _I32, _P],
     "mzk_paged_attend_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, ctypes.POINTER(_I64)],

@@ -451,6 +451,7 @@ struct CompactParams {
   int32_t* refs_out;
   int64_t P;
   int page;
+  int32_t* moved;    // [P] where each page is now, or null
   // workspace
   int64_t* used_in;  // [chunks] used pages of the chunk
   int64_t* used;     // [2] U, and the moves M
@@ -519,15 +520,18 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const CompactParams p
   if (blockIdx.y == 0) {
     if (!first) return;
     for (int64_t i = at; i < M; i += step) p.refs_out[p.to[i]] = p.from_refs[M - 1 - i];
+    // rank[] is written for moved pages only: a page without references, whose word is whatever was
+    // there, is no move's `from`, and a table that names it keeps it
+    auto now = [&](int32_t v) -> int32_t {
+      if (v < U || v >= p.P) return v;
+      const int32_t k = p.rank[v];
+      return k >= 0 && k < M && p.from[k] == v ? p.to[M - 1 - k] : v;
+    };
+    if (p.moved)
+      for (int64_t i = at; i < p.P; i += step) p.moved[i] = now(static_cast<int32_t>(i));
     for (int64_t i = at; i < p.B * p.max_pages; i += step) {
       const int64_t b = i / p.max_pages, j = i - b * p.max_pages;
-      int32_t v = p.tables[b * p.stride + j];
-      if (v >= U && v < p.P) {
-        // rank[] is written for moved pages only: a page without references, whose word is
-        // whatever was there, is no move's `from`, and a table that names it keeps it
-        const int32_t k = p.rank[v];
-        if (k >= 0 && k < M && p.from[k] == v) v = p.to[M - 1 - k];
-      }
+      const int32_t v = now(p.tables[b * p.stride + j]);
       p.tables_out[b * p.stride_out + j] = v;
     }
     return;
@@ -685,6 +689,15 @@ extern "C" int mzk_paged_compact(const int32_t* tables, int64_t table_stride, in
                                  const int32_t* refs, int64_t pages, int page, void* const* pools,
                                  const int64_t* entry_bytes, int npools, int32_t* tables_out, int64_t table_out_stride,
                                  int32_t* refs_out, void* workspace, int64_t workspace_bytes, void* stream) {
+  return mzk_paged_compact_map(tables, table_stride, B, max_pages, refs, pages, page, pools, entry_bytes, npools, tables_out,
+                               table_out_stride, refs_out, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mzk_paged_compact_map(const int32_t* tables, int64_t table_stride, int64_t B, int64_t max_pages,
+                                     const int32_t* refs, int64_t pages, int page, void* const* pools,
+                                     const int64_t* entry_bytes, int npools, int32_t* tables_out, int64_t table_out_stride,
+                                     int32_t* refs_out, int32_t* moved, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
   MZK_CHECK_PAGES("paged_compact", B, max_pages, pages);
   MZK_CHECK_ARG(page >= 1, "paged_compact: pages of at least one entry");
   MZK_CHECK_ARG(table_stride >= max_pages && table_out_stride >= max_pages, "paged_compact: strides smaller than the row");
@@ -692,7 +705,7 @@ extern "C" int mzk_paged_compact(const int32_t* tables, int64_t table_stride, in
   MZK_CHECK_ARG(tables && refs && tables_out && refs_out, "paged_compact: null pointer");
   MZK_CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= compact_bytes(pages),
                 "paged_compact: a 16-byte aligned workspace of %lld bytes is needed", (long long)compact_bytes(pages));
-  CompactParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, refs, refs_out, pages, page};
+  CompactParams p{tables, tables_out, table_stride, table_out_stride, B, max_pages, refs, refs_out, pages, page, moved};
   p.chunks = (pages + kChunk - 1) / kChunk;
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.used_in = reinterpret_cast<int64_t*>(w);

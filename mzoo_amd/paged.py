@@ -325,17 +325,21 @@ def fork(tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: 
     return ot, ol, orf
 
 
-def compact(tables: torch.Tensor, refs: torch.Tensor, *, pools=(), out=None, workspace: torch.Tensor | None = None):
+def compact(tables: torch.Tensor, refs: torch.Tensor, *, pools=(), moved: torch.Tensor | None = None, out=None,
+            workspace: torch.Tensor | None = None):
     """The used pages moved to the front of the pools ([P, page, ...]): of U used ones, those behind
-    page U - 1, in order, into the free ones before it.  Returns (tables, refs); ``out=(tables, refs)``
-    may be the inputs."""
-    _one_device("compact", tables, refs, workspace, *pools)
+    page U - 1, in order, into the free ones before it.  ``moved`` int32 [P] takes where each page's entries are
+    now, for what else than ``tables`` holds pages (``moved[p]`` is p where page p stayed).  Returns (tables,
+    refs); ``out=(tables, refs)`` may be the inputs."""
+    _one_device("compact", tables, refs, moved, workspace, *pools)
     b, width, stride, pages = _book("compact", tables, None, refs)
     page = pools[0].shape[1] if pools and pools[0].dim() >= 2 else 1
     base, size, n = _pool_list("compact", pools, pages, page)
+    if moved is not None and not _is(moved, torch.int32, (pages,)):
+        _refuse("compact", "moved", moved, torch.int32, (pages,))
     ot, _, orf, ostride = _outs("compact", out, b, width, tables, refs, False)
     need = workspace_bytes(b, width, pages)
     ws = _workspace("compact", workspace, need, refs.device)
-    _call(refs.device, "mzk_paged_compact", tables.data_ptr(), stride, b, width, refs.data_ptr(), pages, page, base, size, n,
-          ot.data_ptr(), ostride, orf.data_ptr(), ws.data_ptr(), need)
+    _call(refs.device, "mzk_paged_compact_map", tables.data_ptr(), stride, b, width, refs.data_ptr(), pages, page, base, size, n,
+          ot.data_ptr(), ostride, orf.data_ptr(), _lib.ptr(moved), ws.data_ptr(), need)
     return ot, orf

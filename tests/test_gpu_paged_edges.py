@@ -285,3 +285,26 @@ def test_fork_in_place_of_tables_without_columns(dev):
     _lib.call("mzk_paged_fork", some.data_ptr(), 0, 3, 0, lens.data_ptr(), refs.data_ptr(), 4, parents.data_ptr(), 3, 16,
               some.data_ptr(), 0, lens.data_ptr(), refs.data_ptr(), ws.data_ptr(), 256, _lib.raw_stream(lens.device))
     assert lens.tolist() == [7, 0, 5]
+
+
+# ---- compact ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("pages", [7, 40, 4096, 9000])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_compact_says_where_pages_went(dev, pages, inplace):
+    """Pages that something beside the tables holds are found again by `moved`."""
+    g = _gen(pages)
+    tables = torch.randperm(pages, generator=g)[:pages // 3].int().view(1, -1)
+    refs = _counts(tables, pages)
+    other = torch.randperm(pages, generator=g)[:pages // 4]
+    refs[other] += 1
+    pool = torch.randn(pages, 2, 4, generator=g)
+    d = [t.to(dev) for t in (tables, refs)]
+    dp, moved = pool.to(dev), torch.full((pages,), 99, dtype=torch.int32, device=dev)
+    got = paged.compact(*d, pools=[dp], out=d if inplace else None, moved=moved)
+    m = moved.cpu().long()
+    used = int((refs > 0).sum())
+    assert torch.equal(dp.cpu()[m[other]], pool[other])
+    assert torch.equal(got[0].cpu().long(), m[tables.long()]) and torch.equal(got[1].cpu()[m[refs > 0]], refs[refs > 0])
+    assert sorted(m[refs > 0].tolist()) == list(range(used)) and torch.equal(m[refs == 0], (refs == 0).nonzero()[:, 0])

@@ -191,3 +191,10 @@ def test_room_for_the_new_tokens_positions():
     assert b"twice the new tokens" in lib.mzk_last_error()
     assert lib.mzk_paged_attend(*att[:12], 0x7fffffff, 0x7fffffff - 63, *att[14:]) < 0
     assert b"less than 2^31" in lib.mzk_last_error()
+
+
+def test_compact_refuses_other_maps(fake_gpu):
+    t, _, r = _state()
+    for moved in (torch.zeros(8), torch.zeros(7, dtype=torch.int32), torch.zeros(16, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="moved"):
+            paged.compact(t, r, moved=moved)
