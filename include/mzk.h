@@ -655,13 +655,17 @@ int mzk_paged_compact_map(const int32_t* tables, int64_t table_stride, int64_t B
  *   out [T, H, D] bf16, lse [T, H] fp32; rows behind the last sequence are left as they are, or, with
  *   zero_tail, become 0 (lse -inf).
  *   A sequence and a pool hold less than 2^31 entries, a sequence twice the new tokens (with cu, T) less.
- *   workspace: mzk_paged_attend_workspace_bytes (16-byte aligned, no initialization). */
+ *   workspace: of mzk_paged_attend_workspace_bytes or _call_workspace_bytes (16-byte aligned, no initialization). */
 int mzk_paged_attend(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, int fmt, int nope,
                      const void* pool, int64_t pages, int page, const int32_t* tables, int64_t table_stride,
                      int64_t max_pages, const int64_t* lens, const int32_t* idx, int64_t idx_row_stride, int topk,
                      int64_t window, const float* sinks, void* workspace, int64_t workspace_bytes, void* out,
                      float* lse, int zero_tail, void* stream);
 int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t* bytes);
+/* The first is enough for any table, window and list; the second is what a call with these takes (window as
+ * there, topk -1: no list), 0 where no sequence is split. */
+int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages, int page,
+                                          int64_t window, int topk, int64_t* bytes);
 
 /* Causal attention over packed prompts: the latent_attn and swa_attn levels
  * (layers/attn/latent_attn/fwd.py:45, layers/attn/swa_attn/fwd.py:55) without padding.  q [T, H, D]

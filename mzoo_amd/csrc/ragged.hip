@@ -622,10 +622,23 @@ bool splits(int64_t tiles, int64_t blocks) { return tiles > 12 && tiles > blocks
 
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
-int64_t attend_bytes(int64_t blocks, int64_t B, int D) {
-  const int slots = unit_slots(blocks, B, D);
+// The units that a call is split into (0: none is) by what a sequence can hold, or a token see: the room of its
+// table, its window and the new tokens, or its list (topk -1: none).
+int call_slots(int64_t blocks, int64_t B, int64_t T, int D, int64_t room, int64_t window, int64_t topk) {
+  int64_t most = room;
+  if (window + T < most) most = window + T;
+  if (topk >= 0) most = topk;
+  return B && splits((most + kTile - 1) / kTile, blocks) ? unit_slots(blocks, B, D) : 0;
+}
+
+int64_t slot_bytes(int slots, int64_t blocks, int D) {
   return slots ? 16 + align16_up(static_cast<int64_t>(sizeof(JoinRow)) * blocks) + static_cast<int64_t>(slots) * 64 * 4 * (D + 2) : 0;
 }
+
+// A call's window: without one 2^31 - most_new, with which the position of no new token, as low as -most_new,
+// overflows; it cuts no sequence, as the last of them is at most at room + most_new - 2 (attend's check).
+bool has_window(int64_t window, int64_t most_new) { return window && window < (1ll << 31) - most_new; }
+int64_t call_window(int64_t window, int64_t most_new) { return has_window(window, most_new) ? window : (1ll << 31) - most_new; }
 
 }  // namespace
 }  // namespace mzk
@@ -642,8 +655,6 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                     max_pages <= kMaxInt,
                 "paged_attend: 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(page >= 1, "paged_attend: pages of at least one entry");
-  // A call without a window has one of 2^31 - most_new, with which the position of no new token, as low as
-  // -most_new, overflows; it cuts no sequence, as the last of them is at most at max_pages * page + most_new - 2.
   const int64_t most_new = cu ? T : 1;
   MZK_CHECK_ARG(max_pages * page <= kMaxInt - 64 - 2 * (T ? most_new - 1 : 0) && pages * page <= kMaxInt - 64 && topk <= kMaxInt - 64,
                 "paged_attend: a sequence and a pool hold less than 2^31 entries, a sequence twice the new tokens less");
@@ -679,9 +690,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.idx = idx;
   p.idx_stride = idx_row_stride;
   p.topk = topk;
-  const bool windowed = window && window < (1ll << 31) - most_new;
-  p.window = static_cast<int>(windowed ? window : (1ll << 31) - most_new);
-  p.past = windowed ? p.window : -1;
+  p.window = static_cast<int>(call_window(window, most_new));
+  p.past = has_window(window, most_new) ? p.window : -1;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);
@@ -689,15 +699,11 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.lse = lse;
   p.zero_tail = zero_tail;
   MZK_CHECK_ARG(p.blocks_max < kMaxBlocks && T * H <= kMaxInt - 64, "paged_attend: too many rows");
-  const int64_t need = attend_bytes(p.blocks_max, B, D);
+  p.min_tiles = kMinTiles;
+  p.slots = call_slots(p.blocks_max, B, T, D, max_pages * page, p.window, idx ? topk : -1);
+  const int64_t need = slot_bytes(p.slots, p.blocks_max, D);
   MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attend: workspace needs %lld bytes",
                 (long long)need);
-  // what a sequence can hold, or a token see, in tiles
-  int64_t most = max_pages * page;
-  if (p.window + T < most) most = p.window + T;
-  if (idx) most = topk;
-  p.min_tiles = kMinTiles;
-  p.slots = B && splits((most + kTile - 1) / kTile, p.blocks_max) ? unit_slots(p.blocks_max, B, D) : 0;
   if (p.slots) {
     p.blocks_out = static_cast<int32_t*>(workspace);
     p.joins = reinterpret_cast<JoinRow*>(static_cast<uint8_t*>(workspace) + 16);
@@ -709,8 +715,14 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
 }
 
 extern "C" int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t* bytes) {
+  return mzk_paged_attend_call_workspace_bytes(T, H, D, packed, B, kMaxInt, 1, 0, -1, bytes);
+}
+
+extern "C" int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages,
+                                                     int page, int64_t window, int topk, int64_t* bytes) {
   MZK_CHECK_ARG(bytes != nullptr, "paged_attend_workspace_bytes: null output");
-  MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0, "paged_attend_workspace_bytes: bad sizes");
+  MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && max_pages >= 0 && max_pages <= kMaxInt && page >= 1 && window >= 0,
+                "paged_attend_workspace_bytes: bad sizes");
   MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536 && D <= 65536, "paged_attend_workspace_bytes: sizes of 2^31 or more");
   RaggedParams p{};
   p.T = T;
@@ -720,7 +732,8 @@ extern "C" int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int pac
   const int64_t some = 0;
   p.cu = packed ? &some : nullptr;  // only whether there is one counts
   set_units(p);
-  *bytes = attend_bytes(p.blocks_max, B, D);
+  const int slots = call_slots(p.blocks_max, B, T, D, max_pages * page, call_window(window, packed ? T : 1), topk);
+  *bytes = slot_bytes(slots, p.blocks_max, D);
   return MZK_OK;
 }
 

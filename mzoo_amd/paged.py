@@ -132,10 +132,17 @@ def append(pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, x: torc
 
 
 @functools.lru_cache(maxsize=1024)
-def attend_workspace_bytes(tokens: int, heads: int, dim: int, batch: int, packed: bool) -> int:
-    """What ``attend`` splits long sequences into: the partial results (``mzk_paged_attend_workspace_bytes``)."""
+def attend_workspace_bytes(tokens: int, heads: int, dim: int, batch: int, packed: bool, max_pages: int | None = None, page: int = 1,
+                           window: int = 0, k: int = -1) -> int:
+    """What ``attend`` splits long sequences into: the partial results.  Without ``max_pages`` enough for any
+    tables, windows and lists; with it what a call takes whose tables have so many columns (``window`` 0: none;
+    ``k``: the positions of its lists, -1: none), 0 where no sequence is split."""
     n = ctypes.c_int64(0)
-    _lib.call("mzk_paged_attend_workspace_bytes", tokens, heads, dim, int(packed), batch, ctypes.byref(n))
+    if max_pages is None:
+        _lib.call("mzk_paged_attend_workspace_bytes", tokens, heads, dim, int(packed), batch, ctypes.byref(n))
+    else:
+        _lib.call("mzk_paged_attend_call_workspace_bytes", tokens, heads, dim, int(packed), batch, max_pages, page, window, k,
+                  ctypes.byref(n))
     return n.value
 
 
@@ -191,14 +198,15 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
     else:
         out = torch.empty_like(q)
         lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
-    need = attend_workspace_bytes(t, h, d, b, cu is not None)
+    wide = min(window or 0, (1 << 63) - 1)
+    need = attend_workspace_bytes(t, h, d, b, cu is not None, width, page, wide, k if idx else -1)
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"attend: the workspace must be contiguous uint8 of at least {need} bytes")
     _call(q.device, "mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
-          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, min(window or 0, (1 << 63) - 1), _lib.ptr(sinks),
+          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, wide, _lib.ptr(sinks),
           _lib.ptr(workspace) if need else None, need, out.data_ptr(), lse.data_ptr(), 0 if given else 1)
     return out, lse
 

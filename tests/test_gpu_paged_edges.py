@@ -308,3 +308,17 @@ def test_compact_says_where_pages_went(dev, pages, inplace):
     assert torch.equal(dp.cpu()[m[other]], pool[other])
     assert torch.equal(got[0].cpu().long(), m[tables.long()]) and torch.equal(got[1].cpu()[m[refs > 0]], refs[refs > 0])
     assert sorted(m[refs > 0].tolist()) == list(range(used)) and torch.equal(m[refs == 0], (refs == 0).nonzero()[:, 0])
+
+
+def test_attend_of_short_sequences_takes_no_room_for_shares(dev):
+    """400 sequences of ten tokens are not split, so nothing is allocated but the results."""
+    pool, tables, n64, _, _ = _setup(dev, [10] * 400, 16, 576, "fp8", 97)
+    q = torch.randn(400, 16, 576, generator=_gen(98)).bfloat16().to(dev)
+    want = paged.attend(q, pool, tables, n64)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = paged.attend(q, pool, tables, n64)
+    assert torch.cuda.max_memory_allocated() - before < 2 * (q.numel() * 2 + 400 * 16 * 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

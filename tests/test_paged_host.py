@@ -198,3 +198,19 @@ def test_compact_refuses_other_maps(fake_gpu):
     for moved in (torch.zeros(8), torch.zeros(7, dtype=torch.int32), torch.zeros(16, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="moved"):
             paged.compact(t, r, moved=moved)
+
+
+def test_workspace_of_calls_that_are_not_split():
+    """Short tables, windows and lists take no workspace; a call that is split takes no more than any call may."""
+    size = paged.attend_workspace_bytes
+    most = size(400, 16, 576, 400, False)
+    assert most > 100 << 20
+    assert size(400, 16, 576, 400, False, 10, 16) == 0
+    assert size(400, 16, 576, 400, False, 2000, 16) == most
+    assert size(400, 16, 576, 400, False, 2000, 16, 128) == 0
+    assert size(400, 16, 576, 400, False, 2000, 16, 0, 256) == 0
+    assert size(8, 128, 576, 8, False, 2000, 16, 0, 2048) == size(8, 128, 576, 8, False)
+    assert size(8, 128, 576, 8, False, 2000, 16, 0, 0) == 0
+    assert size(0, 128, 576, 0, False) == size(8, 128, 576, 0, True, 2000, 16) == 0
+    with pytest.raises(_lib.MzkError, match="bad sizes"):
+        size(8, 128, 576, 8, False, -1, 16)
