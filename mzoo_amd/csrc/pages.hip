@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256) grow_count_kernel(const GrowParams p) {
 }
 
 // grow is bound by its three launches in turn, each a chain of loads and scans: 128 sequences over 16384
-// pages take 3.1 + 5.5 + 5.0 us, the copies of the shared last pages in the last.
+// pages take 3.4 + 5.2 + 4.9 us, the copies of the shared last pages in the last.
 //
 // A chunk's free pages by rank, and its counts.  Every workgroup adds up the chunks' and the rows' numbers itself.
 __global__ void __launch_bounds__(256) grow_assign_kernel(const GrowParams p) {

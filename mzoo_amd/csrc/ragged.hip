@@ -617,7 +617,9 @@ int unit_slots(int64_t blocks, int64_t B, int D) {
 // Whether a call is split in whose longest sequence a token may see so many tiles.  The joining launch
 // and the second start of a compute unit cost some 7 and 15 us.  10 sequences x 128 heads over 8 tiles take
 // 19.9 us whole and 23.2 split, 2 over 17 tiles 29.0 and 22.1; 140 blocks over 31 tiles 49 and 75, over 94
-// tiles 115 and 102; 500 blocks over 125 tiles 290 and 317.
+// tiles 115 and 102; 500 blocks over 125 tiles 290 and 317.  The host knows no lengths, so the table's room
+// stands for them: short sequences in wide tables are split too (100 of 500 x 128 heads 34 us with a table of their
+// width, 75 with one of 131072 entries).
 bool splits(int64_t tiles, int64_t blocks) { return tiles > 12 && tiles > blocks / 2; }
 
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }

@@ -5,7 +5,7 @@
 // one arriving).  Per tile:
 //   S^T  wave w: entries 16 w .. + 15 x all 64 rows (v_mfma_f32_16x16x32_bf16, q in registers, one
 //        K operand read for four row groups), so a lane has 4 entries of each of its 4 rows;
-//   P^T  to LDS in bf16 (8 KB);
+//   P^T  to LDS in bf16 (8 KB; the row sums take the unrounded weights: see ragged_wide.h);
 //   O^T  wave w: the 16-channel blocks w, w + 4, .. x 64 rows, one V^T operand read for four row groups.
 // Two barriers a tile.  A tile is some 200 cycles of matrix work at D = 160 and its softmax as many of
 // vector work, so what carries it is two workgroups on a compute unit, each in the other's waits (256
@@ -14,7 +14,8 @@
 //
 // What bounds it: latency and vector work.  17 prompts of up to 700 tokens x 8 heads of 160 channels take 35
 // us (8 at the memory's rate, 6 at the matrix units'), 24 sequences of up to 9000 with four new tokens of 16 heads
-// 26 us and 7 for the join (10 at the memory's rate), 32 of up to 20000 x 16 heads 45 us in all (26).
+// 26 us and 8 for the join (9 at the memory's rate), 32 of up to 20000 x 16 heads 43 us in all (26).  Pages also
+// cost a pause every CT tiles, where the next codes are laid out with no tile in flight.
 //
 // A tile in LDS is D / 32 columns of 64 rows of 64 bytes: a wave's load instruction (16 rows x 64 bytes, a
 // lane 16 of them) fills 1 KB of one column from one address per lane and tile, and an MFMA step of S^T

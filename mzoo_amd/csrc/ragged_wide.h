@@ -6,7 +6,10 @@
 //   S^T  wave (eh, hh): entries 16 eh .. + 15 of the tile x rows 32 hh .. + 31 over all channels
 //        (v_mfma_f32_16x16x32_bf16, two row groups per K operand read), so a score is whole in the
 //        lane that has it;
-//   P^T  goes to LDS in bf16 (4 KB a tile, two of them);
+//   P^T  goes to LDS in bf16 (4 KB a tile, two of them), what the matrix instructions take beside V^T: each
+//        weight is off by up to 2^-8 of itself, while the row sums take the unrounded ones in 32 bits.  Against 64
+//        bits a result is off by 0.0017 to 0.0022 of its norm, by 0.0017 with unrounded weights (its own bf16);
+//        weights as two bf16 terms would double the work of O^T;
 //   O^T  wave w: the 16-channel blocks w, w + 4, .. for all 64 rows, one V^T operand read for four
 //        row groups.
 // One barrier per tile: in iteration u the workgroup runs S(u+1) and PV(u), whose matrix work covers
@@ -15,13 +18,15 @@
 //
 // RG: the unit's row groups of 16, 4, or for one new token of up to 16 or 32 heads 1 or 2 (1: the waves of
 // hh = 1 repeat the scores of hh = 0).  The matrix work falls with them, and the device's clock need not: 32
-// sequences of up to 32k, 8-bit entries, 154 -> 120 us with 16 heads, 158 -> 132 with 32.
+// sequences of up to 32k, 8-bit entries, 154 -> 120 us with 16 heads, 158 -> 128 with 32.
 //
 // What bounds it: the matrix units, shared with one wave's issue of everything else.  8192 tokens x 128 heads of 576
 // channels, causal, take 8.3 to 9.2 ms (1190 to 1080 TFLOP/s, by the clock the device holds); 32 sequences of up
-// to 32768 x 128 heads, 8-bit, 238 us (850 TFLOP/s: shares of unequal length, a start of 15 us); one of
+// to 32768 x 128 heads, 8-bit, 248 us with the join's 12 (820 TFLOP/s; shares of unequal length, a start of 15
+// us), and the launch alone 263 to 305 in twenty calls on end under a kernel trace, presumably by the clock too; one of
 // 4096 21 us, a chain: unit 3, q and tables 5, tiles 5, results 4.  Behind a window of 128, 16 heads,
-// 23.7 K tokens take 420 us: q 4, tiles 6, results 3 of a unit's 18 us, one after the other.
+// 23.7 K tokens take 420 us: q 4, tiles 6, results 3 of a unit's 18 us, one after the other.  Pages also cost a
+// pause every CT tiles, where the next codes are laid out with no tile in flight.
 //
 // A tile in LDS is D / 64 columns of 32 rows of 128 bytes: a wave's load instruction (8 rows x 128
 // bytes, a lane 16 of them) fills 1 KB of one column, in lane order as the hardware wants it, from

@@ -13,8 +13,8 @@ without the host:
   it is written.
 
 ``grow`` makes room and counts the new tokens, ``append`` writes their entries, ``attend`` attends
-them; ``fork`` lets sequences begin as copies of others or end; ``compact`` moves the used pages to
-the front.  One step of decoding::
+them; lowering ``lens`` takes refused tokens back; ``fork`` lets sequences begin as copies of others or
+end; ``compact`` moves the used pages to the front.  One step of decoding::
 
     paged.grow(tables, lens, refs, ones, page, pools=pools, out=(tables, lens, refs), missing=missing)
     paged.append(pool, tables, lens, kv)
@@ -155,10 +155,11 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
     q bf16 [T, H, D]: one token per sequence, or with ``cu`` the last ``cu[b + 1] - cu[b]`` of each (drafted
     tokens, a chunk of a prompt), each at its own position and causal.  A token sees its sequence up
     to itself, the last ``window`` positions of that, or -- one token per sequence -- the positions
-    ``indices`` int32 [B, k] lists (outside the sequence: empty; k 0: none).  ``sinks`` fp32 [H].  Returns (o bf16
-    [T, H, D], lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a
-    given ``out`` and ``lse``.  Positions on no page or past the table are empty; a token that sees nothing gets 0.  ``workspace``: uint8, of
-    ``attend_workspace_bytes``, allocated per call if omitted; calls that overlap need their own."""
+    ``indices`` int32 [B, k] lists (outside the sequence: empty; k 0: none).  Positions on no page or
+    past the table are empty.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D], lse fp32 [T, H]); rows behind
+    the last sequence are 0 (-inf), or as they were in a given ``out`` and ``lse``.  A token that sees
+    nothing gets 0.  ``workspace``: uint8, of ``attend_workspace_bytes``, allocated per call if omitted;
+    calls that overlap need their own."""
     _one_device("attend", q, pool, tables, lens, cu, indices, sinks, workspace, out, lse)
     if q.dim() != 3 or q.shape[1] < 1:
         raise ValueError(f"attend: q must be [T, H, D], got {list(q.shape)}")
