@@ -667,6 +667,16 @@ int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int packed, int64_
 int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages, int page,
                                           int64_t window, int topk, int64_t* bytes);
 
+/* With a window, the first `first` positions (below 2^30) of a sequence stay visible to every token behind
+ * them, too: token t sees position j <= t if j > t - window or j < first.  first 0: as above. */
+int mzk_paged_attend_first(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, int fmt, int nope,
+                           const void* pool, int64_t pages, int page, const int32_t* tables, int64_t table_stride,
+                           int64_t max_pages, const int64_t* lens, const int32_t* idx, int64_t idx_row_stride, int topk,
+                           int64_t window, int64_t first, const float* sinks, void* workspace, int64_t workspace_bytes,
+                           void* out, float* lse, int zero_tail, void* stream);
+int mzk_paged_attend_first_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages, int page,
+                                           int64_t window, int64_t first, int topk, int64_t* bytes);
+
 /* Causal attention over packed prompts: the latent_attn and swa_attn levels
  * (layers/attn/latent_attn/fwd.py:45, layers/attn/swa_attn/fwd.py:55) without padding.  q [T, H, D]
  * bf16; kv [T, G, D] bf16 with rows kv_row_stride elements apart (a multiple of 8), head h attends
@@ -675,6 +685,11 @@ int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, int packed, i
 int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, const void* kv,
                    int64_t kv_row_stride, int G, int64_t window, const float* sinks, void* out, float* lse,
                    int zero_tail, void* stream);
+
+/* The same with `first` as in mzk_paged_attend_first. */
+int mzk_packed_mqa_first(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, const void* kv,
+                         int64_t kv_row_stride, int G, int64_t window, int64_t first, const float* sinks, void* out,
+                         float* lse, int zero_tail, void* stream);
 
 #ifdef __cplusplus
 }

@@ -98,6 +98,11 @@ _SIGS = {
                          _I64, _P, _P, _I64, _P, _P, _I32, _P],
     "mzk_paged_attend_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, ctypes.POINTER(_I64)],
     "mzk_paged_attend_call_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, _I64, _I32, _I64, _I32, ctypes.POINTER(_I64)],
+    "mzk_paged_attend_first": [_P, _I64, _I32, _I32, _P, _I64, _I32, _I32, _P, _I64, _I32, _P, _I64, _I64, _P, _P, _I64,
+                               _I32, _I64, _I64, _P, _P, _I64, _P, _P, _I32, _P],
+    "mzk_paged_attend_first_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, _I64, _I32, _I64, _I64, _I32,
+                                               ctypes.POINTER(_I64)],
+    "mzk_packed_mqa_first": [_P, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _I32, _P],
     "mzk_packed_mqa": [_P, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32, _I64, _P, _P, _P, _I32, _P],
     "mzk_indexer_decode_fused": [_I32, _P, _P, _P, _P, _I64, _I32, _I32, _I64, _I64, _P, _I32, _P, _I64, _P, _P, _P,
                                  _P, _I32, _P, _P, _F32, _P, _P, _I32, _I32, _P, _I64, _I32, _P],

@@ -156,14 +156,14 @@ def attn(q, kv, main_kv, indices, *, window: int, compress_ratio: int, causal: b
 
 
 def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int | None = None,
-           sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+           first: int = 0, sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
     """Causal attention over whole prompts of different lengths, packed one after another: the
     latent_attn / swa_attn levels (``layers/attn/latent_attn/fwd.py:45``, ``layers/attn/swa_attn/fwd.py:55``)
     without padding.
 
     q bf16 [T, H, D]; kv bf16 [T, G, D] (K == V), head h on latent ``h // (H // G)``; cu int64 [B + 1],
     ascending from 0: sequence b is rows ``cu[b] .. cu[b + 1] - 1``.  A token sees its sequence up to
-    itself, or the last ``window`` tokens of that.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D],
+    itself, or the last ``window`` tokens of that and beside them the ``first`` of the sequence.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D],
     lse fp32 [T, H]); rows behind the last sequence are 0 (-inf), or as they were in a given ``out``
     and ``lse``."""
     _lib.require_gpu(q)
@@ -183,6 +183,8 @@ def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int |
         raise ValueError(f"packed: cu must be contiguous int64 [B + 1], got {cu.dtype} {list(cu.shape)}")
     if window is not None and (not isinstance(window, int) or window < 1):
         raise ValueError(f"packed: window must be a positive int or None, got {window!r}")
+    if not isinstance(first, int) or not 0 <= first < 1 << 30 or first and window is None:
+        raise ValueError(f"packed: first must be an int of at least 0, below 2^30, and goes with a window, got {first!r}")
     given = out is not None
     if given != (lse is not None):
         raise ValueError("packed: out and lse go together")
@@ -198,13 +200,13 @@ def packed(q: torch.Tensor, kv: torch.Tensor, cu: torch.Tensor, *, window: int |
     if not given:
         out = torch.empty_like(q)
         lse = torch.empty((t, h), dtype=torch.float32, device=dev)
-    args = (q.data_ptr(), t, h, d, cu.data_ptr(), cu.shape[0] - 1, kv.data_ptr(), row if t > 1 else g * d, g, min(window or 0, 1 << 30),
+    args = (q.data_ptr(), t, h, d, cu.data_ptr(), cu.shape[0] - 1, kv.data_ptr(), row if t > 1 else g * d, g, min(window or 0, 1 << 30), first,
             _lib.ptr(sinks), out.data_ptr(), lse.data_ptr(), 0 if given else 1, _lib.raw_stream(dev))
     if torch.cuda.current_device() == dev.index:
-        _lib.call("mzk_packed_mqa", *args)
+        _lib.call("mzk_packed_mqa_first", *args)
     else:
         with torch.cuda.device(dev):
-            _lib.call("mzk_packed_mqa", *args)
+            _lib.call("mzk_packed_mqa_first", *args)
     return out, lse
 
 

@@ -4,7 +4,8 @@
 //   o[t, h] = sum_j p_j e_j,  p = softmax over the entries j that token t sees of q[t, h] . e_j D^-1/2,
 //   the head's sink one more term of the denominator; lse its logarithm.  K == V == e.
 //   Token i of the n new ones of a sequence with len tokens is at position len - n + i and sees
-//   positions 0 .. its own, the last `window` of them, or the positions of its list.
+//   positions 0 .. its own, the last `window` of them and the `first` of the sequence, or the
+//   positions of its list.
 //
 // A unit of work is a block of 64 rows -- a row is a head of a token, the heads of one latent
 // innermost, so 64 rows are 64 heads of a token or all heads of several -- over all of the
@@ -55,6 +56,7 @@ struct RaggedParams {
   int64_t idx_stride;
   int topk;
   int window;
+  int first;     // with a window: the sequence's first positions that every token behind them sees too
   int64_t past;  // lengths past a table's entries that are told apart: the window; without one -1
   const float* sinks;
   float scale_log2;
@@ -132,7 +134,7 @@ __device__ __forceinline__ int sequence(const RaggedParams& p, int i, int& a, in
   int seen = z - a;
   if (p.lens) seen = static_cast<int>(clamp64(p.lens[i], 0, p.max_pages * p.page));
   if (p.idx) seen = seen > 0 ? p.topk : 0;
-  if (seen - (z - a) > p.window) seen = p.window + (z - a);
+  if (seen - (z - a) - p.first > p.window) seen = p.window + (z - a) + p.first;
   tiles = (seen + kTile - 1) / kTile;
   return ((z - a) * p.HG + (1 << p.unit_shift) - 1) >> p.unit_shift;
 }
@@ -412,15 +414,58 @@ __device__ __forceinline__ void token_range(const RaggedParams& p, const Unit& u
   }
 }
 
-// This unit's share of the tiles that its tokens tok0 .. tok1 - 1 see.
+// This unit's share of the tiles that its tokens tok0 .. tok1 - 1 see.  With first positions that stay visible
+// (FIRST), `head` of them lie before the window's and are counted as if directly before it.
+template <bool FIRST>
 __device__ __forceinline__ void unit_range(const RaggedParams& p, const Unit& u, int tok0, int tok1, int& lo, int& hi) {
   token_range(p, u, tok0, tok1, lo, hi);
+  if (FIRST) lo -= p.first < lo ? p.first : lo;
   if (u.shares > 1) {
     const int tiles = (hi - lo + kTile - 1) / kTile, per = (tiles + u.shares - 1) / u.shares;
     const int64_t from = lo + static_cast<int64_t>(u.share) * per * kTile;
     if (from + per * kTile < hi) hi = static_cast<int>(from) + per * kTile;
     lo = from < hi ? static_cast<int>(from) : hi;
   }
+}
+
+// The entries of a pass: places lo .. hi - 1, of which those from `body` on are positions, and those before it the
+// positions `jump` away: the first of the sequence that stay visible.
+struct Pass {
+  int lo, hi;
+  int body, jump;
+};
+
+// What the tokens sub0 .. sub1 - 1 of a unit of tokens tok0 .. see of its share share_lo .. share_hi - 1
+// (places of the unit, of which the first positions are those before the unit's window).
+template <bool FIRST>
+__device__ __forceinline__ Pass pass_range(const RaggedParams& p, const Unit& u, int tok0, int sub0, int sub1, int share_lo, int share_hi) {
+  Pass w;
+  token_range(p, u, sub0, sub1, w.lo, w.hi);
+  const int seen_lo = w.lo;
+  w.lo = w.lo > share_lo ? w.lo : share_lo;
+  w.hi = w.hi < share_hi ? w.hi : share_hi;
+  if (w.hi < w.lo) w.hi = w.lo;
+  w.body = w.lo;
+  w.jump = 0;
+  if (FIRST) {
+    int unit_lo, unit_hi;  // the unit's window begins there
+    token_range(p, u, tok0, tok0 + 1, unit_lo, unit_hi);
+    // head: positions h0 .. h1 - 1, all before the window of every token of the pass
+    int h0 = share_lo, h1 = share_hi;
+    if (p.first < unit_lo) {
+      h1 = h1 < unit_lo ? h1 : unit_lo;
+      h0 -= unit_lo - p.first;
+      h1 -= unit_lo - p.first;
+    } else {
+      h1 = h1 < p.first ? h1 : p.first;
+      h1 = h1 < seen_lo ? h1 : seen_lo;
+    }
+    if (h1 > h0) {
+      w.jump = h1 - w.body;
+      w.lo = w.body - (h1 - h0);
+    }
+  }
+  return w;
 }
 
 // The entry at position v of the unit's sequence (or of its list) in a pool; -1: none.
@@ -530,8 +575,8 @@ __global__ void __launch_bounds__(256) join_kernel(const RaggedParams p) {
   *reinterpret_cast<uint2*>(p.out + (j.row0 + row) * D + 16 * blk + c) = uint2{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
 }
 
-template <int FMT, int D, int NOPE>
-int launch_ragged(const RaggedParams& p, hipStream_t s) {
+template <int FMT, int D, int NOPE, bool FIRST>
+int launch_ragged_as(const RaggedParams& p, hipStream_t s) {
   // (find_unit's order takes 16 workgroups at a time)
   const int64_t grid = p.slots ? p.slots : p.blocks_max / 16 * 16 + 16;
   using M = std::conditional_t<(D > 256), WideLds<FMT, D>, NarrowLds<FMT, D>>;
@@ -539,9 +584,11 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   int which = 0;
   if constexpr (D > 256) {
     which = p.cu || p.H > 32 ? 0 : p.H > 16 ? 1 : 2;
-    kern = which == 0 ? ragged_wide_kernel<FMT, D, NOPE, 4> : which == 1 ? ragged_wide_kernel<FMT, D, NOPE, 2> : ragged_wide_kernel<FMT, D, NOPE, 1>;
+    kern = which == 0   ? ragged_wide_kernel<FMT, D, NOPE, 4, FIRST>
+           : which == 1 ? ragged_wide_kernel<FMT, D, NOPE, 2, FIRST>
+                        : ragged_wide_kernel<FMT, D, NOPE, 1, FIRST>;
   } else {
-    kern = ragged_narrow_kernel<FMT, D, NOPE>;
+    kern = ragged_narrow_kernel<FMT, D, NOPE, FIRST>;
   }
   // the dynamic-LDS limit is a per-device function attribute: set once per device
   static std::atomic<bool> attr_set[3][kMaxDevices] = {};  // setting it twice is harmless
@@ -567,6 +614,11 @@ int launch_ragged(const RaggedParams& p, hipStream_t s) {
   }
   MZK_LAUNCH_CHECK("ragged attention");
   return MZK_OK;
+}
+
+template <int FMT, int D, int NOPE>
+int launch_ragged(const RaggedParams& p, hipStream_t s) {
+  return p.first ? launch_ragged_as<FMT, D, NOPE, true>(p, s) : launch_ragged_as<FMT, D, NOPE, false>(p, s);
 }
 
 int dispatch_ragged(const char* name, int fmt, int nope, const RaggedParams& p, hipStream_t s) {
@@ -625,10 +677,10 @@ bool splits(int64_t tiles, int64_t blocks) { return tiles > 12 && tiles > blocks
 int64_t align16_up(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 // The units that a call is split into (0: none is) by what a sequence can hold, or a token see: the room of its
-// table, its window and the new tokens, or its list (topk -1: none).
-int call_slots(int64_t blocks, int64_t B, int64_t T, int D, int64_t room, int64_t window, int64_t topk) {
+// table, its window, first positions and new tokens, or its list (topk -1: none).
+int call_slots(int64_t blocks, int64_t B, int64_t T, int D, int64_t room, int64_t window, int64_t first, int64_t topk) {
   int64_t most = room;
-  if (window + T < most) most = window + T;
+  if (window + first + T < most) most = window + first + T;
   if (topk >= 0) most = topk;
   return B && splits((most + kTile - 1) / kTile, blocks) ? unit_slots(blocks, B, D) : 0;
 }
@@ -652,6 +704,15 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                                 int64_t max_pages, const int64_t* lens, const int32_t* idx, int64_t idx_row_stride,
                                 int topk, int64_t window, const float* sinks, void* workspace, int64_t workspace_bytes,
                                 void* out, float* lse, int zero_tail, void* stream) {
+  return mzk_paged_attend_first(q, T, H, D, cu, B, fmt, nope, pool, pages, page, tables, table_stride, max_pages, lens, idx,
+                                idx_row_stride, topk, window, 0, sinks, workspace, workspace_bytes, out, lse, zero_tail, stream);
+}
+
+extern "C" int mzk_paged_attend_first(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, int fmt, int nope,
+                                      const void* pool, int64_t pages, int page, const int32_t* tables, int64_t table_stride,
+                                      int64_t max_pages, const int64_t* lens, const int32_t* idx, int64_t idx_row_stride,
+                                      int topk, int64_t window, int64_t first, const float* sinks, void* workspace,
+                                      int64_t workspace_bytes, void* out, float* lse, int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0, "paged_attend: bad sizes");
   MZK_CHECK_ARG(T < kNoWindow && B <= kMaxInt && H <= 65536 && pages >= 0 && pages <= kMaxInt && max_pages >= 0 &&
                     max_pages <= kMaxInt,
@@ -662,6 +723,8 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
                 "paged_attend: a sequence and a pool hold less than 2^31 entries, a sequence twice the new tokens less");
   MZK_CHECK_ARG(fmt == 0 || fmt == 1, "paged_attend: fmt must be 0 (bf16) or 1 (fp8-b128)");
   MZK_CHECK_ARG(window >= 0 && topk >= 0, "paged_attend: negative window or list");
+  MZK_CHECK_ARG(first >= 0 && first < kNoWindow && (first == 0 || window > 0),
+                "paged_attend: first positions, less than 2^30, go with a window");
   MZK_CHECK_ARG(cu || T == B, "paged_attend: without cu one token per sequence (%lld tokens, %lld sequences)",
                 (long long)T, (long long)B);
   MZK_CHECK_ARG(!idx || (cu == nullptr && window == 0 && idx_row_stride >= topk),
@@ -694,6 +757,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.topk = topk;
   p.window = static_cast<int>(call_window(window, most_new));
   p.past = has_window(window, most_new) ? p.window : -1;
+  p.first = has_window(window, most_new) ? static_cast<int>(first) : 0;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);
@@ -702,7 +766,7 @@ extern "C" int mzk_paged_attend(const void* q, int64_t T, int H, int D, const in
   p.zero_tail = zero_tail;
   MZK_CHECK_ARG(p.blocks_max < kMaxBlocks && T * H <= kMaxInt - 64, "paged_attend: too many rows");
   p.min_tiles = kMinTiles;
-  p.slots = call_slots(p.blocks_max, B, T, D, max_pages * page, p.window, idx ? topk : -1);
+  p.slots = call_slots(p.blocks_max, B, T, D, max_pages * page, p.window, p.first, idx ? topk : -1);
   const int64_t need = slot_bytes(p.slots, p.blocks_max, D);
   MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attend: workspace needs %lld bytes",
                 (long long)need);
@@ -722,8 +786,14 @@ extern "C" int mzk_paged_attend_workspace_bytes(int64_t T, int H, int D, int pac
 
 extern "C" int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages,
                                                      int page, int64_t window, int topk, int64_t* bytes) {
+  return mzk_paged_attend_first_workspace_bytes(T, H, D, packed, B, max_pages, page, window, 0, topk, bytes);
+}
+
+extern "C" int mzk_paged_attend_first_workspace_bytes(int64_t T, int H, int D, int packed, int64_t B, int64_t max_pages,
+                                                      int page, int64_t window, int64_t first, int topk, int64_t* bytes) {
   MZK_CHECK_ARG(bytes != nullptr, "paged_attend_workspace_bytes: null output");
-  MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && max_pages >= 0 && max_pages <= kMaxInt && page >= 1 && window >= 0,
+  MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && max_pages >= 0 && max_pages <= kMaxInt && page >= 1 && window >= 0 &&
+                    first >= 0 && first < kNoWindow && (first == 0 || window > 0),
                 "paged_attend_workspace_bytes: bad sizes");
   MZK_CHECK_ARG(T <= kMaxInt && B <= kMaxInt && H <= 65536 && D <= 65536, "paged_attend_workspace_bytes: sizes of 2^31 or more");
   RaggedParams p{};
@@ -734,7 +804,8 @@ extern "C" int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, in
   const int64_t some = 0;
   p.cu = packed ? &some : nullptr;  // only whether there is one counts
   set_units(p);
-  const int slots = call_slots(p.blocks_max, B, T, D, max_pages * page, call_window(window, packed ? T : 1), topk);
+  const int slots = call_slots(p.blocks_max, B, T, D, max_pages * page, call_window(window, packed ? T : 1),
+                               has_window(window, packed ? T : 1) ? first : 0, topk);
   *bytes = slot_bytes(slots, p.blocks_max, D);
   return MZK_OK;
 }
@@ -742,10 +813,18 @@ extern "C" int mzk_paged_attend_call_workspace_bytes(int64_t T, int H, int D, in
 extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, const void* kv,
                               int64_t kv_row_stride, int G, int64_t window, const float* sinks, void* out, float* lse,
                               int zero_tail, void* stream) {
+  return mzk_packed_mqa_first(q, T, H, D, cu, B, kv, kv_row_stride, G, window, 0, sinks, out, lse, zero_tail, stream);
+}
+
+extern "C" int mzk_packed_mqa_first(const void* q, int64_t T, int H, int D, const int64_t* cu, int64_t B, const void* kv,
+                                    int64_t kv_row_stride, int G, int64_t window, int64_t first, const float* sinks, void* out,
+                                    float* lse, int zero_tail, void* stream) {
   MZK_CHECK_ARG(T >= 0 && B >= 0 && H >= 1 && D > 0 && G >= 1, "packed_mqa: bad sizes");
   MZK_CHECK_ARG(T < kNoWindow && B <= kMaxInt && H <= 65536, "packed_mqa: 2^30 tokens, or sizes of 2^31");
   MZK_CHECK_ARG(H % G == 0, "packed_mqa: %d heads do not divide into %d latents", H, G);
   MZK_CHECK_ARG(window >= 0, "packed_mqa: negative window");
+  MZK_CHECK_ARG(first >= 0 && first < kNoWindow && (first == 0 || window > 0),
+                "packed_mqa: first positions, less than 2^30, go with a window");
   MZK_CHECK_ARG(kv_row_stride >= static_cast<int64_t>(G) * D && kv_row_stride % 8 == 0 && kv_row_stride < 1ll << 30,
                 "packed_mqa: kv rows must be G * D apart or more, a multiple of 8 elements below 2^30");
   if (T == 0) return MZK_OK;
@@ -763,6 +842,7 @@ extern "C" int mzk_packed_mqa(const void* q, int64_t T, int H, int D, const int6
   p.entries = static_cast<const uint8_t*>(kv);
   p.entry_stride = 2 * kv_row_stride;
   p.window = window && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
+  p.first = p.window < kNoWindow ? static_cast<int>(first) : 0;
   p.sinks = sinks;
   p.scale_log2 = (1.0f / __builtin_sqrtf(static_cast<float>(D))) * kLog2e;
   set_units(p);

@@ -54,7 +54,7 @@ struct NarrowLds {
   static_assert(LDS <= 80 * 1024, "two workgroups a compute unit");
 };
 
-template <int FMT, int D, int NOPE>
+template <int FMT, int D, int NOPE, bool FIRST>
 __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(const RaggedParams p) {
   using M = NarrowLds<FMT, D>;
   using L = Layout<FMT, D, NOPE>;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
   const int shift = u.len - u.n;
   int share_lo, share_hi;
-  unit_range(p, u, tok0, tok1, share_lo, share_hi);
+  unit_range<FIRST>(p, u, tok0, tok1, share_lo, share_hi);
   const bool paged = p.tables != nullptr;
   const uint64_t first_entry = reinterpret_cast<uint64_t>(p.entries) +
                                (paged ? 0 : static_cast<uint64_t>(u.t0) * p.entry_stride + static_cast<uint64_t>(u.g) * L::kEntryBytes);
@@ -96,17 +96,21 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   const uint64_t piece = first_entry + (M::kDirect ? 16u * ((lane & 3) ^ narrow_swz(ld_row)) : 0u);
 
   int lo = 0, hi = 0, c0 = 0, nt = 0;
+  int body = 0, jump = 0;  // with first positions: places from `body` on are positions, the others `jump` from theirs
+  auto position = [&](int v) __attribute__((always_inline)) -> int { return FIRST && v < body ? v + jump : v; };
   int sub0 = tok0, sub1 = tok1;
-  int row_lo[4], row_span[4], tok_h[4];
+  int row_lo[4], row_span[4], row_head[4], tok_h[4];
   int full_lo = 0, full_hi = 0;
   auto set_range = [&]() __attribute__((always_inline)) {
-    token_range(p, u, sub0, sub1, lo, hi);
-    lo = lo > share_lo ? lo : share_lo;
-    hi = hi < share_hi ? hi : share_hi;
-    if (hi < lo) hi = lo;
+    const Pass w = pass_range<FIRST>(p, u, tok0, sub0, sub1, share_lo, share_hi);
+    lo = w.lo;
+    hi = w.hi;
+    body = w.body;
+    jump = w.jump;
     int most_lo = lo, least_hi = hi;
     if (!p.idx) {
       most_lo = clamp32(shift + sub1 - p.window, lo, 0x7fffffff - kTile64);
+      if (FIRST && most_lo <= body) most_lo = lo;
       least_hi = shift + sub0 + 1 < hi ? shift + sub0 + 1 : hi;
     }
     full_lo = (most_lo - lo + kTile64 - 1) / kTile64;
@@ -120,6 +124,10 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
         const int pos = shift + tok_h[hg];
         if (pos - p.window + 1 > a) a = pos - p.window + 1;
         if (pos + 1 < z) z = pos + 1;
+      }
+      if (FIRST) {
+        const int end = body > p.first ? body : p.first, past = shift + tok_h[hg] + 1;
+        row_head[hg] = (end < past ? (end < hi ? end : hi) : past < hi ? past : hi) - lo;
       }
       row_lo[hg] = a - lo;
       row_span[hg] = z > a ? z - a : 0;
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
     for (int e0 = 0; e0 < nt * kTile64; e0 += NT) {
       const int e = e0 + tid;
       uint32_t code = kEmpty;
-      if (e < nt * kTile64 && e < left) code = static_cast<uint32_t>(pool_entry(p, u, lo + c0 + e));  // -1: kEmpty
+      if (e < nt * kTile64 && e < left) code = static_cast<uint32_t>(pool_entry(p, u, position(lo + c0 + e)));  // -1: kEmpty
       const uint64_t bal = __ballot(code != kEmpty);
       if (e < nt * kTile64) {
         tab[e] = code;
@@ -168,7 +176,7 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
   auto code_of = [&](int t, int row) __attribute__((always_inline)) -> uint32_t {
     if (paged) return tab[t * kTile64 + row];
     const int v = c0 + t * kTile64 + row;
-    return static_cast<uint32_t>(lo + (v < hi - lo ? v : hi - lo - 1));
+    return static_cast<uint32_t>(position(lo + (v < hi - lo ? v : hi - lo - 1)));
   };
   Piece raw[M::kDirect ? 1 : PPT];
   // tile t requested: straight into its buffer, or into registers
@@ -234,7 +242,8 @@ __global__ void __launch_bounds__(256, D > 160 ? 1 : 2) ragged_narrow_kernel(con
       for (int hg = 0; hg < 4; ++hg)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool in = ((bits >> (4 * g + r)) & 1u) != 0u && static_cast<uint32_t>(e0 + r - row_lo[hg]) < static_cast<uint32_t>(row_span[hg]);
+          const bool in = ((bits >> (4 * g + r)) & 1u) != 0u &&
+                          (static_cast<uint32_t>(e0 + r - row_lo[hg]) < static_cast<uint32_t>(row_span[hg]) || (FIRST && e0 + r < row_head[hg]));
           v[hg][r] = in ? v[hg][r] : -__builtin_huge_valf();
         }
     }

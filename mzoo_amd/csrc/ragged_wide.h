@@ -86,7 +86,7 @@ struct WideRaw {
   u32x4 s;  // the entry's four block scales
 };
 
-template <int FMT, int D, int NOPE, int RG>
+template <int FMT, int D, int NOPE, int RG, bool FIRST>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 ragged_wide_kernel(const RaggedParams p) {
   using M = WideLds<FMT, D>;
@@ -137,7 +137,7 @@ ragged_wide_kernel(const RaggedParams p) {
   const int tok0 = p.by_heads(u.r0), tok1 = p.by_heads(u.r1 - 1) + 1;
   const int shift = u.len - u.n;
   int share_lo, share_hi;
-  unit_range(p, u, tok0, tok1, share_lo, share_hi);
+  unit_range<FIRST>(p, u, tok0, tok1, share_lo, share_hi);
   int tok_b[SB];  // the tokens of this lane's rows
 #pragma unroll
   for (int b = 0; b < SB; ++b) {
@@ -197,15 +197,18 @@ ragged_wide_kernel(const RaggedParams p) {
   v4f s_acc[SB];
   WideRaw raw[2];
 
-  int lo = 0, hi = 0;       // the pass's entries: positions lo .. hi - 1
+  int lo = 0, hi = 0;       // the pass's entries: places lo .. hi - 1
+  int body = 0, jump = 0;   // with first positions: those from `body` on are positions, the others `jump` from theirs
+  auto position = [&](int v) __attribute__((always_inline)) -> int { return FIRST && v < body ? v + jump : v; };
   int c0 = 0, nt = 0;       // the chunk at hand: its first entry (from lo), its tiles
   int row_lo[SB], row_span[SB];  // of this lane's rows, entries seen, from lo
+  int row_head[SB];              // and, with first positions, all before here
   int full_lo = 0, full_hi = 0;  // tiles (from lo) of which every row sees every entry
   // the entry that a lane fetches for tile t of the chunk: past the end of the range its last one
   auto code_of = [&](int t) __attribute__((always_inline)) -> uint32_t {
     if (paged) return tab[t * kTile + te];
     const int v = c0 + t * kTile + te;
-    return static_cast<uint32_t>(lo + (v < hi - lo ? v : hi - lo - 1));
+    return static_cast<uint32_t>(position(lo + (v < hi - lo ? v : hi - lo - 1)));
   };
   auto direct = [&](gptr_t e, uint32_t buf) __attribute__((always_inline)) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + buf);
@@ -246,7 +249,7 @@ ragged_wide_kernel(const RaggedParams p) {
       const int e = e0 + tid;
       uint32_t code = kEmpty;
       if (e < nt * kTile && e < left) {
-        code = static_cast<uint32_t>(pool_entry(p, u, lo + c0 + e));  // -1: kEmpty
+        code = static_cast<uint32_t>(pool_entry(p, u, position(lo + c0 + e)));  // -1: kEmpty
       }
       const uint64_t bal = __ballot(code != kEmpty);
       if (e < n_tab) {
@@ -277,7 +280,7 @@ ragged_wide_kernel(const RaggedParams p) {
   // entry r (of 4) of this lane in tile t, for row group b
   auto sees = [&](int t, uint32_t bits, int b, int r) __attribute__((always_inline)) -> bool {
     const int v = c0 + t * kTile + 16 * eh + 4 * g + r;
-    return ((bits >> (16 * eh + 4 * g + r)) & 1u) != 0u && static_cast<uint32_t>(v - row_lo[b]) < static_cast<uint32_t>(row_span[b]);
+    return ((bits >> (16 * eh + 4 * g + r)) & 1u) != 0u && (static_cast<uint32_t>(v - row_lo[b]) < static_cast<uint32_t>(row_span[b]) || (FIRST && v < row_head[b]));
   };
   auto scores = [&](int t, float (&v)[SB][4]) __attribute__((always_inline)) {
     const uint32_t bits = paged ? masks[t] : 0xffffffffu;
@@ -558,13 +561,15 @@ ragged_wide_kernel(const RaggedParams p) {
   // the entries that tokens sub0 .. sub1 - 1 see of this unit's share, and what the rows see of them
   int sub0 = tok0, sub1 = tok1;
   auto set_range = [&]() __attribute__((always_inline)) {
-    token_range(p, u, sub0, sub1, lo, hi);
-    lo = lo > share_lo ? lo : share_lo;
-    hi = hi < share_hi ? hi : share_hi;
-    if (hi < lo) hi = lo;
+    const Pass w = pass_range<FIRST>(p, u, tok0, sub0, sub1, share_lo, share_hi);
+    lo = w.lo;
+    hi = w.hi;
+    body = w.body;
+    jump = w.jump;
     int most_lo = lo, least_hi = hi;
     if (!p.idx) {
       most_lo = clamp32(shift + sub1 - p.window, lo, 0x7fffffff - kTile);
+      if (FIRST && most_lo <= body) most_lo = lo;
       least_hi = shift + sub0 + 1 < hi ? shift + sub0 + 1 : hi;
     }
     full_lo = (most_lo - lo + kTile - 1) / kTile;
@@ -576,6 +581,10 @@ ragged_wide_kernel(const RaggedParams p) {
         const int pos = shift + tok_b[b];
         if (pos - p.window + 1 > a) a = pos - p.window + 1;
         if (pos + 1 < z) z = pos + 1;
+      }
+      if (FIRST) {
+        const int end = body > p.first ? body : p.first, past = shift + tok_b[b] + 1;
+        row_head[b] = (end < past ? (end < hi ? end : hi) : past < hi ? past : hi) - lo;
       }
       row_lo[b] = a - lo;
       row_span[b] = z > a ? z - a : 0;

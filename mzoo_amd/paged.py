@@ -133,28 +133,28 @@ def append(pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, x: torc
 
 @functools.lru_cache(maxsize=1024)
 def attend_workspace_bytes(tokens: int, heads: int, dim: int, batch: int, packed: bool, max_pages: int | None = None, page: int = 1,
-                           window: int = 0, k: int = -1) -> int:
+                           window: int = 0, k: int = -1, first: int = 0) -> int:
     """What ``attend`` splits long sequences into: the partial results.  Without ``max_pages`` enough for any
     tables, windows and lists; with it what a call takes whose tables have so many columns (``window`` 0: none;
-    ``k``: the positions of its lists, -1: none), 0 where no sequence is split."""
+    ``k``: the positions of its lists, -1: none; ``first``: its first positions), 0 where no sequence is split."""
     n = ctypes.c_int64(0)
     if max_pages is None:
         _lib.call("mzk_paged_attend_workspace_bytes", tokens, heads, dim, int(packed), batch, ctypes.byref(n))
     else:
-        _lib.call("mzk_paged_attend_call_workspace_bytes", tokens, heads, dim, int(packed), batch, max_pages, page, window, k,
-                  ctypes.byref(n))
+        _lib.call("mzk_paged_attend_first_workspace_bytes", tokens, heads, dim, int(packed), batch, max_pages, page, window,
+                  first, k, ctypes.byref(n))
     return n.value
 
 
 def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, *,
-           cu: torch.Tensor | None = None, window: int | None = None, indices: torch.Tensor | None = None,
+           cu: torch.Tensor | None = None, window: int | None = None, first: int = 0, indices: torch.Tensor | None = None,
            sinks: torch.Tensor | None = None, rope: int = quant.ENTRY_ROPE, workspace: torch.Tensor | None = None,
            out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
     """Attention of the newest tokens over their sequences' pages (their own entries appended).
 
     q bf16 [T, H, D]: one token per sequence, or with ``cu`` the last ``cu[b + 1] - cu[b]`` of each (drafted
     tokens, a chunk of a prompt), each at its own position and causal.  A token sees its sequence up
-    to itself, the last ``window`` positions of that, or -- one token per sequence -- the positions
+    to itself, the last ``window`` positions of that and beside them the ``first`` of the sequence, or -- one token per sequence -- the positions
     ``indices`` int32 [B, k] lists (outside the sequence: empty; k 0: none).  Positions on no page or
     past the table are empty.  ``sinks`` fp32 [H].  Returns (o bf16 [T, H, D], lse fp32 [T, H]); rows behind
     the last sequence are 0 (-inf), or as they were in a given ``out`` and ``lse``.  A token that sees
@@ -179,6 +179,8 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
         _refuse("attend", "sinks", sinks, torch.float32, (h,))
     if window is not None and (not isinstance(window, int) or window < 1):
         raise ValueError(f"attend: window must be a positive int or None, got {window!r}")
+    if not isinstance(first, int) or not 0 <= first < 1 << 30 or first and window is None:
+        raise ValueError(f"attend: first must be an int of at least 0, below 2^30, and goes with a window, got {first!r}")
     k = istride = idx = 0
     if indices is not None:
         if cu is not None or window is not None:
@@ -200,14 +202,14 @@ def attend(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, lens: torc
         out = torch.empty_like(q)
         lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
     wide = min(window or 0, (1 << 63) - 1)
-    need = attend_workspace_bytes(t, h, d, b, cu is not None, width, page, wide, k if idx else -1)
+    need = attend_workspace_bytes(t, h, d, b, cu is not None, width, page, wide, k if idx else -1, first)
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
             raise ValueError(f"attend: the workspace must be contiguous uint8 of at least {need} bytes")
-    _call(q.device, "mzk_paged_attend", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
-          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, wide, _lib.ptr(sinks),
+    _call(q.device, "mzk_paged_attend_first", q.data_ptr(), t, h, d, _lib.ptr(cu), b, fmt, nope, pool.data_ptr(), pages, page,
+          tables.data_ptr(), stride, width, lens.data_ptr(), idx, istride, k, wide, first, _lib.ptr(sinks),
           _lib.ptr(workspace) if need else None, need, out.data_ptr(), lse.data_ptr(), 0 if given else 1)
     return out, lse
 
