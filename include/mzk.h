@@ -691,6 +691,47 @@ int mzk_packed_mqa_first(const void* q, int64_t T, int H, int D, const int64_t* 
                          int64_t kv_row_stride, int G, int64_t window, int64_t first, const float* sinks, void* out,
                          float* lse, int zero_tail, void* stream);
 
+/* ---- from logits to the next tokens -------------------------------------------------------
+ * A row's tokens stand in the order of falling logits, equal ones by rising index, with weights w =
+ * exp((l - max l) / T).  top-k keeps the first k of them (<= 0: all), top-p the shortest prefix of those whose
+ * weights reach p of their sum (>= 1: all, at least the first), min-p those of at least min_p times the first
+ * one's weight (<= 0: all).  temperature <= 0: the first alone.  NaN and -inf are no tokens; +inf counts as
+ * the largest finite number.
+ *   logits [rows, row_stride elements] fp32, bf16 or fp16, V of a row (at most 2^20), rows at any alignment.
+ *   temperature, top_k, top_p, min_p: device arrays of one value for each row, or NULL: the value behind, for all.
+ *   workspace: of the call's _workspace_bytes (16-byte aligned, no initialization); calls that overlap
+ *   need their own. */
+
+/* tokens[r]: the first of the kept ones whose running sum of weights exceeds u[r] (in [0, 1)) times their
+ * sum; logprobs[r] the logarithm of its share of that.  A row without a token: -1, -inf. */
+int mzk_sample_workspace_bytes(int64_t rows, int64_t V, int dtype, int64_t* bytes);
+int mzk_sample(const void* logits, int dtype, int64_t rows, int64_t V, int64_t row_stride, const float* u,
+               const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p,
+               float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, float* logprobs, void* workspace,
+               int64_t workspace_bytes, void* stream);
+
+/* Drafted tokens against the target's logits.  Rows cu[b] .. cu[b + 1] - 1 (int64 [B + 1], ascending from 0, not
+ * checked) are sequence b's: row i holds the logits behind tokens[i], so the drafted token tokens[i + 1] of the same
+ * sequence is judged by row i.  With p its probability behind the filters and q the draft's (draft_probs[i,
+ * tokens[i + 1]], rows draft_row_stride elements apart; NULL: 1) it is accepted if u[i] q < p.  accepted[b]: the
+ * tokens before the first refused one.  next[b]: drawn with draw[b] from the last row, or from the refused
+ * token's row: without draft_probs as mzk_sample does, without that token; with them from max(p - q, 0) by rising index
+ * (from p where that is nothing).  A sequence of no rows: 0 and -1. */
+int mzk_verify_workspace_bytes(int64_t T, int64_t B, int64_t V, int dtype, int probs, int64_t* bytes);
+int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, int64_t row_stride, const int64_t* tokens,
+               const int64_t* cu, int64_t B, const float* u, const float* draw, const float* draft_probs,
+               int64_t draft_row_stride, const float* temperature, float temperature_all, const int32_t* top_k,
+               int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* accepted,
+               int64_t* next, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A step of a beam search: of each group of `width` rows the `keep` best continuations by scores[row] + logit -
+ * log sum exp, best first, equal ones by row and token (width * keep at most 4096).  parents: their rows, tokens,
+ * out_scores; -1, -1 and -inf where a group has fewer.  A row whose score is -inf or NaN has none. */
+int mzk_beams_workspace_bytes(int64_t rows, int64_t V, int dtype, int keep, int64_t* bytes);
+int mzk_beams(const void* logits, int dtype, int64_t rows, int64_t V, int64_t row_stride, const float* scores, int width,
+              int keep, int32_t* parents, int64_t* tokens, float* out_scores, void* workspace, int64_t workspace_bytes,
+              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -103,6 +103,13 @@ _SIGS = {
     "mzk_paged_attend_first_workspace_bytes": [_I64, _I32, _I32, _I32, _I64, _I64, _I32, _I64, _I64, _I32,
                                                ctypes.POINTER(_I64)],
     "mzk_packed_mqa_first": [_P, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _I32, _P],
+    "mzk_sample_workspace_bytes": [_I64, _I64, _I32, ctypes.POINTER(_I64)],
+    "mzk_sample": [_P, _I32, _I64, _I64, _I64, _P, _P, _F32, _P, _I32, _P, _F32, _P, _F32, _P, _P, _P, _I64, _P],
+    "mzk_verify_workspace_bytes": [_I64, _I64, _I64, _I32, _I32, ctypes.POINTER(_I64)],
+    "mzk_verify": [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _F32, _P, _I32, _P, _F32, _P, _F32, _P,
+                   _P, _P, _I64, _P],
+    "mzk_beams_workspace_bytes": [_I64, _I64, _I32, _I32, ctypes.POINTER(_I64)],
+    "mzk_beams": [_P, _I32, _I64, _I64, _I64, _P, _I32, _I32, _P, _P, _P, _P, _I64, _P],
     "mzk_packed_mqa": [_P, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32, _I64, _P, _P, _P, _I32, _P],
     "mzk_indexer_decode_fused": [_I32, _P, _P, _P, _P, _I64, _I32, _I32, _I64, _I64, _P, _I32, _P, _I64, _P, _P, _P,
                                  _P, _I32, _P, _P, _F32, _P, _P, _I32, _I32, _P, _I64, _I32, _P],
