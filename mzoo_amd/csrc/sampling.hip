@@ -11,47 +11,38 @@
 // Tokens are whole numbers, so a token beside a border of the running sum has to come out right: weights
 // are computed in 64 bits to about 2^-50 of themselves, and summed as whole numbers, in any order the same.
 //
-// No row is sorted.  Three launches, none of which needs another's workgroups at the same time:
-//   survey   chunks of a row: the chunk's maximum and a histogram of its weights over bins of 1/10 octave,
-//            51 octaves down; what lies below them is 2^-50 of the largest weight and counts as 0
-//   narrow   every chunk's workgroup joins the row's histograms, finds the few bins in which the cuts of
-//            the filters and the drawn token lie, and lists its tokens of these bins
-//   finish   a workgroup for each row finds the exact cuts and the token among the listed ones, by
-//            weighted radix selection: a histogram over the bits that the open range of keys has left
+// No row is sorted, and none is looked at twice in full arithmetic.  A row's workgroup has a histogram of its weights
+// over bins of 1/10 octave, from the largest down (survey: of its own, or joined from those of chunks where there are
+// too few rows for the compute units); finds the few bins in which the cuts of the filters and the token lie; lists
+// the row's tokens of these bins; and selects among those, bin by bin.
 #include "common.h"
 
 namespace mzk {
 namespace {
 
-constexpr int kBins = 512, kRest = kBins - 1;  // the last bin takes what is too small to count
+constexpr int kBins = 512, kRest = kBins - 1;  // bins of a histogram; the last takes what is too small to count, 2^-51
 constexpr double kPerOctave = 10.0;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
-constexpr int kCap = 16384;  // listed tokens of a row; where there are more, finish reads the row itself
+constexpr double kBelow = 1.0 - 0x1p-30, kAbove = 1.0 + 0x1p-30;  // slack of bounds
+constexpr int kCap = 16384;  // listed tokens of a row
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr uint32_t kNone = 0xffffffffu;
+constexpr int kNoTop = -0x7fffffff;
 
 enum Mode { kSample, kVerify, kBeams };
 
-// Bins b0 .. b1 in which something has to be found (none: b1 < b0), and the weights of the bins before them.
-struct Window {
-  int b0, b1;
-  double before;
+// What a survey finds besides its bins.
+struct Surveyed {
+  int top;    // the largest bin; kNoTop: no token
+  float max;  // the largest logit
 };
 
-// What narrow leaves of a row for finish.
-struct Plan {
-  double total;       // all weights
-  Window k, p, f, d;  // top-k's cut, top-p's, min-p's, the drawn token
-  uint32_t count_before;  // tokens in the bins before k.b0
-  float max;
-};
-
-// What finish leaves of a row for the launches behind it.
+// What a row leaves for the launches behind it.
 struct Row {
-  double kept;             // W
-  uint32_t ik, idx;        // the last token of the order that top-k and top-p keep: its key and index
-  float max;
-  int32_t accepted, token;
+  double kept;    // W, in units of 2^-scale
+  uint64_t cut;   // key and index of the last token that top-k and top-p keep
+  float max, origin;
+  int32_t top, accepted, token;
 };
 
 struct Filter {
@@ -63,13 +54,13 @@ struct Filter {
 struct SamplingParams {
   const uint8_t* logits;
   int64_t stride;  // bytes from row to row
-  int V, rows, chunks;
+  int V, rows;
+  int chunks, chunk_pieces;  // of a row's survey; 1: the row's workgroup surveys it
+  int scale;                 // log2 of the whole number that stands for the weight at the largest bin: V of them stay below 2^63
   Mode mode;
   Filter temperature, top_p, min_p;
   const int32_t* top_k;
   int top_k_all;
-  int count;  // whether tokens are counted: some row may have a top-k
-  int scale;  // log2 of the whole number that stands for the largest weight: V of them stay below 2^63
   const float* u;  // [rows]
   // verify
   const int64_t* tokens;  // [rows]
@@ -78,19 +69,17 @@ struct SamplingParams {
   const float* draw;   // [B]
   const float* probs;  // [rows, V] or null
   int64_t probs_stride;
+  int rest_chunks;
   // beams
   const float* scores;  // [rows]
   int width, keep;
   // workspace
-  float* heads;      // [rows][chunks] maxima
-  uint64_t* hist;    // [rows][chunks][kBins] weights, 2^50 the chunk's largest
+  Surveyed* heads;   // [rows][chunks]
+  uint64_t* hist;    // [rows][chunks][kBins] from the largest down
   uint32_t* counts;  // the same, tokens
-  Plan* plans;       // [rows]
-  uint32_t* listed;  // [rows]
-  uint2* list;       // [rows][kCap] key and index
   Row* rowres;       // [rows]
   int32_t* refused;  // [B] the row of a refused token, or -1
-  uint64_t* rest;    // [B][chunks] sums of what the target has above the draft
+  uint64_t* rest;    // [B][rest_chunks] sums of what the target has above the draft
   uint2* best;       // [rows][keep]
   uint32_t* nbest;   // [rows]
   // results
@@ -103,9 +92,9 @@ struct SamplingParams {
 
 // ---- numbers --------------------------------------------------------------------------------
 
-// 2^t for t <= 0, to about 2^-51 of itself: the power series of exp(f ln 2) for |f| <= 1/2, whose
+// 2^t for t <= 1, to about 2^-51 of itself: the power series of exp(f ln 2) for |f| <= 1/2, whose
 // first term left out is (ln 2 / 2)^13 / 13! = 1.7e-16.
-__device__ __forceinline__ double exp2_neg(double t) {
+__device__ __forceinline__ double exp2_of(double t) {
   t = fmax(t, -1100.0);
   const double n = __builtin_rint(t);
   const double x = (t - n) * kLn2D;
@@ -125,18 +114,30 @@ __device__ __forceinline__ double exp2_neg(double t) {
   return __builtin_ldexp(e, static_cast<int>(n));
 }
 
-// A number of 0 .. 2^51 to the nearest whole one: the low bits of its sum with 2^52.
-__device__ __forceinline__ uint64_t whole(double x) {
-  return static_cast<uint64_t>(__double_as_longlong(x + 4503599627370496.0)) & 0xfffffffffffffull;
+// 2^43 2^(r / 10) as a whole number for |r| <= 1/2: seven terms of the power series, the first left out
+// (ln 2 / 20)^8 / 8! = 5e-17; the last sum is with 2^52 more, which rounds it and leaves it in the low bits.
+constexpr int kWhole = 43;
+__device__ __forceinline__ uint64_t whole_exp2(double r) {
+  constexpr double c = kLn2D / kPerOctave, one = 8796093022208.0;
+  double e = one * c * c * c * c * c * c * c / 5040.0;
+  e = __builtin_fma(e, r, one * c * c * c * c * c * c / 720.0);
+  e = __builtin_fma(e, r, one * c * c * c * c * c / 120.0);
+  e = __builtin_fma(e, r, one * c * c * c * c / 24.0);
+  e = __builtin_fma(e, r, one * c * c * c / 6.0);
+  e = __builtin_fma(e, r, one * c * c / 2.0);
+  e = __builtin_fma(e, r, one * c);
+  e = __builtin_fma(e, r, one + 4503599627370496.0);
+  return static_cast<uint64_t>(__double_as_longlong(e)) & 0xfffffffffffffull;
 }
 
 // A random number as one of [0, 1): NaN as 0.
 __device__ __forceinline__ double unit(float u) { return u > 0.0f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0; }
 
+constexpr float kBig = 3.402823466e38f;
 // A logit as it counts: NaN as -inf, +inf as the largest finite number, -0 as 0.
 __device__ __forceinline__ float logit_of(float x) {
   x = x != x ? -__builtin_huge_valf() : x + 0.0f;
-  return x > 3.402823466e38f ? 3.402823466e38f : x;
+  return x > kBig ? kBig : x;
 }
 // Keys rise as logits fall.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -148,66 +149,71 @@ __device__ __forceinline__ float logit_of_key(uint32_t ik) { return __uint_as_fl
 // ---- a row's settings -------------------------------------------------------------------------
 
 struct Settings {
-  double s, s_bin;  // log2 e / T, and bins
-  int k;            // 0: none
-  double p;         // 1: none
-  double f;         // log2 min_p; -inf: none
-  bool first;       // T <= 0: the first of the order
+  double s;    // 10 log2 e / T: bins of a logit
+  int k;       // 0: none
+  double p;    // 1: none
+  double f;    // 10 log2 min_p; -inf: none
+  bool first;  // T <= 0: the first of the order
 };
 __device__ __forceinline__ Settings settings(const SamplingParams& q, int row) {
   Settings z;
-  const float t = q.mode == kBeams ? 1.0f : q.temperature(row);
+  const bool beams = q.mode == kBeams;
+  const float t = beams ? 1.0f : q.temperature(row);
   z.first = !(t > 0.0f);
-  z.s = kLog2eD / (z.first ? 1.0 : static_cast<double>(t));
-  z.s_bin = z.s * kPerOctave;
-  z.k = q.mode == kBeams ? q.keep : q.top_k ? q.top_k[row] : q.top_k_all;
-  if (q.mode != kBeams && (z.k < 0 || z.k >= q.V)) z.k = 0;
-  const float p = q.mode == kBeams ? 1.0f : q.top_p(row);
+  z.s = kPerOctave * kLog2eD / (z.first ? 1.0 : static_cast<double>(t));
+  z.k = beams ? q.keep : q.top_k ? q.top_k[row] : q.top_k_all;
+  if (!beams && (z.k < 0 || z.k >= q.V)) z.k = 0;
+  const float p = beams ? 1.0f : q.top_p(row);
   z.p = z.first ? 0.0 : p < 1.0f ? (p > 0.0f ? static_cast<double>(p) : 0.0) : 1.0;
-  const float f = q.mode == kBeams ? 0.0f : q.min_p(row);
-  z.f = f > 0.0f ? (f < 1.0f ? log2(static_cast<double>(f)) : 0.0) : -__builtin_huge_val();
+  const float f = beams ? 0.0f : q.min_p(row);
+  z.f = f > 0.0f ? (f < 1.0f ? kPerOctave * log2(static_cast<double>(f)) : 0.0) : -__builtin_huge_val();
   if (z.first) z.k = 0, z.f = -__builtin_huge_val();
   return z;
 }
 
-// The bin below a maximum whose place on the grid is `top`; kRest for what is too small.
-__device__ __forceinline__ int bin_of(float l, double s_bin, double top) {
-  return static_cast<int>(fmin(top - __builtin_floor(static_cast<double>(l) * s_bin), static_cast<double>(kRest)));
-}
-
 // ---- loads ------------------------------------------------------------------------------------
 
-// A chunk: 256 threads, EPT elements each, in whole 16-byte pieces of memory as far as they lie inside the row.
-template <int DT, int EPT>
-struct Chunk {
-  static constexpr int SIZE = DT == MZK_F32 ? 4 : 2, N = 16 / SIZE, PIECES = EPT / N;
-  // elements of a row before the first whole piece are counted from the piece that they lie in
-  __device__ static int mis(const uint8_t* row) { return static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / SIZE); }
-  __device__ static float value(const uint8_t* row, int i) { return logit_of(load_as_f32<DT>(row, i)); }
-  // the index of element i (of EPT) of this thread
-  __device__ static int index(int chunk, int tid, int i, int mis) { return (chunk * 256 * PIECES + (i / N) * 256 + tid) * N + i % N - mis; }
-  __device__ static void load(const uint8_t* row, int V, int chunk, int tid, int mis, float (&v)[EPT]) {
+// A row in pieces of 16 bytes of memory, the first and the last of which may lie partly outside it.
+template <int DT>
+struct Pieces {
+  static constexpr int SIZE = DT == MZK_F32 ? 4 : 2, N = 16 / SIZE;
+  const uint8_t* row;
+  int V, mis;  // elements of the first piece before the row
+  __device__ Pieces(const uint8_t* r, int v) : row(r), V(v), mis(static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15u) / SIZE)) {}
+  __device__ int count() const { return (V + mis + N - 1) / N; }
+  __device__ int first(int piece) const { return piece * N - mis; }  // index of its first element
+  __device__ uint32_t raw(int i) const {
+    if constexpr (DT == MZK_F32) return reinterpret_cast<const uint32_t*>(row)[i];
+    else return reinterpret_cast<const uint16_t*>(row)[i];
+  }
+  __device__ static float value(uint32_t bits) {
+    return DT == MZK_F32 ? __uint_as_float(bits) : DT == MZK_BF16 ? bf16_to_f32(static_cast<uint16_t>(bits)) : f16_to_f32(static_cast<uint16_t>(bits));
+  }
+  __device__ float operator[](int i) const { return logit_of(value(raw(i))); }
+  __device__ uint4 load(int piece) const {  // (what lies outside the row is -inf)
+    constexpr uint32_t none = DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80u : 0xfc00u;
+    const int e = first(piece);
+    if (e >= 0 && e + N <= V) return *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(e) * SIZE);
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int e = index(chunk, tid, k * N, mis);
-      if (e >= 0 && e + N <= V) {
-        const uint4 x = *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(e) * SIZE);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (DT == MZK_F32) {
-            v[k * N + j] = logit_of(__uint_as_float(w[j]));
-          } else {
-            const uint16_t h[2] = {static_cast<uint16_t>(w[j] & 0xffffu), static_cast<uint16_t>(w[j] >> 16)};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) v[k * N + 2 * j + i] = logit_of(DT == MZK_BF16 ? bf16_to_f32(h[i]) : f16_to_f32(h[i]));
-          }
-        }
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == MZK_F32) {
+        w[j] = e + j >= 0 && e + j < V ? raw(e + j) : none;
       } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[k * N + j] = e + j >= 0 && e + j < V ? value(row, e + j) : -__builtin_huge_valf();
+        const int i = e + 2 * j;
+        w[j] = (i >= 0 && i < V ? raw(i) : none) | (i + 1 >= 0 && i + 1 < V ? raw(i + 1) : none) << 16;
       }
     }
+    return uint4{w[0], w[1], w[2], w[3]};
+  }
+  __device__ static uint4 none() {
+    constexpr uint32_t w = DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    return uint4{w, w, w, w};
+  }
+  // element j (of N) of a loaded piece, not yet as it counts
+  __device__ static float at(const uint4& x, int j) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    return DT == MZK_F32 ? value(w[j]) : value(w[j / 2] >> (16 * (j & 1)) & 0xffffu);
   }
 };
 
@@ -244,581 +250,616 @@ __device__ __forceinline__ T wave_scan(T v, int lane) {
 
 // ---- survey -------------------------------------------------------------------------------------
 
-template <int DT, int EPT>
+// Where a logit lies: t = (l - origin) s, in bins; its bin is the nearest whole number k, and its weight 2^(k / 10)
+// times 2^((t - k) / 10).  A bin sums the second factors, as whole numbers of 2^43; the first is its own.
+struct Grid {
+  float origin;
+  double s;
+  __device__ double place(float l) const { return (static_cast<double>(l) - static_cast<double>(origin)) * s; }
+};
+
+// The origin: the largest of the row's first 1024 logits, the same for all its chunks.  With equal logits all weights
+// are whole powers of two, and sums of them exact.
+template <int DT, int NT>
+__device__ __forceinline__ float origin_of(const Pieces<DT>& x, int tid, float* lds) {
+  float m = -__builtin_huge_valf();
+  for (int i = tid; i < 1024 && i < x.V; i += NT) m = fmaxf(m, x[i]);
+  m = wave_max(m);
+  if ((tid & 63) == 0) lds[tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, lds[w]);
+  __syncthreads();
+  return m > -__builtin_huge_valf() ? m : 0.0f;
+}
+
+constexpr int kFar = 1 << 28;  // bins from the origin that are told apart
+
+// The bin of a maximum.
+__device__ __forceinline__ int top_of(const Grid& g, float m) {
+  return static_cast<int>(__builtin_rint(fmin(fmax(g.place(fminf(m, kBig)), -static_cast<double>(kFar)), static_cast<double>(kFar))));
+}
+
+// Pieces from .. to - 1 of a row into the histogram (and, counting, the numbers of tokens): bin k in place k mod
+// kBins, for the kBins - 1 bins from the largest on.  As that rises, places of bins that fall behind become its.
+// Bound by the 64-bit arithmetic, 13 instructions of a quarter of the rate an element, and the LDS's atomic sums, in two
+// copies by the lane's parity, so that fewer lanes meet; the next pieces are in flight meanwhile.
+template <int DT, int NT>
+__device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, bool counting, int from, int to, int tid,
+                                           unsigned long long* hist /* [2][kBins] */, uint32_t* counts /* [kBins] */, int* tops /* [2] */,
+                                           float* lds /* [NT / 64] */) {
+  using P = Pieces<DT>;
+  constexpr int PER = 16 / P::N;  // pieces of a thread at a time: 16 elements
+  for (int i = tid; i < 2 * kBins; i += NT) hist[i] = 0;
+  if (counting)
+    for (int i = tid; i < kBins; i += NT) counts[i] = 0;
+  if (tid < 2) tops[tid] = kNoTop;
+  uint4 next[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) next[i] = from + i * NT + tid < to ? x.load(from + i * NT + tid) : P::none();
+  float max_all = -__builtin_huge_valf();
+  int top = kNoTop, turn = 0;
+  unsigned long long* const mine = hist + (tid & 1) * kBins;
+  __syncthreads();
+  for (int at = from; at < to; at += PER * NT) {
+    float v[16];
+    float m = -__builtin_huge_valf();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[i] = P::at(next[i / P::N], i % P::N);
+      m = fmaxf(m, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int piece = at + (PER + i) * NT + tid;
+      if (at + PER * NT < to) next[i] = piece < to ? x.load(piece) : P::none();
+    }
+    m = wave_max(m);
+    max_all = fmaxf(max_all, m);
+    if ((tid & 63) == 0 && m > -__builtin_huge_valf())
+      atomicMax(&tops[turn], top_of(g, m));
+    __syncthreads();
+    const int now = max(top, tops[turn]);
+    turn ^= 1;
+    if (now > top) {  // uniform
+      if (top > kNoTop) {
+        const int n = now - top < kBins ? now - top : kBins;
+        for (int i = tid; i < n; i += NT) {
+          const int j = (now - i) & kRest;
+          hist[j] = hist[kBins + j] = 0;
+          if (counting) counts[j] = 0;
+        }
+        __syncthreads();
+      }
+      top = now;
+    }
+    const double bottom = static_cast<double>(top - kRest);  // bins above it are kept
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const double t = g.place(fminf(v[i], kBig));
+      const double n = __builtin_rint(t);
+      if (n > bottom && v[i] > -__builtin_huge_valf()) {  // (not a NaN)
+        const int k = static_cast<int>(fmin(n, static_cast<double>(kFar))) & kRest;
+        atomicAdd(&mine[k], static_cast<unsigned long long>(whole_exp2(t - n)));
+        if (counting) atomicAdd(&counts[k], 1u);
+      }
+    }
+  }
+  if ((tid & 63) == 0) lds[tid >> 6] = max_all;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) max_all = fmaxf(max_all, lds[w]);
+  return Surveyed{top, logit_of(max_all)};
+}
+
+template <int DT>
 __global__ void __launch_bounds__(256) survey_kernel(const SamplingParams q) {
-  using C = Chunk<DT, EPT>;
-  __shared__ unsigned long long hist[kBins];
+  __shared__ unsigned long long hist[2 * kBins];
   __shared__ uint32_t counts[kBins];
-  __shared__ float top[4];
+  __shared__ float lds[4];
+  __shared__ int tops[2];
   const int tid = threadIdx.x;
   const int row = blockIdx.x / q.chunks, chunk = blockIdx.x - row * q.chunks;
   if (q.mode == kVerify && q.cu[q.B] <= row) return;  // a row of no sequence
-  const uint8_t* const base = q.logits + row * q.stride;
-  float v[EPT];
-  C::load(base, q.V, chunk, tid, C::mis(base), v);
+  const Pieces<DT> x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
-  for (int i = tid; i < kBins; i += 256) {
-    hist[i] = 0;
-    counts[i] = 0;
-  }
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < EPT; ++i) m = fmaxf(m, v[i]);
-  m = wave_max(m);
-  if ((tid & 63) == 0) top[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  const bool counting = z.k > 0;
+  const Grid g{origin_of<DT, 256>(x, tid, lds), z.s};
+  const int from = chunk * q.chunk_pieces, all = x.count(), to = from + q.chunk_pieces < all ? from + q.chunk_pieces : all;
+  const Surveyed r = survey<DT, 256>(x, g, counting, from, to, tid, hist, counts, tops, lds);
   const int64_t at = static_cast<int64_t>(row) * q.chunks + chunk;
-  if (tid == 0) {
-    q.heads[at] = m;
-    if (chunk == 0) q.listed[row] = 0;
-  }
-  if (m == -__builtin_huge_valf()) return;  // uniform
-  const double grid = __builtin_floor(static_cast<double>(m) * z.s_bin);
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int j = bin_of(v[i], z.s_bin, grid);
-    if (j < kRest) {
-      const double t = (static_cast<double>(v[i]) - static_cast<double>(m)) * z.s;
-      atomicAdd(&hist[j], static_cast<unsigned long long>(whole(exp2_neg(t) * 0x1p50)));
-      if (q.count) atomicAdd(&counts[j], 1u);
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < kBins; i += 256) {
-    q.hist[at * kBins + i] = hist[i];
-    if (q.count) q.counts[at * kBins + i] = counts[i];
+  if (tid == 0) q.heads[at] = r;
+  if (r.top == kNoTop) return;  // uniform
+  for (int j = tid; j < kBins; j += 256) {
+    const int i = (r.top - j) & kRest;
+    q.hist[at * kBins + j] = j < kRest ? hist[i] + hist[kBins + i] : 0;
+    if (counting) q.counts[at * kBins + j] = j < kRest ? counts[i] : 0;
   }
 }
 
-// ---- narrow -------------------------------------------------------------------------------------
+// ---- a row --------------------------------------------------------------------------------------
 
-template <int DT, int EPT>
-__global__ void __launch_bounds__(256) narrow_kernel(const SamplingParams q) {
-  using C = Chunk<DT, EPT>;
-  constexpr int kMost = 1024;  // chunks of a row
-  __shared__ float heads[kMost];
-  __shared__ double factor[kMost];
-  __shared__ int shift[kMost];
+constexpr int kRowThreads = 1024;
+
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q) {
+  constexpr int NT = kRowThreads, NW = NT / 64;
+  using P = Pieces<DT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint2* const list = reinterpret_cast<uint2*>(smem);  // [kCap] key; index, and the bin above bit 20
+  __shared__ unsigned long long hist[1024];            // (survey: two copies of the bins)
+  __shared__ uint32_t counts[kBins];
   __shared__ uint64_t cw[kBins];  // running sums of the bins' weights
-  __shared__ uint32_t cn[kBins];
-  __shared__ uint64_t part_w[4];
-  __shared__ uint32_t part_n[4];
-  __shared__ float top[4];
-  __shared__ int found[3][4][4];
-  __shared__ uint32_t base_at;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x / q.chunks, chunk = blockIdx.x - row * q.chunks;
+  __shared__ uint32_t cn[kBins];  // and of their tokens
+  __shared__ uint64_t part[NW], ext[4], sel[4];
+  __shared__ uint32_t partn[NW], number[2];
+  __shared__ int found[2][2][NW];
+  __shared__ float lds[NW];
+  __shared__ int tops[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   int b = 0, end = 0;
   if (q.mode == kVerify && !sequence_of(q, row, lane, b, end)) return;  // uniform
-  const uint8_t* const base = q.logits + row * q.stride;
+  const P x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
+  const bool counting = z.k > 0;
 
-  // the row's maximum, and where the chunks' bins lie among the row's
-  float m = -__builtin_huge_valf();
-  for (int c = tid; c < q.chunks; c += 256) {
-    const float h = q.heads[static_cast<int64_t>(row) * q.chunks + c];
-    heads[c] = h;
-    m = fmaxf(m, h);
-  }
-  m = wave_max(m);
-  if (lane == 0) top[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  Plan plan{};
-  plan.max = m;
-  plan.k = plan.p = plan.f = plan.d = Window{1, 0, 0.0};
-  if (m == -__builtin_huge_valf()) {  // uniform: no token at all
-    if (chunk == 0 && tid == 0) q.plans[row] = plan;
-    return;
-  }
-  const double grid = __builtin_floor(static_cast<double>(m) * z.s_bin);
-  for (int c = tid; c < q.chunks; c += 256) {
-    const float h = heads[c];
-    const bool some = h > -__builtin_huge_valf();
-    shift[c] = some ? bin_of(h, z.s_bin, grid) : kBins;
-    factor[c] = some ? exp2_neg((static_cast<double>(h) - static_cast<double>(m)) * z.s) * 0x1p-50 : 0.0;
-  }
-  __syncthreads();
-  double w0 = 0.0, w1 = 0.0;  // bins 2 tid, 2 tid + 1 of the row
-  uint32_t n0 = 0, n1 = 0;
-  const int64_t at = static_cast<int64_t>(row) * q.chunks;
-  for (int c = 0; c < q.chunks; ++c) {
-    const int j = 2 * tid - shift[c];
-    const double f = factor[c];
-    const uint64_t* const h = q.hist + (at + c) * kBins;
-    if (j >= 0) w0 = w0 + static_cast<double>(h[j]) * f;
-    if (j + 1 >= 0 && j + 1 < kRest && 2 * tid + 1 < kRest) w1 = w1 + static_cast<double>(h[j + 1]) * f;
-    if (q.count) {
-      const uint32_t* const n = q.counts + (at + c) * kBins;
-      if (j >= 0) n0 += n[j];
-      if (j + 1 >= 0 && j + 1 < kRest && 2 * tid + 1 < kRest) n1 += n[j + 1];
-    }
-  }
-  // As whole numbers from here: sums of them do not depend on their order, and a bin of nothing adds nothing.
-  const double scale = __builtin_ldexp(1.0, q.scale), unscale = __builtin_ldexp(1.0, -q.scale);
-  {
-    const uint64_t i0 = static_cast<uint64_t>(w0 * scale + 0.5), i1 = static_cast<uint64_t>(w1 * scale + 0.5);
-    const uint64_t s = wave_scan(i0 + i1, lane);
-    const uint32_t n = wave_scan(n0 + n1, lane);
-    if (lane == 63) part_w[wave] = s, part_n[wave] = n;
-    __syncthreads();
-    uint64_t before = s - (i0 + i1);
-    uint32_t nbefore = n - (n0 + n1);
-    for (int w = 0; w < wave; ++w) before += part_w[w], nbefore += part_n[w];
-    cw[2 * tid] = before + i0;
-    cw[2 * tid + 1] = before + i0 + i1;
-    cn[2 * tid] = nbefore + n0;
-    cn[2 * tid + 1] = nbefore + n0 + n1;
-  }
-  __syncthreads();
-  auto upto = [&](int j) -> double { return static_cast<double>(cw[j]); };  // of `scale`
-  auto before = [&](int j) -> double { return j > 0 ? static_cast<double>(cw[j - 1]) : 0.0; };
-  const double total = upto(kRest);
-  plan.total = total * unscale;
-  // the first bin whose running sum is not below x
-  int round = 0;
-  auto find = [&](auto below_a, auto below_c, int& a, int& c) {
-    const int na = __popcll(__ballot(below_a(2 * tid))) + __popcll(__ballot(below_a(2 * tid + 1)));
-    const int nc = __popcll(__ballot(below_c(2 * tid))) + __popcll(__ballot(below_c(2 * tid + 1)));
-    if (lane == 0) found[round][wave][0] = na, found[round][wave][1] = nc;
-    __syncthreads();
-    a = c = 0;
-    for (int w = 0; w < 4; ++w) a += found[round][w][0], c += found[round][w][1];
-    ++round;
-  };
-  int last, unused;
-  // weights kept: between least and most
-  double k_least = total, k_most = total;
-  if (z.k) {
-    int kb;
-    find([&](int j) { return cn[j] < static_cast<uint32_t>(z.k); }, [&](int j) { return upto(j) < total; }, kb, last);
-    if (kb < kRest) {
-      plan.k = Window{kb, kb, before(kb) * unscale};
-      plan.count_before = kb > 0 ? cn[kb - 1] : 0;
-      k_least = before(kb);
-      k_most = upto(kb);
-    }
-  } else {
-    find([&](int j) { return upto(j) < total; }, [&](int) { return false; }, last, unused);
-  }
-  double least = k_least, most = k_most;
-  if (z.p < 1.0) {
-    int lo, hi;
-    find([&](int j) { return upto(j) < z.p * k_least; }, [&](int j) { return upto(j) < z.p * k_most; }, lo, hi);
-    if (hi > last) hi = last;
-    if (lo > hi) lo = hi;
-    plan.p = Window{lo, hi, before(lo) * unscale};
-    // a token of bin j weighs 2^-((j - 1) / 10) at most
-    const double over = z.p * k_most + exp2_neg(-(lo > 1 ? lo - 1 : 0) / kPerOctave) * scale;
-    least = fmin(least, z.p * k_least);
-    most = fmin(most, fmin(upto(hi), over));
-  }
-  if (z.f > -__builtin_huge_val()) {
-    const double y = (static_cast<double>(m) * z.s + z.f) * kPerOctave, eps = 1e-6 + fabs(y) * 1e-13;
-    const int lo = static_cast<int>(fmin(fmax(grid - __builtin_floor(y + eps), 0.0), static_cast<double>(kRest)));
-    int hi = static_cast<int>(fmin(fmax(grid - __builtin_floor(y - eps), 0.0), static_cast<double>(kRest)));
-    if (lo < kRest) {
-      if (hi >= kRest) hi = kRest - 1;
-      plan.f = Window{lo, hi, before(lo) * unscale};
-      least = fmin(least, before(lo));
-      most = fmin(most, upto(hi));
-    }
-  }
-  if (q.mode == kBeams) {
-    // with fewer tokens than wanted among the bins that count, all of the row's
-    plan.k = Window{0, plan.k.b1 >= plan.k.b0 ? plan.k.b1 : kRest, 0.0};
-    plan.count_before = 0;
-    if (plan.k.b1 == kRest && chunk == 0 && tid == 0) atomicAdd(&q.listed[row], static_cast<uint32_t>(kCap) + 1u);
-  } else {
-    // The drawn token.  In verify a refused token that the draft was sure of leaves the row: with its bin
-    // before the cuts it is kept, behind them not, among them one or the other.
-    const double u = z.first ? 0.0 : unit(q.mode == kVerify ? q.draw[b] : q.u[row]);
-    double wd = 0.0;
-    int bd = kBins;
-    bool sure = true;
-    if (q.mode == kVerify && !q.probs && row + 1 < end) {
-      const int64_t d = q.tokens[row + 1];
-      if (d >= 0 && d < q.V) {
-        const float l = C::value(base, static_cast<int>(d));
-        if (l > -__builtin_huge_valf()) {
-          bd = bin_of(l, z.s_bin, grid);
-          int cut = kRest - 1, open = kBins;  // bins before `open` are kept, behind `cut` are not
-          if (plan.k.b1 >= plan.k.b0) open = plan.k.b0, cut = plan.k.b1;
-          if (plan.p.b1 >= plan.p.b0) open = min(open, plan.p.b0), cut = min(cut, plan.p.b1);
-          if (plan.f.b1 >= plan.f.b0) open = min(open, plan.f.b0), cut = min(cut, plan.f.b1);
-          if (bd <= cut) wd = exp2_neg((static_cast<double>(l) - static_cast<double>(m)) * z.s) * scale;
-          sure = bd < open || bd > cut;
+  // ---- the row's histogram: bin j, from the largest down, is thread j's ----
+  Grid g{origin_of<DT, NT>(x, tid, lds), z.s};
+  uint64_t sum = 0;  // of the second factors
+  uint32_t num = 0;
+  Surveyed r{kNoTop, -__builtin_huge_valf()};
+  for (bool whole_row = q.chunks == 1;; whole_row = true) {
+    if (whole_row) {
+      r = survey<DT, NT>(x, g, counting, 0, x.count(), tid, hist, counts, tops, lds);
+      if (tid < kRest && r.top > kNoTop) {
+        const int i = (r.top - tid) & kRest;
+        sum = hist[i] + hist[kBins + i];
+        num = counting ? counts[i] : 0;
+      }
+    } else {
+      const Surveyed* const heads = q.heads + static_cast<int64_t>(row) * q.chunks;
+      for (int c = 0; c < q.chunks; ++c) {
+        const Surveyed h = heads[c];
+        r.top = max(r.top, h.top);
+        r.max = fmaxf(r.max, h.max);
+      }
+      if (tid < kRest) {
+        const uint64_t* const h = q.hist + static_cast<int64_t>(row) * q.chunks * kBins;
+        const uint32_t* const n = q.counts + static_cast<int64_t>(row) * q.chunks * kBins;
+#pragma unroll 4
+        for (int c = 0; c < q.chunks; ++c) {
+          const int top = heads[c].top;
+          const uint32_t j = static_cast<uint32_t>(tid) - (static_cast<uint32_t>(r.top) - static_cast<uint32_t>(top));
+          if (top > kNoTop && r.top - top <= tid) {
+            sum += h[static_cast<int64_t>(c) * kBins + j];
+            if (counting) num += n[static_cast<int64_t>(c) * kBins + j];
+          }
         }
       }
     }
-    // (the slack covers the roundings of the bins' sums and of wd)
-    const double slack = bd < kBins ? 2048.0 : 0.0;
-    const double lo_x = u * fmax(least - wd, 0.0) - slack, hi_x = u * (sure ? most - wd : most) + slack;
-    int lo, hi;
-    find([&](int j) { return (sure && j >= bd ? upto(j) - wd : upto(j)) <= lo_x; },
-         [&](int j) { return (j >= bd ? upto(j) - wd : upto(j)) <= hi_x; }, lo, hi);
-    if (hi > last) hi = last;
-    if (lo > hi) lo = hi;
-    plan.d = Window{lo, hi, before(lo) * unscale};
-  }
-  if (chunk == 0 && tid == 0) q.plans[row] = plan;
-
-  // this chunk's tokens of the windows
-  const Window win[4] = {plan.k, plan.p, plan.f, plan.d};
-  int hull0 = kBins, hull1 = -1;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (win[i].b1 >= win[i].b0) {
-      hull0 = min(hull0, win[i].b0);
-      hull1 = max(hull1, win[i].b1);
-    }
-  if (shift[chunk] > hull1) return;  // uniform: all of it lies below
-  const int mis = C::mis(base);
-  float v[EPT];
-  C::load(base, q.V, chunk, tid, mis, v);
-  uint32_t mine = 0;
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int j = bin_of(v[i], z.s_bin, grid);
-    if (j < kRest && j >= hull0 && j <= hull1) {
-      bool in = false;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) in = in || (j >= win[w].b0 && j <= win[w].b1);
-      mine |= static_cast<uint32_t>(in) << i;
-    }
-  }
-  const uint32_t n = __popc(mine);
-  const uint32_t incl = wave_scan(n, lane);
-  __shared__ uint32_t sums[4];
-  if (lane == 63) sums[wave] = incl;
-  __syncthreads();
-  if (tid == 0) {
-    const uint32_t all = sums[0] + sums[1] + sums[2] + sums[3];
-    base_at = all ? atomicAdd(&q.listed[row], all) : 0;
-  }
-  __syncthreads();
-  uint32_t to = base_at + incl - n;
-  for (int w = 0; w < wave; ++w) to += sums[w];
-#pragma unroll
-  for (int i = 0; i < EPT; ++i)
-    if (mine >> i & 1u) {
-      if (to < kCap) q.list[static_cast<int64_t>(row) * kCap + to] = uint2{key_of(v[i]), static_cast<uint32_t>(C::index(chunk, tid, i, mis))};
-      ++to;
-    }
-}
-
-// ---- finish -------------------------------------------------------------------------------------
-
-constexpr int kFinish = 1024;  // threads
-
-// A token of the order: weights up to and with it.
-struct Found {
-  uint32_t ik, idx;
-  double upto, w;
-};
-
-template <int DT>
-struct Finish {
-  const SamplingParams& q;
-  const Settings& z;
-  const Plan& plan;
-  const uint8_t* base;
-  double grid;
-  bool in_list;
-  int n;
-  int tid, lane, wave;
-  // LDS
-  uint2* own;                 // [kCap] the listed tokens
-  unsigned long long* hist;   // [1024]
-  unsigned long long* hist2;  // [1024]
-  unsigned long long* sums;   // [2][16]
-  unsigned long long* sel;    // [4]
-  uint32_t* ext;              // [16]
-
-  __device__ double weight(uint32_t k) const {
-    return exp2_neg((static_cast<double>(logit_of_key(k)) - static_cast<double>(plan.max)) * z.s);
-  }
-  __device__ int bin(uint32_t k) const { return bin_of(logit_of_key(k), z.s_bin, grid); }
-
-  __device__ void fetch(int row) {
-    if (!in_list) return;
-    const uint2* const from = q.list + static_cast<int64_t>(row) * kCap;
-    for (int i = tid; i < n; i += kFinish) own[i] = from[i];  // (each thread reads its own only)
-  }
-
-  // f(key, index, weight) for the tokens with keys lo .. hi (weight only if WEIGHT)
-  template <bool WEIGHT, typename F>
-  __device__ void each(uint32_t lo, uint32_t hi, F f) const {
-    if (in_list) {
-      for (int i = tid; i < n; i += kFinish) {
-        const uint2 x = own[i];
-        if (x.x >= lo && x.x <= hi) f(x.x, x.y, WEIGHT ? weight(x.x) : 0.0);
-      }
-    } else {
-      for (int e = tid; e < q.V; e += kFinish) {
-        const float l = Chunk<DT, 8>::value(base, e);
-        const uint32_t k = key_of(l);
-        if (k >= lo && k <= hi && l > -__builtin_huge_valf()) f(k, static_cast<uint32_t>(e), WEIGHT ? weight(k) : 0.0);
-      }
-    }
-  }
-
-  __device__ uint64_t block_scan(uint64_t v, uint64_t* part, uint64_t& total) const {
-    const uint64_t s = wave_scan(v, lane);
-    if (lane == 63) part[wave] = s;
+    if (whole_row && g.origin == r.max) break;
+    // far from the origin bins are not told apart: once more, from the largest logit
+    if (r.max == -__builtin_huge_valf() || (r.top < kFar / 2 && r.top > -kFar / 2)) break;
+    g.origin = r.max;
+    sum = 0;
+    num = 0;
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kFinish / 64; ++i) {
-      const uint64_t x = part[i];
-      if (i < wave) before += x;
-      total += x;
-    }
-    return before + s;
   }
-
-  // The least and largest key of a window's tokens; false: it has none.
-  __device__ bool range(const Window& win, uint32_t& lo, uint32_t& hi) {
-    if (win.b1 < win.b0) return false;
-    if (tid == 0) ext[0] = kNone, ext[1] = 0;
-    __syncthreads();
-    uint32_t a = kNone, c = 0;
-    each<false>(0, kNone, [&](uint32_t k, uint32_t, double) {
-      const int j = bin(k);
-      if (j >= win.b0 && j <= win.b1) a = min(a, k), c = max(c, k);
-    });
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      a = min(a, static_cast<uint32_t>(__shfl_xor(static_cast<int>(a), d, 64)));
-      c = max(c, static_cast<uint32_t>(__shfl_xor(static_cast<int>(c), d, 64)));
-    }
-    if (lane == 0 && a != kNone) {
-      atomicMin(&ext[0], a);
-      atomicMax(&ext[1], c);
-    }
-    __syncthreads();
-    lo = ext[0];
-    hi = ext[1];
-    __syncthreads();
-    return lo <= hi;
-  }
-
-  __device__ bool reaches(float l) const { return (static_cast<double>(l) - static_cast<double>(plan.max)) * z.s >= z.f; }
-
-  // The weights of a window's tokens, of keys lo .. hi, that reach min-p.
-  __device__ double reaching(uint32_t lo, uint32_t hi, const Window& win) {
-    const int octave = static_cast<int>((win.b0 > 0 ? win.b0 - 1 : 0) / kPerOctave);
-    const double scale = __builtin_ldexp(1.0, octave + 43), unscale = __builtin_ldexp(1.0, -(octave + 43));
-    if (tid == 0) sel[0] = 0;
-    __syncthreads();
-    uint64_t sum = 0;
-    each<true>(lo, hi, [&](uint32_t k, uint32_t, double wt) {
-      if (reaches(logit_of_key(k))) sum += whole(wt * scale);
-    });
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    if (lane == 0 && sum) atomicAdd(&sel[0], static_cast<unsigned long long>(sum));
-    __syncthreads();
-    const double w = static_cast<double>(sel[0]) * unscale;
-    __syncthreads();
-    return w;
-  }
-
-  // Of the tokens with keys lo .. hi, in the order, the first at which `before` + the running sum reaches x
-  // (strict: exceeds it) -- of the weights, or, by_count, of ones (before and x: numbers of them); the last if none
-  // does.  `skip` is left out.  Whole numbers: 2^43 the largest weight of bin b0.
-  __device__ Found select(uint32_t lo, uint32_t hi, int b0, bool by_count, bool strict, double before, double x, uint32_t skip,
-                          double weights_before) {
-    const int octave = static_cast<int>((b0 > 0 ? b0 - 1 : 0) / kPerOctave);
-    const double scale = __builtin_ldexp(1.0, octave + 43), unscale = __builtin_ldexp(1.0, -(octave + 43));
-    uint64_t need;
-    {
-      const double y = fmin(fmax((x - before) * (by_count ? 1.0 : scale), 0.0), 0x1p63);
-      need = strict ? static_cast<uint64_t>(y) + 1 : static_cast<uint64_t>(__builtin_ceil(y));
-      if (need == 0) need = 1;
-    }
-    uint64_t sum = 0, sum2 = 0;  // of what lies before the open range: the measure, and by_count the weights
-    bool begin = true;
-    while (true) {
-      const uint32_t span = hi - lo;
-      const int bits = span ? 32 - __builtin_clz(span) : 0, sh = bits > 10 ? bits - 10 : 0;
-      hist[tid] = 0;
-      if (by_count) hist2[tid] = 0;
-      __syncthreads();
-      each<true>(lo, hi, [&](uint32_t k, uint32_t i, double wt) {
-        if (i == skip) return;
-        const uint32_t at = (k - lo) >> sh;
-        const unsigned long long m = whole(wt * scale);
-        atomicAdd(&hist[at], by_count ? 1ull : m);
-        if (by_count) atomicAdd(&hist2[at], m);
-      });
-      __syncthreads();
-      const uint64_t v = hist[tid];
-      uint64_t total, total2;
-      const uint64_t incl = sum + block_scan(v, reinterpret_cast<uint64_t*>(sums), total);
-      uint64_t incl2 = 0, v2 = 0;
-      if (by_count) {
-        v2 = hist2[tid];
-        incl2 = sum2 + block_scan(v2, reinterpret_cast<uint64_t*>(sums) + 16, total2);
-      }
-      if (begin && need > total) need = total ? total : 1;
-      if (tid == 0) sel[0] = 0, sel[1] = sum, sel[2] = sum2;
-      __syncthreads();
-      if (incl - v < need && need <= incl) sel[0] = tid, sel[1] = incl - v, sel[2] = incl2 - v2;
-      __syncthreads();
-      const uint32_t digit = static_cast<uint32_t>(sel[0]);
-      sum = sel[1];
-      sum2 = sel[2];
-      begin = false;
-      lo = lo + (digit << sh);
-      if (sh == 0) break;
-      const uint32_t top = lo + ((1u << sh) - 1u);
-      hi = top < hi ? top : hi;
-    }
-    // equal logits: the one in question by its place among them
-    if (tid == 0) ext[0] = kNone, ext[1] = 0, ext[2] = 0;
-    __syncthreads();
-    each<false>(lo, lo, [&](uint32_t, uint32_t i, double) {
-      if (i == skip) return;
-      atomicMin(&ext[0], i);
-      atomicMax(&ext[1], i);
-      atomicAdd(&ext[2], 1u);
-    });
-    __syncthreads();
-    Found r;
-    r.ik = lo;
-    r.w = weight(lo);
-    const uint64_t m = whole(r.w * scale);
-    uint32_t i0 = ext[0], i1 = ext[1];
-    const uint32_t ties = ext[2];
-    uint64_t place = by_count ? need - sum : m ? (need - sum + m - 1) / m : 1;
-    if (place > ties) place = ties;
-    if (place < 1) place = 1;
-    r.upto = (by_count ? weights_before : before) + static_cast<double>((by_count ? sum2 : sum) + place * m) * unscale;
-    uint32_t rank = static_cast<uint32_t>(place);
-    __syncthreads();
-    if (rank == 1) i1 = i0;
-    if (rank == ties) i0 = i1;
-    uint64_t seen = 0;
-    while (i0 < i1) {
-      const uint32_t span = i1 - i0;
-      const int bits = 32 - __builtin_clz(span), sh = bits > 10 ? bits - 10 : 0;
-      hist[tid] = 0;
-      if (tid == 0) sel[0] = 0, sel[1] = seen;
-      __syncthreads();
-      each<false>(lo, lo, [&](uint32_t, uint32_t i, double) {
-        if (i != skip && i >= i0 && i <= i1) atomicAdd(&hist[(i - i0) >> sh], 1ull);
-      });
-      __syncthreads();
-      const uint64_t v = hist[tid];
-      uint64_t total;
-      const uint64_t incl = seen + block_scan(v, reinterpret_cast<uint64_t*>(sums), total);
-      if (incl - v < rank && rank <= incl) sel[0] = tid, sel[1] = incl - v;
-      __syncthreads();
-      i0 = i0 + (static_cast<uint32_t>(sel[0]) << sh);
-      seen = sel[1];
-      const uint32_t top = i0 + ((1u << sh) - 1u);
-      i1 = top < i1 ? top : i1;
-      __syncthreads();
-    }
-    r.idx = i0;
-    return r;
-  }
-};
-
-template <int DT>
-__global__ void __launch_bounds__(kFinish) finish_kernel(const SamplingParams q) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ unsigned long long hist[1024], hist2[1024], sums[32], sel[4];
-  __shared__ uint32_t ext[16];
-  const int tid = threadIdx.x, row = blockIdx.x;
-  int b = 0, end = 0;
-  if (q.mode == kVerify && !sequence_of(q, row, tid & 63, b, end)) return;  // uniform
-  const Plan plan = q.plans[row];
-  const Settings z = settings(q, row);
-  const uint8_t* const base = q.logits + row * q.stride;
-  if (plan.max == -__builtin_huge_valf()) {  // uniform: no token
+  if (r.max == -__builtin_huge_valf()) {  // uniform: no token
     if (tid == 0) {
       if (q.mode == kSample) q.token[row] = -1, q.logprob[row] = -__builtin_huge_valf();
-      if (q.mode == kVerify) q.rowres[row] = Row{0.0, 0, 0, plan.max, 0, -1};
+      if (q.mode == kVerify) q.rowres[row] = Row{0.0, 0, r.max, 0.0f, 0, 0, -1};
       if (q.mode == kBeams) q.nbest[row] = 0;
     }
     return;
   }
-  const uint32_t listed = q.listed[row];
-  Finish<DT> f{q, z, plan, base, __builtin_floor(static_cast<double>(plan.max) * z.s_bin), listed <= kCap, static_cast<int>(listed),
-               tid, tid & 63, tid >> 6, reinterpret_cast<uint2*>(smem), hist, hist2, sums, sel, ext};
-  f.fetch(row);
-  // the last token of the order that top-k and top-p keep, and the weights of what is kept
-  uint32_t ik = kNone, idx = kNone;
-  double kept = plan.total;
-  auto cut = [&](uint32_t k, uint32_t i) {
-    if (k < ik || (k == ik && i < idx)) ik = k, idx = i;
+  // ---- running sums, as whole numbers: a bin of nothing adds nothing ----
+  // a unit of a bin's sum, in units of 2^-scale of the weight at the largest bin's middle
+  auto unit_of = [&](int j) -> double { return exp2_of(static_cast<double>(-j) / kPerOctave) * __builtin_ldexp(1.0, q.scale - kWhole); };
+  const double my_unit = unit_of(tid);
+  uint64_t my_w = static_cast<uint64_t>(static_cast<double>(sum) * my_unit + 0.5);
+  if (tid < kBins) {
+    const uint64_t s = wave_scan(my_w, lane);
+    const uint32_t n = wave_scan(num, lane);
+    if (lane == 63) part[wave] = s, partn[wave] = n;
+    cw[tid] = s;
+    cn[tid] = n;
+  }
+  __syncthreads();
+  uint64_t my_cw = ~0ull;
+  uint32_t my_cn = kNone;
+  if (tid < kBins) {
+    my_cw = cw[tid];
+    my_cn = cn[tid];
+    for (int w = 0; w < wave; ++w) my_cw += part[w], my_cn += partn[w];
+    cw[tid] = my_cw;
+    cn[tid] = my_cn;
+  }
+  __syncthreads();
+  const double total = static_cast<double>(cw[kRest]);
+  auto upto = [&](int j) -> double { return static_cast<double>(cw[j]); };
+  auto before = [&](int j) -> double { return j > 0 ? static_cast<double>(cw[j - 1]) : 0.0; };
+  int round = 0;
+  // the numbers of bins of which a and c hold: the first of which they do not, if they hold for all before it
+  auto find = [&](bool a, bool c, int& na, int& nc) {
+    const int pa = __popcll(__ballot(tid < kBins && a)), pc = __popcll(__ballot(tid < kBins && c));
+    if (lane == 0) found[round & 1][0][wave] = pa, found[round & 1][1][wave] = pc;
+    __syncthreads();
+    na = nc = 0;
+#pragma unroll
+    for (int w = 0; w < kBins / 64; ++w) na += found[round & 1][0][w], nc += found[round & 1][1][w];
+    ++round;
   };
-  uint32_t skip = kNone, token = kNone;
-  double logprob = 0.0;
-  bool accepted = false;
-  // top-k's cut, top-p's and min-p's, then the token (one loop: the code is fetched once)
-#pragma unroll 1
-  for (int step = 0; step < 4; ++step) {
-    const Window win = step == 0 ? plan.k : step == 1 ? plan.p : step == 2 ? plan.f : plan.d;
-    double before = win.before, x = 0.0;
-    if (step == 0) before = static_cast<double>(plan.count_before), x = static_cast<double>(z.k);
-    if (step == 1) x = z.p * kept;
-    if (step == 3) {
-      const double u = z.first ? 0.0 : unit(q.mode == kSample ? q.u[row] : q.mode == kVerify ? q.draw[b] : 0.0f);
-      double left = kept;
-      const int64_t d = q.mode == kVerify && row + 1 < end ? q.tokens[row + 1] : -1;
-      if (d >= 0 && d < q.V) {
-        const float l = Chunk<DT, 8>::value(base, static_cast<int>(d));
-        const uint32_t k = key_of(l);
-        const int j = bin_of(l, z.s_bin, f.grid);
-        if (j < kRest && f.reaches(l) && (k < ik || (k == ik && static_cast<uint32_t>(d) <= idx))) {
-          const double wd = f.weight(k);
-          const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + d]) : 1.0;
-          accepted = static_cast<double>(q.u[row]) * sure * kept < wd;
-          if (!q.probs && kept - wd > 0.0) {
-            skip = static_cast<uint32_t>(d);
-            left = kept - wd;
-            if (j < plan.d.b0) before -= wd;
-          }
-        }
+  auto in_bin = [&](float l) -> int {  // its bin from the largest down; kRest: too small to count
+    const double n = __builtin_rint(g.place(l));
+    return static_cast<int>(fmin(static_cast<double>(r.top) - n, static_cast<double>(kRest)));
+  };
+  auto reaches = [&](float l) -> bool { return (static_cast<double>(l) - static_cast<double>(r.max)) * z.s >= z.f; };
+  // the logarithm of a sum of weights, of the largest token's
+  auto log_of = [&](double w) -> double {
+    return log(w * __builtin_ldexp(1.0, -q.scale)) + (static_cast<double>(r.top) - g.place(r.max)) * (kLn2D / kPerOctave);
+  };
+  auto second = [&](float l) -> uint64_t {
+    const double t = g.place(l);
+    return whole_exp2(t - __builtin_rint(t));
+  };
+
+  // ---- a drafted token that its row judges ----
+  uint32_t drafted = kNone, drafted_key = 0;
+  int drafted_bin = kBins;
+  uint64_t drafted_sum = 0;  // its second factor
+  if (q.mode == kVerify && row + 1 < end) {
+    const int64_t d = q.tokens[row + 1];
+    if (d >= 0 && d < q.V) {
+      const float l = x[static_cast<int>(d)];
+      if (l > -__builtin_huge_valf() && in_bin(l) < kRest) {
+        drafted = static_cast<uint32_t>(d);
+        drafted_key = key_of(l);
+        drafted_bin = in_bin(l);
+        drafted_sum = second(l);
       }
-      x = u * left;
-    }
-    uint32_t lo, hi;
-    const bool some = f.range(win, lo, hi);  // uniform
-    if (step == 2 && win.b1 >= win.b0) kept = fmin(kept, win.before + (some ? f.reaching(lo, hi, win) : 0.0));
-    if (!some || step == 2) continue;
-    const Found c = f.select(lo, hi, win.b0, step == 0, step == 3, before, x, skip, plan.k.before);
-    if (step < 3) {
-      cut(c.ik, c.idx);
-      kept = fmin(kept, c.upto);
-    } else {
-      token = c.idx;
-      logprob = (static_cast<double>(logit_of_key(c.ik)) - static_cast<double>(plan.max)) * (z.s * kLn2D) - log(kept);
     }
   }
-  if (q.mode == kBeams) {
-    if (tid == 0) ext[4] = 0;
+  const bool leaves = drafted != kNone && !q.probs;  // refused, it leaves the row
+  // what it adds to the running sums
+  double drafted_w = 0.0;
+  if (leaves) {
+    if (tid == drafted_bin) sel[0] = my_w - static_cast<uint64_t>(static_cast<double>(sum - drafted_sum) * my_unit + 0.5);
     __syncthreads();
-    f.template each<false>(0, ik, [&](uint32_t k, uint32_t i, double) {
-      if (k == ik && i > idx) return;
-      const uint32_t at = atomicAdd(&ext[4], 1u);
-      if (at < static_cast<uint32_t>(q.keep)) q.best[static_cast<int64_t>(row) * q.keep + at] = uint2{k, i};
+    drafted_w = static_cast<double>(sel[0]);
+  }
+  const double u = z.first || q.mode == kBeams ? 0.0 : unit(q.mode == kVerify ? q.draw[b] : q.u[row]);
+
+  // ---- the bins in which something is to be found, before the cuts are known ----
+  // windows: top-k's cut, top-p's, min-p's, the token
+  int w0[4] = {1, 1, 1, 1}, w1[4] = {0, 0, 0, 0};
+  int last;
+  {
+    int kb;
+    find(my_cn < static_cast<uint32_t>(z.k), static_cast<double>(my_cw) < total, kb, last);
+    double least = total, most = total;
+    if (counting && kb < kRest) {
+      w0[0] = w1[0] = kb;
+      least = before(kb);
+      most = upto(kb);
+    }
+    if (q.mode == kBeams) {
+      // (with fewer tokens than wanted among the bins that count, all of the row's)
+      w0[0] = 0;
+      w1[0] = kb < kRest ? kb : kRest;
+    } else {
+      if (z.p < 1.0) {
+        const double a = z.p * least * kBelow, c = z.p * most * kAbove;
+        find(static_cast<double>(my_cw) < a, static_cast<double>(my_cw) < c, w0[1], w1[1]);
+        w1[1] = min(w1[1], last);
+        w0[1] = min(w0[1], w1[1]);
+        // a token of bin j weighs less than 2^((1 - j) / 10)
+        const double one = exp2_of(static_cast<double>(1 - w0[1]) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
+        least = a;
+        most = fmin(upto(w1[1]), c + one);
+      }
+      if (z.f > -__builtin_huge_val()) {
+        // tokens whose place is not below this reach min-p
+        const double y = g.place(r.max) + z.f, eps = 1e-6 + fabs(y) * 1e-13, top = static_cast<double>(r.top);
+        w0[2] = static_cast<int>(fmin(fmax(top - __builtin_rint(y + eps), 0.0), static_cast<double>(kRest)));
+        w1[2] = static_cast<int>(fmin(fmax(top - __builtin_rint(y - eps), 0.0), static_cast<double>(kRest - 1)));
+        if (w0[2] < kRest) {
+          least = fmin(least, before(w0[2]));
+          most = fmin(most, upto(w1[2]));
+        }
+      }
+      // with its bin before the cuts the drafted token is kept, behind them not, among them one or the other
+      double gone = 0.0;
+      bool sure = true;
+      if (leaves) {
+        int open = kBins, cut = kRest;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (w1[i] >= w0[i]) open = min(open, w0[i]), cut = min(cut, w1[i]);
+        gone = drafted_bin <= cut ? drafted_w : 0.0;
+        sure = drafted_bin < open || drafted_bin > cut;
+      }
+      const double a = u * fmax(least - gone, 0.0) * kBelow, c = u * (sure ? most - gone : most) * kAbove;
+      const double w = static_cast<double>(my_cw), without = tid >= drafted_bin ? w - gone : w;
+      find((sure ? without : w) <= a, without <= c, w0[3], w1[3]);
+      w1[3] = min(w1[3], kRest - 1);
+      w0[3] = min(w0[3], w1[3]);
+    }
+  }
+
+  // ---- the cuts and the token ----
+  bool in_list = false, relist = false;
+  int n = 0;
+  uint64_t cut = ~0ull;  // key and index of the last token that top-k and top-p keep
+  double kept = total;
+  uint32_t skip = kNone, token = kNone;
+  bool accepted = false;
+  double logprob = 0.0;
+#pragma unroll 1
+  for (int step = -1; step < 4; ++step) {
+    double target = 0.0;
+    int b0 = w0[3], b1 = w1[3];
+    if (step == 0) b0 = w0[0], b1 = w1[0];
+    if (step == 1) b0 = w0[1], b1 = w1[1];
+    if (step == 2) b0 = w0[2], b1 = w1[2];
+    double start = 0.0;  // what lies before the bin
+    if (step >= 0) {
+      if (b1 < b0) continue;  // uniform
+      if (step == 1) target = z.p * kept;
+      if (step == 3) {
+        double left = kept;
+        if (drafted != kNone) {
+          const uint64_t me = static_cast<uint64_t>(drafted_key) << 20 | drafted;
+          if (me <= cut && reaches(logit_of_key(drafted_key))) {
+            const double w = static_cast<double>(drafted_sum) * unit_of(drafted_bin);
+            const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + drafted]) : 1.0;
+            accepted = static_cast<double>(q.u[row]) * sure * kept < w;
+            // (what leaves less than 2^12 units is not refused: u is at most 1 - 2^-24)
+            if (leaves && kept - w > 4096.0) {
+              skip = drafted;
+              left = kept - w;
+            }
+          }
+        }
+        target = u * left;
+      }
+      if (step == 1 || step == 3) {
+        // the bin: the first whose running sum reaches the target, or for the token exceeds it
+        const double w = static_cast<double>(my_cw), gone = skip != kNone && tid >= drafted_bin ? drafted_w : 0.0;
+        int at, end_at;
+        const double whole_w = total - (skip != kNone ? drafted_w : 0.0);
+        find(step == 3 ? w - gone <= target : w < target, w - gone < whole_w, at, end_at);
+        at = min(at, end_at);
+        b0 = b1 = min(max(at, b0), b1);
+        start = before(b0) - (skip != kNone && b0 > drafted_bin ? drafted_w : 0.0);
+      }
+    }
+    // ---- the tokens of the bins: all windows' at once, or, where those are too many, the bin's ----
+    if (step < 0 || relist) {
+      __syncthreads();
+      if (tid == 0) number[0] = 0;
+      __syncthreads();
+      // two ranges of bins, the cuts' and the token's, as ranges of logits a little wider
+      int h[2][2] = {{b0, b1}, {1, 0}};
+      if (step < 0) {
+        h[0][0] = min(min(w1[0] < w0[0] ? kBins : w0[0], w1[1] < w0[1] ? kBins : w0[1]), w1[2] < w0[2] ? kBins : w0[2]);
+        h[0][1] = max(max(w1[0], w1[1]), w1[2]);
+        h[1][0] = w0[3];
+        h[1][1] = w1[3];
+      }
+      float from[2], to[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const double top = static_cast<double>(r.top), o = static_cast<double>(g.origin);
+        const float a = static_cast<float>(o + (top - h[i][1] - 0.5) / z.s), c = static_cast<float>(o + (top - h[i][0] + 0.5) / z.s);
+        from[i] = h[i][1] >= kRest ? -kBig : a - fabsf(a) * 0x1p-20f - 1e-37f;
+        to[i] = c + fabsf(c) * 0x1p-20f + 1e-37f;
+        if (h[i][1] < h[i][0]) from[i] = __builtin_huge_valf(), to[i] = -from[i];
+        from[i] = fmaxf(from[i], -kBig);
+      }
+      const int pieces = x.count();
+      constexpr int AHEAD = 4;
+      for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
+        uint4 v[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) v[a] = p0 + a * NT + tid < pieces ? x.load(p0 + a * NT + tid) : P::none();
+        uint32_t mine = 0;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) {
+            const float l = fminf(P::at(v[a], i), kBig), was = P::at(v[a], i);
+            const bool in = ((l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1])) && was == was;
+            mine |= static_cast<uint32_t>(in) << (a * P::N + i);
+          }
+        if (__ballot(mine != 0) == 0) continue;
+        const uint32_t many = __popc(mine), s = wave_scan(many, lane);
+        uint32_t at = 0;
+        if (lane == 63) at = atomicAdd(&number[0], s);
+        at = static_cast<uint32_t>(__shfl(static_cast<int>(at), 63, 64)) + s - many;
+        while (mine) {
+          const int i = __builtin_ctz(mine);
+          mine &= mine - 1;
+          const int idx = x.first(p0 + i / P::N * NT + tid) + i % P::N;
+          const float l = x[idx];
+          if (at < kCap) list[at] = uint2{key_of(l), static_cast<uint32_t>(idx) | static_cast<uint32_t>(in_bin(l)) << 20};
+          ++at;
+        }
+      }
+      __syncthreads();
+      n = static_cast<int>(min(number[0], static_cast<uint32_t>(kCap)));
+      in_list = number[0] <= kCap;
+      if (step < 0) {
+        relist = !in_list;
+        continue;
+      }
+    }
+    // f(key and index, logit) for the tokens of bins b0 .. b1 with keys and indices lo .. hi
+    auto each = [&](uint64_t lo, uint64_t hi, auto f) __attribute__((always_inline)) {
+      if (in_list) {
+        for (int i = tid; i < n; i += NT) {
+          const uint2 e = list[i];
+          const int j = static_cast<int>(e.y >> 20);
+          const uint32_t idx = e.y & 0xfffffu;
+          const uint64_t me = static_cast<uint64_t>(e.x) << 20 | idx;
+          if (j >= b0 && j <= b1 && me >= lo && me <= hi && idx != skip) f(me, logit_of_key(e.x));
+        }
+      } else {
+        for (int i = tid; i < x.V; i += NT) {
+          const float l = x[i];
+          const int j = in_bin(l);
+          const uint64_t me = static_cast<uint64_t>(key_of(l)) << 20 | static_cast<uint32_t>(i);
+          if (j >= b0 && j <= b1 && l > -__builtin_huge_valf() && me >= lo && me <= hi && static_cast<uint32_t>(i) != skip) f(me, l);
+        }
+      }
+    };
+    uint64_t lo = 0, hi = ~0ull;
+    const bool by_count = step == 0;
+    const double u_bin = unit_of(b0);
+    if (step != 2) {
+      // ---- the token at which the running sum reaches `need` ----
+      uint64_t need;
+      if (by_count) {
+        need = static_cast<uint64_t>(z.k) - (b0 > 0 ? cn[b0 - 1] : 0u);
+      } else {
+        const double y = fmax((target - start) / u_bin, 0.0);
+        need = step == 3 ? static_cast<uint64_t>(y) + 1 : static_cast<uint64_t>(__builtin_ceil(y));
+      }
+      if (need < 1) need = 1;
+      uint64_t passed = 0;
+      while (true) {
+        // how many are left, and between which keys and indices
+        __syncthreads();
+        if (tid == 0) ext[0] = ~0ull, ext[1] = 0, number[0] = 0, number[1] = 0;
+        hist[tid] = 0;
+        __syncthreads();
+        uint64_t a = ~0ull, c = 0;
+        uint32_t m = 0;
+        each(lo, hi, [&](uint64_t me, float) {
+          a = me < a ? me : a;
+          c = me > c ? me : c;
+          ++m;
+        });
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) {
+          const uint64_t a2 = __shfl_xor(a, d, 64), c2 = __shfl_xor(c, d, 64);
+          a = a2 < a ? a2 : a;
+          c = c2 > c ? c2 : c;
+          m += __shfl_xor(m, d, 64);
+        }
+        if (lane == 0 && m) {
+          atomicMin(reinterpret_cast<unsigned long long*>(&ext[0]), a);
+          atomicMax(reinterpret_cast<unsigned long long*>(&ext[1]), c);
+          atomicAdd(&number[0], m);
+        }
+        __syncthreads();
+        const uint32_t left = number[0];
+        lo = ext[0];
+        hi = ext[1];
+        if (left <= 64) break;  // uniform
+        const uint64_t span = hi - lo;
+        const int bits = 64 - __builtin_clzll(span), sh = bits > 10 ? bits - 10 : 0;
+        each(lo, hi, [&](uint64_t me, float l) { atomicAdd(&hist[(me - lo) >> sh], by_count ? 1ull : static_cast<unsigned long long>(second(l))); });
+        __syncthreads();
+        const uint64_t v = hist[tid];
+        const uint64_t s = wave_scan(v, lane);
+        if (lane == 63) part[wave] = s;
+        __syncthreads();
+        uint64_t before_me = passed, all = passed;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const uint64_t p = part[w];
+          if (w < wave) before_me += p;
+          all += p;
+        }
+        if (need > all) need = all;
+        if (before_me + s - v < need && need <= before_me + s) sel[0] = tid, sel[1] = before_me + s - v;
+        __syncthreads();
+        lo = lo + (sel[0] << sh);
+        const uint64_t top = lo + ((1ull << sh) - 1ull);
+        hi = top < hi ? top : hi;
+        passed = sel[1];
+      }
+      // ---- at most 64: gathered, and one wave sums them in their order ----
+      each(lo, hi, [&](uint64_t me, float l) {
+        const uint32_t to = atomicAdd(&number[1], 1u);
+        hist[2 * to] = me;
+        hist[2 * to + 1] = by_count ? 1ull : static_cast<unsigned long long>(second(l));
+      });
+      __syncthreads();
+      const int m = static_cast<int>(number[1]);
+      const uint64_t me = lane < m ? hist[2 * lane] : ~0ull, mine = lane < m ? hist[2 * lane + 1] : 0;
+      uint64_t sums = passed, all = passed;
+      for (int i = 0; i < m; ++i) {
+        const uint64_t o = hist[2 * i], w = hist[2 * i + 1];
+        sums += o <= me ? w : 0;
+        all += w;
+      }
+      if (need > all) need = all;
+      const uint64_t hit = __ballot(lane < m && sums >= need && sums - mine < need);
+      lo = hit ? __shfl(me, __builtin_ctzll(hit), 64) : ~0ull;  // (every wave finds the same)
+    }
+    if (step == 3) {
+      if (lo != ~0ull) {
+        token = static_cast<uint32_t>(lo & 0xfffffu);
+        logprob = (static_cast<double>(logit_of_key(static_cast<uint32_t>(lo >> 20))) - static_cast<double>(r.max)) * z.s * (kLn2D / kPerOctave) - log_of(kept);
+      }
+      continue;
+    }
+    if (step < 2) cut = lo < cut ? lo : cut;
+    if (q.mode == kBeams) break;  // uniform
+    // ---- the weights up to the cut, or of those that reach min-p ----
+    __syncthreads();
+    if (tid == 0) sel[2] = 0;
+    __syncthreads();
+    uint64_t mine = 0;
+    each(0, step == 2 ? ~0ull : lo, [&](uint64_t, float l) {
+      uint64_t w = second(l);
+      if (step == 2) {
+        if (!reaches(l)) return;
+        if (in_bin(l) != b0) w = static_cast<uint64_t>(static_cast<double>(w) * exp2_of(static_cast<double>(b0 - in_bin(l)) / kPerOctave));
+      }
+      mine += w;
     });
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mine += __shfl_xor(mine, d, 64);
+    if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&sel[2]), static_cast<unsigned long long>(mine));
     __syncthreads();
-    if (tid == 0) q.nbest[row] = ext[4] < static_cast<uint32_t>(q.keep) ? ext[4] : static_cast<uint32_t>(q.keep);
+    kept = fmin(kept, before(b0) + static_cast<double>(sel[2]) * u_bin);
+  }
+  if (q.mode == kBeams) {
+    __syncthreads();
+    if (tid == 0) number[1] = 0;
+    __syncthreads();
+    auto take = [&](uint32_t k, uint32_t i) {
+      const uint32_t to = atomicAdd(&number[1], 1u);
+      if (to < static_cast<uint32_t>(q.keep)) q.best[static_cast<int64_t>(row) * q.keep + to] = uint2{k, i};
+    };
+    if (in_list) {
+      for (int i = tid; i < n; i += NT) {
+        const uint32_t idx = list[i].y & 0xfffffu;
+        if ((static_cast<uint64_t>(list[i].x) << 20 | idx) <= cut) take(list[i].x, idx);
+      }
+    } else {
+      for (int i = tid; i < x.V; i += NT) {
+        const uint32_t k = key_of(x[i]);
+        if ((static_cast<uint64_t>(k) << 20 | static_cast<uint32_t>(i)) <= cut && x[i] > -__builtin_huge_valf()) take(k, static_cast<uint32_t>(i));
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      q.nbest[row] = min(number[1], static_cast<uint32_t>(q.keep));
+      q.rowres[row] = Row{log_of(total), 0, r.max, g.origin, r.top, 0, 0};
+    }
     return;
   }
   if (tid != 0) return;
   if (q.mode == kSample) {
     q.token[row] = token == kNone ? -1 : static_cast<int64_t>(token);
-    q.logprob[row] = static_cast<float>(logprob);
+    // (a difference below what the sums tell apart is none)
+    q.logprob[row] = logprob > -0x1p-40 ? 0.0f : static_cast<float>(logprob);
   } else {
-    q.rowres[row] = Row{kept, ik, idx, plan.max, accepted ? 1 : 0, static_cast<int32_t>(token)};
+    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, accepted ? 1 : 0, static_cast<int32_t>(token)};
   }
 }
 
@@ -839,87 +880,76 @@ __global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
 }
 
 // What the target has above the draft at token i, 2^52 a probability of 1.
-template <int DT>
 __device__ __forceinline__ uint64_t above(const SamplingParams& q, const Settings& z, const Row& r, int row, float l, int i) {
-  const uint32_t k = key_of(l);
-  const double t = (static_cast<double>(l) - static_cast<double>(r.max)) * z.s;
-  if (!(l > -__builtin_huge_valf()) || t < z.f || k > r.ik || (k == r.ik && static_cast<uint32_t>(i) > r.idx)) return 0;
-  const double d = exp2_neg(t) / r.kept - static_cast<double>(fmaxf(q.probs[row * q.probs_stride + i], 0.0f));
+  const uint64_t me = static_cast<uint64_t>(key_of(l)) << 20 | static_cast<uint32_t>(i);
+  if (!(l > -__builtin_huge_valf()) || me > r.cut || (static_cast<double>(l) - static_cast<double>(r.max)) * z.s < z.f) return 0;
+  const double t = Grid{r.origin, z.s}.place(l) - static_cast<double>(r.top);
+  const double p = exp2_of(t / kPerOctave) * __builtin_ldexp(1.0, q.scale) / r.kept;
+  const double d = p - static_cast<double>(fmaxf(q.probs[row * q.probs_stride + i], 0.0f));
   return d > 0.0 ? static_cast<uint64_t>(d * 0x1p52) : 0;
 }
 
-template <int DT, int EPT>
+constexpr int kRestElements = 4096;  // of a chunk
+
+template <int DT>
 __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
-  using C = Chunk<DT, EPT>;
   __shared__ unsigned long long sums[4];
   const int tid = threadIdx.x;
-  const int b = blockIdx.x / q.chunks, chunk = blockIdx.x - b * q.chunks;
+  const int b = blockIdx.x / q.rest_chunks, chunk = blockIdx.x - b * q.rest_chunks;
   const int row = q.refused[b];
   if (row < 0) return;
-  const uint8_t* const base = q.logits + row * q.stride;
+  const Pieces<DT> x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
-  const int mis = C::mis(base);
-  float v[EPT];
-  C::load(base, q.V, chunk, tid, mis, v);
   uint64_t s = 0;
-#pragma unroll
-  for (int i = 0; i < EPT; ++i)
-    if (v[i] > -__builtin_huge_valf()) s += above<DT>(q, z, r, row, v[i], C::index(chunk, tid, i, mis));
+#pragma unroll 4
+  for (int k = 0; k < kRestElements / 256; ++k) {
+    const int i = chunk * kRestElements + 256 * k + tid;
+    if (i < q.V) s += above(q, z, r, row, x[i], i);
+  }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
   if ((tid & 63) == 0) sums[tid >> 6] = s;
   __syncthreads();
-  if (tid == 0) q.rest[static_cast<int64_t>(b) * q.chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
+  if (tid == 0) q.rest[static_cast<int64_t>(b) * q.rest_chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 // The token of a refused row from what the target has above the draft, by rising index (where that is
 // nothing it stays the one from the target itself).
-template <int DT, int EPT>
+template <int DT>
 __global__ void __launch_bounds__(256) redraw_kernel(const SamplingParams q) {
-  using C = Chunk<DT, EPT>;
-  __shared__ unsigned long long sums[4];
-  __shared__ unsigned long long at_before[2];
+  __shared__ unsigned long long sums[4], at_before;
   __shared__ int at_chunk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   const int row = q.refused[b];
   if (row < 0) return;
-  const uint64_t* const rest = q.rest + static_cast<int64_t>(b) * q.chunks;
-  uint64_t total = 0;
-  for (int c = tid; c < q.chunks; c += 256) total += rest[c];
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, 64);
-  if (lane == 0) sums[wave] = total;
+  // a chunk is a thread's: at most 2^20 / 4096 of them
+  const uint64_t mine = tid < q.rest_chunks ? q.rest[static_cast<int64_t>(b) * q.rest_chunks + tid] : 0;
+  const uint64_t upto = wave_scan(mine, lane);
+  if (lane == 63) sums[wave] = upto;
   __syncthreads();
-  total = sums[0] + sums[1] + sums[2] + sums[3];
+  const uint64_t total = sums[0] + sums[1] + sums[2] + sums[3];
   if (total == 0) return;  // uniform
   uint64_t need = static_cast<uint64_t>(unit(q.draw[b]) * static_cast<double>(total)) + 1;
   if (need > total) need = total;
-  if (tid == 0) {
-    uint64_t s = 0;
-    int c = 0;
-    while (c < q.chunks - 1 && s + rest[c] < need) s += rest[c++];
-    at_chunk = c;
-    at_before[0] = s;
-  }
+  uint64_t before = upto - mine;
+  for (int w = 0; w < wave; ++w) before += sums[w];
+  if (before < need && need <= before + mine) at_chunk = tid, at_before = before;
   __syncthreads();
-  const int chunk = at_chunk;
-  uint64_t sum = at_before[0];
-  const uint8_t* const base = q.logits + row * q.stride;
+  uint64_t sum = at_before;
+  const Pieces<DT> x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
-  const int mis = C::mis(base);
-  const int first = C::index(chunk, 0, 0, mis);
-  for (int e0 = 0; e0 < 256 * EPT; e0 += 256) {
-    const int i = first + e0 + tid;
-    const uint64_t v = i >= 0 && i < q.V ? above<DT>(q, z, r, row, C::value(base, i), i) : 0;
+  for (int k = 0; k < kRestElements / 256; ++k) {
+    const int i = at_chunk * kRestElements + 256 * k + tid;
+    const uint64_t v = i < q.V ? above(q, z, r, row, x[i], i) : 0;
     const uint64_t s = wave_scan(v, lane);
     __syncthreads();
     if (lane == 63) sums[wave] = s;
     __syncthreads();
-    uint64_t before = sum;
-    for (int w = 0; w < wave; ++w) before += sums[w];
-    if (before + s - v < need && need <= before + s) q.token[b] = i;
+    uint64_t at = sum;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+    if (at + s - v < need && need <= at + s) q.token[b] = i;
     sum += sums[0] + sums[1] + sums[2] + sums[3];
     if (sum >= need) break;  // uniform
   }
@@ -944,8 +974,8 @@ __global__ void __launch_bounds__(1024) beams_kernel(const SamplingParams q, int
       const float score = q.scores[row];
       if (static_cast<uint32_t>(j) < q.nbest[row] && score > -__builtin_huge_valf()) {
         const uint2 x = q.best[static_cast<int64_t>(row) * q.keep + j];
-        const Plan& plan = q.plans[row];
-        v = static_cast<double>(score) + ((static_cast<double>(logit_of_key(x.x)) - static_cast<double>(plan.max)) - log(plan.total));
+        const Row& r = q.rowres[row];  // (kept: the logarithm of the sum)
+        v = static_cast<double>(score) + ((static_cast<double>(logit_of_key(x.x)) - static_cast<double>(r.max)) - r.kept);
         w = static_cast<uint64_t>(row) << 32 | x.y;
       }
     }
@@ -977,12 +1007,6 @@ __global__ void __launch_bounds__(1024) beams_kernel(const SamplingParams q, int
 
 // ---- host -----------------------------------------------------------------------------------------
 
-// Elements of a chunk's thread: 32, or 8 where chunks of 8192 would leave compute units idle.
-int chunk_elements(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) < 512 ? 8 : 32; }
-
-// Chunks of a row, whatever its alignment: up to 7 elements of the first piece belong to no row.
-int chunk_count(int64_t V, int per) { return static_cast<int>((V + 7 + 256 * per - 1) / (256 * per)); }
-
 int64_t up(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
 
 // The workspace's parts, in order; returns the bytes.
@@ -992,19 +1016,14 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
     to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(ws + at);
     at += up(n * static_cast<int64_t>(sizeof(*to)));
   };
-  const int64_t r = q.rows, rc = r * q.chunks;
+  const int64_t r = q.rows, rc = q.chunks > 1 ? r * q.chunks : 0;
   take(q.heads, rc);
   take(q.hist, rc * kBins);
-  if (q.count) take(q.counts, rc * kBins);
-  take(q.plans, r);
-  take(q.listed, r);
-  take(q.list, r * kCap);
-  if (q.mode == kVerify) {
-    take(q.rowres, r);
-    if (q.probs) {
-      take(q.refused, q.B);
-      take(q.rest, static_cast<int64_t>(q.B) * q.chunks);
-    }
+  take(q.counts, rc * kBins);
+  if (q.mode != kSample) take(q.rowres, r);
+  if (q.mode == kVerify && q.probs) {
+    take(q.refused, q.B);
+    take(q.rest, static_cast<int64_t>(q.B) * q.rest_chunks);
   }
   if (q.mode == kBeams) {
     take(q.best, r * q.keep);
@@ -1013,7 +1032,7 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
   return at;
 }
 
-constexpr int kFinishLds = kCap * static_cast<int>(sizeof(uint2));
+constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2));
 
 // The dynamic-LDS limit is a per-device function attribute: set once per device.
 template <typename K>
@@ -1033,19 +1052,17 @@ bool raise_lds(K kern, int bytes, std::atomic<bool> (&set)[kMaxDevices]) {
   return true;
 }
 
-template <int DT, int EPT>
-int launch_as(const SamplingParams& q, hipStream_t s) {
-  static std::atomic<bool> finish_set[kMaxDevices] = {};
-  if (!raise_lds(finish_kernel<DT>, kFinishLds, finish_set)) return MZK_ELAUNCH;
-  const unsigned grid = static_cast<unsigned>(q.rows) * static_cast<unsigned>(q.chunks);
-  survey_kernel<DT, EPT><<<grid, 256, 0, s>>>(q);
-  narrow_kernel<DT, EPT><<<grid, 256, 0, s>>>(q);
-  finish_kernel<DT><<<static_cast<unsigned>(q.rows), kFinish, kFinishLds, s>>>(q);
+template <int DT>
+int launch(const SamplingParams& q, hipStream_t s) {
+  static std::atomic<bool> row_set[kMaxDevices] = {};
+  if (!raise_lds(row_kernel<DT>, kRowLds, row_set)) return MZK_ELAUNCH;
+  if (q.chunks > 1) survey_kernel<DT><<<static_cast<unsigned>(q.rows) * static_cast<unsigned>(q.chunks), 256, 0, s>>>(q);
+  row_kernel<DT><<<static_cast<unsigned>(q.rows), kRowThreads, kRowLds, s>>>(q);
   if (q.mode == kVerify) {
     verify_kernel<<<static_cast<unsigned>((q.B + 255) / 256), 256, 0, s>>>(q);
     if (q.probs) {
-      rest_kernel<DT, EPT><<<static_cast<unsigned>(q.B) * static_cast<unsigned>(q.chunks), 256, 0, s>>>(q);
-      redraw_kernel<DT, EPT><<<static_cast<unsigned>(q.B), 256, 0, s>>>(q);
+      rest_kernel<DT><<<static_cast<unsigned>(q.B) * static_cast<unsigned>(q.rest_chunks), 256, 0, s>>>(q);
+      redraw_kernel<DT><<<static_cast<unsigned>(q.B), 256, 0, s>>>(q);
     }
   }
   if (q.mode == kBeams) {
@@ -1057,11 +1074,6 @@ int launch_as(const SamplingParams& q, hipStream_t s) {
   return MZK_OK;
 }
 
-template <int DT>
-int launch(const SamplingParams& q, hipStream_t s) {
-  return chunk_elements(q.rows, q.V) == 8 ? launch_as<DT, 8>(q, s) : launch_as<DT, 32>(q, s);
-}
-
 int size_of(int dtype) { return dtype == MZK_F32 ? 4 : 2; }
 
 // What every call checks of its rows, and the parts of the parameters that follow from them.
@@ -1069,26 +1081,34 @@ int rows_of(SamplingParams& q, const char* name, int64_t rows, int64_t V, int dt
   MZK_CHECK_ARG(dtype >= MZK_F32 && dtype <= MZK_F16, "%s: unsupported dtype %d", name, dtype);
   MZK_CHECK_ARG(rows >= 0 && V >= 1, "%s: bad sizes", name);
   MZK_CHECK_ARG(V <= kMaxVocab, "%s: at most %lld logits a row, got %lld", name, (long long)kMaxVocab, (long long)V);
-  const int per = chunk_elements(rows, V);
+  // a launch has less than 2^32 threads
+  MZK_CHECK_ARG(rows < (1 << 22), "%s: too many rows: %lld", name, (long long)rows);
   q.V = static_cast<int>(V);
-  q.chunks = chunk_count(V, per);
   q.scale = 62;
   while ((static_cast<int64_t>(1) << (62 - q.scale)) < V) --q.scale;
-  // a launch has less than 2^32 threads
-  MZK_CHECK_ARG(rows < (1 << 22) && rows * q.chunks < (1 << 24), "%s: too many rows: %lld of %lld logits", name, (long long)rows, (long long)V);
+  // Chunks: of whole steps of a survey's workgroup, 4096 elements, so that there are some 1024 workgroups; none
+  // from 128 rows on, and 7 elements of the first piece may belong to no row.
+  const int64_t steps = (V + 7 + 4095) / 4096;
+  int64_t chunks = rows >= 128 || rows == 0 ? 1 : 1024 / rows;
+  if (chunks > 64) chunks = 64;
+  if (chunks > steps) chunks = steps;
+  const int64_t per = (steps + chunks - 1) / chunks;
+  q.chunk_pieces = static_cast<int>(per * 4096 * size_of(dtype) / 16);
+  q.chunks = static_cast<int>((steps + per - 1) / per);
+  q.rest_chunks = static_cast<int>((V + kRestElements - 1) / kRestElements);
   q.rows = static_cast<int>(rows);
   return MZK_OK;
 }
 
 int run(SamplingParams& q, const char* name, const void* logits, int64_t stride, int dtype, void* workspace, int64_t workspace_bytes,
         void* stream) {
-  MZK_CHECK_ARG(logits && workspace, "%s: null pointer", name);
+  MZK_CHECK_ARG(logits, "%s: null pointer", name);
   MZK_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % size_of(dtype) == 0 && aligned16(workspace), "%s: misaligned logits or workspace", name);
   MZK_CHECK_ARG(stride >= q.V || q.rows <= 1, "%s: rows of logits overlap", name);
   q.logits = static_cast<const uint8_t*>(logits);
   q.stride = stride * size_of(dtype);
   const int64_t need = lay(q, static_cast<uint8_t*>(workspace));
-  MZK_CHECK_ARG(workspace_bytes >= need, "%s: workspace needs %lld bytes", name, (long long)need);
+  MZK_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace needs %lld bytes", name, (long long)need);
   const hipStream_t s = as_stream(stream);
   return dtype == MZK_F32 ? launch<MZK_F32>(q, s) : dtype == MZK_BF16 ? launch<MZK_BF16>(q, s) : launch<MZK_F16>(q, s);
 }
@@ -1107,7 +1127,6 @@ extern "C" int mzk_sample_workspace_bytes(int64_t rows, int64_t V, int dtype, in
   MZK_CHECK_ARG(bytes != nullptr, "sample_workspace_bytes: null output");
   SamplingParams q{};
   q.mode = kSample;
-  q.count = 1;
   if (const int rc = rows_of(q, "sample_workspace_bytes", rows, V, dtype)) return rc;
   return bytes_of(q, bytes);
 }
@@ -1126,7 +1145,6 @@ extern "C" int mzk_sample(const void* logits, int dtype, int64_t rows, int64_t V
   q.min_p = Filter{min_p, min_p_all};
   q.top_k = top_k;
   q.top_k_all = top_k_all;
-  q.count = top_k || top_k_all > 0;
   q.u = u;
   q.token = tokens;
   q.logprob = logprobs;
@@ -1138,7 +1156,6 @@ extern "C" int mzk_verify_workspace_bytes(int64_t T, int64_t B, int64_t V, int d
   MZK_CHECK_ARG(B >= 0 && B < 1 << 22, "verify_workspace_bytes: bad sizes");
   SamplingParams q{};
   q.mode = kVerify;
-  q.count = 1;
   if (const int rc = rows_of(q, "verify_workspace_bytes", T, V, dtype)) return rc;
   q.B = static_cast<int>(B);
   const float some = 0.0f;
@@ -1155,7 +1172,7 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   SamplingParams q{};
   q.mode = kVerify;
   if (const int rc = rows_of(q, "verify", T, V, dtype)) return rc;
-  MZK_CHECK_ARG(B >= 0 && B < 1 << 22 && B * q.chunks < 1 << 24, "verify: bad sizes");
+  MZK_CHECK_ARG(B >= 0 && B < 1 << 22 && B * q.rest_chunks < 1 << 24, "verify: bad sizes");
   if (B == 0) return MZK_OK;
   MZK_CHECK_ARG(cu && accepted && next && draw && (T == 0 || (tokens && u)), "verify: null pointer");
   MZK_CHECK_ARG(!draft_probs || draft_row_stride >= V || T <= 1, "verify: rows of the draft's probabilities overlap");
@@ -1164,7 +1181,6 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   q.min_p = Filter{min_p, min_p_all};
   q.top_k = top_k;
   q.top_k_all = top_k_all;
-  q.count = top_k || top_k_all > 0;
   q.u = u;
   q.tokens = tokens;
   q.cu = cu;
@@ -1188,7 +1204,6 @@ extern "C" int mzk_beams_workspace_bytes(int64_t rows, int64_t V, int dtype, int
   MZK_CHECK_ARG(keep >= 1 && keep <= kMostBeams, "beams_workspace_bytes: bad sizes");
   SamplingParams q{};
   q.mode = kBeams;
-  q.count = 1;
   if (const int rc = rows_of(q, "beams_workspace_bytes", rows, V, dtype)) return rc;
   q.keep = keep;
   return bytes_of(q, bytes);
@@ -1205,7 +1220,6 @@ extern "C" int mzk_beams(const void* logits, int dtype, int64_t rows, int64_t V,
   MZK_CHECK_ARG(rows % width == 0, "beams: %lld rows are no groups of %d", (long long)rows, width);
   if (rows == 0) return MZK_OK;
   MZK_CHECK_ARG(scores && parents && tokens && out_scores, "beams: null pointer");
-  q.count = 1;
   q.scores = scores;
   q.width = width;
   q.keep = keep;

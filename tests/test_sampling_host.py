@@ -80,12 +80,11 @@ def test_entry_points_check_their_arguments():
         assert text in lib.mzk_last_error().decode(), lib.mzk_last_error()
 
     big = 1 << 40
-    sm = [p, 0, 4, 1000, 1000, p, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, big, None]
-    for i, v, text in ((0, None, "null"), (0, odd, "misaligned"), (1, 7, "dtype"), (2, -1, "bad sizes"), (2, 1 << 23, "too many rows"), (3, 0, "bad sizes"),
-                       (3, (1 << 20) + 1, "at most"), (4, 999, "overlap"), (5, None, "null"), (14, None, "null"), (15, None, "null"), (16, None, "null"),
+    sm = [p, 0, 4, 100000, 100000, p, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, big, None]
+    for i, v, text in ((0, None, "null"), (0, odd, "misaligned"), (1, 7, "dtype"), (2, -1, "bad sizes"), (2, 1 << 22, "too many rows"), (3, 0, "bad sizes"),
+                       (3, (1 << 20) + 1, "at most"), (4, 99999, "overlap"), (5, None, "null"), (14, None, "null"), (15, None, "null"), (16, None, "workspace needs"),
                        (16, ctypes.c_void_p(264), "misaligned"), (17, 8, "workspace needs")):
         refuse("mzk_sample", sm[:i] + [v] + sm[i + 1:], text)
-    refuse("mzk_sample", sm[:2] + [1 << 20, 1 << 20, 1 << 20] + sm[5:], "too many rows")
     assert lib.mzk_sample(None, 0, 0, 1000, 1000, *sm[5:14], None, None, None, 0, None) == 0   # no rows
     vf = [p, 0, 6, 1000, 1000, p, p, 2, p, p, None, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, p, big, None]
     for i, v, text in ((0, None, "null"), (5, None, "null"), (6, None, "null"), (7, -1, "bad sizes"), (7, 1 << 22, "bad sizes"), (8, None, "null"),
@@ -96,7 +95,7 @@ def test_entry_points_check_their_arguments():
     for i, v, text in ((6, 4, "no groups"), (6, 0, "at least 1"), (7, 0, "at least 1"), (7, 4096, "at most"), (5, None, "null"), (8, None, "null"),
                        (12, 8, "workspace needs"), (1, 3, "dtype")):
         refuse("mzk_beams", bm[:i] + [v] + bm[i + 1:], text)
-    for f, args in (("sample", (4, 1000, 0)), ("verify", (4, 2, 1000, 0, 1)), ("beams", (4, 1000, 0, 2))):
+    for f, args in (("sample", (4, 100000, 0)), ("verify", (4, 2, 100000, 0, 1)), ("beams", (4, 100000, 0, 2))):
         assert getattr(lib, f"mzk_{f}_workspace_bytes")(*args, ctypes.byref(n)) == 0 and n.value > 0
         assert getattr(lib, f"mzk_{f}_workspace_bytes")(*args, None) < 0
         assert getattr(lib, f"mzk_{f}_workspace_bytes")(4, *args[1:-2], 1 << 30, *args[-1:], ctypes.byref(n)) < 0
