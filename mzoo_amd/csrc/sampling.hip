@@ -12,7 +12,7 @@
 // are computed in 64 bits to about 2^-50 of themselves, and summed as whole numbers, in any order the same.
 //
 // No row is sorted, and none is looked at twice in full arithmetic.  A row's workgroup has a histogram of its weights
-// over bins of 1/10 octave, from the largest down (survey: of its own, or joined from those of chunks where there are
+// over bins of 1/20 octave, from the largest down (survey: of its own, or joined from those of chunks where there are
 // too few rows for the compute units); finds the few bins in which the cuts of the filters and the token lie; lists
 // the row's tokens of these bins; and selects among those, bin by bin.
 #include "common.h"
@@ -20,8 +20,8 @@
 namespace mzk {
 namespace {
 
-constexpr int kBins = 512, kRest = kBins - 1;  // bins of a histogram; the last takes what is too small to count, 2^-51
-constexpr double kPerOctave = 10.0;
+constexpr int kBins = 1024, kRest = kBins - 1;  // bins of a histogram; the last takes what is too small to count, 2^-51
+constexpr double kPerOctave = 20.0;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr double kBelow = 1.0 - 0x1p-30, kAbove = 1.0 + 0x1p-30;  // slack of bounds
 constexpr int kCap = 16384;  // listed tokens of a row
@@ -35,6 +35,7 @@ enum Mode { kSample, kVerify, kBeams };
 struct Surveyed {
   int top;    // the largest bin; kNoTop: no token
   float max;  // the largest logit
+  float origin;
 };
 
 // What a row leaves for the launches behind it.
@@ -114,30 +115,57 @@ __device__ __forceinline__ double exp2_of(double t) {
   return __builtin_ldexp(e, static_cast<int>(n));
 }
 
-// 2^43 2^(r / 10) as a whole number for |r| <= 1/2: seven terms of the power series, the first left out
-// (ln 2 / 20)^8 / 8! = 5e-17; the last sum is with 2^52 more, which rounds it and leaves it in the low bits.
+// a b + c with c in scalar registers: left to itself the compiler copies c for the two-operand form.
+__device__ __forceinline__ double fma_scalar(double a, double b, double c) {
+  double d;
+  asm volatile("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));  // (kept in this order)
+  return d;
+}
+
+// 2^43 2^(r / 20) as a whole number for |r| <= 1/2, to about 2^-43.9: the power series to the sixth power, which is
+// replaced by the lower ones that come nearest, but the constant one (its Chebyshev polynomial's), 2^-48; the last
+// sum is with 2^52 more, which rounds it and leaves it in the low bits.
 constexpr int kWhole = 43;
-__device__ __forceinline__ uint64_t whole_exp2(double r) {
+template <int N>
+__device__ __forceinline__ void whole_exp2(const double (&r)[N], uint64_t (&w)[N]) {
   constexpr double c = kLn2D / kPerOctave, one = 8796093022208.0;
-  double e = one * c * c * c * c * c * c * c / 5040.0;
-  e = __builtin_fma(e, r, one * c * c * c * c * c * c / 720.0);
-  e = __builtin_fma(e, r, one * c * c * c * c * c / 120.0);
-  e = __builtin_fma(e, r, one * c * c * c * c / 24.0);
-  e = __builtin_fma(e, r, one * c * c * c / 6.0);
-  e = __builtin_fma(e, r, one * c * c / 2.0);
-  e = __builtin_fma(e, r, one * c);
-  e = __builtin_fma(e, r, one + 4503599627370496.0);
-  return static_cast<uint64_t>(__double_as_longlong(e)) & 0xfffffffffffffull;
+  // r^6 = (48 (r^4 / 4) - 18 (r^2 / 16)) / 32 nearly
+  constexpr double c6 = one * c * c * c * c * c * c / 720.0;
+  constexpr double by[6] = {one + 4503599627370496.0, one * c, one * c * c / 2.0 - c6 * 0.03515625, one * c * c * c / 6.0,
+                            one * c * c * c * c / 24.0 + c6 * 0.375, one * c * c * c * c * c / 120.0};
+  double e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) e[j] = fma_scalar(r[j], by[5], by[4]);
+#pragma unroll
+  for (int i = 3; i >= 0; --i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) e[j] = fma_scalar(e[j], r[j], by[i]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) w[j] = static_cast<uint64_t>(__double_as_longlong(e[j])) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ uint64_t whole_exp2(double r) {
+  const double x[1] = {r};
+  uint64_t w[1];
+  whole_exp2(x, w);
+  return w[0];
+}
+
+// log2 x for x >= 2^-190: the hardware's, and what it leaves, 1 + d with |d| < 2^-20, by the series.
+__device__ __forceinline__ double log2_of(double x) {
+  const double y = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(x * 0x1p64))) - 64.0;
+  const double d = x * exp2_of(-y) - 1.0;
+  return y + (d - d * d * (0.5 - d * (1.0 / 3.0))) * kLog2eD;
 }
 
 // A random number as one of [0, 1): NaN as 0.
 __device__ __forceinline__ double unit(float u) { return u > 0.0f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0; }
 
 constexpr float kBig = 3.402823466e38f;
-// A logit as it counts: NaN as -inf, +inf as the largest finite number, -0 as 0.
+// A logit as it counts: NaN as -inf, +inf as its type's largest finite number, -0 as 0.
+template <int DT>
 __device__ __forceinline__ float logit_of(float x) {
-  x = x != x ? -__builtin_huge_valf() : x + 0.0f;
-  return x > kBig ? kBig : x;
+  constexpr float big = DT == MZK_F32 ? kBig : DT == MZK_BF16 ? 0x1.fep127f : 65504.0f;
+  return x != x ? -__builtin_huge_valf() : fminf(x + 0.0f, big);
 }
 // Keys rise as logits fall.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -149,10 +177,10 @@ __device__ __forceinline__ float logit_of_key(uint32_t ik) { return __uint_as_fl
 // ---- a row's settings -------------------------------------------------------------------------
 
 struct Settings {
-  double s;    // 10 log2 e / T: bins of a logit
+  double s;    // 20 log2 e / T: bins of a logit
   int k;       // 0: none
   double p;    // 1: none
-  double f;    // 10 log2 min_p; -inf: none
+  double f;    // 20 log2 min_p; -inf: none
   bool first;  // T <= 0: the first of the order
 };
 __device__ __forceinline__ Settings settings(const SamplingParams& q, int row) {
@@ -166,7 +194,7 @@ __device__ __forceinline__ Settings settings(const SamplingParams& q, int row) {
   const float p = beams ? 1.0f : q.top_p(row);
   z.p = z.first ? 0.0 : p < 1.0f ? (p > 0.0f ? static_cast<double>(p) : 0.0) : 1.0;
   const float f = beams ? 0.0f : q.min_p(row);
-  z.f = f > 0.0f ? (f < 1.0f ? kPerOctave * log2(static_cast<double>(f)) : 0.0) : -__builtin_huge_val();
+  z.f = f > 0.0f ? (f < 1.0f ? kPerOctave * log2_of(static_cast<double>(f)) : 0.0) : -__builtin_huge_val();
   if (z.first) z.k = 0, z.f = -__builtin_huge_val();
   return z;
 }
@@ -189,7 +217,23 @@ struct Pieces {
   __device__ static float value(uint32_t bits) {
     return DT == MZK_F32 ? __uint_as_float(bits) : DT == MZK_BF16 ? bf16_to_f32(static_cast<uint16_t>(bits)) : f16_to_f32(static_cast<uint16_t>(bits));
   }
-  __device__ float operator[](int i) const { return logit_of(value(raw(i))); }
+  __device__ float operator[](int i) const { return logit_of<DT>(value(raw(i))); }
+  static constexpr float BIG = DT == MZK_F32 ? kBig : DT == MZK_BF16 ? 0x1.fep127f : 65504.0f;
+  // a piece with its type's largest finite number in the place of +inf
+  __device__ static uint4 finite(uint4 x) {
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      constexpr uint32_t inf = DT == MZK_F32 ? 0x7f800000u : DT == MZK_BF16 ? 0x7f80u : 0x7c00u;
+      if (DT == MZK_F32) {
+        w[j] -= w[j] == inf;
+      } else {
+        w[j] -= (w[j] & 0xffffu) == inf;
+        w[j] -= (w[j] >> 16) == inf ? 0x10000u : 0u;
+      }
+    }
+    return uint4{w[0], w[1], w[2], w[3]};
+  }
   __device__ uint4 load(int piece) const {  // (what lies outside the row is -inf)
     constexpr uint32_t none = DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80u : 0xfc00u;
     const int e = first(piece);
@@ -233,33 +277,60 @@ __device__ __forceinline__ bool sequence_of(const SamplingParams& q, int row, in
   return false;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+// Across the wave with data-parallel moves: steps of 1, 2, 4, 8 within 16 lanes, then the sums of the lanes before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, ROWS == 0xf));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  return static_cast<uint64_t>(moved<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 | moved<CTRL, ROWS>(static_cast<uint32_t>(v));
+}
+// The sums up to each lane.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  return static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), lane)) << 32 | lane_of(static_cast<uint32_t>(v), lane);
+}
 template <typename T>
-__device__ __forceinline__ T wave_scan(T v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
+__device__ __forceinline__ T wave_sum(T v) { return lane_of(wave_scan(v), 63); }
+// The largest of the wave (a NaN is none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float larger(float v) {
+  const int low = __float_as_int(-__builtin_huge_valf());
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = larger<0x111, 0xf>(v);
+  v = larger<0x112, 0xf>(v);
+  v = larger<0x114, 0xf>(v);
+  v = larger<0x118, 0xf>(v);
+  v = larger<0x142, 0xa>(v);
+  v = larger<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // ---- survey -------------------------------------------------------------------------------------
 
-// Where a logit lies: t = (l - origin) s, in bins; its bin is the nearest whole number k, and its weight 2^(k / 10)
-// times 2^((t - k) / 10).  A bin sums the second factors, as whole numbers of 2^43; the first is its own.
+// Where a logit lies: t = (l - origin) s, in bins; its bin is the nearest whole number k, and its weight 2^(k / 20)
+// times 2^((t - k) / 20).  A bin sums the second factors, as whole numbers of 2^43; the first is its own.
 struct Grid {
   float origin;
   double s;
   __device__ double place(float l) const { return (static_cast<double>(l) - static_cast<double>(origin)) * s; }
 };
 
-// The origin: the largest of the row's first 1024 logits, the same for all its chunks.  With equal logits all weights
-// are whole powers of two, and sums of them exact.
+// The origin: the largest of the row's first 1024 logits, the same for all its chunks.  With equal logits the
+// second factors are 1, and sums of them exact.
 template <int DT, int NT>
 __device__ __forceinline__ float origin_of(const Pieces<DT>& x, int tid, float* lds) {
   float m = -__builtin_huge_valf();
@@ -273,129 +344,174 @@ __device__ __forceinline__ float origin_of(const Pieces<DT>& x, int tid, float* 
   return m > -__builtin_huge_valf() ? m : 0.0f;
 }
 
+constexpr int kCopies = 2;     // of each bin, side by side, by the lane
+constexpr int kAhead = 4;      // pieces of a chunk's thread that are asked for at once
+constexpr int kAside = 64;     // places behind the bins for what is too small to count
 constexpr int kFar = 1 << 28;  // bins from the origin that are told apart
 
 // The bin of a maximum.
 __device__ __forceinline__ int top_of(const Grid& g, float m) {
-  return static_cast<int>(__builtin_rint(fmin(fmax(g.place(fminf(m, kBig)), -static_cast<double>(kFar)), static_cast<double>(kFar))));
+  return static_cast<int>(__builtin_rint(fmin(fmax(g.place(m), -static_cast<double>(kFar)), static_cast<double>(kFar))));
 }
 
 // Pieces from .. to - 1 of a row into the histogram (and, counting, the numbers of tokens): bin k in place k mod
 // kBins, for the kBins - 1 bins from the largest on.  As that rises, places of bins that fall behind become its.
-// Bound by the 64-bit arithmetic, 13 instructions of a quarter of the rate an element, and the LDS's atomic sums, in two
-// copies by the lane's parity, so that fewer lanes meet; the next pieces are in flight meanwhile.
-template <int DT, int NT>
+// Bound by the LDS's atomic sums and the arithmetic, some 22 instructions an element; the next pieces are in flight meanwhile.
+template <int DT, int NT, int AHEAD>
 __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, bool counting, int from, int to, int tid,
-                                           unsigned long long* hist /* [2][kBins] */, uint32_t* counts /* [kBins] */, int* tops /* [2] */,
-                                           float* lds /* [NT / 64] */) {
+                                           unsigned long long* hist /* [kBins][kCopies], and kAside */, uint32_t* counts /* the same */,
+                                           int* tops /* [2] */, float* lds /* [NT / 64] */) {
   using P = Pieces<DT>;
-  constexpr int PER = 16 / P::N;  // pieces of a thread at a time: 16 elements
-  for (int i = tid; i < 2 * kBins; i += NT) hist[i] = 0;
+  constexpr int PER = AHEAD, ELEMENTS = PER * P::N;
+  for (int i = tid; i < kCopies * kBins; i += NT) hist[i] = 0;
   if (counting)
-    for (int i = tid; i < kBins; i += NT) counts[i] = 0;
+    for (int i = tid; i < kCopies * kBins; i += NT) counts[i] = 0;
   if (tid < 2) tops[tid] = kNoTop;
   uint4 next[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) next[i] = from + i * NT + tid < to ? x.load(from + i * NT + tid) : P::none();
-  float max_all = -__builtin_huge_valf();
+  float known = -__builtin_huge_valf();  // a maximum of this wave's that the others have heard of
   int top = kNoTop, turn = 0;
-  unsigned long long* const mine = hist + (tid & 1) * kBins;
+  // offsets in bytes: the copy's, and a place's that nobody reads
+  const int copy = 8 * (tid & (kCopies - 1)), aside = 8 * (kCopies * kBins + (tid & 63));
   __syncthreads();
   for (int at = from; at < to; at += PER * NT) {
-    float v[16];
+    uint4 now[PER];
     float m = -__builtin_huge_valf();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      v[i] = P::at(next[i / P::N], i % P::N);
-      m = fmaxf(m, v[i]);
+    for (int i = 0; i < PER; ++i) {
+      now[i] = next[i];
+#pragma unroll
+      for (int j = 0; j < P::N; ++j) m = fmaxf(m, P::at(now[i], j));
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int piece = at + (PER + i) * NT + tid;
       if (at + PER * NT < to) next[i] = piece < to ? x.load(piece) : P::none();
     }
-    m = wave_max(m);
-    max_all = fmaxf(max_all, m);
-    if ((tid & 63) == 0 && m > -__builtin_huge_valf())
-      atomicMax(&tops[turn], top_of(g, m));
+    if (__ballot(m > known)) {
+      known = wave_max(m);
+      if ((tid & 63) == 0) atomicMax(&tops[turn], top_of(g, logit_of<DT>(known)));
+    }
     __syncthreads();
-    const int now = max(top, tops[turn]);
+    const int risen = max(top, tops[turn]);
     turn ^= 1;
-    if (now > top) {  // uniform
+    if (risen > top) {  // uniform
       if (top > kNoTop) {
-        const int n = now - top < kBins ? now - top : kBins;
-        for (int i = tid; i < n; i += NT) {
-          const int j = (now - i) & kRest;
-          hist[j] = hist[kBins + j] = 0;
+        const int n = risen - top < kBins ? risen - top : kBins;
+        for (int i = tid; i < n * kCopies; i += NT) {
+          const int j = ((risen - i / kCopies) & kRest) * kCopies + i % kCopies;
+          hist[j] = 0;
           if (counting) counts[j] = 0;
         }
         __syncthreads();
       }
-      top = now;
+      top = risen;
+    }
+    if (__ballot(m > P::BIG)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) now[i] = P::finite(now[i]);
     }
     const double bottom = static_cast<double>(top - kRest);  // bins above it are kept
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const double t = g.place(fminf(v[i], kBig));
-      const double n = __builtin_rint(t);
-      if (n > bottom && v[i] > -__builtin_huge_valf()) {  // (not a NaN)
-        const int k = static_cast<int>(fmin(n, static_cast<double>(kFar))) & kRest;
-        atomicAdd(&mine[k], static_cast<unsigned long long>(whole_exp2(t - n)));
-        if (counting) atomicAdd(&counts[k], 1u);
+    for (int i = 0; i < ELEMENTS; i += 4) {  // (four at a time, so that the steps of one wait for nothing)
+      double t[4];
+      uint64_t w[4];
+      int k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = g.place(P::at(now[(i + j) / P::N], (i + j) % P::N));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // the nearest whole number: the low bits of the sum with 3 2^51
+        const double sum = t[j] + 0x1.8p52, n = sum - 0x1.8p52;
+        k[j] = (static_cast<int>(__double_as_longlong(sum)) * (8 * kCopies) & 8 * kCopies * kRest) | copy;
+        k[j] = n > bottom ? k[j] : aside;  // (not of a NaN, nor of -inf)
+        t[j] = t[j] - n;
+      }
+      whole_exp2(t, w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) atomicAdd(reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(hist) + k[j]), static_cast<unsigned long long>(w[j]));
+      if (counting) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) atomicAdd(&counts[k[j] >> 3], 1u);
       }
     }
   }
+  float max_all = known;
   if ((tid & 63) == 0) lds[tid >> 6] = max_all;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) max_all = fmaxf(max_all, lds[w]);
-  return Surveyed{top, logit_of(max_all)};
+  return Surveyed{top, logit_of<DT>(max_all), g.origin};
+}
+
+// Bin j from the largest down.
+__device__ __forceinline__ void surveyed_bin(const Surveyed& r, int j, bool counting, const unsigned long long* hist, const uint32_t* counts,
+                                             uint64_t& sum, uint32_t& num) {
+  sum = 0;
+  num = 0;
+  if (j >= kRest) return;
+  const int i = ((r.top - j) & kRest) * kCopies;
+#pragma unroll
+  for (int c = 0; c < kCopies; ++c) sum += hist[i + c];
+  if (counting)
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) num += counts[i + c];
 }
 
 template <int DT>
 __global__ void __launch_bounds__(256) survey_kernel(const SamplingParams q) {
-  __shared__ unsigned long long hist[2 * kBins];
-  __shared__ uint32_t counts[kBins];
+  __shared__ unsigned long long hist[kCopies * kBins + kAside];
+  __shared__ uint32_t counts[kCopies * kBins + kAside];
   __shared__ float lds[4];
   __shared__ int tops[2];
   const int tid = threadIdx.x;
-  const int row = blockIdx.x / q.chunks, chunk = blockIdx.x - row * q.chunks;
-  if (q.mode == kVerify && q.cu[q.B] <= row) return;  // a row of no sequence
+  // workgroups go to the 8 XCDs in turn: a row's chunks to the one that its own workgroup reads it from again
+  const int of8 = blockIdx.x >> 3, row = of8 / q.chunks * 8 + (blockIdx.x & 7), chunk = of8 % q.chunks;
+  if (row >= q.rows || (q.mode == kVerify && q.cu[q.B] <= row)) return;  // (a row of no sequence)
   const Pieces<DT> x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
   const bool counting = z.k > 0;
   const Grid g{origin_of<DT, 256>(x, tid, lds), z.s};
   const int from = chunk * q.chunk_pieces, all = x.count(), to = from + q.chunk_pieces < all ? from + q.chunk_pieces : all;
-  const Surveyed r = survey<DT, 256>(x, g, counting, from, to, tid, hist, counts, tops, lds);
+  const Surveyed r = survey<DT, 256, kAhead>(x, g, counting, from, to, tid, hist, counts, tops, lds);
   const int64_t at = static_cast<int64_t>(row) * q.chunks + chunk;
   if (tid == 0) q.heads[at] = r;
   if (r.top == kNoTop) return;  // uniform
   for (int j = tid; j < kBins; j += 256) {
-    const int i = (r.top - j) & kRest;
-    q.hist[at * kBins + j] = j < kRest ? hist[i] + hist[kBins + i] : 0;
-    if (counting) q.counts[at * kBins + j] = j < kRest ? counts[i] : 0;
+    uint64_t sum;
+    uint32_t num;
+    surveyed_bin(r, j, counting, hist, counts, sum, num);
+    q.hist[at * kBins + j] = sum;
+    if (counting) q.counts[at * kBins + j] = num;
   }
 }
 
 // ---- a row --------------------------------------------------------------------------------------
 
-constexpr int kRowThreads = 1024;
+constexpr int kRowThreads = kBins / 2;
+constexpr int kMostChunks = 64;
+constexpr int kDigits = 1024;  // of a selection's step
 
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q) {
   constexpr int NT = kRowThreads, NW = NT / 64;
+  constexpr int KS = DT == MZK_F32 ? 0 : DT == MZK_BF16 ? 16 : 13;  // low bits of a key that are all the same
   using P = Pieces<DT>;
   extern __shared__ __align__(16) uint8_t smem[];
   uint2* const list = reinterpret_cast<uint2*>(smem);  // [kCap] key; index, and the bin above bit 20
-  __shared__ unsigned long long hist[1024];            // (survey: two copies of the bins)
-  __shared__ uint32_t counts[kBins];
+  // (the survey's bins are there before the list is)
+  unsigned long long* const bins = reinterpret_cast<unsigned long long*>(smem);
+  uint32_t* const bin_counts = reinterpret_cast<uint32_t*>(smem + 8 * (kCopies * kBins + kAside));
+  __shared__ unsigned long long hist[kDigits];
+  __shared__ uint32_t counts[kDigits];
   __shared__ uint64_t cw[kBins];  // running sums of the bins' weights
   __shared__ uint32_t cn[kBins];  // and of their tokens
-  __shared__ uint64_t part[NW], ext[4], sel[4];
+  __shared__ uint64_t part[NW], sel[4], last_ones[64][2];
   __shared__ uint32_t partn[NW], number[2];
   __shared__ int found[2][2][NW];
   __shared__ float lds[NW];
-  __shared__ int tops[2];
+  __shared__ int tops[kMostChunks];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   int b = 0, end = 0;
   if (q.mode == kVerify && !sequence_of(q, row, lane, b, end)) return;  // uniform
@@ -403,46 +519,60 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   const Settings z = settings(q, row);
   const bool counting = z.k > 0;
 
-  // ---- the row's histogram: bin j, from the largest down, is thread j's ----
-  Grid g{origin_of<DT, NT>(x, tid, lds), z.s};
-  uint64_t sum = 0;  // of the second factors
-  uint32_t num = 0;
-  Surveyed r{kNoTop, -__builtin_huge_valf()};
+  // ---- the row's histogram: bins 2 tid, 2 tid + 1, from the largest down, are this thread's ----
+  Grid g{q.chunks == 1 ? origin_of<DT, NT>(x, tid, lds) : q.heads[static_cast<int64_t>(row) * q.chunks].origin, z.s};
+  uint64_t sum[2] = {0, 0};  // of the second factors
+  uint32_t num[2] = {0, 0};
+  Surveyed r{kNoTop, -__builtin_huge_valf(), 0.0f};
   for (bool whole_row = q.chunks == 1;; whole_row = true) {
     if (whole_row) {
-      r = survey<DT, NT>(x, g, counting, 0, x.count(), tid, hist, counts, tops, lds);
-      if (tid < kRest && r.top > kNoTop) {
-        const int i = (r.top - tid) & kRest;
-        sum = hist[i] + hist[kBins + i];
-        num = counting ? counts[i] : 0;
+      r = survey<DT, NT, 8>(x, g, counting, 0, x.count(), tid, bins, bin_counts, tops, lds);
+      if (r.top > kNoTop) {
+        surveyed_bin(r, 2 * tid, counting, bins, bin_counts, sum[0], num[0]);
+        surveyed_bin(r, 2 * tid + 1, counting, bins, bin_counts, sum[1], num[1]);
       }
     } else {
-      const Surveyed* const heads = q.heads + static_cast<int64_t>(row) * q.chunks;
-      for (int c = 0; c < q.chunks; ++c) {
-        const Surveyed h = heads[c];
-        r.top = max(r.top, h.top);
-        r.max = fmaxf(r.max, h.max);
-      }
-      if (tid < kRest) {
-        const uint64_t* const h = q.hist + static_cast<int64_t>(row) * q.chunks * kBins;
-        const uint32_t* const n = q.counts + static_cast<int64_t>(row) * q.chunks * kBins;
-#pragma unroll 4
-        for (int c = 0; c < q.chunks; ++c) {
-          const int top = heads[c].top;
-          const uint32_t j = static_cast<uint32_t>(tid) - (static_cast<uint32_t>(r.top) - static_cast<uint32_t>(top));
-          if (top > kNoTop && r.top - top <= tid) {
-            sum += h[static_cast<int64_t>(c) * kBins + j];
-            if (counting) num += n[static_cast<int64_t>(c) * kBins + j];
+      const Surveyed h = lane < q.chunks ? q.heads[static_cast<int64_t>(row) * q.chunks + lane] : Surveyed{kNoTop, -__builtin_huge_valf(), 0.0f};
+      r = h;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) r.top = max(r.top, __shfl_xor(r.top, d, 64));
+      r.max = wave_max(r.max);
+      if (wave == 0) tops[lane] = h.top;
+      __syncthreads();
+      const uint64_t* const hs = q.hist + static_cast<int64_t>(row) * q.chunks * kBins;
+      const uint32_t* const ns = q.counts + static_cast<int64_t>(row) * q.chunks * kBins;
+      constexpr int AT_ONCE = 8;  // (unconditional loads: bins that a chunk lacks are fetched as its last)
+      for (int c0 = 0; c0 < q.chunks; c0 += AT_ONCE) {
+        uint64_t h8[AT_ONCE][2];
+        uint32_t n8[AT_ONCE][2];
+        bool some[AT_ONCE][2];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int c = min(c0 + i, q.chunks - 1), t = tops[c];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            some[i][e] = c0 + i < q.chunks && t > kNoTop && r.top - t <= 2 * tid + e;
+            const int at = c * kBins + (some[i][e] ? 2 * tid + e - (r.top - t) : kRest);
+            h8[i][e] = hs[at];
+            n8[i][e] = counting ? ns[at] : 0;
           }
         }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sum[e] += some[i][e] ? h8[i][e] : 0;
+            num[e] += some[i][e] ? n8[i][e] : 0;
+          }
       }
+      if (tid == NT - 1) sum[1] = 0, num[1] = 0;  // kRest
     }
     if (whole_row && g.origin == r.max) break;
     // far from the origin bins are not told apart: once more, from the largest logit
     if (r.max == -__builtin_huge_valf() || (r.top < kFar / 2 && r.top > -kFar / 2)) break;
     g.origin = r.max;
-    sum = 0;
-    num = 0;
+    sum[0] = sum[1] = 0;
+    num[0] = num[1] = 0;
     __syncthreads();
   }
   if (r.max == -__builtin_huge_valf()) {  // uniform: no token
@@ -455,25 +585,28 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   }
   // ---- running sums, as whole numbers: a bin of nothing adds nothing ----
   // a unit of a bin's sum, in units of 2^-scale of the weight at the largest bin's middle
-  auto unit_of = [&](int j) -> double { return exp2_of(static_cast<double>(-j) / kPerOctave) * __builtin_ldexp(1.0, q.scale - kWhole); };
-  const double my_unit = unit_of(tid);
-  uint64_t my_w = static_cast<uint64_t>(static_cast<double>(sum) * my_unit + 0.5);
-  if (tid < kBins) {
-    const uint64_t s = wave_scan(my_w, lane);
-    const uint32_t n = wave_scan(num, lane);
-    if (lane == 63) part[wave] = s, partn[wave] = n;
-    cw[tid] = s;
-    cn[tid] = n;
-  }
-  __syncthreads();
-  uint64_t my_cw = ~0ull;
-  uint32_t my_cn = kNone;
-  if (tid < kBins) {
-    my_cw = cw[tid];
-    my_cn = cn[tid];
-    for (int w = 0; w < wave; ++w) my_cw += part[w], my_cn += partn[w];
-    cw[tid] = my_cw;
-    cn[tid] = my_cn;
+  auto unit_of = [&](int j) __attribute__((always_inline)) -> double {
+    return exp2_of(static_cast<double>(-j) / kPerOctave) * __builtin_ldexp(1.0, q.scale - kWhole);
+  };
+  const double my_unit[2] = {unit_of(2 * tid), unit_of(2 * tid + 1)};
+  const uint64_t my_w0 = static_cast<uint64_t>(static_cast<double>(sum[0]) * my_unit[0] + 0.5);
+  const uint64_t my_w1 = static_cast<uint64_t>(static_cast<double>(sum[1]) * my_unit[1] + 0.5);
+  double my_upto[2];
+  uint32_t my_cn[2];
+  {
+    uint64_t w = wave_scan(my_w0 + my_w1);
+    uint32_t m = wave_scan(num[0] + num[1]);
+    if (lane == 63) part[wave] = w, partn[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+      if (i < wave) w += part[i], m += partn[i];
+    cw[2 * tid] = w - my_w1;
+    cw[2 * tid + 1] = w;
+    cn[2 * tid] = my_cn[0] = m - num[1];
+    cn[2 * tid + 1] = my_cn[1] = m;
+    my_upto[0] = static_cast<double>(w - my_w1);
+    my_upto[1] = static_cast<double>(w);
   }
   __syncthreads();
   const double total = static_cast<double>(cw[kRest]);
@@ -481,14 +614,16 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   auto before = [&](int j) -> double { return j > 0 ? static_cast<double>(cw[j - 1]) : 0.0; };
   int round = 0;
   // the numbers of bins of which a and c hold: the first of which they do not, if they hold for all before it
-  auto find = [&](bool a, bool c, int& na, int& nc) {
-    const int pa = __popcll(__ballot(tid < kBins && a)), pc = __popcll(__ballot(tid < kBins && c));
-    if (lane == 0) found[round & 1][0][wave] = pa, found[round & 1][1][wave] = pc;
+  auto find = [&](auto a, auto c, int& na, int& nc) __attribute__((always_inline)) {
+    const int pa = __popcll(__ballot(a(0))) + __popcll(__ballot(a(1))), pc = __popcll(__ballot(c(0))) + __popcll(__ballot(c(1)));
+    if (lane == 0) found[round][0][wave] = pa, found[round][1][wave] = pc;
     __syncthreads();
     na = nc = 0;
 #pragma unroll
-    for (int w = 0; w < kBins / 64; ++w) na += found[round & 1][0][w], nc += found[round & 1][1][w];
-    ++round;
+    for (int w = 0; w < NW; ++w) na += found[round][0][w], nc += found[round][1][w];
+    na = __builtin_amdgcn_readfirstlane(na);
+    nc = __builtin_amdgcn_readfirstlane(nc);
+    round ^= 1;
   };
   auto in_bin = [&](float l) -> int {  // its bin from the largest down; kRest: too small to count
     const double n = __builtin_rint(g.place(l));
@@ -497,34 +632,42 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   auto reaches = [&](float l) -> bool { return (static_cast<double>(l) - static_cast<double>(r.max)) * z.s >= z.f; };
   // the logarithm of a sum of weights, of the largest token's
   auto log_of = [&](double w) -> double {
-    return log(w * __builtin_ldexp(1.0, -q.scale)) + (static_cast<double>(r.top) - g.place(r.max)) * (kLn2D / kPerOctave);
+    return (log2_of(w * __builtin_ldexp(1.0, -q.scale)) + (static_cast<double>(r.top) - g.place(r.max)) / kPerOctave) * kLn2D;
   };
   auto second = [&](float l) -> uint64_t {
     const double t = g.place(l);
     return whole_exp2(t - __builtin_rint(t));
   };
+  // a token's place in the order
+  auto order_of = [&](uint32_t key, uint32_t idx) -> uint64_t { return static_cast<uint64_t>(key >> KS) << 20 | idx; };
+  // the logits of bins b0 .. b1, a little more
+  auto logits_of = [&](int b0, int b1, float& from, float& to) {
+    const double top = static_cast<double>(r.top), o = static_cast<double>(g.origin);
+    const float a = static_cast<float>(o + (top - b1 - 0.5) / z.s), c = static_cast<float>(o + (top - b0 + 0.5) / z.s);
+    from = b1 >= kRest ? -kBig : fmaxf(a - fabsf(a) * 0x1p-20f - 1e-37f, -kBig);
+    to = b0 == 0 ? __builtin_huge_valf() : fminf(c + fabsf(c) * 0x1p-20f + 1e-37f, kBig);
+  };
 
   // ---- a drafted token that its row judges ----
   uint32_t drafted = kNone, drafted_key = 0;
   int drafted_bin = kBins;
-  uint64_t drafted_sum = 0;  // its second factor
+  double drafted_w = 0.0;  // what it adds to the running sums, if it leaves the row once refused
   if (q.mode == kVerify && row + 1 < end) {
     const int64_t d = q.tokens[row + 1];
     if (d >= 0 && d < q.V) {
       const float l = x[static_cast<int>(d)];
-      if (l > -__builtin_huge_valf() && in_bin(l) < kRest) {
+      if (l > -__builtin_huge_valf()) {
         drafted = static_cast<uint32_t>(d);
         drafted_key = key_of(l);
         drafted_bin = in_bin(l);
-        drafted_sum = second(l);
       }
     }
   }
-  const bool leaves = drafted != kNone && !q.probs;  // refused, it leaves the row
-  // what it adds to the running sums
-  double drafted_w = 0.0;
-  if (leaves) {
-    if (tid == drafted_bin) sel[0] = my_w - static_cast<uint64_t>(static_cast<double>(sum - drafted_sum) * my_unit + 0.5);
+  const bool leaves = drafted_bin < kRest && !q.probs;
+  if (leaves) {  // uniform
+    const int e = drafted_bin & 1;
+    if (tid == drafted_bin >> 1)
+      sel[0] = (e ? my_w1 : my_w0) - static_cast<uint64_t>(static_cast<double>(sum[e] - second(logit_of_key(drafted_key))) * my_unit[e] + 0.5);
     __syncthreads();
     drafted_w = static_cast<double>(sel[0]);
   }
@@ -536,7 +679,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   int last;
   {
     int kb;
-    find(my_cn < static_cast<uint32_t>(z.k), static_cast<double>(my_cw) < total, kb, last);
+    find([&](int e) { return my_cn[e] < static_cast<uint32_t>(z.k); }, [&](int e) { return my_upto[e] < total; }, kb, last);
     double least = total, most = total;
     if (counting && kb < kRest) {
       w0[0] = w1[0] = kb;
@@ -550,10 +693,10 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     } else {
       if (z.p < 1.0) {
         const double a = z.p * least * kBelow, c = z.p * most * kAbove;
-        find(static_cast<double>(my_cw) < a, static_cast<double>(my_cw) < c, w0[1], w1[1]);
+        find([&](int e) { return my_upto[e] < a; }, [&](int e) { return my_upto[e] < c; }, w0[1], w1[1]);
         w1[1] = min(w1[1], last);
         w0[1] = min(w0[1], w1[1]);
-        // a token of bin j weighs less than 2^((1 - j) / 10)
+        // a token of bin j weighs less than 2^((1 - j) / 20)
         const double one = exp2_of(static_cast<double>(1 - w0[1]) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
         least = a;
         most = fmin(upto(w1[1]), c + one);
@@ -580,38 +723,55 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         sure = drafted_bin < open || drafted_bin > cut;
       }
       const double a = u * fmax(least - gone, 0.0) * kBelow, c = u * (sure ? most - gone : most) * kAbove;
-      const double w = static_cast<double>(my_cw), without = tid >= drafted_bin ? w - gone : w;
-      find((sure ? without : w) <= a, without <= c, w0[3], w1[3]);
+      auto without = [&](int e) { return 2 * tid + e >= drafted_bin ? my_upto[e] - gone : my_upto[e]; };
+      find([&](int e) { return (sure ? without(e) : my_upto[e]) <= a; }, [&](int e) { return without(e) <= c; }, w0[3], w1[3]);
       w1[3] = min(w1[3], kRest - 1);
       w0[3] = min(w0[3], w1[3]);
     }
   }
 
   // ---- the cuts and the token ----
-  bool in_list = false, relist = false;
+  // whether the windows' tokens fit the list: a second factor is 1, nearly
+  bool in_list = false, relist;
+  {
+    uint64_t many = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      bool in = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) in = in || (2 * tid + e >= w0[i] && 2 * tid + e <= w1[i]);
+      many += in ? sum[e] >> kWhole : 0;
+    }
+    many = wave_sum(many);
+    if (lane == 0) part[wave] = many;
+    __syncthreads();
+    many = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) many += part[w];
+    relist = many > static_cast<uint64_t>(kCap - kCap / 16);
+  }
   int n = 0;
-  uint64_t cut = ~0ull;  // key and index of the last token that top-k and top-p keep
+  uint64_t cut = ~0ull;  // the last token that top-k and top-p keep
   double kept = total;
   uint32_t skip = kNone, token = kNone;
   bool accepted = false;
-  double logprob = 0.0;
+  float drawn = 0.0f;  // the token's logit
 #pragma unroll 1
   for (int step = -1; step < 4; ++step) {
-    double target = 0.0;
     int b0 = w0[3], b1 = w1[3];
     if (step == 0) b0 = w0[0], b1 = w1[0];
     if (step == 1) b0 = w0[1], b1 = w1[1];
     if (step == 2) b0 = w0[2], b1 = w1[2];
-    double start = 0.0;  // what lies before the bin
+    double target = 0.0, start = 0.0;  // what is looked for, what lies before the bin
     if (step >= 0) {
       if (b1 < b0) continue;  // uniform
       if (step == 1) target = z.p * kept;
       if (step == 3) {
         double left = kept;
         if (drafted != kNone) {
-          const uint64_t me = static_cast<uint64_t>(drafted_key) << 20 | drafted;
-          if (me <= cut && reaches(logit_of_key(drafted_key))) {
-            const double w = static_cast<double>(drafted_sum) * unit_of(drafted_bin);
+          const float l = logit_of_key(drafted_key);
+          if (order_of(drafted_key, drafted) <= cut && reaches(l)) {
+            const double w = exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
             const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + drafted]) : 1.0;
             accepted = static_cast<double>(q.u[row]) * sure * kept < w;
             // (what leaves less than 2^12 units is not refused: u is at most 1 - 2^-24)
@@ -625,100 +785,126 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
       }
       if (step == 1 || step == 3) {
         // the bin: the first whose running sum reaches the target, or for the token exceeds it
-        const double w = static_cast<double>(my_cw), gone = skip != kNone && tid >= drafted_bin ? drafted_w : 0.0;
+        const double gone = skip != kNone ? drafted_w : 0.0;
+        auto w = [&](int e) { return 2 * tid + e >= drafted_bin ? my_upto[e] - gone : my_upto[e]; };
         int at, end_at;
-        const double whole_w = total - (skip != kNone ? drafted_w : 0.0);
-        find(step == 3 ? w - gone <= target : w < target, w - gone < whole_w, at, end_at);
+        find([&](int e) { return step == 3 ? w(e) <= target : w(e) < target; }, [&](int e) { return w(e) < total - gone; }, at, end_at);
         at = min(at, end_at);
         b0 = b1 = min(max(at, b0), b1);
-        start = before(b0) - (skip != kNone && b0 > drafted_bin ? drafted_w : 0.0);
+        start = before(b0) - (b0 > drafted_bin ? gone : 0.0);
       }
     }
     // ---- the tokens of the bins: all windows' at once, or, where those are too many, the bin's ----
+    if (step < 0 && relist) continue;
     if (step < 0 || relist) {
       __syncthreads();
       if (tid == 0) number[0] = 0;
       __syncthreads();
-      // two ranges of bins, the cuts' and the token's, as ranges of logits a little wider
-      int h[2][2] = {{b0, b1}, {1, 0}};
-      if (step < 0) {
-        h[0][0] = min(min(w1[0] < w0[0] ? kBins : w0[0], w1[1] < w0[1] ? kBins : w0[1]), w1[2] < w0[2] ? kBins : w0[2]);
-        h[0][1] = max(max(w1[0], w1[1]), w1[2]);
-        h[1][0] = w0[3];
-        h[1][1] = w1[3];
-      }
+      // two ranges of bins: the cuts' and the token's
+      int h0 = b0, h1 = b1;
       float from[2], to[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const double top = static_cast<double>(r.top), o = static_cast<double>(g.origin);
-        const float a = static_cast<float>(o + (top - h[i][1] - 0.5) / z.s), c = static_cast<float>(o + (top - h[i][0] + 0.5) / z.s);
-        from[i] = h[i][1] >= kRest ? -kBig : a - fabsf(a) * 0x1p-20f - 1e-37f;
-        to[i] = c + fabsf(c) * 0x1p-20f + 1e-37f;
-        if (h[i][1] < h[i][0]) from[i] = __builtin_huge_valf(), to[i] = -from[i];
-        from[i] = fmaxf(from[i], -kBig);
+      if (step < 0) {
+        logits_of(w0[3], w1[3], from[1], to[1]);
+        h0 = min(min(w1[0] < w0[0] ? kBins : w0[0], w1[1] < w0[1] ? kBins : w0[1]), w1[2] < w0[2] ? kBins : w0[2]);
+        h1 = max(max(w1[0], w1[1]), w1[2]);
       }
+      logits_of(h0, h1, from[0], to[0]);
+      if (h1 < h0) from[0] = __builtin_huge_valf();
+      if (step >= 0 || w1[3] < w0[3]) from[1] = __builtin_huge_valf(), to[1] = 0.0f;
       const int pieces = x.count();
-      constexpr int AHEAD = 4;
+      constexpr int AHEAD = 32 / P::N;  // 32 elements a thread
+      uint4 next[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) next[a] = a * NT + tid < pieces ? x.load(a * NT + tid) : P::none();
       for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
         uint4 v[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) v[a] = p0 + a * NT + tid < pieces ? x.load(p0 + a * NT + tid) : P::none();
+        for (int a = 0; a < AHEAD; ++a) {
+          v[a] = next[a];
+          const int piece = p0 + (AHEAD + a) * NT + tid;
+          if (p0 + AHEAD * NT < pieces) next[a] = piece < pieces ? x.load(piece) : P::none();
+        }
         uint32_t mine = 0;
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
 #pragma unroll
           for (int i = 0; i < P::N; ++i) {
-            const float l = fminf(P::at(v[a], i), kBig), was = P::at(v[a], i);
-            const bool in = ((l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1])) && was == was;
+            const float l = P::at(v[a], i);  // (a NaN is in no range)
+            const bool in = (l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1]);
             mine |= static_cast<uint32_t>(in) << (a * P::N + i);
           }
         if (__ballot(mine != 0) == 0) continue;
-        const uint32_t many = __popc(mine), s = wave_scan(many, lane);
+        const uint32_t many = __popc(mine), s = wave_scan(many);
         uint32_t at = 0;
         if (lane == 63) at = atomicAdd(&number[0], s);
-        at = static_cast<uint32_t>(__shfl(static_cast<int>(at), 63, 64)) + s - many;
+        at = lane_of(at, 63) + s - many;
         while (mine) {
           const int i = __builtin_ctz(mine);
           mine &= mine - 1;
-          const int idx = x.first(p0 + i / P::N * NT + tid) + i % P::N;
-          const float l = x[idx];
-          if (at < kCap) list[at] = uint2{key_of(l), static_cast<uint32_t>(idx) | static_cast<uint32_t>(in_bin(l)) << 20};
+          if (at < kCap) list[at].y = static_cast<uint32_t>(x.first(p0 + i / P::N * NT + tid) + i % P::N);
           ++at;
         }
       }
       __syncthreads();
-      n = static_cast<int>(min(number[0], static_cast<uint32_t>(kCap)));
       in_list = number[0] <= kCap;
+      n = in_list ? static_cast<int>(number[0]) : 0;
+#pragma unroll 4
+      for (int i = tid; i < n; i += NT) {  // (each thread comes back to its own)
+        const uint32_t idx = list[i].y;
+        const float l = x[static_cast<int>(idx)];
+        list[i] = uint2{key_of(l), idx | static_cast<uint32_t>(in_bin(l)) << 20};
+      }
       if (step < 0) {
         relist = !in_list;
         continue;
       }
     }
-    // f(key and index, logit) for the tokens of bins b0 .. b1 with keys and indices lo .. hi
+    // f(place in the order, logit) for the tokens of bins b0 .. b1 between lo and hi
     auto each = [&](uint64_t lo, uint64_t hi, auto f) __attribute__((always_inline)) {
       if (in_list) {
         for (int i = tid; i < n; i += NT) {
           const uint2 e = list[i];
           const int j = static_cast<int>(e.y >> 20);
           const uint32_t idx = e.y & 0xfffffu;
-          const uint64_t me = static_cast<uint64_t>(e.x) << 20 | idx;
+          const uint64_t me = order_of(e.x, idx);
           if (j >= b0 && j <= b1 && me >= lo && me <= hi && idx != skip) f(me, logit_of_key(e.x));
         }
       } else {
         for (int i = tid; i < x.V; i += NT) {
           const float l = x[i];
           const int j = in_bin(l);
-          const uint64_t me = static_cast<uint64_t>(key_of(l)) << 20 | static_cast<uint32_t>(i);
+          const uint64_t me = order_of(key_of(l), static_cast<uint32_t>(i));
           if (j >= b0 && j <= b1 && l > -__builtin_huge_valf() && me >= lo && me <= hi && static_cast<uint32_t>(i) != skip) f(me, l);
         }
       }
     };
-    uint64_t lo = 0, hi = ~0ull;
-    const bool by_count = step == 0;
     const double u_bin = unit_of(b0);
-    if (step != 2) {
-      // ---- the token at which the running sum reaches `need` ----
-      uint64_t need;
+    if (step == 2) {
+      // ---- the weights of those that reach min-p ----
+      __syncthreads();
+      if (tid == 0) sel[2] = 0;
+      __syncthreads();
+      uint64_t mine = 0;
+      each(0, ~0ull, [&](uint64_t, float l) {
+        if (!reaches(l)) return;
+        const uint64_t w = second(l);
+        const int j = in_bin(l);
+        mine += j == b0 ? w : static_cast<uint64_t>(static_cast<double>(w) * exp2_of(static_cast<double>(b0 - j) / kPerOctave));
+      });
+      mine = wave_sum(mine);
+      if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&sel[2]), static_cast<unsigned long long>(mine));
+      __syncthreads();
+      kept = fmin(kept, before(b0) + static_cast<double>(sel[2]) * u_bin);
+      continue;
+    }
+    // ---- the token at which the running sum, of ones or of weights, reaches `need` ----
+    const bool by_count = step == 0;
+    uint64_t lo, hi, need;
+    {
+      float from, to;
+      logits_of(b0, b1, from, to);
+      lo = order_of(key_of(fminf(to, kBig) + 0.0f), 0);
+      hi = order_of(key_of(from + 0.0f), 0xfffffu);
       if (by_count) {
         need = static_cast<uint64_t>(z.k) - (b0 > 0 ? cn[b0 - 1] : 0u);
       } else {
@@ -726,106 +912,77 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         need = step == 3 ? static_cast<uint64_t>(y) + 1 : static_cast<uint64_t>(__builtin_ceil(y));
       }
       if (need < 1) need = 1;
-      uint64_t passed = 0;
-      while (true) {
-        // how many are left, and between which keys and indices
-        __syncthreads();
-        if (tid == 0) ext[0] = ~0ull, ext[1] = 0, number[0] = 0, number[1] = 0;
-        hist[tid] = 0;
-        __syncthreads();
-        uint64_t a = ~0ull, c = 0;
-        uint32_t m = 0;
-        each(lo, hi, [&](uint64_t me, float) {
-          a = me < a ? me : a;
-          c = me > c ? me : c;
-          ++m;
-        });
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
-          const uint64_t a2 = __shfl_xor(a, d, 64), c2 = __shfl_xor(c, d, 64);
-          a = a2 < a ? a2 : a;
-          c = c2 > c ? c2 : c;
-          m += __shfl_xor(m, d, 64);
-        }
-        if (lane == 0 && m) {
-          atomicMin(reinterpret_cast<unsigned long long*>(&ext[0]), a);
-          atomicMax(reinterpret_cast<unsigned long long*>(&ext[1]), c);
-          atomicAdd(&number[0], m);
-        }
-        __syncthreads();
-        const uint32_t left = number[0];
-        lo = ext[0];
-        hi = ext[1];
-        if (left <= 64) break;  // uniform
-        const uint64_t span = hi - lo;
-        const int bits = 64 - __builtin_clzll(span), sh = bits > 10 ? bits - 10 : 0;
-        each(lo, hi, [&](uint64_t me, float l) { atomicAdd(&hist[(me - lo) >> sh], by_count ? 1ull : static_cast<unsigned long long>(second(l))); });
-        __syncthreads();
-        const uint64_t v = hist[tid];
-        const uint64_t s = wave_scan(v, lane);
-        if (lane == 63) part[wave] = s;
-        __syncthreads();
-        uint64_t before_me = passed, all = passed;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const uint64_t p = part[w];
-          if (w < wave) before_me += p;
-          all += p;
-        }
-        if (need > all) need = all;
-        if (before_me + s - v < need && need <= before_me + s) sel[0] = tid, sel[1] = before_me + s - v;
-        __syncthreads();
-        lo = lo + (sel[0] << sh);
-        const uint64_t top = lo + ((1ull << sh) - 1ull);
-        hi = top < hi ? top : hi;
-        passed = sel[1];
-      }
-      // ---- at most 64: gathered, and one wave sums them in their order ----
+    }
+    uint64_t passed = 0;  // weights and numbers before lo
+    uint32_t passed_n = 0;
+    while (true) {
+      const int bits = 64 - __builtin_clzll(hi - lo | 1), sh = bits > 10 ? bits - 10 : 0;
+      __syncthreads();
+      hist[tid] = hist[NT + tid] = 0;
+      counts[tid] = counts[NT + tid] = 0;
+      if (tid == 0) sel[0] = 0, sel[1] = passed, sel[2] = passed_n, number[1] = 0;
+      __syncthreads();
       each(lo, hi, [&](uint64_t me, float l) {
-        const uint32_t to = atomicAdd(&number[1], 1u);
-        hist[2 * to] = me;
-        hist[2 * to + 1] = by_count ? 1ull : static_cast<unsigned long long>(second(l));
+        atomicAdd(&hist[(me - lo) >> sh], static_cast<unsigned long long>(second(l)));
+        atomicAdd(&counts[(me - lo) >> sh], 1u);
       });
       __syncthreads();
-      const int m = static_cast<int>(number[1]);
-      const uint64_t me = lane < m ? hist[2 * lane] : ~0ull, mine = lane < m ? hist[2 * lane + 1] : 0;
-      uint64_t sums = passed, all = passed;
-      for (int i = 0; i < m; ++i) {
-        const uint64_t o = hist[2 * i], w = hist[2 * i + 1];
-        sums += o <= me ? w : 0;
-        all += w;
-      }
-      if (need > all) need = all;
-      const uint64_t hit = __ballot(lane < m && sums >= need && sums - mine < need);
-      lo = hit ? __shfl(me, __builtin_ctzll(hit), 64) : ~0ull;  // (every wave finds the same)
-    }
-    if (step == 3) {
-      if (lo != ~0ull) {
-        token = static_cast<uint32_t>(lo & 0xfffffu);
-        logprob = (static_cast<double>(logit_of_key(static_cast<uint32_t>(lo >> 20))) - static_cast<double>(r.max)) * z.s * (kLn2D / kPerOctave) - log_of(kept);
-      }
-      continue;
-    }
-    if (step < 2) cut = lo < cut ? lo : cut;
-    if (q.mode == kBeams) break;  // uniform
-    // ---- the weights up to the cut, or of those that reach min-p ----
-    __syncthreads();
-    if (tid == 0) sel[2] = 0;
-    __syncthreads();
-    uint64_t mine = 0;
-    each(0, step == 2 ? ~0ull : lo, [&](uint64_t, float l) {
-      uint64_t w = second(l);
-      if (step == 2) {
-        if (!reaches(l)) return;
-        if (in_bin(l) != b0) w = static_cast<uint64_t>(static_cast<double>(w) * exp2_of(static_cast<double>(b0 - in_bin(l)) / kPerOctave));
-      }
-      mine += w;
-    });
+      // digits 2 tid, 2 tid + 1
+      const uint64_t v0 = hist[2 * tid], v1 = hist[2 * tid + 1];
+      const uint32_t n0 = counts[2 * tid], n1 = counts[2 * tid + 1];
+      const uint64_t s = wave_scan(v0 + v1);
+      const uint32_t sn = wave_scan(n0 + n1);
+      if (lane == 63) part[wave] = s, partn[wave] = sn;
+      __syncthreads();
+      uint64_t w = passed + s - v0 - v1, all = passed;
+      uint32_t k = passed_n + sn - n0 - n1, all_n = passed_n;
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) mine += __shfl_xor(mine, d, 64);
-    if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&sel[2]), static_cast<unsigned long long>(mine));
+      for (int i = 0; i < NW; ++i) {
+        if (i < wave) w += part[i], k += partn[i];
+        all += part[i];
+        all_n += partn[i];
+      }
+      const uint64_t most = by_count ? all_n : all;
+      if (need > most) need = most;
+      const uint64_t a = by_count ? k : w, c = a + (by_count ? n0 : v0), e = c + (by_count ? n1 : v1);
+      if (a < need && need <= c) sel[0] = static_cast<uint64_t>(2 * tid) | static_cast<uint64_t>(n0) << 32, sel[1] = w, sel[2] = k;
+      if (c < need && need <= e) sel[0] = static_cast<uint64_t>(2 * tid + 1) | static_cast<uint64_t>(n1) << 32, sel[1] = w + v0, sel[2] = k + n0;
+      __syncthreads();
+      const uint64_t got = sel[0];
+      passed = sel[1];
+      passed_n = static_cast<uint32_t>(sel[2]);
+      lo = lo + ((got & 0xffffffffu) << sh);
+      const uint64_t top = lo + ((1ull << sh) - 1ull);
+      hi = top < hi ? top : hi;
+      if ((got >> 32) <= 64 || sh == 0) break;  // uniform
+    }
+    // ---- at most 64: gathered, and every wave sums them in their order ----
+    each(lo, hi, [&](uint64_t me, float l) {
+      const uint32_t to = atomicAdd(&number[1], 1u);
+      last_ones[to][0] = me;
+      last_ones[to][1] = second(l);
+    });
     __syncthreads();
-    kept = fmin(kept, before(b0) + static_cast<double>(sel[2]) * u_bin);
+    const int m = static_cast<int>(number[1]);
+    const uint64_t me = lane < m ? last_ones[lane][0] : ~0ull, mine = lane < m ? last_ones[lane][1] : 0;
+    uint64_t w = passed;
+    uint32_t k = passed_n;
+    for (int i = 0; i < m; ++i)
+      if (last_ones[i][0] <= me) w += last_ones[i][1], ++k;
+    const uint64_t measure = by_count ? k : w, one = by_count ? 1 : mine;
+    const uint64_t hit = __ballot(lane < m && measure >= need && measure - one < need);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      const uint64_t found_at = __shfl(me, at, 64);
+      if (step == 3) {
+        token = static_cast<uint32_t>(found_at & 0xfffffu);
+        drawn = x[static_cast<int>(token)];
+      } else {
+        cut = found_at < cut ? found_at : cut;
+        kept = fmin(kept, before(b0) + static_cast<double>(__shfl(w, at, 64)) * u_bin);
+      }
+    }
+    if (q.mode == kBeams) break;  // uniform
   }
   if (q.mode == kBeams) {
     __syncthreads();
@@ -838,12 +995,12 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     if (in_list) {
       for (int i = tid; i < n; i += NT) {
         const uint32_t idx = list[i].y & 0xfffffu;
-        if ((static_cast<uint64_t>(list[i].x) << 20 | idx) <= cut) take(list[i].x, idx);
+        if (order_of(list[i].x, idx) <= cut) take(list[i].x, idx);
       }
     } else {
       for (int i = tid; i < x.V; i += NT) {
         const uint32_t k = key_of(x[i]);
-        if ((static_cast<uint64_t>(k) << 20 | static_cast<uint32_t>(i)) <= cut && x[i] > -__builtin_huge_valf()) take(k, static_cast<uint32_t>(i));
+        if (order_of(k, static_cast<uint32_t>(i)) <= cut && x[i] > -__builtin_huge_valf()) take(k, static_cast<uint32_t>(i));
       }
     }
     __syncthreads();
@@ -857,7 +1014,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   if (q.mode == kSample) {
     q.token[row] = token == kNone ? -1 : static_cast<int64_t>(token);
     // (a difference below what the sums tell apart is none)
-    q.logprob[row] = logprob > -0x1p-40 ? 0.0f : static_cast<float>(logprob);
+    const double lp = (static_cast<double>(drawn) - static_cast<double>(r.max)) * z.s * (kLn2D / kPerOctave) - log_of(kept);
+    q.logprob[row] = lp > -0x1p-40 ? 0.0f : static_cast<float>(lp);
   } else {
     q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, accepted ? 1 : 0, static_cast<int32_t>(token)};
   }
@@ -880,8 +1038,10 @@ __global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
 }
 
 // What the target has above the draft at token i, 2^52 a probability of 1.
+template <int DT>
 __device__ __forceinline__ uint64_t above(const SamplingParams& q, const Settings& z, const Row& r, int row, float l, int i) {
-  const uint64_t me = static_cast<uint64_t>(key_of(l)) << 20 | static_cast<uint32_t>(i);
+  constexpr int KS = DT == MZK_F32 ? 0 : DT == MZK_BF16 ? 16 : 13;
+  const uint64_t me = static_cast<uint64_t>(key_of(l) >> KS) << 20 | static_cast<uint32_t>(i);
   if (!(l > -__builtin_huge_valf()) || me > r.cut || (static_cast<double>(l) - static_cast<double>(r.max)) * z.s < z.f) return 0;
   const double t = Grid{r.origin, z.s}.place(l) - static_cast<double>(r.top);
   const double p = exp2_of(t / kPerOctave) * __builtin_ldexp(1.0, q.scale) / r.kept;
@@ -905,10 +1065,9 @@ __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
 #pragma unroll 4
   for (int k = 0; k < kRestElements / 256; ++k) {
     const int i = chunk * kRestElements + 256 * k + tid;
-    if (i < q.V) s += above(q, z, r, row, x[i], i);
+    if (i < q.V) s += above<DT>(q, z, r, row, x[i], i);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+  s = wave_sum(s);
   if ((tid & 63) == 0) sums[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) q.rest[static_cast<int64_t>(b) * q.rest_chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
@@ -925,7 +1084,7 @@ __global__ void __launch_bounds__(256) redraw_kernel(const SamplingParams q) {
   if (row < 0) return;
   // a chunk is a thread's: at most 2^20 / 4096 of them
   const uint64_t mine = tid < q.rest_chunks ? q.rest[static_cast<int64_t>(b) * q.rest_chunks + tid] : 0;
-  const uint64_t upto = wave_scan(mine, lane);
+  const uint64_t upto = wave_scan(mine);
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
   const uint64_t total = sums[0] + sums[1] + sums[2] + sums[3];
@@ -942,8 +1101,8 @@ __global__ void __launch_bounds__(256) redraw_kernel(const SamplingParams q) {
   const Row r = q.rowres[row];
   for (int k = 0; k < kRestElements / 256; ++k) {
     const int i = at_chunk * kRestElements + 256 * k + tid;
-    const uint64_t v = i < q.V ? above(q, z, r, row, x[i], i) : 0;
-    const uint64_t s = wave_scan(v, lane);
+    const uint64_t v = i < q.V ? above<DT>(q, z, r, row, x[i], i) : 0;
+    const uint64_t s = wave_scan(v);
     __syncthreads();
     if (lane == 63) sums[wave] = s;
     __syncthreads();
@@ -1056,7 +1215,7 @@ template <int DT>
 int launch(const SamplingParams& q, hipStream_t s) {
   static std::atomic<bool> row_set[kMaxDevices] = {};
   if (!raise_lds(row_kernel<DT>, kRowLds, row_set)) return MZK_ELAUNCH;
-  if (q.chunks > 1) survey_kernel<DT><<<static_cast<unsigned>(q.rows) * static_cast<unsigned>(q.chunks), 256, 0, s>>>(q);
+  if (q.chunks > 1) survey_kernel<DT><<<static_cast<unsigned>((q.rows + 7) / 8 * 8 * q.chunks), 256, 0, s>>>(q);
   row_kernel<DT><<<static_cast<unsigned>(q.rows), kRowThreads, kRowLds, s>>>(q);
   if (q.mode == kVerify) {
     verify_kernel<<<static_cast<unsigned>((q.B + 255) / 256), 256, 0, s>>>(q);
@@ -1086,14 +1245,14 @@ int rows_of(SamplingParams& q, const char* name, int64_t rows, int64_t V, int dt
   q.V = static_cast<int>(V);
   q.scale = 62;
   while ((static_cast<int64_t>(1) << (62 - q.scale)) < V) --q.scale;
-  // Chunks: of whole steps of a survey's workgroup, 4096 elements, so that there are some 1024 workgroups; none
-  // from 128 rows on, and 7 elements of the first piece may belong to no row.
-  const int64_t steps = (V + 7 + 4095) / 4096;
+  // Chunks: of whole steps of a survey's workgroup, so that there are some 1024 workgroups; none from 128 rows on.
+  // (7 elements of the first piece may belong to no row.)
+  const int64_t step = 256 * kAhead, pieces = (V + 7) * size_of(dtype) / 16 + 1, steps = (pieces + step - 1) / step;
   int64_t chunks = rows >= 128 || rows == 0 ? 1 : 1024 / rows;
-  if (chunks > 64) chunks = 64;
+  if (chunks > kMostChunks) chunks = kMostChunks;
   if (chunks > steps) chunks = steps;
   const int64_t per = (steps + chunks - 1) / chunks;
-  q.chunk_pieces = static_cast<int>(per * 4096 * size_of(dtype) / 16);
+  q.chunk_pieces = static_cast<int>(per * step);
   q.chunks = static_cast<int>((steps + per - 1) / per);
   q.rest_chunks = static_cast<int>((V + kRestElements - 1) / kRestElements);
   q.rows = static_cast<int>(rows);

@@ -18,7 +18,7 @@ A row's tokens stand in the order of falling logits, equal ones by rising index.
 logits; ``top_k`` keeps the first k tokens of the order; ``top_p`` the fewest of those that hold that share of
 their probability; ``min_p`` those of at least that share of the first one's.  Each is a number for all
 rows, a tensor of one for each row (float32; ``top_k`` int32), or None: off.  Temperature 0 takes the
-first token of the order.  NaN and -inf are no tokens; +inf counts as the largest finite number.
+first token of the order.  NaN and -inf are no tokens; +inf counts as the largest finite number of its type.
 
 Logits are fp32, bf16 or fp16 [rows, V], V at most 2^20, rows of wider tensors among them.
 """
