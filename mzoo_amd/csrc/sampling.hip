@@ -38,6 +38,14 @@ struct Surveyed {
   float origin;
 };
 
+// What a row's bins say to the launches that list and finish it.
+struct Plan {
+  Surveyed r;
+  int w0[4], w1[4];       // bins in which a cut or the token is (w1 < w0: none)
+  float from[2], to[2];   // the logits to be listed
+  double drafted_w;
+};
+
 // What a row leaves for the launches behind it.
 struct Row {
   double kept;    // W, in units of 2^-scale
@@ -78,6 +86,11 @@ struct SamplingParams {
   Surveyed* heads;   // [rows][chunks]
   uint64_t* hist;    // [rows][chunks][kBins] from the largest down
   uint32_t* counts;  // the same, tokens
+  Plan* plans;       // [rows]
+  uint64_t* sums;    // [rows][kBins] running sums of the joined bins
+  uint32_t* sum_counts;
+  uint32_t* listed;  // [rows]
+  uint2* list;       // [rows][kCap] key; index, and the bin above bit 20
   Row* rowres;       // [rows]
   int32_t* refused;  // [B] the row of a refused token, or -1
   uint64_t* rest;    // [B][rest_chunks] sums of what the target has above the draft
@@ -345,7 +358,7 @@ __device__ __forceinline__ float origin_of(const Pieces<DT>& x, int tid, float* 
 }
 
 constexpr int kCopies = 2;     // of each bin, side by side, by the lane
-constexpr int kAhead = 4;      // pieces of a chunk's thread that are asked for at once
+constexpr int kSurveyThreads = 1024, kSurveyElements = 16;  // of a chunk's workgroup; of its thread at once
 constexpr int kAside = 64;     // places behind the bins for what is too small to count
 constexpr int kFar = 1 << 28;  // bins from the origin that are told apart
 
@@ -460,10 +473,10 @@ __device__ __forceinline__ void surveyed_bin(const Surveyed& r, int j, bool coun
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) survey_kernel(const SamplingParams q) {
+__global__ void __launch_bounds__(kSurveyThreads) survey_kernel(const SamplingParams q) {
   __shared__ unsigned long long hist[kCopies * kBins + kAside];
   __shared__ uint32_t counts[kCopies * kBins + kAside];
-  __shared__ float lds[4];
+  __shared__ float lds[kSurveyThreads / 64];
   __shared__ int tops[2];
   const int tid = threadIdx.x;
   // workgroups go to the 8 XCDs in turn: a row's chunks to the one that its own workgroup reads it from again
@@ -472,18 +485,76 @@ __global__ void __launch_bounds__(256) survey_kernel(const SamplingParams q) {
   const Pieces<DT> x(q.logits + row * q.stride, q.V);
   const Settings z = settings(q, row);
   const bool counting = z.k > 0;
-  const Grid g{origin_of<DT, 256>(x, tid, lds), z.s};
+  const Grid g{origin_of<DT, kSurveyThreads>(x, tid, lds), z.s};
   const int from = chunk * q.chunk_pieces, all = x.count(), to = from + q.chunk_pieces < all ? from + q.chunk_pieces : all;
-  const Surveyed r = survey<DT, 256, kAhead>(x, g, counting, from, to, tid, hist, counts, tops, lds);
+  const Surveyed r = survey<DT, kSurveyThreads, kSurveyElements / Pieces<DT>::N>(x, g, counting, from, to, tid, hist, counts, tops, lds);
   const int64_t at = static_cast<int64_t>(row) * q.chunks + chunk;
   if (tid == 0) q.heads[at] = r;
   if (r.top == kNoTop) return;  // uniform
-  for (int j = tid; j < kBins; j += 256) {
+  for (int j = tid; j < kBins; j += kSurveyThreads) {
     uint64_t sum;
     uint32_t num;
     surveyed_bin(r, j, counting, hist, counts, sum, num);
     q.hist[at * kBins + j] = sum;
     if (counting) q.counts[at * kBins + j] = num;
+  }
+}
+
+// ---- list -----------------------------------------------------------------------------------------
+
+// The tokens of a chunk with logits in the plan's ranges.
+template <int DT>
+__global__ void __launch_bounds__(kSurveyThreads) list_kernel(const SamplingParams q) {
+  using P = Pieces<DT>;
+  constexpr int NT = kSurveyThreads, NW = NT / 64, PER = kSurveyElements / P::N;
+  __shared__ uint32_t part[NW], base;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int of8 = blockIdx.x >> 3, row = of8 / q.chunks * 8 + (blockIdx.x & 7), chunk = of8 % q.chunks;
+  if (row >= q.rows || (q.mode == kVerify && q.cu[q.B] <= row)) return;
+  const P x(q.logits + row * q.stride, q.V);
+  const int first = chunk * q.chunk_pieces, all = x.count(), end = first + q.chunk_pieces < all ? first + q.chunk_pieces : all;
+  uint4 next[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) next[i] = first + i * NT + tid < end ? x.load(first + i * NT + tid) : P::none();
+  const Plan p = q.plans[row];
+  const Grid g{p.r.origin, settings(q, row).s};
+  if (fmaxf(p.to[0], p.to[1]) == -__builtin_huge_valf()) return;  // uniform: no list
+  for (int at = first; at < end; at += PER * NT) {
+    uint4 now[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      now[i] = next[i];
+      const int piece = at + (PER + i) * NT + tid;
+      if (at + PER * NT < end) next[i] = piece < end ? x.load(piece) : P::none();
+    }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kSurveyElements; ++i) {
+      const float l = P::at(now[i / P::N], i % P::N);  // (a NaN is in no range)
+      mine |= static_cast<uint32_t>((l >= p.from[0] && l <= p.to[0]) || (l >= p.from[1] && l <= p.to[1])) << i;
+    }
+    const uint32_t many = __popc(mine), s = wave_scan(many);
+    if (lane == 63) part[wave] = s;
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < wave) before += part[w];
+      total += part[w];
+    }
+    if (tid == 0 && total) base = atomicAdd(&q.listed[row], total);
+    __syncthreads();
+    uint32_t to = base + before + s - many;
+#pragma unroll
+    for (int i = 0; i < kSurveyElements; ++i) {
+      if (mine >> i & 1u) {
+        const float l = logit_of<DT>(P::at(now[i / P::N], i % P::N));
+        const int j = static_cast<int>(fmin(static_cast<double>(p.r.top) - __builtin_rint(g.place(l)), static_cast<double>(kRest)));
+        const int idx = x.first(at + i / P::N * NT + tid) + i % P::N;
+        if (to < kCap) q.list[static_cast<int64_t>(row) * kCap + to] = uint2{key_of(l), static_cast<uint32_t>(idx) | static_cast<uint32_t>(j) << 20};
+        ++to;
+      }
+    }
   }
 }
 
@@ -493,7 +564,11 @@ constexpr int kRowThreads = kBins / 2;
 constexpr int kMostChunks = 64;
 constexpr int kDigits = 1024;  // of a selection's step
 
-template <int DT>
+// A row in one launch, or, where its chunks are surveyed and listed by workgroups of their own, in two: up to the bins
+// in which something is to be found, and from the list on.
+enum Part { kWholeRow, kPlanPart, kFinishPart };
+
+template <int DT, Part PART>
 __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q) {
   constexpr int NT = kRowThreads, NW = NT / 64;
   constexpr int KS = DT == MZK_F32 ? 0 : DT == MZK_BF16 ? 16 : 13;  // low bits of a key that are all the same
@@ -520,11 +595,16 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   const bool counting = z.k > 0;
 
   // ---- the row's histogram: bins 2 tid, 2 tid + 1, from the largest down, are this thread's ----
-  Grid g{q.chunks == 1 ? origin_of<DT, NT>(x, tid, lds) : q.heads[static_cast<int64_t>(row) * q.chunks].origin, z.s};
+  Plan* const plan = q.plans + row;
+  Grid g{PART == kWholeRow ? 0.0f : PART == kPlanPart ? q.heads[static_cast<int64_t>(row) * q.chunks].origin : plan->r.origin, z.s};
   uint64_t sum[2] = {0, 0};  // of the second factors
   uint32_t num[2] = {0, 0};
   Surveyed r{kNoTop, -__builtin_huge_valf(), 0.0f};
-  for (bool whole_row = q.chunks == 1;; whole_row = true) {
+  bool by_value = false;  // 16-bit logits: the counts of their values say where to look
+
+  if (PART == kWholeRow && !by_value) g.origin = origin_of<DT, NT>(x, tid, lds);
+  if (PART == kFinishPart) r = plan->r;
+  for (bool whole_row = PART == kWholeRow; PART != kFinishPart && !by_value; whole_row = true) {
     if (whole_row) {
       r = survey<DT, NT, 8>(x, g, counting, 0, x.count(), tid, bins, bin_counts, tops, lds);
       if (r.top > kNoTop) {
@@ -577,6 +657,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   }
   if (r.max == -__builtin_huge_valf()) {  // uniform: no token
     if (tid == 0) {
+      if (PART == kPlanPart) plan->r = r, plan->to[0] = plan->to[1] = -__builtin_huge_valf(), q.listed[row] = 0;
       if (q.mode == kSample) q.token[row] = -1, q.logprob[row] = -__builtin_huge_valf();
       if (q.mode == kVerify) q.rowres[row] = Row{0.0, 0, r.max, 0.0f, 0, 0, -1};
       if (q.mode == kBeams) q.nbest[row] = 0;
@@ -594,19 +675,40 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   double my_upto[2];
   uint32_t my_cn[2];
   {
-    uint64_t w = wave_scan(my_w0 + my_w1);
-    uint32_t m = wave_scan(num[0] + num[1]);
-    if (lane == 63) part[wave] = w, partn[wave] = m;
-    __syncthreads();
+    // (by value the sums are there)
+    const int at = kBins * row;
+    uint64_t w = 0;
+    uint32_t m = 0;
+    if (PART != kFinishPart && !by_value) {
+      w = wave_scan(my_w0 + my_w1);
+      m = wave_scan(num[0] + num[1]);
+      if (lane == 63) part[wave] = w, partn[wave] = m;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NW; ++i)
-      if (i < wave) w += part[i], m += partn[i];
-    cw[2 * tid] = w - my_w1;
-    cw[2 * tid + 1] = w;
-    cn[2 * tid] = my_cn[0] = m - num[1];
-    cn[2 * tid + 1] = my_cn[1] = m;
-    my_upto[0] = static_cast<double>(w - my_w1);
-    my_upto[1] = static_cast<double>(w);
+      for (int i = 0; i < NW; ++i)
+        if (i < wave) w += part[i], m += partn[i];
+      cw[2 * tid] = w - my_w1;
+      cw[2 * tid + 1] = w;
+      cn[2 * tid] = m - num[1];
+      cn[2 * tid + 1] = m;
+    }
+    if (PART == kFinishPart) {
+      cw[2 * tid] = q.sums[at + 2 * tid];
+      cw[2 * tid + 1] = q.sums[at + 2 * tid + 1];
+      cn[2 * tid] = q.sum_counts[at + 2 * tid];
+      cn[2 * tid + 1] = q.sum_counts[at + 2 * tid + 1];
+    }
+    if (PART == kPlanPart) {
+      q.sums[at + 2 * tid] = w - my_w1;
+      q.sums[at + 2 * tid + 1] = w;
+      q.sum_counts[at + 2 * tid] = m - num[1];
+      q.sum_counts[at + 2 * tid + 1] = m;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // (each thread its own)
+      my_upto[e] = static_cast<double>(cw[2 * tid + e]);
+      my_cn[e] = cn[2 * tid + e];
+    }
   }
   __syncthreads();
   const double total = static_cast<double>(cw[kRest]);
@@ -664,7 +766,9 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     }
   }
   const bool leaves = drafted_bin < kRest && !q.probs;
-  if (leaves) {  // uniform
+  if (PART == kFinishPart) {
+    drafted_w = plan->drafted_w;
+  } else if (leaves && !by_value) {  // uniform
     const int e = drafted_bin & 1;
     if (tid == drafted_bin >> 1)
       sel[0] = (e ? my_w1 : my_w0) - static_cast<uint64_t>(static_cast<double>(sum[e] - second(logit_of_key(drafted_key))) * my_unit[e] + 0.5);
@@ -676,9 +780,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   // ---- the bins in which something is to be found, before the cuts are known ----
   // windows: top-k's cut, top-p's, min-p's, the token
   int w0[4] = {1, 1, 1, 1}, w1[4] = {0, 0, 0, 0};
-  int last;
-  {
-    int kb;
+  if (PART != kFinishPart && !by_value) {
+    int kb, last;
     find([&](int e) { return my_cn[e] < static_cast<uint32_t>(z.k); }, [&](int e) { return my_upto[e] < total; }, kb, last);
     double least = total, most = total;
     if (counting && kb < kRest) {
@@ -706,7 +809,12 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         const double y = g.place(r.max) + z.f, eps = 1e-6 + fabs(y) * 1e-13, top = static_cast<double>(r.top);
         w0[2] = static_cast<int>(fmin(fmax(top - __builtin_rint(y + eps), 0.0), static_cast<double>(kRest)));
         w1[2] = static_cast<int>(fmin(fmax(top - __builtin_rint(y - eps), 0.0), static_cast<double>(kRest - 1)));
-        if (w0[2] < kRest) {
+        // the shortest prefix counts: of two cuts whose bins do not meet, the one before the other
+        const int o0 = z.p < 1.0 ? w0[1] : w0[0], o1 = z.p < 1.0 ? w1[1] : w1[0];
+        if (w0[2] >= kRest || (o1 >= o0 && w0[2] > o1)) {
+          w0[2] = 1, w1[2] = 0;
+        } else {
+          if (o1 >= o0 && w1[2] < o0) w0[0] = w0[1] = 1, w1[0] = w1[1] = 0;
           least = fmin(least, before(w0[2]));
           most = fmin(most, upto(w1[2]));
         }
@@ -731,16 +839,20 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   }
 
   // ---- the cuts and the token ----
-  // whether the windows' tokens fit the list: a second factor is 1, nearly
-  bool in_list = false, relist;
-  {
+  // the bins from the first cut's to the last's
+  const int cuts0 = min(min(w1[0] < w0[0] ? kBins : w0[0], w1[1] < w0[1] ? kBins : w0[1]), w1[2] < w0[2] ? kBins : w0[2]);
+  const int cuts1 = max(max(w1[0], w1[1]), w1[2]);
+  // whether the tokens fit the list: a second factor is 1, nearly
+  bool in_list = false, relist = by_value;
+  if (PART == kFinishPart) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w0[i] = plan->w0[i], w1[i] = plan->w1[i];
+  } else if (!by_value) {
     uint64_t many = 0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      bool in = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) in = in || (2 * tid + e >= w0[i] && 2 * tid + e <= w1[i]);
-      many += in ? sum[e] >> kWhole : 0;
+      const int j = 2 * tid + e;
+      many += (j >= cuts0 && j <= cuts1) || (j >= w0[3] && j <= w1[3]) ? sum[e] >> kWhole : 0;
     }
     many = wave_sum(many);
     if (lane == 0) part[wave] = many;
@@ -749,6 +861,25 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
 #pragma unroll
     for (int w = 0; w < NW; ++w) many += part[w];
     relist = many > static_cast<uint64_t>(kCap - kCap / 16);
+  }
+  // two ranges of logits: the cuts' and the token's bins
+  float from[2], to[2];
+  logits_of(cuts0, cuts1, from[0], to[0]);
+  logits_of(w0[3], w1[3], from[1], to[1]);
+  if (cuts1 < cuts0) from[0] = __builtin_huge_valf(), to[0] = -__builtin_huge_valf();
+  if (w1[3] < w0[3]) from[1] = __builtin_huge_valf(), to[1] = -__builtin_huge_valf();
+  if (PART == kPlanPart) {
+    if (tid == 0) {
+      Plan p{r, {}, {}, {}, {}, drafted_w};
+      p.r.origin = g.origin;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p.w0[i] = w0[i], p.w1[i] = w1[i];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) p.from[i] = from[i], p.to[i] = relist ? -__builtin_huge_valf() : to[i];
+      *plan = p;
+      q.listed[row] = relist ? static_cast<uint32_t>(kCap) + 1u : 0;
+    }
+    return;
   }
   int n = 0;
   uint64_t cut = ~0ull;  // the last token that top-k and top-p keep
@@ -796,54 +927,62 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     }
     // ---- the tokens of the bins: all windows' at once, or, where those are too many, the bin's ----
     if (step < 0 && relist) continue;
+    if (PART == kFinishPart && step < 0) {
+      const uint32_t many = q.listed[row];
+      in_list = many <= kCap;
+      relist = !in_list;
+      n = in_list ? static_cast<int>(many) : 0;
+      const uint2* const theirs = q.list + static_cast<int64_t>(row) * kCap;
+#pragma unroll 8
+      for (int i = tid; i < n; i += NT) list[i] = theirs[i];  // (each thread comes back to its own)
+      continue;
+    }
     if (step < 0 || relist) {
       __syncthreads();
       if (tid == 0) number[0] = 0;
       __syncthreads();
-      // two ranges of bins: the cuts' and the token's
-      int h0 = b0, h1 = b1;
-      float from[2], to[2];
-      if (step < 0) {
-        logits_of(w0[3], w1[3], from[1], to[1]);
-        h0 = min(min(w1[0] < w0[0] ? kBins : w0[0], w1[1] < w0[1] ? kBins : w0[1]), w1[2] < w0[2] ? kBins : w0[2]);
-        h1 = max(max(w1[0], w1[1]), w1[2]);
+      if (step >= 0) {
+        if (!by_value) logits_of(b0, b1, from[0], to[0]);
+        from[1] = __builtin_huge_valf();
+        to[1] = -__builtin_huge_valf();
       }
-      logits_of(h0, h1, from[0], to[0]);
-      if (h1 < h0) from[0] = __builtin_huge_valf();
-      if (step >= 0 || w1[3] < w0[3]) from[1] = __builtin_huge_valf(), to[1] = 0.0f;
       const int pieces = x.count();
-      constexpr int AHEAD = 32 / P::N;  // 32 elements a thread
+      constexpr int AHEAD = 8, MASKS = AHEAD * P::N / 32;
       uint4 next[AHEAD];
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) next[a] = a * NT + tid < pieces ? x.load(a * NT + tid) : P::none();
       for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
-        uint4 v[AHEAD];
+        uint32_t mine[MASKS];
+#pragma unroll
+        for (int k = 0; k < MASKS; ++k) mine[k] = 0;
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-          v[a] = next[a];
+          const uint4 v = next[a];
           const int piece = p0 + (AHEAD + a) * NT + tid;
           if (p0 + AHEAD * NT < pieces) next[a] = piece < pieces ? x.load(piece) : P::none();
-        }
-        uint32_t mine = 0;
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
 #pragma unroll
           for (int i = 0; i < P::N; ++i) {
-            const float l = P::at(v[a], i);  // (a NaN is in no range)
+            const float l = P::at(v, i);  // (a NaN is in no range)
             const bool in = (l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1]);
-            mine |= static_cast<uint32_t>(in) << (a * P::N + i);
+            mine[a * P::N / 32] |= static_cast<uint32_t>(in) << (a * P::N % 32 + i);
           }
-        if (__ballot(mine != 0) == 0) continue;
-        const uint32_t many = __popc(mine), s = wave_scan(many);
+        }
+        uint32_t many = 0;
+#pragma unroll
+        for (int k = 0; k < MASKS; ++k) many += __popc(mine[k]);
+        if (__ballot(many != 0) == 0) continue;
+        const uint32_t s = wave_scan(many);
         uint32_t at = 0;
         if (lane == 63) at = atomicAdd(&number[0], s);
         at = lane_of(at, 63) + s - many;
-        while (mine) {
-          const int i = __builtin_ctz(mine);
-          mine &= mine - 1;
-          if (at < kCap) list[at].y = static_cast<uint32_t>(x.first(p0 + i / P::N * NT + tid) + i % P::N);
-          ++at;
-        }
+#pragma unroll
+        for (int k = 0; k < MASKS; ++k)
+          while (mine[k]) {
+            const int i = 32 * k + __builtin_ctz(mine[k]);
+            mine[k] &= mine[k] - 1;
+            if (at < kCap) list[at].y = static_cast<uint32_t>(x.first(p0 + i / P::N * NT + tid) + i % P::N);
+            ++at;
+          }
       }
       __syncthreads();
       in_list = number[0] <= kCap;
@@ -1166,6 +1305,9 @@ __global__ void __launch_bounds__(1024) beams_kernel(const SamplingParams q, int
 
 // ---- host -----------------------------------------------------------------------------------------
 
+// fp32 rows from so many on, or so short ones, are a workgroup's each; 16-bit ones always.
+constexpr int kWholeRows = 192, kWholeVocab = 65536;
+
 int64_t up(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
 
 // The workspace's parts, in order; returns the bytes.
@@ -1179,6 +1321,12 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
   take(q.heads, rc);
   take(q.hist, rc * kBins);
   take(q.counts, rc * kBins);
+  const int64_t split = q.chunks > 1 ? r : 0;
+  take(q.plans, split);
+  take(q.sums, split * kBins);
+  take(q.sum_counts, split * kBins);
+  take(q.listed, split);
+  take(q.list, split * kCap);
   if (q.mode != kSample) take(q.rowres, r);
   if (q.mode == kVerify && q.probs) {
     take(q.refused, q.B);
@@ -1191,7 +1339,8 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
   return at;
 }
 
-constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2));
+constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2)), kBinsLds = 12 * (kCopies * kBins + kAside);
+static_assert(kBinsLds <= kRowLds && kBinsLds + 20 * 1024 <= 64 * 1024, "LDS");
 
 // The dynamic-LDS limit is a per-device function attribute: set once per device.
 template <typename K>
@@ -1213,10 +1362,19 @@ bool raise_lds(K kern, int bytes, std::atomic<bool> (&set)[kMaxDevices]) {
 
 template <int DT>
 int launch(const SamplingParams& q, hipStream_t s) {
-  static std::atomic<bool> row_set[kMaxDevices] = {};
-  if (!raise_lds(row_kernel<DT>, kRowLds, row_set)) return MZK_ELAUNCH;
-  if (q.chunks > 1) survey_kernel<DT><<<static_cast<unsigned>((q.rows + 7) / 8 * 8 * q.chunks), 256, 0, s>>>(q);
-  row_kernel<DT><<<static_cast<unsigned>(q.rows), kRowThreads, kRowLds, s>>>(q);
+  static std::atomic<bool> whole_set[kMaxDevices] = {}, finish_set[kMaxDevices] = {};
+  const unsigned rows = static_cast<unsigned>(q.rows);
+  if (q.chunks == 1) {
+    if (!raise_lds(row_kernel<DT, kWholeRow>, kRowLds, whole_set)) return MZK_ELAUNCH;
+    row_kernel<DT, kWholeRow><<<rows, kRowThreads, kRowLds, s>>>(q);
+  } else if constexpr (DT == MZK_F32) {
+    if (!raise_lds(row_kernel<DT, kFinishPart>, kRowLds, finish_set)) return MZK_ELAUNCH;
+    const unsigned grid = (rows + 7) / 8 * 8 * static_cast<unsigned>(q.chunks);
+    survey_kernel<DT><<<grid, kSurveyThreads, 0, s>>>(q);
+    row_kernel<DT, kPlanPart><<<rows, kRowThreads, kBinsLds, s>>>(q);
+    list_kernel<DT><<<grid, kSurveyThreads, 0, s>>>(q);
+    row_kernel<DT, kFinishPart><<<rows, kRowThreads, kRowLds, s>>>(q);
+  }
   if (q.mode == kVerify) {
     verify_kernel<<<static_cast<unsigned>((q.B + 255) / 256), 256, 0, s>>>(q);
     if (q.probs) {
@@ -1245,10 +1403,11 @@ int rows_of(SamplingParams& q, const char* name, int64_t rows, int64_t V, int dt
   q.V = static_cast<int>(V);
   q.scale = 62;
   while ((static_cast<int64_t>(1) << (62 - q.scale)) < V) --q.scale;
-  // Chunks: of whole steps of a survey's workgroup, so that there are some 1024 workgroups; none from 128 rows on.
+  // Chunks: of whole steps of a survey's workgroup, so that there are some 512 workgroups; none from 128 rows on.
   // (7 elements of the first piece may belong to no row.)
-  const int64_t step = 256 * kAhead, pieces = (V + 7) * size_of(dtype) / 16 + 1, steps = (pieces + step - 1) / step;
-  int64_t chunks = rows >= 128 || rows == 0 ? 1 : 1024 / rows;
+  const int64_t step = kSurveyThreads * kSurveyElements * size_of(dtype) / 16, pieces = (V + 7) * size_of(dtype) / 16 + 1;
+  const int64_t steps = (pieces + step - 1) / step;
+  int64_t chunks = dtype != MZK_F32 || rows >= kWholeRows || rows == 0 || V <= kWholeVocab ? 1 : 512 / rows;
   if (chunks > kMostChunks) chunks = kMostChunks;
   if (chunks > steps) chunks = steps;
   const int64_t per = (steps + chunks - 1) / chunks;
