@@ -696,7 +696,7 @@ int mzk_packed_mqa_first(const void* q, int64_t T, int H, int D, const int64_t* 
  * exp((l - max l) / T).  top-k keeps the first k of them (<= 0: all), top-p the shortest prefix of those whose
  * weights reach p of their sum (>= 1: all, at least the first), min-p those of at least min_p times the first
  * one's weight (<= 0: all).  temperature <= 0: the first alone.  NaN and -inf are no tokens; +inf counts as
- * the largest finite number.
+ * its type's largest finite number.
  *   logits [rows, row_stride elements] fp32, bf16 or fp16, V of a row (at most 2^20), rows at any alignment.
  *   temperature, top_k, top_p, min_p: device arrays of one value for each row, or NULL: the value behind, for all.
  *   workspace: of the call's _workspace_bytes (16-byte aligned, no initialization); calls that overlap

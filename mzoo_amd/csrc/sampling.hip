@@ -6,15 +6,24 @@
 // top-k keeps the first k of the order, top-p the shortest prefix of those whose weights reach p of their
 // sum, min-p those of at least min_p times the first one's weight: each keeps a prefix, so together the
 // shortest.  The token drawn is the first whose running sum exceeds u times the kept sum W.  (T <= 0: the
-// first of the order.)  NaN and -inf are no tokens; +inf counts as the largest finite number, -0 as 0.
+// first of the order.)  NaN and -inf are no tokens; +inf counts as its type's largest finite number, -0 as 0.
 //
 // Tokens are whole numbers, so a token beside a border of the running sum has to come out right: weights
 // are computed in 64 bits to about 2^-50 of themselves, and summed as whole numbers, in any order the same.
 //
-// No row is sorted, and none is looked at twice in full arithmetic.  A row's workgroup has a histogram of its weights
-// over bins of 1/20 octave, from the largest down (survey: of its own, or joined from those of chunks where there are
-// too few rows for the compute units); finds the few bins in which the cuts of the filters and the token lie; lists
-// the row's tokens of these bins; and selects among those, bin by bin.
+// No row is sorted.  What is to be found lies in few places of the order, and those are found from sums:
+//   bins      weights are summed in bins of 1/20 octave, from the largest down, by atomic sums in LDS (survey);
+//   by value  of bf16 logits the tokens of each of the 2^16 values are counted instead, and weights computed once a value.
+// Running sums say in which bins (at which value) the cuts and the token are; the row is read once more to list its
+// tokens there, and the token is selected among those.
+// One workgroup does this for a row (row_kernel); where rows are fewer than compute units that way is bound by the 25 to
+// 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
+// row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
+//
+// Measured: fp32, 1 row of 131072: 7.1 + 10.2 + 4.7 + 13.1 us in four launches, of which reading would be 0.1 us: bound
+// by the launches' own steps, most of them barriers.  256 rows of 200019, with top-k, top-p and min-p by turns: 108 us,
+// 1.9 TB/s: bound by a compute unit's arithmetic on its row, some 22 instructions an element.  bf16, 64 rows of 131072:
+// 45.8 us; 160 rows: 64 us.  fp16, 16 rows of 32000: 23 us.
 #include "common.h"
 
 namespace mzk {
@@ -214,15 +223,28 @@ __device__ __forceinline__ Settings settings(const SamplingParams& q, int row) {
 
 // ---- loads ------------------------------------------------------------------------------------
 
-// A row in pieces of 16 bytes of memory, the first and the last of which may lie partly outside it.
+// A row in pieces of 16 bytes of memory: the whole ones in order, then what of the row lies before them and behind
+// them, filled up with -inf; those two are laid into LDS by `edges`, before a barrier of the caller.
 template <int DT>
 struct Pieces {
   static constexpr int SIZE = DT == MZK_F32 ? 4 : 2, N = 16 / SIZE;
   const uint8_t* row;
-  int V, mis;  // elements of the first piece before the row
-  __device__ Pieces(const uint8_t* r, int v) : row(r), V(v), mis(static_cast<int>((reinterpret_cast<uintptr_t>(r) & 15u) / SIZE)) {}
-  __device__ int count() const { return (V + mis + N - 1) / N; }
-  __device__ int first(int piece) const { return piece * N - mis; }  // index of its first element
+  int V, head, whole;  // elements before the first whole piece, whole pieces
+  const uint4* edge;   // [2] in LDS
+  __device__ Pieces(const uint8_t* r, int v, const uint4* e) : row(r), V(v), edge(e) {
+    head = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(r) & 15u)) & 15u) / SIZE;
+    if (head > V) head = V;
+    whole = (V - head) / N;
+  }
+  __device__ void edges(int tid, uint4* e) const {
+    if (tid >= 2 * N) return;
+    const int i = tid < N ? tid : tid - N + head + whole * N;
+    const uint32_t bits = i < (tid < N ? head : V) ? raw(i) : DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80u : 0xfc00u;
+    if constexpr (DT == MZK_F32) reinterpret_cast<uint32_t*>(e)[tid] = bits;
+    else reinterpret_cast<uint16_t*>(e)[tid] = static_cast<uint16_t>(bits);
+  }
+  __device__ int count() const { return whole + 2; }
+  __device__ int first(int piece) const { return piece < whole ? head + piece * N : piece == whole ? 0 : head + whole * N; }  // index of its first element
   __device__ uint32_t raw(int i) const {
     if constexpr (DT == MZK_F32) return reinterpret_cast<const uint32_t*>(row)[i];
     else return reinterpret_cast<const uint16_t*>(row)[i];
@@ -247,21 +269,10 @@ struct Pieces {
     }
     return uint4{w[0], w[1], w[2], w[3]};
   }
-  __device__ uint4 load(int piece) const {  // (what lies outside the row is -inf)
-    constexpr uint32_t none = DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80u : 0xfc00u;
-    const int e = first(piece);
-    if (e >= 0 && e + N <= V) return *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(e) * SIZE);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (DT == MZK_F32) {
-        w[j] = e + j >= 0 && e + j < V ? raw(e + j) : none;
-      } else {
-        const int i = e + 2 * j;
-        w[j] = (i >= 0 && i < V ? raw(i) : none) | (i + 1 >= 0 && i + 1 < V ? raw(i + 1) : none) << 16;
-      }
-    }
-    return uint4{w[0], w[1], w[2], w[3]};
+  __device__ uint4 load(int piece, int end) const {  // from `end` on: -inf
+    if (piece < whole && piece < end) return *reinterpret_cast<const uint4*>(row + (head + static_cast<int64_t>(piece) * N) * SIZE);
+    if (piece >= end) return none();
+    return edge[piece - whole];
   }
   __device__ static uint4 none() {
     constexpr uint32_t w = DT == MZK_F32 ? 0xff800000u : DT == MZK_BF16 ? 0xff80ff80u : 0xfc00fc00u;
@@ -382,7 +393,7 @@ __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, b
   if (tid < 2) tops[tid] = kNoTop;
   uint4 next[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) next[i] = from + i * NT + tid < to ? x.load(from + i * NT + tid) : P::none();
+  for (int i = 0; i < PER; ++i) next[i] = x.load(from + i * NT + tid, to);
   float known = -__builtin_huge_valf();  // a maximum of this wave's that the others have heard of
   int top = kNoTop, turn = 0;
   // offsets in bytes: the copy's, and a place's that nobody reads
@@ -400,7 +411,7 @@ __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, b
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int piece = at + (PER + i) * NT + tid;
-      if (at + PER * NT < to) next[i] = piece < to ? x.load(piece) : P::none();
+      if (at + PER * NT < to) next[i] = x.load(piece, to);
     }
     if (__ballot(m > known)) {
       known = wave_max(m);
@@ -482,7 +493,9 @@ __global__ void __launch_bounds__(kSurveyThreads) survey_kernel(const SamplingPa
   // workgroups go to the 8 XCDs in turn: a row's chunks to the one that its own workgroup reads it from again
   const int of8 = blockIdx.x >> 3, row = of8 / q.chunks * 8 + (blockIdx.x & 7), chunk = of8 % q.chunks;
   if (row >= q.rows || (q.mode == kVerify && q.cu[q.B] <= row)) return;  // (a row of no sequence)
-  const Pieces<DT> x(q.logits + row * q.stride, q.V);
+  __shared__ uint4 edge[2];
+  const Pieces<DT> x(q.logits + row * q.stride, q.V, edge);
+  x.edges(tid, edge);  // (barriers follow)
   const Settings z = settings(q, row);
   const bool counting = z.k > 0;
   const Grid g{origin_of<DT, kSurveyThreads>(x, tid, lds), z.s};
@@ -511,11 +524,14 @@ __global__ void __launch_bounds__(kSurveyThreads) list_kernel(const SamplingPara
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int of8 = blockIdx.x >> 3, row = of8 / q.chunks * 8 + (blockIdx.x & 7), chunk = of8 % q.chunks;
   if (row >= q.rows || (q.mode == kVerify && q.cu[q.B] <= row)) return;
-  const P x(q.logits + row * q.stride, q.V);
+  __shared__ uint4 edge[2];
+  const P x(q.logits + row * q.stride, q.V, edge);
+  x.edges(tid, edge);
+  __syncthreads();
   const int first = chunk * q.chunk_pieces, all = x.count(), end = first + q.chunk_pieces < all ? first + q.chunk_pieces : all;
   uint4 next[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) next[i] = first + i * NT + tid < end ? x.load(first + i * NT + tid) : P::none();
+  for (int i = 0; i < PER; ++i) next[i] = x.load(first + i * NT + tid, end);
   const Plan p = q.plans[row];
   const Grid g{p.r.origin, settings(q, row).s};
   if (fmaxf(p.to[0], p.to[1]) == -__builtin_huge_valf()) return;  // uniform: no list
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(kSurveyThreads) list_kernel(const SamplingPara
     for (int i = 0; i < PER; ++i) {
       now[i] = next[i];
       const int piece = at + (PER + i) * NT + tid;
-      if (at + PER * NT < end) next[i] = piece < end ? x.load(piece) : P::none();
+      if (at + PER * NT < end) next[i] = x.load(piece, end);
     }
     uint32_t mine = 0;
 #pragma unroll
@@ -563,6 +579,7 @@ __global__ void __launch_bounds__(kSurveyThreads) list_kernel(const SamplingPara
 constexpr int kRowThreads = kBins / 2;
 constexpr int kMostChunks = 64;
 constexpr int kDigits = 1024;  // of a selection's step
+constexpr int kByValue = 16384;  // longer rows of bf16 logits are counted by value
 
 // A row in one launch, or, where its chunks are surveyed and listed by workgroups of their own, in two: up to the bins
 // in which something is to be found, and from the list on.
@@ -590,7 +607,10 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   int b = 0, end = 0;
   if (q.mode == kVerify && !sequence_of(q, row, lane, b, end)) return;  // uniform
-  const P x(q.logits + row * q.stride, q.V);
+  __shared__ uint4 edge[2];
+  const P x(q.logits + row * q.stride, q.V, edge);
+  x.edges(tid, edge);
+  __syncthreads();
   const Settings z = settings(q, row);
   const bool counting = z.k > 0;
 
@@ -600,8 +620,190 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   uint64_t sum[2] = {0, 0};  // of the second factors
   uint32_t num[2] = {0, 0};
   Surveyed r{kNoTop, -__builtin_huge_valf(), 0.0f};
-  bool by_value = false;  // 16-bit logits: the counts of their values say where to look
-
+  bool by_value = false;  // bf16 logits: the counts of their values say where to look
+  // ---- bf16 logits: how many tokens have each value ----
+  // (4096 logits: 25.6 us by value, 24.4 with bins; 32768: 31.1 and 33.8; 131072: 46.4 and 60.6, 64 rows)
+  // Two counters a word, the negative value's above the positive's, from the order's first 128 values (a block) on:
+  // block j is thread j's.  A counter that passes 2^16 is found out by the sum of all.
+  uint32_t* const tally = reinterpret_cast<uint32_t*>(smem);
+  [[maybe_unused]] uint64_t reached = 0;  // the weights of the tokens that reach min-p
+  // value o (of 2^16) of the order, 0 the largest of its sign's patterns
+  auto pattern = [&](uint32_t o) -> uint32_t { return o < 0x8000u ? 0x7fffu - o : o; };
+  auto value_of = [&](uint32_t o) -> float { return P::value(pattern(o)); };
+  // the counters of values o, o + 1 (o even)
+  auto tallied = [&](uint32_t o, uint32_t& c0, uint32_t& c1) __attribute__((always_inline)) {
+    const uint2 w = *reinterpret_cast<const uint2*>(tally + (pattern(o) & 0x7ffeu));
+    c0 = o < 0x8000u ? w.y & 0xffffu : w.x >> 16;
+    c1 = o < 0x8000u ? w.x & 0xffffu : w.y >> 16;
+  };
+  // the weight of a logit, in units of 2^-scale of the largest's
+  auto weight = [&](float l) __attribute__((always_inline)) -> double {
+    return exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
+  };
+  if (DT == MZK_BF16 && PART == kWholeRow && q.V > kByValue) {
+    // blocks of numbers: before them NaN and +inf, behind them -inf and NaN
+    constexpr int FIRST = 1, END = 511, INF = 0x7f80, AHEAD = 8;
+    for (int i = tid; i < 8192; i += NT) reinterpret_cast<uint4*>(tally)[i] = uint4{0, 0, 0, 0};
+    uint4 next[AHEAD];
+    const int pieces = x.count();
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) next[a] = x.load(a * NT + tid, pieces);
+    __syncthreads();
+    uint32_t all = 0;
+    for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const uint32_t v[4] = {next[a].x, next[a].y, next[a].z, next[a].w};
+        const int piece = p0 + (AHEAD + a) * NT + tid;
+        if (p0 + AHEAD * NT < pieces) next[a] = x.load(piece, pieces);
+        if (p0 + a * NT + tid >= pieces) continue;
+        all += P::N;
+        uint8_t* const at = reinterpret_cast<uint8_t*>(tally);
+        // one value throughout the wave, as in a masked vocabulary: one lane counts for all
+        const uint64_t here = __ballot(true);
+        const uint32_t one = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v[0])));
+        if (__builtin_expect(__ballot(v[0] == one && v[1] == one && v[2] == one && v[3] == one && (one & 0xffffu) == one >> 16) == here, 0)) {
+          if (lane == __builtin_ctzll(here))
+            atomicAdd(reinterpret_cast<uint32_t*>(at + (one << 2 & 0x1fffcu)), (1u + (one >> 31) * 0xffffu) * static_cast<uint32_t>(P::N * __popcll(here)));
+          continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          atomicAdd(reinterpret_cast<uint32_t*>(at + (v[i] << 2 & 0x1fffcu)), 1u + (v[i] >> 15 & 1u) * 0xffffu);
+          atomicAdd(reinterpret_cast<uint32_t*>(at + (v[i] >> 14 & 0x1fffcu)), 1u + (v[i] >> 31) * 0xffffu);
+        }
+      }
+    }
+    all = wave_sum(all);
+    if (lane == 0) partn[wave] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += partn[w];
+    if (tid == 0) {  // -0 is 0, +inf the largest number
+      const uint32_t zero = tally[0], most = tally[INF - 1];
+      const uint32_t z2 = (zero & 0xffffu) + (zero >> 16), m2 = (most & 0xffffu) + (tally[INF] & 0xffffu);
+      tally[0] = z2;
+      tally[INF - 1] = (most & 0xffff0000u) | (m2 & 0xffffu);
+      tally[INF] &= 0xffff0000u;
+      number[0] = z2 > 0xffffu || m2 > 0xffffu;
+    }
+    __syncthreads();
+    cw[tid] = 0;
+    uint32_t mine = 0;  // tokens of block tid: 128 words, from another one on in every lane, so that no two meet
+    {
+      const uint32_t* const words = tally + (tid < 256 ? 255 - tid : tid - 256) * 128;
+      const int sh = tid < 256 ? 0 : 16;
+#pragma unroll 16
+      for (int i = 0; i < 128; ++i) mine += words[(i + tid) & 127] >> sh & 0xffffu;
+      cn[tid] = mine;
+    }
+    // the first block of numbers with a token, and the sum of all counters
+    const uint64_t some = __ballot(mine != 0 && tid >= FIRST && tid < END);
+    const uint32_t sums = wave_sum(mine);
+    if (lane == 0) found[0][0][wave] = some ? 64 * wave + __builtin_ctzll(some) : END, partn[wave] = sums;
+    __syncthreads();
+    int first = END;
+    uint32_t counted = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) first = min(first, found[0][0][w]), counted += partn[w];
+    const bool exact = counted == all && number[0] == 0;
+    by_value = true;
+    if (first < END) {
+      uint32_t c0, c1;
+      tallied(128u * first + 2u * lane, c0, c1);
+      const int at = __builtin_ctzll(__ballot((c0 | c1) != 0));
+      r.max = value_of(128u * first + 2u * at + (lane_of(c0, at) ? 0u : 1u));
+      r.top = 0;
+      g.origin = r.max;
+    }
+    // blocks with weights that count
+    const bool light = !(first < END) || tid < first || !(g.place(value_of(128u * tid)) > -static_cast<double>(kRest));
+    const uint64_t heavy = __ballot(!light);
+    __syncthreads();
+    if (lane == 0) found[0][0][wave] = __popcll(heavy);
+    __syncthreads();
+    int end_heavy = first;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) end_heavy += found[0][0][w];
+    end_heavy = min(end_heavy, END);
+    int end_count = END;
+    if (!exact) {
+      // Some counter has run over.  It may be one of those that do not count, as of a masked vocabulary: are the
+      // others' tokens as many as there are?
+      end_count = end_heavy;
+      const float least = first < END ? value_of(128u * end_heavy - 1u) : -P::BIG;
+      uint32_t are = 0;
+      for (int p = tid; p < pieces; p += NT) {
+        const uint4 v = x.load(p, pieces);
+#pragma unroll
+        for (int i = 0; i < P::N; ++i) are += P::at(v, i) >= least;
+      }
+      const uint32_t theirs = wave_sum(tid < end_count && tid >= FIRST ? mine : 0u), seen = wave_sum(are);
+      if (lane == 0) partn[wave] = theirs - seen;
+      __syncthreads();
+      uint32_t differ = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) differ |= partn[w];
+      by_value = differ == 0 && number[0] == 0 && q.mode != kBeams;
+      __syncthreads();
+    }
+    if (by_value && first < END) {
+      // the blocks whose weights count, one after another
+      const uint64_t live = __ballot(tid >= first && tid < end_heavy && mine != 0);
+      if (lane == 0) found[1][0][wave] = __popcll(live);
+      __syncthreads();
+      int before_me = 0, lives = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w < wave) before_me += found[1][0][w];
+        lives += found[1][0][w];
+      }
+      if (live >> lane & 1u) counts[before_me + __popcll(live & ((1ull << lane) - 1ull))] = static_cast<uint32_t>(tid);
+      __syncthreads();
+      uint64_t reach = 0;
+      const double m = static_cast<double>(r.max);
+      for (int i = 2 * wave; i < lives; i += 2 * NW) {
+        float l[4];
+        uint32_t c[4];
+        int j[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          j[e] = static_cast<int>(counts[i + e < lives ? i + e : i]);
+          const uint32_t o = 128u * j[e] + 2u * lane;
+          tallied(o, c[2 * e], c[2 * e + 1]);
+          l[2 * e] = value_of(o);
+          l[2 * e + 1] = value_of(o + 1u);
+        }
+        uint64_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = static_cast<uint64_t>(static_cast<double>(c[e]) * weight(l[e]) + 0.5);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (i + e >= lives) continue;
+          const uint64_t s = wave_sum(w[2 * e] + w[2 * e + 1]);
+          if (lane == 0) cw[j[e]] = s;
+          if (z.f > -__builtin_huge_val())
+            reach += wave_sum(((static_cast<double>(l[2 * e]) - m) * z.s >= z.f ? w[2 * e] : 0) + ((static_cast<double>(l[2 * e + 1]) - m) * z.s >= z.f ? w[2 * e + 1] : 0));
+        }
+      }
+      __syncthreads();
+      if (tid < FIRST || tid >= end_count) mine = 0;
+      uint64_t w = wave_scan(cw[tid]);
+      uint32_t k = wave_scan(mine);
+      if (lane == 63) part[wave] = w, partn[wave] = k;
+      if (lane == 0) last_ones[wave][0] = reach;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        if (i < wave) w += part[i], k += partn[i];
+        reached += last_ones[i][0];
+      }
+      cw[tid] = w;
+      cn[tid] = k;
+    }
+    __syncthreads();
+  }
   if (PART == kWholeRow && !by_value) g.origin = origin_of<DT, NT>(x, tid, lds);
   if (PART == kFinishPart) r = plan->r;
   for (bool whole_row = PART == kWholeRow; PART != kFinishPart && !by_value; whole_row = true) {
@@ -669,7 +871,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   auto unit_of = [&](int j) __attribute__((always_inline)) -> double {
     return exp2_of(static_cast<double>(-j) / kPerOctave) * __builtin_ldexp(1.0, q.scale - kWhole);
   };
-  const double my_unit[2] = {unit_of(2 * tid), unit_of(2 * tid + 1)};
+  const double my_unit[2] = {by_value ? 0.0 : unit_of(2 * tid), by_value ? 0.0 : unit_of(2 * tid + 1)};
   const uint64_t my_w0 = static_cast<uint64_t>(static_cast<double>(sum[0]) * my_unit[0] + 0.5);
   const uint64_t my_w1 = static_cast<uint64_t>(static_cast<double>(sum[1]) * my_unit[1] + 0.5);
   double my_upto[2];
@@ -705,13 +907,13 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
       q.sum_counts[at + 2 * tid + 1] = m;
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {  // (each thread its own)
-      my_upto[e] = static_cast<double>(cw[2 * tid + e]);
-      my_cn[e] = cn[2 * tid + e];
+    for (int e = 0; e < 2; ++e) {  // (each thread its own; by value it has one block)
+      my_upto[e] = by_value ? static_cast<double>(cw[tid]) : static_cast<double>(cw[2 * tid + e]);
+      my_cn[e] = by_value ? cn[tid] : cn[2 * tid + e];
     }
   }
   __syncthreads();
-  const double total = static_cast<double>(cw[kRest]);
+  const double total = static_cast<double>(cw[by_value ? 511 : kRest]);
   auto upto = [&](int j) -> double { return static_cast<double>(cw[j]); };
   auto before = [&](int j) -> double { return j > 0 ? static_cast<double>(cw[j - 1]) : 0.0; };
   int round = 0;
@@ -864,8 +1066,10 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   }
   // two ranges of logits: the cuts' and the token's bins
   float from[2], to[2];
-  logits_of(cuts0, cuts1, from[0], to[0]);
-  logits_of(w0[3], w1[3], from[1], to[1]);
+  if (!by_value) {
+    logits_of(cuts0, cuts1, from[0], to[0]);
+    logits_of(w0[3], w1[3], from[1], to[1]);
+  }
   if (cuts1 < cuts0) from[0] = __builtin_huge_valf(), to[0] = -__builtin_huge_valf();
   if (w1[3] < w0[3]) from[1] = __builtin_huge_valf(), to[1] = -__builtin_huge_valf();
   if (PART == kPlanPart) {
@@ -887,21 +1091,33 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   uint32_t skip = kNone, token = kNone;
   bool accepted = false;
   float drawn = 0.0f;  // the token's logit
+  // by value: how many of the equal ones at the cut are kept, and their logit
+  uint64_t cut_need = ~0ull;
+  bool beyond = false;  // a drafted token among them that is not
+  float cut_value = 0.0f;
+  const uint32_t my_total_n = by_value ? cn[511] : 0;
+  auto order_index = [&](uint32_t key) -> uint32_t { return key >> 16; };  // of a value, from the key of its logit
 #pragma unroll 1
-  for (int step = -1; step < 4; ++step) {
+  for (int step = -1; step < 5; ++step) {
     int b0 = w0[3], b1 = w1[3];
     if (step == 0) b0 = w0[0], b1 = w1[0];
     if (step == 1) b0 = w0[1], b1 = w1[1];
     if (step == 2) b0 = w0[2], b1 = w1[2];
     double target = 0.0, start = 0.0;  // what is looked for, what lies before the bin
+    uint64_t need = 1;
+    if (by_value) {
+      if (step < 0 || (step == 0 && !counting) || (step == 1 && !(z.p < 1.0))) continue;  // uniform
+      b0 = 0;
+      b1 = kBins;
+    }
     if (step >= 0) {
-      if (b1 < b0) continue;  // uniform
-      if (step == 1) target = z.p * kept;
+      if (b1 < b0 || (step == 4 && !by_value)) continue;  // uniform
+      if (step == 1) target = by_value ? fmax(z.p * kept, 0.5) : z.p * kept;
       if (step == 3) {
         double left = kept;
         if (drafted != kNone) {
           const float l = logit_of_key(drafted_key);
-          if (order_of(drafted_key, drafted) <= cut && reaches(l)) {
+          if (order_of(drafted_key, drafted) <= cut && !beyond && reaches(l)) {
             const double w = exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
             const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + drafted]) : 1.0;
             accepted = static_cast<double>(q.u[row]) * sure * kept < w;
@@ -914,7 +1130,94 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         }
         target = u * left;
       }
-      if (step == 1 || step == 3) {
+      if (by_value) {
+        if (step == 2) {
+          if (z.f > -__builtin_huge_val()) kept = fmin(kept, static_cast<double>(reached));
+          // a drafted token of the cut's value: kept if fewer equal ones than the cut keeps are before it
+          if (drafted == kNone || order_of(drafted_key, 0xfffffu) != cut) continue;
+          const float l = logit_of_key(drafted_key);
+          uint32_t c0, c1;
+          tallied(order_index(drafted_key) & ~1u, c0, c1);
+          if ((order_index(drafted_key) & 1u ? c1 : c0) == 1u) continue;  // (it alone)
+          uint32_t m = 0;
+          for (int p = tid; p < x.count(); p += NT) {
+            const uint4 v = x.load(p, x.count());
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) m += logit_of<DT>(P::at(v, i)) == l && x.first(p) + i < static_cast<int>(drafted);
+          }
+          m = wave_sum(m);
+          __syncthreads();
+          if (lane == 0) partn[wave] = m;
+          __syncthreads();
+          m = 0;
+#pragma unroll
+          for (int i = 0; i < NW; ++i) m += partn[i];
+          beyond = m >= cut_need;
+          continue;
+        } else if (step == 4) {
+          // which of the equal ones at the cut are kept: wanted by the launches behind
+          if (!q.probs || cut == ~0ull) continue;
+          need = cut_need;
+          from[0] = to[0] = cut_value;
+          skip = kNone;
+        } else if (step == 0 && my_total_n < static_cast<uint32_t>(z.k)) {
+          if (q.mode != kBeams) continue;
+          need = z.k;  // all of them
+          from[0] = -P::BIG;
+          to[0] = P::BIG;
+        } else {
+          // the block: the first whose running sum reaches the target, or for the token exceeds it
+          double gone = 0.0;  // what the drafted token's value loses without it
+          if (skip != kNone) {
+            uint32_t c0, c1;
+            tallied(order_index(drafted_key) & ~1u, c0, c1);
+            const uint32_t c = order_index(drafted_key) & 1u ? c1 : c0;
+            const double w = weight(logit_of_key(drafted_key));
+            gone = static_cast<double>(static_cast<uint64_t>(c * w + 0.5) - static_cast<uint64_t>((c - 1) * w + 0.5));
+          }
+          const int gone_block = skip != kNone ? static_cast<int>(order_index(drafted_key) >> 7) : kBins;
+          auto w = [&](int) { return tid >= gone_block ? my_upto[0] - gone : my_upto[0]; };
+          int at, end_at;
+          find([&](int e) { return e == 0 && (step == 0 ? my_cn[0] < static_cast<uint32_t>(z.k) : step == 3 ? w(0) <= target : w(0) < target); },
+               [&](int e) { return e == 0 && (step == 0 ? my_cn[0] < my_total_n : w(0) < total - gone); }, at, end_at);
+          at = min(at, end_at);
+          // the value in it
+          const uint32_t o = 128u * at + 2u * lane;
+          uint32_t c0, c1;
+          tallied(o, c0, c1);
+          if (skip != kNone) c0 -= o == order_index(drafted_key), c1 -= o + 1u == order_index(drafted_key);
+          const float l0 = value_of(o), l1 = value_of(o + 1u);
+          const double one0 = weight(l0), one1 = weight(l1);
+          const uint64_t a = static_cast<uint64_t>(c0 * one0 + 0.5), c = static_cast<uint64_t>(c1 * one1 + 0.5);
+          const uint64_t sw = wave_scan(a + c);
+          const uint32_t sn = wave_scan(c0 + c1);
+          const double w0 = before(at) - (at > gone_block ? gone : 0.0), u1 = w0 + static_cast<double>(sw), u0 = w0 + static_cast<double>(sw - c);
+          const uint32_t n0 = at > 0 ? cn[at - 1] : 0, k1 = n0 + sn, k0 = k1 - c1;
+          const bool hit0 = c0 && (step == 0 ? k0 >= static_cast<uint32_t>(z.k) : step == 3 ? u0 > target : u0 >= target);
+          const bool hit1 = c1 && (step == 0 ? k1 >= static_cast<uint32_t>(z.k) : step == 3 ? u1 > target : u1 >= target);
+          const uint64_t hits = __ballot(hit0 || hit1), any = __ballot((c0 | c1) != 0);
+          const int who = hits ? __builtin_ctzll(hits) : any ? 63 - __builtin_clzll(any) : 0;
+          const bool second_one = !(hits ? hit0 : c1 == 0);
+          const uint32_t odd = lane_of(static_cast<uint32_t>(second_one), who);
+          const uint32_t many = lane_of(odd ? c1 : c0, who), k_before = lane_of(odd ? k0 : k0 - c0, who);
+          const double w_before = w0 + static_cast<double>(lane_of(odd ? sw - c : sw - c - a, who));
+          const float l = value_of(128u * at + 2u * who + odd);
+          const double one = __longlong_as_double(static_cast<long long>(lane_of(static_cast<uint64_t>(__double_as_longlong(odd ? one1 : one0)), who)));
+          // the token's place among the equal ones
+          const double y = step == 0 ? static_cast<double>(z.k) - static_cast<double>(k_before) : fmax((target - w_before) / one, 0.0);
+          need = static_cast<uint64_t>(fmin(step == 3 ? __builtin_floor(y) + 1.0 : fmax(__builtin_ceil(y), 1.0), static_cast<double>(many)));
+          from[0] = to[0] = l;
+          if (step < 2) {
+            const uint64_t at_cut = order_of(key_of(l), 0xfffffu);
+            kept = fmin(kept, w_before + static_cast<double>(need) * one);
+            if (at_cut < cut || (at_cut == cut && need < cut_need)) cut = at_cut, cut_need = need, cut_value = l;
+            if (q.mode != kBeams) continue;
+            need = z.k;
+            to[0] = P::BIG;
+          }
+        }
+        if (to[0] == P::BIG) to[0] = __builtin_huge_valf();
+      } else if (step == 1 || step == 3) {
         // the bin: the first whose running sum reaches the target, or for the token exceeds it
         const double gone = skip != kNone ? drafted_w : 0.0;
         auto w = [&](int e) { return 2 * tid + e >= drafted_bin ? my_upto[e] - gone : my_upto[e]; };
@@ -946,26 +1249,46 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         from[1] = __builtin_huge_valf();
         to[1] = -__builtin_huge_valf();
       }
+      // bf16, one value: its pattern in both halves of a word (of 0 without the sign)
+      const bool one_value = by_value && from[0] == to[0];
+      const uint32_t sign = from[0] == 0.0f ? 0x7fff7fffu : 0xffffffffu, half = __float_as_uint(from[0]) >> 16, same = (half << 16 | half) & sign;
       const int pieces = x.count();
       constexpr int AHEAD = 8, MASKS = AHEAD * P::N / 32;
       uint4 next[AHEAD];
 #pragma unroll
-      for (int a = 0; a < AHEAD; ++a) next[a] = a * NT + tid < pieces ? x.load(a * NT + tid) : P::none();
+      for (int a = 0; a < AHEAD; ++a) next[a] = x.load(a * NT + tid, pieces);
       for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
         uint32_t mine[MASKS];
+        uint4 now[AHEAD];
 #pragma unroll
         for (int k = 0; k < MASKS; ++k) mine[k] = 0;
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-          const uint4 v = next[a];
+          now[a] = next[a];
           const int piece = p0 + (AHEAD + a) * NT + tid;
-          if (p0 + AHEAD * NT < pieces) next[a] = piece < pieces ? x.load(piece) : P::none();
+          if (p0 + AHEAD * NT < pieces) next[a] = x.load(piece, pieces);
+        }
+        if (DT == MZK_BF16 && one_value) {
+          // halves of words equal to one pattern: of the exclusive or, those that are 0
 #pragma unroll
-          for (int i = 0; i < P::N; ++i) {
-            const float l = P::at(v, i);  // (a NaN is in no range)
-            const bool in = (l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1]);
-            mine[a * P::N / 32] |= static_cast<uint32_t>(in) << (a * P::N % 32 + i);
+          for (int a = 0; a < AHEAD; ++a) {
+            const uint32_t v[4] = {now[a].x, now[a].y, now[a].z, now[a].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t d = (v[i] & sign) ^ same, other = ((d & 0x7fff7fffu) + 0x7fff7fffu) | d;  // bits 15, 31: not equal
+              const uint32_t equal = ~other & 0x80008000u;
+              mine[a * P::N / 32] |= (equal >> 15 & 1u) << (a * P::N % 32 + 2 * i) | (equal >> 31) << (a * P::N % 32 + 2 * i + 1);
+            }
           }
+        } else {
+#pragma unroll
+          for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) {
+              const float l = P::at(now[a], i);  // (a NaN is in no range)
+              const bool in = (l >= from[0] && l <= to[0]) || (l >= from[1] && l <= to[1]);
+              mine[a * P::N / 32] |= static_cast<uint32_t>(in) << (a * P::N % 32 + i);
+            }
         }
         uint32_t many = 0;
 #pragma unroll
@@ -1017,8 +1340,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         }
       }
     };
-    const double u_bin = unit_of(b0);
-    if (step == 2) {
+    const double u_bin = by_value ? 0.0 : unit_of(b0);
+    if (step == 2 && !by_value) {
       // ---- the weights of those that reach min-p ----
       __syncthreads();
       if (tid == 0) sel[2] = 0;
@@ -1037,14 +1360,16 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
       continue;
     }
     // ---- the token at which the running sum, of ones or of weights, reaches `need` ----
-    const bool by_count = step == 0;
-    uint64_t lo, hi, need;
+    const bool by_count = step == 0 || by_value;
+    uint64_t lo, hi;
     {
-      float from, to;
-      logits_of(b0, b1, from, to);
-      lo = order_of(key_of(fminf(to, kBig) + 0.0f), 0);
-      hi = order_of(key_of(from + 0.0f), 0xfffffu);
-      if (by_count) {
+      float least = from[0], most = to[0];
+      if (!by_value) logits_of(b0, b1, least, most);
+      lo = order_of(key_of(fminf(most, kBig) + 0.0f), 0);
+      hi = order_of(key_of(least + 0.0f), 0xfffffu);
+      if (by_value) {
+        // (known)
+      } else if (by_count) {
         need = static_cast<uint64_t>(z.k) - (b0 > 0 ? cn[b0 - 1] : 0u);
       } else {
         const double y = fmax((target - start) / u_bin, 0.0);
@@ -1118,7 +1443,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         drawn = x[static_cast<int>(token)];
       } else {
         cut = found_at < cut ? found_at : cut;
-        kept = fmin(kept, before(b0) + static_cast<double>(__shfl(w, at, 64)) * u_bin);
+        if (!by_value) kept = fmin(kept, before(b0) + static_cast<double>(__shfl(w, at, 64)) * u_bin);
       }
     }
     if (q.mode == kBeams) break;  // uniform
@@ -1197,7 +1522,7 @@ __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
   const int b = blockIdx.x / q.rest_chunks, chunk = blockIdx.x - b * q.rest_chunks;
   const int row = q.refused[b];
   if (row < 0) return;
-  const Pieces<DT> x(q.logits + row * q.stride, q.V);
+  const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
   uint64_t s = 0;
@@ -1235,7 +1560,7 @@ __global__ void __launch_bounds__(256) redraw_kernel(const SamplingParams q) {
   if (before < need && need <= before + mine) at_chunk = tid, at_before = before;
   __syncthreads();
   uint64_t sum = at_before;
-  const Pieces<DT> x(q.logits + row * q.stride, q.V);
+  const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
   for (int k = 0; k < kRestElements / 256; ++k) {
@@ -1305,8 +1630,12 @@ __global__ void __launch_bounds__(1024) beams_kernel(const SamplingParams q, int
 
 // ---- host -----------------------------------------------------------------------------------------
 
-// fp32 rows from so many on, or so short ones, are a workgroup's each; 16-bit ones always.
-constexpr int kWholeRows = 192, kWholeVocab = 65536;
+// Up to how many rows of V their chunks have workgroups of their own.  Four launches cost some 29 us and 2e-6 us an
+// element of all rows; one launch some 20 us and 3.2e-4 us an element of a row, of bf16 by value 25 us and 1.45e-4 us.
+// So the borders' two sides, split and whole: fp32, 131072: 52.9 and 62.6 us with 64 rows, 68.7 and 63.8 with 128;
+// 65536: 31.5 and 41.1 with 32, 52.6 and 42.7 with 128, 32768: 28.8 and 30.0 with 1; fp16, 65536: 38.5 and 43.4 with 64, 49.5 and 44.9 with 128;
+// bf16, 131072: 39.6 and 45.9 with 32, 48.4 and 46.4 with 64; 65536: 31.7 and 36.0 with 32, 38.4 and 36.3 with 64.
+int64_t split_rows(int64_t V, int dtype) { return dtype == MZK_BF16 ? 72 - (3 << 20) / V : 144 - (5 << 20) / V; }
 
 int64_t up(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
 
@@ -1367,7 +1696,7 @@ int launch(const SamplingParams& q, hipStream_t s) {
   if (q.chunks == 1) {
     if (!raise_lds(row_kernel<DT, kWholeRow>, kRowLds, whole_set)) return MZK_ELAUNCH;
     row_kernel<DT, kWholeRow><<<rows, kRowThreads, kRowLds, s>>>(q);
-  } else if constexpr (DT == MZK_F32) {
+  } else {
     if (!raise_lds(row_kernel<DT, kFinishPart>, kRowLds, finish_set)) return MZK_ELAUNCH;
     const unsigned grid = (rows + 7) / 8 * 8 * static_cast<unsigned>(q.chunks);
     survey_kernel<DT><<<grid, kSurveyThreads, 0, s>>>(q);
@@ -1403,11 +1732,10 @@ int rows_of(SamplingParams& q, const char* name, int64_t rows, int64_t V, int dt
   q.V = static_cast<int>(V);
   q.scale = 62;
   while ((static_cast<int64_t>(1) << (62 - q.scale)) < V) --q.scale;
-  // Chunks: of whole steps of a survey's workgroup, so that there are some 512 workgroups; none from 128 rows on.
-  // (7 elements of the first piece may belong to no row.)
-  const int64_t step = kSurveyThreads * kSurveyElements * size_of(dtype) / 16, pieces = (V + 7) * size_of(dtype) / 16 + 1;
+  // Chunks: of whole steps of a survey's workgroup, so that there are some 512 workgroups.
+  const int64_t step = kSurveyThreads * kSurveyElements * size_of(dtype) / 16, pieces = V * size_of(dtype) / 16 + 2;
   const int64_t steps = (pieces + step - 1) / step;
-  int64_t chunks = dtype != MZK_F32 || rows >= kWholeRows || rows == 0 || V <= kWholeVocab ? 1 : 512 / rows;
+  int64_t chunks = rows == 0 || rows > split_rows(V, dtype) ? 1 : 512 / rows;
   if (chunks > kMostChunks) chunks = kMostChunks;
   if (chunks > steps) chunks = steps;
   const int64_t per = (steps + chunks - 1) / chunks;
