@@ -1505,18 +1505,36 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
 
 // ---- verify: the sequences ------------------------------------------------------------------------
 
-// The first refused token of each sequence; without the draft's probabilities, and where none is refused, the
-// token of that row is the next.
-__global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
-  const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b >= q.B) return;
+// The rows of sequence b: the first whose drafted token is refused, or the last (by a whole wave; -1: no rows).
+__device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, int& first, int& end, int& token) {
   auto clamp = [&](int64_t v, int lo) -> int { return v < lo ? lo : v > q.rows ? q.rows : static_cast<int>(v); };
-  const int a = clamp(q.cu[b], 0), z = clamp(q.cu[b + 1], a);
-  int i = a;
-  while (i + 1 < z && q.rowres[i].accepted) ++i;
-  q.accepted[b] = i - a;
-  q.token[b] = z > a ? q.rowres[i].token : -1;
-  if (q.probs) q.refused[b] = i + 1 < z ? i : -1;
+  first = clamp(q.cu[b], 0);
+  end = clamp(q.cu[b + 1], first);
+  token = -1;
+  for (int i0 = first; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    const Row* const r = q.rowres + (i < end ? i : end - 1);
+    const int accepted = r->accepted, its = r->token;
+    const uint64_t stop = __ballot(i < end && (i + 1 == end || !accepted));
+    if (stop) {
+      const int at = __builtin_ctzll(stop);
+      token = __builtin_amdgcn_readlane(its, at);
+      return i0 + at;
+    }
+  }
+  return -1;
+}
+
+// The sequences, a wave each: without the draft's probabilities, and where no token is refused, the token of that row is
+// the next.
+__global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
+  const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b >= q.B) return;
+  int first, end, token;
+  const int i = judged(q, b, lane, first, end, token);
+  if (lane != 0) return;
+  q.accepted[b] = i < 0 ? 0 : i - first;
+  q.token[b] = token;
 }
 
 // What the target has above the draft at token i, 2^52 a probability of 1.
@@ -1531,26 +1549,34 @@ __device__ __forceinline__ uint64_t above(const SamplingParams& q, const Setting
   return d > 0.0 ? static_cast<uint64_t>(d * 0x1p52) : 0;
 }
 
-constexpr int kRestElements = 4096;  // of a chunk
+constexpr int kRestElements = 1024;  // of a chunk: 4 of a thread
 
+// With the draft's probabilities: the sequences, and of refused tokens' rows the sums of what the target has above the draft.
 template <int DT>
 __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
   __shared__ unsigned long long sums[4];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.x / q.rest_chunks, chunk = blockIdx.x - b * q.rest_chunks;
-  const int row = q.refused[b];
-  if (row < 0) return;
+  int first, end, token;
+  const int row = judged(q, b, lane, first, end, token);
+  const bool refused = row >= 0 && row + 1 < end;  // uniform
+  if (chunk == 0 && tid == 0) {
+    q.accepted[b] = row < 0 ? 0 : row - first;
+    q.token[b] = token;
+    q.refused[b] = refused ? row : -1;
+  }
+  if (!refused) return;
   const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
   uint64_t s = 0;
-#pragma unroll 4
+#pragma unroll
   for (int k = 0; k < kRestElements / 256; ++k) {
     const int i = chunk * kRestElements + 256 * k + tid;
     if (i < q.V) s += above<DT>(q, z, r, row, x[i], i);
   }
   s = wave_sum(s);
-  if ((tid & 63) == 0) sums[tid >> 6] = s;
+  if (lane == 0) sums[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) q.rest[static_cast<int64_t>(b) * q.rest_chunks + chunk] = sums[0] + sums[1] + sums[2] + sums[3];
 }
@@ -1559,40 +1585,55 @@ __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
 // nothing it stays the one from the target itself).
 template <int DT>
 __global__ void __launch_bounds__(256) redraw_kernel(const SamplingParams q) {
-  __shared__ unsigned long long sums[4], at_before;
+  constexpr int PER = 4;  // chunks of a thread, at most 2^20 / kRestElements in all, and elements
+  static_assert(kMaxVocab / kRestElements <= 256 * PER && kRestElements == 256 * PER, "redraw");
+  __shared__ unsigned long long sums[4], part[4], at_before;
   __shared__ int at_chunk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   const int row = q.refused[b];
   if (row < 0) return;
-  // a chunk is a thread's: at most 2^20 / 4096 of them
-  const uint64_t mine = tid < q.rest_chunks ? q.rest[static_cast<int64_t>(b) * q.rest_chunks + tid] : 0;
-  const uint64_t upto = wave_scan(mine);
+  uint64_t mine[PER], upto = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = PER * tid + k;
+    mine[k] = c < q.rest_chunks ? q.rest[static_cast<int64_t>(b) * q.rest_chunks + c] : 0;
+    upto += mine[k];
+  }
+  const uint64_t of_me = upto;
+  upto = wave_scan(upto);
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
   const uint64_t total = sums[0] + sums[1] + sums[2] + sums[3];
   if (total == 0) return;  // uniform
   uint64_t need = static_cast<uint64_t>(unit(q.draw[b]) * static_cast<double>(total)) + 1;
   if (need > total) need = total;
-  uint64_t before = upto - mine;
-  for (int w = 0; w < wave; ++w) before += sums[w];
-  if (before < need && need <= before + mine) at_chunk = tid, at_before = before;
+  uint64_t at = upto - of_me;
+  for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (at < need && need <= at + mine[k]) at_chunk = PER * tid + k, at_before = at;
+    at += mine[k];
+  }
   __syncthreads();
-  uint64_t sum = at_before;
   const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
   const Settings z = settings(q, row);
   const Row r = q.rowres[row];
-  for (int k = 0; k < kRestElements / 256; ++k) {
-    const int i = at_chunk * kRestElements + 256 * k + tid;
-    const uint64_t v = i < q.V ? above<DT>(q, z, r, row, x[i], i) : 0;
-    const uint64_t s = wave_scan(v);
-    __syncthreads();
-    if (lane == 63) sums[wave] = s;
-    __syncthreads();
-    uint64_t at = sum;
-    for (int w = 0; w < wave; ++w) at += sums[w];
-    if (at + s - v < need && need <= at + s) q.token[b] = i;
-    sum += sums[0] + sums[1] + sums[2] + sums[3];
-    if (sum >= need) break;  // uniform
+  const int i0 = at_chunk * kRestElements + PER * tid;
+  uint64_t s = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    mine[k] = i0 + k < q.V ? above<DT>(q, z, r, row, x[i0 + k], i0 + k) : 0;
+    s += mine[k];
+  }
+  upto = wave_scan(s);
+  if (lane == 63) part[wave] = upto;
+  __syncthreads();
+  at = at_before + upto - s;
+  for (int w = 0; w < wave; ++w) at += part[w];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (at < need && need <= at + mine[k]) q.token[b] = i0 + k;
+    at += mine[k];
   }
 }
 
@@ -1723,8 +1764,9 @@ int launch(const SamplingParams& q, hipStream_t s) {
     row_kernel<DT, kFinishPart><<<rows, kRowThreads, kRowLds, s>>>(q);
   }
   if (q.mode == kVerify) {
-    verify_kernel<<<static_cast<unsigned>((q.B + 255) / 256), 256, 0, s>>>(q);
-    if (q.probs) {
+    if (!q.probs) {
+      verify_kernel<<<static_cast<unsigned>((q.B + 3) / 4), 256, 0, s>>>(q);
+    } else {
       rest_kernel<DT><<<static_cast<unsigned>(q.B) * static_cast<unsigned>(q.rest_chunks), 256, 0, s>>>(q);
       redraw_kernel<DT><<<static_cast<unsigned>(q.B), 256, 0, s>>>(q);
     }
@@ -1836,7 +1878,7 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   SamplingParams q{};
   q.mode = kVerify;
   if (const int rc = rows_of(q, "verify", T, V, dtype)) return rc;
-  MZK_CHECK_ARG(B >= 0 && B < 1 << 22 && B * q.rest_chunks < 1 << 24, "verify: bad sizes");
+  MZK_CHECK_ARG(B >= 0 && B < 1 << 22 && (!draft_probs || B * q.rest_chunks < 1 << 24), "verify: bad sizes");
   if (B == 0) return MZK_OK;
   MZK_CHECK_ARG(cu && accepted && next && draw && (T == 0 || (tokens && u)), "verify: null pointer");
   MZK_CHECK_ARG(!draft_probs || draft_row_stride >= V || T <= 1, "verify: rows of the draft's probabilities overlap");
@@ -1856,7 +1898,7 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   q.token = next;
   if (T == 0) {  // no rows: sequences of nothing
     q.probs = nullptr;
-    verify_kernel<<<static_cast<unsigned>((B + 255) / 256), 256, 0, as_stream(stream)>>>(q);
+    verify_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, as_stream(stream)>>>(q);
     MZK_LAUNCH_CHECK("verify");
     return MZK_OK;
   }
