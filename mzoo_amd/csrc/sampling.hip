@@ -20,10 +20,10 @@
 // 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
 // row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
 //
-// Measured: fp32, 1 row of 131072: 7.1 + 10.2 + 4.7 + 13.1 us in four launches, of which reading would be 0.1 us: bound
-// by the launches' own steps, most of them barriers.  256 rows of 200019, with top-k, top-p and min-p by turns: 108 us,
-// 1.9 TB/s: bound by a compute unit's arithmetic on its row, some 22 instructions an element.  bf16, 64 rows of 131072:
-// 45.8 us; 160 rows: 64 us.  fp16, 16 rows of 32000: 23 us.
+// Measured: fp32, 1 row of 131072: 7.0 + 9.8 + 4.3 + 13.0 us in four launches, of which reading would be 0.1 us: bound
+// by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
+// turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
+// rows of 131072: 43 us, of which the count 10.8; 160 drafted rows: 48.  fp16, 16 rows of 32000: 23 us.
 #include "common.h"
 
 namespace mzk {
@@ -380,7 +380,8 @@ __device__ __forceinline__ int top_of(const Grid& g, float m) {
 
 // Pieces from .. to - 1 of a row into the histogram (and, counting, the numbers of tokens): bin k in place k mod
 // kBins, for the kBins - 1 bins from the largest on.  As that rises, places of bins that fall behind become its.
-// Bound by the LDS's atomic sums and the arithmetic, some 22 instructions an element; the next pieces are in flight meanwhile.
+// Bound by memory where all compute units read, else by the arithmetic, some 20 instructions an element, 12 of them in 64
+// bits (110 cycles a wave, of which they are 80; the atomic sums hide behind them: 56 us of 58 with narrower ones).
 template <int DT, int NT, int AHEAD>
 __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, bool counting, int from, int to, int tid,
                                            unsigned long long* hist /* [kBins][kCopies], and kAside */, uint32_t* counts /* the same */,
@@ -811,7 +812,9 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   if (PART == kFinishPart) r = plan->r;
   for (bool whole_row = PART == kWholeRow; PART != kFinishPart && !by_value; whole_row = true) {
     if (whole_row) {
-      r = survey<DT, NT, 8>(x, g, counting, 0, x.count(), tid, bins, bin_counts, tops, lds);
+      // (8 pieces at a time are more code to fetch than they gain: 64 rows of 4096, bf16, 27.6 us and 24.7 with 4, 23.5 with 2;
+      // 256 rows of 200019, fp32, 94.0, 93.5 and 99.1)
+      r = survey<DT, NT, 4>(x, g, counting, 0, x.count(), tid, bins, bin_counts, tops, lds);
       if (r.top > kNoTop) {
         surveyed_bin(r, 2 * tid, counting, bins, bin_counts, sum[0], num[0]);
         surveyed_bin(r, 2 * tid + 1, counting, bins, bin_counts, sum[1], num[1]);
