@@ -23,7 +23,7 @@
 // Measured: fp32, 1 row of 131072: 7.0 + 9.8 + 4.3 + 13.0 us in four launches, of which reading would be 0.1 us: bound
 // by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
 // turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
-// rows of 131072: 43 us, of which the count 10.8; 160 drafted rows: 48.  fp16, 16 rows of 32000: 23 us.
+// rows of 131072: 45 us, of which the count 12; 160 drafted rows: 49.5.  fp16, 16 rows of 32000: 23 us.
 #include "common.h"
 
 namespace mzk {
@@ -651,7 +651,32 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     for (int a = 0; a < AHEAD; ++a) next[a] = x.load(a * NT + tid, pieces);
     __syncthreads();
     uint32_t all = 0;
+    // A value that many lanes have, as that of a masked vocabulary, would be summed one lane after the other: each wave has a
+    // hot one, looked for in the first and the last of every 8 pieces, whose tokens each lane sums in a place of its own.
+    // (80 rows of 131072, whole calls: 45 us, 44 without this; all but 5000 tokens masked at random 45, and 178.)
+    uint8_t* const at = reinterpret_cast<uint8_t*>(tally);
+    uint32_t* const own = tally + 32768 + tid;
+    const uint32_t own_at = 4u * (32768u + tid);
+    uint32_t hot = 0xffffu;  // (a NaN)
+    *own = 0;
+    auto flush = [&]() {  // (its lanes' own; the order of a wave's accesses is kept)
+      const uint32_t n = *own;
+      if (hot == 0xff80u) all -= n >> 16;  // -inf: no tokens
+      else if (const uint32_t sum = wave_sum(n); lane == 0 && sum) atomicAdd(&tally[hot & 0x7fffu], sum);
+      *own = 0;
+    };
     for (int p0 = 0; p0 < pieces; p0 += AHEAD * NT) {
+      {
+        const bool full = p0 + AHEAD * NT <= pieces;  // (behind the row -inf is loaded)
+        const uint32_t v0 = next[0].x & 0xffffu, v1 = (full ? next[AHEAD - 1].x : next[0].x) & 0xffffu;
+        const uint32_t c0 = lane_of(v0, 0), c1 = lane_of(v1, 37);
+        const int n0 = __popcll(__ballot(v0 == c0)), n1 = __popcll(__ballot(v1 == c1));
+        const uint32_t c = n0 >= n1 ? c0 : c1;
+        if (max(n0, n1) >= 6 && c != hot) {  // uniform
+          flush();
+          hot = c;
+        }
+      }
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
         const uint32_t v[4] = {next[a].x, next[a].y, next[a].z, next[a].w};
@@ -659,25 +684,15 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         if (p0 + AHEAD * NT < pieces) next[a] = x.load(piece, pieces);
         if (p0 + a * NT + tid >= pieces) continue;
         all += P::N;
-        uint8_t* const at = reinterpret_cast<uint8_t*>(tally);
-        // one value throughout the wave, as in a masked vocabulary: one lane counts for all (the first word says that it
-        // is not, mostly; 64 rows of 131072: 10.8 us with both tests, 13.3 with the second alone, 9.3 with none)
-        const uint32_t one = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v[0])));
-        if (__builtin_expect(__ballot(v[0] != one) == 0, 0)) {
-          if (__ballot(v[1] != one || v[2] != one || v[3] != one || (one & 0xffffu) != one >> 16) == 0) {
-            const uint64_t here = __ballot(true);
-            if (lane == __builtin_ctzll(here))
-              atomicAdd(reinterpret_cast<uint32_t*>(at + (one << 2 & 0x1fffcu)), (1u + (one >> 31) * 0xffffu) * static_cast<uint32_t>(P::N * __popcll(here)));
-            continue;
-          }
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          atomicAdd(reinterpret_cast<uint32_t*>(at + (v[i] << 2 & 0x1fffcu)), 1u + (v[i] >> 15 & 1u) * 0xffffu);
-          atomicAdd(reinterpret_cast<uint32_t*>(at + (v[i] >> 14 & 0x1fffcu)), 1u + (v[i] >> 31) * 0xffffu);
+          const uint32_t low = (v[i] & 0xffffu) == hot ? own_at : v[i] << 2 & 0x1fffcu, high = v[i] >> 16 == hot ? own_at : v[i] >> 14 & 0x1fffcu;
+          atomicAdd(reinterpret_cast<uint32_t*>(at + low), 1u + (v[i] >> 15 & 1u) * 0xffffu);
+          atomicAdd(reinterpret_cast<uint32_t*>(at + high), 1u + (v[i] >> 31) * 0xffffu);
         }
       }
     }
+    flush();
     all = wave_sum(all);
     if (lane == 0) partn[wave] = all;
     __syncthreads();
@@ -738,17 +753,21 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
       end_count = end_heavy;
       const float least = first < END ? value_of(128u * end_heavy - 1u) : -P::BIG;
       uint32_t are = 0;
-      for (int p = tid; p < pieces; p += NT) {
-        const uint4 v = x.load(p, pieces);
+      for (int p0 = tid; p0 < pieces; p0 += 8 * NT) {
+        uint4 v[8];
 #pragma unroll
-        for (int i = 0; i < P::N; ++i) are += P::at(v, i) >= least;
+        for (int i = 0; i < 8; ++i) v[i] = x.load(p0 + i * NT, pieces);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < P::N; ++e) are += P::at(v[i], e) >= least;
       }
       const uint32_t theirs = wave_sum(tid < end_count && tid >= FIRST ? mine : 0u), seen = wave_sum(are);
       if (lane == 0) partn[wave] = theirs - seen;
       __syncthreads();
       uint32_t differ = 0;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) differ |= partn[w];
+      for (int w = 0; w < NW; ++w) differ += partn[w];
       by_value = differ == 0 && number[0] == 0 && q.mode != kBeams;
       __syncthreads();
     }
@@ -1730,7 +1749,7 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
   return at;
 }
 
-constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2)), kBinsLds = 12 * (kCopies * kBins + kAside);
+constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2)) + 4 * kRowThreads, kBinsLds = 12 * (kCopies * kBins + kAside);
 static_assert(kBinsLds <= kRowLds && kBinsLds + 20 * 1024 <= 64 * 1024, "LDS");
 
 // The dynamic-LDS limit is a per-device function attribute: set once per device.

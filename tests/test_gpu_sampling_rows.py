@@ -231,3 +231,28 @@ def test_many_rows_captured(dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [20000, 99991])
+def test_sample_runs_of_values(dev, v, dtype):
+    """Runs of one value after another, of any length, between other tokens: counts of values change over within the row."""
+    g = torch.Generator().manual_seed(v)
+    x = _logits(MANY, v, v, dtype)
+    values = torch.tensor([-float("inf"), 0.0, -0.0, 1.5, -2.0, 3.0, float("nan"), torch.finfo(dtype).min])
+    for row in range(12):
+        at = 0
+        while at < v:
+            n = int(2 ** (16 * torch.rand(1, generator=g)))
+            if row % 2 == 0 or torch.rand(1, generator=g) < 0.5:
+                x[row, at:at + n] = values[torch.randint(0, 8, (1,), generator=g)].to(dtype)
+            at += n
+    for row in range(12, 16):                         # some of each everywhere
+        some = torch.rand(v, generator=g) < 0.2 * (row - 11)
+        x[row, some] = values[torch.randint(0, 8, (int(some.sum()),), generator=g)].to(dtype)
+    for i, f in enumerate((dict(), dict(top_k=500), dict(min_p=0.1), dict(temperature=0.5))):
+        u = _u(MANY, v + i)
+        print(f"{v} {dtype} {f}", flush=True)
+        got = sampling.sample(x.to(dev), u.to(dev), **f)
+        _check_near([t[:20].cpu() for t in got], x[:20], u[:20], f)
+    _check_beams(dev, x[:16], -_u(16, 1), 4, 20)
