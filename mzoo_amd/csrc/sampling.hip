@@ -20,7 +20,7 @@
 // 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
 // row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
 //
-// Measured: fp32, 1 row of 131072: 7.0 + 9.8 + 4.3 + 13.0 us in four launches, of which reading would be 0.1 us: bound
+// Measured: fp32, 1 row of 131072: 7.0 + 9.8 + 4.3 + 11.0 us in four launches, of which reading would be 0.1 us: bound
 // by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
 // turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
 // rows of 131072: 45 us, of which the count 12; 160 drafted rows: 49.5.  fp16, 16 rows of 32000: 23 us.
@@ -1134,6 +1134,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     }
     return;
   }
+  // the windows that the listed tokens are from (by value: of one alone)
+  const int windows = by_value ? 1 : (w1[0] >= w0[0]) + (w1[1] >= w0[1]) + (w1[2] >= w0[2]) + (w1[3] >= w0[3]);
   int n = 0;
   uint64_t cut = ~0ull;  // the last token that top-k and top-p keep
   double kept = total;
@@ -1464,82 +1466,98 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     }
     uint64_t passed = 0;  // weights and numbers before lo
     uint32_t passed_n = 0;
-    while (true) {
-      const int bits = 64 - __builtin_clzll(hi - lo | 1), sh = bits > 10 ? bits - 10 : 0;
-      __syncthreads();
-      hist[tid] = hist[NT + tid] = 0;
-      counts[tid] = counts[NT + tid] = 0;
-      if (tid == 0) sel[0] = 0, sel[1] = passed, sel[2] = passed_n, number[1] = 0;
-      __syncthreads();
-      each(lo, hi, [&](uint64_t me, float l) {
-        const uint32_t digit = static_cast<uint32_t>((me - lo) >> sh), bits = __float_as_uint(l);
-        const uint64_t w = second(l);
-        bool left = true;
-        if (!in_list) {
-          // the lanes with the same logit and digit, of which a row of few values has many, by one of them
-#pragma unroll 1
-          for (uint64_t todo = __ballot(true); todo;) {
-            const int leader = __builtin_ctzll(todo);
-            const bool like = left && digit == lane_of(digit, leader) && bits == lane_of(bits, leader);
-            const uint64_t same = __ballot(like);
-            const uint32_t many = static_cast<uint32_t>(__popcll(same));
-            if (many < 8) break;  // uniform
-            if (lane == leader) {
-              atomicAdd(&hist[digit], static_cast<unsigned long long>(many * w));
-              atomicAdd(&counts[digit], many);
+    // Of a short list the tokens are gathered at once, without a digit: mostly few of them are in these bins.  (fp32, whole
+    // calls, top-k, top-p and min-p: 1 row of 131072 32.4 us for 34.3, 64 of 4096 20.4 for 22.8; the others +-1.)
+    for (bool direct = in_list && n <= 64 * windows;; direct = false) {
+      while (!direct) {
+        const int bits = 64 - __builtin_clzll(hi - lo | 1), sh = bits > 10 ? bits - 10 : 0;
+        __syncthreads();
+        hist[tid] = hist[NT + tid] = 0;
+        counts[tid] = counts[NT + tid] = 0;
+        if (tid == 0) sel[0] = 0, sel[1] = passed, sel[2] = passed_n, number[1] = 0;
+        __syncthreads();
+        each(lo, hi, [&](uint64_t me, float l) {
+          const uint32_t digit = static_cast<uint32_t>((me - lo) >> sh), bits = __float_as_uint(l);
+          const uint64_t w = second(l);
+          bool left = true;
+          if (!in_list) {
+            // the lanes with the same logit and digit, of which a row of few values has many, by one of them
+  #pragma unroll 1
+            for (uint64_t todo = __ballot(true); todo;) {
+              const int leader = __builtin_ctzll(todo);
+              const bool like = left && digit == lane_of(digit, leader) && bits == lane_of(bits, leader);
+              const uint64_t same = __ballot(like);
+              const uint32_t many = static_cast<uint32_t>(__popcll(same));
+              if (many < 8) break;  // uniform
+              if (lane == leader) {
+                atomicAdd(&hist[digit], static_cast<unsigned long long>(many * w));
+                atomicAdd(&counts[digit], many);
+              }
+              left = left && !like;
+              todo &= ~same;
             }
-            left = left && !like;
-            todo &= ~same;
           }
+          if (left) {
+            atomicAdd(&hist[digit], static_cast<unsigned long long>(w));
+            atomicAdd(&counts[digit], 1u);
+          }
+        });
+        __syncthreads();
+        // digits 2 tid, 2 tid + 1
+        const uint64_t v0 = hist[2 * tid], v1 = hist[2 * tid + 1];
+        const uint32_t n0 = counts[2 * tid], n1 = counts[2 * tid + 1];
+        const uint64_t s = wave_scan(v0 + v1);
+        const uint32_t sn = wave_scan(n0 + n1);
+        if (lane == 63) part[wave] = s, partn[wave] = sn;
+        __syncthreads();
+        uint64_t w = passed + s - v0 - v1, all = passed;
+        uint32_t k = passed_n + sn - n0 - n1, all_n = passed_n;
+  #pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          if (i < wave) w += part[i], k += partn[i];
+          all += part[i];
+          all_n += partn[i];
         }
-        if (left) {
-          atomicAdd(&hist[digit], static_cast<unsigned long long>(w));
-          atomicAdd(&counts[digit], 1u);
+        const uint64_t most = by_count ? all_n : all;
+        if (need > most) need = most;
+        const uint64_t a = by_count ? k : w, c = a + (by_count ? n0 : v0), e = c + (by_count ? n1 : v1);
+        if (a < need && need <= c) sel[0] = static_cast<uint64_t>(2 * tid) | static_cast<uint64_t>(n0) << 32, sel[1] = w, sel[2] = k;
+        if (c < need && need <= e) sel[0] = static_cast<uint64_t>(2 * tid + 1) | static_cast<uint64_t>(n1) << 32, sel[1] = w + v0, sel[2] = k + n0;
+        __syncthreads();
+        const uint64_t got = sel[0];
+        passed = sel[1];
+        passed_n = static_cast<uint32_t>(sel[2]);
+        lo = lo + ((got & 0xffffffffu) << sh);
+        const uint64_t top = lo + ((1ull << sh) - 1ull);
+        hi = top < hi ? top : hi;
+        if ((got >> 32) <= 64 || sh == 0) break;  // uniform
+      }
+      if (direct) {  // uniform
+        __syncthreads();
+        if (tid == 0) number[1] = 0;
+        __syncthreads();
+      }
+      // ---- at most 64: gathered, and every wave sums them in their order ----
+      each(lo, hi, [&](uint64_t me, float l) {
+        const uint32_t to = atomicAdd(&number[1], 1u);
+        if (to < 64) {
+          last_ones[to][0] = me;
+          last_ones[to][1] = second(l);
         }
       });
       __syncthreads();
-      // digits 2 tid, 2 tid + 1
-      const uint64_t v0 = hist[2 * tid], v1 = hist[2 * tid + 1];
-      const uint32_t n0 = counts[2 * tid], n1 = counts[2 * tid + 1];
-      const uint64_t s = wave_scan(v0 + v1);
-      const uint32_t sn = wave_scan(n0 + n1);
-      if (lane == 63) part[wave] = s, partn[wave] = sn;
-      __syncthreads();
-      uint64_t w = passed + s - v0 - v1, all = passed;
-      uint32_t k = passed_n + sn - n0 - n1, all_n = passed_n;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        if (i < wave) w += part[i], k += partn[i];
-        all += part[i];
-        all_n += partn[i];
-      }
-      const uint64_t most = by_count ? all_n : all;
-      if (need > most) need = most;
-      const uint64_t a = by_count ? k : w, c = a + (by_count ? n0 : v0), e = c + (by_count ? n1 : v1);
-      if (a < need && need <= c) sel[0] = static_cast<uint64_t>(2 * tid) | static_cast<uint64_t>(n0) << 32, sel[1] = w, sel[2] = k;
-      if (c < need && need <= e) sel[0] = static_cast<uint64_t>(2 * tid + 1) | static_cast<uint64_t>(n1) << 32, sel[1] = w + v0, sel[2] = k + n0;
-      __syncthreads();
-      const uint64_t got = sel[0];
-      passed = sel[1];
-      passed_n = static_cast<uint32_t>(sel[2]);
-      lo = lo + ((got & 0xffffffffu) << sh);
-      const uint64_t top = lo + ((1ull << sh) - 1ull);
-      hi = top < hi ? top : hi;
-      if ((got >> 32) <= 64 || sh == 0) break;  // uniform
+      if (!direct || number[1] <= 64) break;  // uniform
     }
-    // ---- at most 64: gathered, and every wave sums them in their order ----
-    each(lo, hi, [&](uint64_t me, float l) {
-      const uint32_t to = atomicAdd(&number[1], 1u);
-      last_ones[to][0] = me;
-      last_ones[to][1] = second(l);
-    });
-    __syncthreads();
     const int m = static_cast<int>(number[1]);
     const uint64_t me = lane < m ? last_ones[lane][0] : ~0ull, mine = lane < m ? last_ones[lane][1] : 0;
     uint64_t w = passed;
     uint32_t k = passed_n;
-    for (int i = 0; i < m; ++i)
+    uint64_t all = passed;
+    for (int i = 0; i < m; ++i) {
+      all += last_ones[i][1];
       if (last_ones[i][0] <= me) w += last_ones[i][1], ++k;
+    }
+    need = min(need, by_count ? passed_n + static_cast<uint64_t>(m) : all);
     const uint64_t measure = by_count ? k : w, one = by_count ? 1 : mine;
     const uint64_t hit = __ballot(lane < m && measure >= need && measure - one < need);
     if (hit) {
