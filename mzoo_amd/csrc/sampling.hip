@@ -20,10 +20,10 @@
 // 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
 // row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
 //
-// Measured: fp32, 1 row of 131072: 7.0 + 9.8 + 4.3 + 11.0 us in four launches, of which reading would be 0.1 us: bound
+// Measured: fp32, 1 row of 131072: 6.9 + 9.7 + 4.5 + 10.3 us in four launches, of which reading would be 0.1 us: bound
 // by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
 // turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
-// rows of 131072: 45 us, of which the count 12; 160 drafted rows: 49.5.  fp16, 16 rows of 32000: 23 us.
+// rows of 131072: 44 us, of which the count 12; 160 drafted rows: 50.  fp16, 16 rows of 32000: 22 us.
 #include "common.h"
 
 namespace mzk {
