@@ -715,8 +715,8 @@ int mzk_sample(const void* logits, int dtype, int64_t rows, int64_t V, int64_t r
  * sequence is judged by row i.  With p its probability behind the filters and q the draft's (draft_probs[i,
  * tokens[i + 1]], rows draft_row_stride elements apart; NULL: 1) it is accepted if u[i] q < p.  accepted[b]: the
  * tokens before the first refused one.  next[b]: drawn with draw[b] from the last row, or from the refused
- * token's row: without draft_probs as mzk_sample does, without that token; with them from max(p - q, 0) by rising index
- * (from p where that is nothing).  A sequence of no rows: 0 and -1. */
+ * token's row: without draft_probs as mzk_sample does, without that token; with them from max(p - q, 0) by rising index,
+ * in units of 2^-52 (from p where that is nothing).  A sequence of no rows: 0 and -1. */
 int mzk_verify_workspace_bytes(int64_t T, int64_t B, int64_t V, int dtype, int probs, int64_t* bytes);
 int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, int64_t row_stride, const int64_t* tokens,
                const int64_t* cu, int64_t B, const float* u, const float* draw, const float* draft_probs,

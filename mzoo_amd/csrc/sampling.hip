@@ -1441,7 +1441,9 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         need = static_cast<uint64_t>(z.k) - (b0 > 0 ? cn[b0 - 1] : 0u);
       } else {
         const double y = fmax((target - start) / u_bin, 0.0);
-        need = step == 3 ? static_cast<uint64_t>(y) + 1 : static_cast<uint64_t>(__builtin_ceil(y));
+        // (a border that is hit exactly, as with equal weights, is: y is off by some 2^-51 of itself, and a float32's share
+        // of at most 2^20 equal ones that is on no border lies 2^-45 and more from it)
+        need = step == 3 ? static_cast<uint64_t>(y * (1.0 + 0x1p-48)) + 1 : static_cast<uint64_t>(__builtin_ceil(y * (1.0 - 0x1p-48)));
       }
       if (need < 1) need = 1;
     }

@@ -152,8 +152,8 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu: torch.Tensor, u: torc
     the vocabulary are refused.  Returns (accepted int64 [B], next int64 [B]): the drafted tokens before the first
     refused one, and the token behind those, drawn with ``draw`` fp32 [B]: where none was refused from the
     last row as ``sample`` does; else from what the refused token's row has above the draft -- without
-    ``draft_probs`` its other tokens, in their order, with them ``max(p - q, 0)`` by rising index (from p where that
-    is nothing).  A sequence of no rows gives 0 and -1; rows behind the last sequence are not read.  Filters, ``out=(accepted,
+    ``draft_probs`` its other tokens, in their order, with them ``max(p - q, 0)`` by rising index, in units of 2^-52 (from p
+    where that is nothing).  A sequence of no rows gives 0 and -1; rows behind the last sequence are not read.  Filters, ``out=(accepted,
     next)`` and ``workspace`` (``verify_workspace_bytes``) as in ``sample``."""
     _one_device("verify", logits, tokens, cu, u, draw, draft_probs, workspace)
     logits, rows, v, stride = _logits("verify", logits)

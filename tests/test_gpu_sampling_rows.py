@@ -256,3 +256,22 @@ def test_sample_runs_of_values(dev, v, dtype):
         got = sampling.sample(x.to(dev), u.to(dev), **f)
         _check_near([t[:20].cpu() for t in got], x[:20], u[:20], f)
     _check_beams(dev, x[:16], -_u(16, 1), 4, 20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 150])
+def test_sample_equal_logits_behind_a_mask(dev, dtype, rows):
+    """All weights 1, and none among a row's first logits: borders that are hit exactly."""
+    v, n = 46130, 15430
+    x = torch.full((rows, v), -float("inf"))
+    x[:, v - 2 * n::2] = -100.0
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(3))
+    u[0], u[1] = 0.5, 0.25
+    for t in (1.7, 0.3, 1.0, 77.0):
+        for f in (dict(top_p=0.5), dict(), dict(top_p=0.25, top_k=n // 2 * 2), dict(top_p=0.75, min_p=1.0), dict(top_k=8192)):
+            _check_sample(dev, x[:2], u[:2], temperature=t, **f)
+            if rows > 2:
+                got = sampling.sample(x.to(dev), u.to(dev), temperature=t, **f)
+                for i in range(0, rows, 7):
+                    assert got[0][i].item() == R.sample(x[i].float().numpy(), u[i].item(), temperature=t, **f)[0]
