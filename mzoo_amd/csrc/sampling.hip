@@ -1168,7 +1168,22 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         double left = kept;
         if (drafted != kNone) {
           const float l = logit_of_key(drafted_key);
-          if (order_of(drafted_key, drafted) <= cut && !beyond && reaches(l)) {
+          const uint64_t its = order_of(drafted_key, drafted);
+          bool stays = its <= cut && !beyond && reaches(l);
+          if (__builtin_expect(stays && counting && cut == ~0ull && drafted_bin == kRest, 0)) {  // uniform
+            // top-k may end among tokens too light for the sums, of which this is one: those before it are counted
+            uint32_t m = 0;
+            x.template walk<NT>(tid, [&](int i, float of) __attribute__((always_inline)) { m += order_of(key_of(of), static_cast<uint32_t>(i)) < its; });
+            m = wave_sum(m);
+            __syncthreads();
+            if (lane == 0) partn[wave] = m;
+            __syncthreads();
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) m += partn[i];
+            stays = m < static_cast<uint32_t>(z.k);
+          }
+          if (stays) {
             const double w = exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
             const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + drafted]) : 1.0;
             accepted = static_cast<double>(q.u[row]) * sure * kept < w;
