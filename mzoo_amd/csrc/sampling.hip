@@ -25,13 +25,11 @@
 // turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
 // rows of 131072: 44 us, of which the count 12; 160 drafted rows: 50.  fp16, 16 rows of 32000: 22 us.
 #include "common.h"
+#include "sampling_numbers.h"
 
 namespace mzk {
 namespace {
 
-constexpr int kBins = 1024, kRest = kBins - 1;  // bins of a histogram; the last takes what is too small to count, 2^-51
-constexpr double kPerOctave = 20.0;
-constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr double kBelow = 1.0 - 0x1p-30, kAbove = 1.0 + 0x1p-30;  // slack of bounds
 constexpr int kCap = 16384;  // listed tokens of a row
 constexpr int64_t kMaxVocab = 1 << 20;
@@ -114,28 +112,6 @@ struct SamplingParams {
 };
 
 // ---- numbers --------------------------------------------------------------------------------
-
-// 2^t for t <= 1, to about 2^-51 of itself: the power series of exp(f ln 2) for |f| <= 1/2, whose
-// first term left out is (ln 2 / 2)^13 / 13! = 1.7e-16.
-__device__ __forceinline__ double exp2_of(double t) {
-  t = fmax(t, -1100.0);
-  const double n = __builtin_rint(t);
-  const double x = (t - n) * kLn2D;
-  double e = 1.0 / 479001600.0;
-  e = __builtin_fma(e, x, 1.0 / 39916800.0);
-  e = __builtin_fma(e, x, 1.0 / 3628800.0);
-  e = __builtin_fma(e, x, 1.0 / 362880.0);
-  e = __builtin_fma(e, x, 1.0 / 40320.0);
-  e = __builtin_fma(e, x, 1.0 / 5040.0);
-  e = __builtin_fma(e, x, 1.0 / 720.0);
-  e = __builtin_fma(e, x, 1.0 / 120.0);
-  e = __builtin_fma(e, x, 1.0 / 24.0);
-  e = __builtin_fma(e, x, 1.0 / 6.0);
-  e = __builtin_fma(e, x, 0.5);
-  e = __builtin_fma(e, x, 1.0);
-  e = __builtin_fma(e, x, 1.0);
-  return __builtin_ldexp(e, static_cast<int>(n));
-}
 
 // a b + c with c in scalar registers: left to itself the compiler copies c for the two-operand form.
 __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
@@ -661,10 +637,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     c0 = o < 0x8000u ? w.y & 0xffffu : w.x >> 16;
     c1 = o < 0x8000u ? w.x & 0xffffu : w.y >> 16;
   };
-  // the weight of a logit, in units of 2^-scale of the largest's
-  auto weight = [&](float l) __attribute__((always_inline)) -> double {
-    return exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
-  };
+  auto weight = [&](float l) __attribute__((always_inline)) -> double { return weight_of(l, r.max, z.s, q.scale); };
   if (DT == MZK_BF16 && PART == kWholeRow && q.V > kByValue) {
     // blocks of numbers: before them NaN and +inf, behind them -inf and NaN
     constexpr int FIRST = 1, END = 511, INF = 0x7f80, AHEAD = 8;

@@ -17,6 +17,42 @@ def _in_chunks(rows, v, dtype):
     return sampling.sample_workspace_bytes(rows, v, dtype) > 0
 
 
+def _verify(logits, tokens, u, draw, probs=None, **filters):
+    """One sequence, as ``R.verify``, also where probabilities are far below 2^-28.  A drafted token is accepted if u q W < w; w is off by at most
+    2^-45 of itself (2^-51 of its power, 2^-52 of at most 1100 of its exponent), W by less than 2^-29 of itself: the
+    comparison is sure unless u q and p are within 2^-28 of p.  What a refused token's row has above the draft is in units of 2^-52, so a
+    draw is off by at most V 2^-52 of their sum: 2^-32 for 2^17 tokens and a sum of 2^-3."""
+    n, v, clear = len(tokens), logits.shape[1], True
+    for i in range(n):
+        order, w, sure = R.kept(logits[i], **filters)
+        clear &= sure
+        if i == n - 1:
+            break
+        d = int(tokens[i + 1])
+        at = np.flatnonzero(order == d) if 0 <= d < v else []
+        p = w[at[0]] / w.sum() if len(at) else np.longdouble(0)
+        q = 1.0 if probs is None or not 0 <= d < v else float(probs[i][d])
+        a = np.longdouble(float(np.float32(u[i]))) * np.longdouble(q)
+        if p < np.longdouble(2) ** -1100:             # below the numbers of 64 bits
+            p = np.longdouble(0)
+        clear &= not (0 < p < 2.0 ** -1000 and a < 2.0 ** -900) and not (p > 0 and abs(a - p) <= 2.0 ** -28 * p and not p == q == 1)
+        if a < p:
+            continue
+        if probs is None:
+            if p < 1:
+                order, w = order[order != d], w[order != d]
+        elif order.size:
+            left = np.zeros(v, np.longdouble)
+            left[order] = w / w.sum()
+            left = np.maximum(left - np.asarray(probs[i], np.float64).astype(np.longdouble), 0)
+            if left.sum() > 0:
+                clear &= bool(left.sum() >= 0.125)
+                order, w = np.arange(v), left
+        break
+    token, sure = R.pick(order, w, draw)
+    return i, token, clear and sure
+
+
 # ---- tokens too light for the sums ------------------------------------------------------------
 
 @pytest.mark.parametrize("probs", [False, True])
@@ -63,3 +99,63 @@ def test_verify_top_k_ends_among_light_tokens(dev, dtype, v, sequences, chunks, 
         token, sure = R.pick(among, w, draw[b].item())
         assert clear and sure
         assert (acc[b], nxt[b]) == (0, token), f"sequence {b}: place {at[b]} of {k[2 * b]} kept ones: {acc[b]}, {nxt[b]}"
+
+
+# ---- temperatures at the ends of float32 ------------------------------------------------------
+
+ENDS = [1.401298464324817e-45, 1e-30, 1e-3, 0.01, 1e30, 3.4028234663852886e38, float("inf")]
+
+
+def _sharp(rows, v, dtype, seed):
+    """Rows whose largest logit lies low in its octave, high, at the ends of the type and below 0."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, v, generator=g) * 2.5
+    top = torch.finfo(dtype).max
+    for i, m in enumerate((40.0, 33.0, 63.5, 0.0, -17.0, top, 1e-4, -1e-4)):
+        x[i] = torch.minimum(x[i], torch.tensor(min(m, 60000.0))) if m >= 0 else -x[i].abs() + m
+        x[i, 7 + 1000 * i] = m
+    x[8] = -float("inf")
+    x[8, v - 3] = -top
+    x[9, ::2] = float("nan")
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,rows,v,chunks", [(torch.bfloat16, 80, 17000, False), (torch.bfloat16, 80, 131072, False),
+                                                 (torch.float16, 160, 17000, False), (torch.float32, 160, 17000, False),
+                                                 (torch.bfloat16, 10, 131072, True), (torch.float16, 10, 131072, True),
+                                                 (torch.float32, 10, 131072, True)])
+def test_temperatures_at_the_ends(dev, dtype, rows, v, chunks):
+    assert _in_chunks(rows, v, dtype) == chunks
+    x = _sharp(rows, v, dtype, v)
+    see, host = 10, x.float().numpy()
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(1))
+    for t in ENDS:
+        for f in (dict(), dict(top_k=20, top_p=0.9), dict(min_p=0.5)):
+            print(f"{rows} rows of {v} {dtype} temperature {t} {f}", flush=True)
+            token, lp = [r.tolist() for r in sampling.sample(x.to(dev), u.to(dev), temperature=t, **f)]
+            for i in range(see):
+                want, want_lp, clear = R.sample(host[i], u[i].item(), temperature=t, **f)
+                assert clear, f"row {i}: a border is near"
+                assert token[i] == want, f"row {i}: {token[i]}, expected {want}"
+                assert abs(lp[i] - want_lp) <= 2.0 ** -24 * abs(want_lp) + 2.0 ** -29, f"row {i}: {lp[i]} {want_lp}"
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("dtype,rows,v", [(torch.bfloat16, 80, 17000), (torch.float16, 12, 70000), (torch.float32, 12, 20000)])
+def test_verify_at_the_ends_of_temperature(dev, dtype, rows, v, probs):
+    x = _sharp(rows, v, dtype, v)
+    cu = [0, 2, 4, 6, 8, 10, rows]
+    tokens = torch.randint(0, v, (rows,), generator=torch.Generator().manual_seed(2))
+    tokens[1:10:4] = x.float().nan_to_num(-9e9).argmax(1)[0:9:4]
+    q = torch.softmax(x.float().clamp(-1e4, 1e4).nan_to_num(-1e4), 1) if probs else None
+    u, draw = torch.rand(rows, generator=torch.Generator().manual_seed(3)), torch.rand(6, generator=torch.Generator().manual_seed(4))
+    for t in ENDS:
+        print(f"verify {rows} rows of {v} {dtype} temperature {t} probs {probs}", flush=True)
+        acc, nxt = sampling.verify(x.to(dev), tokens.to(dev), torch.tensor(cu, device=dev), u.to(dev), draw.to(dev),
+                                   draft_probs=None if q is None else q.to(dev), temperature=t)
+        for b in range(5):
+            a, z = cu[b], cu[b + 1]
+            n, token, clear = _verify(x[a:z].float().numpy(), tokens[a:z].tolist(), u[a:z].numpy(), draw[b].item(),
+                                      None if q is None else q[a:z].numpy(), temperature=t)
+            assert clear, f"sequence {b}: a border is near"
+            assert (int(acc[b]), int(nxt[b])) == (n, token), f"sequence {b}: {int(acc[b])}, {int(nxt[b])}; expected {n}, {token}"
