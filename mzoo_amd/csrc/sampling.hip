@@ -34,7 +34,6 @@ constexpr double kBelow = 1.0 - 0x1p-30, kAbove = 1.0 + 0x1p-30;  // slack of bo
 constexpr int kCap = 16384;  // listed tokens of a row
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr int kNoTop = -0x7fffffff;
 
 enum Mode { kSample, kVerify, kBeams };
 
@@ -437,7 +436,7 @@ __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, b
 #pragma unroll
       for (int i = 0; i < PER; ++i) now[i] = P::finite(now[i]);
     }
-    const double bottom = static_cast<double>(top - kRest);  // bins above it are kept
+    const double bottom = bottom_of(top);
 #pragma unroll
     for (int i = 0; i < ELEMENTS; i += 4) {  // (four at a time, so that the steps of one wait for nothing)
       double t[4];

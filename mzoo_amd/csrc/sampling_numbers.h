@@ -37,4 +37,9 @@ __device__ __forceinline__ double weight_of(float l, float largest, double s, in
   return exp2_of(bins / kPerOctave) * __builtin_ldexp(1.0, scale);  // (a NaN, of -inf at an infinite temperature, is 0)
 }
 
+constexpr int kNoTop = -0x7fffffff;  // the largest bin of no token
+
+// The bin above which a survey's bins are kept whose largest is `top`.
+__device__ __forceinline__ double bottom_of(int top) { return static_cast<double>(top) - kRest; }
+
 }  // namespace mzk

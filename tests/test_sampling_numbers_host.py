@@ -72,3 +72,11 @@ def test_weights_of_all_values_of_a_block(tmp_path):
     }
   if (weight_of(-INFINITY, 1.0f, 0.0, 62) != 0.0) return 4;  // at an infinite temperature
 """)
+
+
+def test_the_bottom_of_no_token(tmp_path):
+    """A row that begins masked has no largest bin yet: nothing is below what is kept, and -inf is not above it."""
+    _run(tmp_path, r"""
+  if (bottom_of(0) != -1023.0 || bottom_of(1 << 28) != 268434433.0) return 1;
+  if (!(bottom_of(kNoTop) < -0x1p31) || -INFINITY > bottom_of(kNoTop)) return 2;
+""")
