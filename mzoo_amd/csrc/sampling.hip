@@ -367,7 +367,6 @@ __device__ __forceinline__ float origin_of(const Pieces<DT>& x, int tid, float* 
   return m > -__builtin_huge_valf() ? m : 0.0f;
 }
 
-constexpr int kCopies = 2;     // of each bin, side by side, by the lane
 constexpr int kSurveyThreads = 1024, kSurveyElements = 16;  // of a chunk's workgroup; of its thread at once
 constexpr int kAside = 64;     // places behind the bins for what is too small to count
 constexpr int kFar = 1 << 28;  // bins from the origin that are told apart
@@ -448,7 +447,7 @@ __device__ __forceinline__ Surveyed survey(const Pieces<DT>& x, const Grid& g, b
       for (int j = 0; j < 4; ++j) {
         // the nearest whole number: the low bits of the sum with 3 2^51
         const double sum = t[j] + 0x1.8p52, n = sum - 0x1.8p52;
-        k[j] = (static_cast<int>(__double_as_longlong(sum)) * (8 * kCopies) & 8 * kCopies * kRest) | copy;
+        k[j] = place_of(sum) | copy;
         k[j] = n > bottom ? k[j] : aside;  // (not of a NaN, nor of -inf)
         t[j] = t[j] - n;
       }

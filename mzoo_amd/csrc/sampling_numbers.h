@@ -42,4 +42,11 @@ constexpr int kNoTop = -0x7fffffff;  // the largest bin of no token
 // The bin above which a survey's bins are kept whose largest is `top`.
 __device__ __forceinline__ double bottom_of(int top) { return static_cast<double>(top) - kRest; }
 
+constexpr int kCopies = 2;  // of each bin, side by side, by the lane
+
+// The offset in bytes of the place of bin n, n mod kBins; n, however far, in the low bits of n + 3 2^51.
+__device__ __forceinline__ int place_of(double sum) {
+  return static_cast<int>(static_cast<unsigned>(__builtin_bit_cast(unsigned long long, sum)) * (8u * kCopies) & 8u * kCopies * kRest);
+}
+
 }  // namespace mzk
