@@ -85,11 +85,13 @@ def test_the_bottom_of_no_token(tmp_path):
 def test_places_of_far_bins(tmp_path):
     """A masked token lies any number of bins below the largest; its place, which nobody reads, is one of the histogram's."""
     _run(tmp_path, r"""
-  for (double n : {0.0, 1.0, -1.0, 1023.0, 1024.0, -1024.0, 1e6, -1e6, 134217727.0, 134217728.0, 268435456.0, -268435456.0, -3e9, 1e12, -1e15}) {
+  const double near[] = {0.0, 1.0, -1.0, 1023.0, 1024.0, -1024.0, 1e6, -1e6, 134217727.0, 134217728.0, 268435456.0, -268435456.0, -3e9, 1e12, -1e15};
+  const double farther[] = {-1e30, -1e85, -INFINITY, NAN};
+  for (double n : near) {
     const int at = place_of(n + 0x1.8p52), want = static_cast<int>(static_cast<long long>(n) & kRest) * 8 * kCopies;
     if (at != want) { std::printf("%g: %d\n", n, at); return 1; }
   }
-  for (double far : {-1e30, -1e85, -INFINITY, static_cast<double>(NAN)}) {
+  for (double far : farther) {
     const int at = place_of(far + 0x1.8p52);
     if (at < 0 || at > 8 * kCopies * kRest || at % (8 * kCopies)) return 2;
   }
