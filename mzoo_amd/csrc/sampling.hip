@@ -284,20 +284,24 @@ struct Pieces {
   }
 };
 
-// The sequence of a row of packed ones and the row behind its last; false: none.
+// The sequence of a row of packed ones and the row behind its last; false: none.  The first that ends behind the row, by 64 of
+// them at a time, evenly spaced: 2 dependent loads for 4096 sequences, 4 for 2^22.  (One after another, 65536 rows of as many
+// sequences took 27.8 ms, of which reading and drawing is 3.8.)
 __device__ __forceinline__ bool sequence_of(const SamplingParams& q, int row, int lane, int& b, int& end) {
-  for (int b0 = 0; b0 < q.B; b0 += 64) {
-    const int64_t z = b0 + lane < q.B ? q.cu[b0 + lane + 1] : 0;
-    const uint64_t in = __ballot(b0 + lane < q.B && z > row);
-    if (in) {
-      const int at = __builtin_ctzll(in);
-      b = b0 + at;
-      const int64_t e = q.cu[b + 1];
-      end = e < q.rows ? static_cast<int>(e) : q.rows;
-      return q.cu[b] <= row;
-    }
+  b = 0;
+  for (int n = q.B; n > 0;) {  // among b .. b + n - 1
+    const int step = (n + 63) / 64, last = (lane + 1) * step < n ? (lane + 1) * step - 1 : n - 1;
+    const uint64_t in = __ballot(q.cu[b + last + 1] > row);
+    if (in == 0) return false;
+    const int before = __builtin_ctzll(in) * step;
+    b += before;
+    n = step < n - before ? step : n - before;
+    if (step == 1) break;
   }
-  return false;
+  if (q.B == 0) return false;
+  const int64_t e = q.cu[b + 1];
+  end = e < q.rows ? static_cast<int>(e) : q.rows;
+  return q.cu[b] <= row;
 }
 
 // Across the wave with data-parallel moves: steps of 1, 2, 4, 8 within 16 lanes, then the sums of the lanes before.
