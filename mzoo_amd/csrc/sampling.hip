@@ -59,6 +59,8 @@ struct Row {
   float max, origin;
   int32_t top, accepted, token;
 };
+// Accepted if top-k keeps it: the drafted token is too light for the sums, and top-k may end among such ones.
+constexpr int kIfKept = 2;
 
 struct Filter {
   const float* f;  // one for each row, or null: `all` for every row
@@ -1143,22 +1145,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
         double left = kept;
         if (drafted != kNone) {
           const float l = logit_of_key(drafted_key);
-          const uint64_t its = order_of(drafted_key, drafted);
-          bool stays = its <= cut && !beyond && reaches(l);
-          if (__builtin_expect(stays && counting && cut == ~0ull && drafted_bin == kRest, 0)) {  // uniform
-            // top-k may end among tokens too light for the sums, of which this is one: those before it are counted
-            uint32_t m = 0;
-            x.template walk<NT>(tid, [&](int i, float of) __attribute__((always_inline)) { m += order_of(key_of(of), static_cast<uint32_t>(i)) < its; });
-            m = wave_sum(m);
-            __syncthreads();
-            if (lane == 0) partn[wave] = m;
-            __syncthreads();
-            m = 0;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) m += partn[i];
-            stays = m < static_cast<uint32_t>(z.k);
-          }
-          if (stays) {
+          if (order_of(drafted_key, drafted) <= cut && !beyond && reaches(l)) {
             const double w = exp2_of((g.place(l) - static_cast<double>(r.top)) / kPerOctave) * __builtin_ldexp(1.0, q.scale);
             const double sure = q.probs ? static_cast<double>(q.probs[row * q.probs_stride + drafted]) : 1.0;
             accepted = static_cast<double>(q.u[row]) * sure * kept < w;
@@ -1600,13 +1587,33 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     const double lp = (static_cast<double>(drawn) - static_cast<double>(r.max)) * z.s * (kLn2D / kPerOctave) - log_of(kept);
     q.logprob[row] = lp > -0x1p-40 ? 0.0f : static_cast<float>(lp);
   } else {
-    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, accepted ? 1 : 0, static_cast<int32_t>(token)};
+    const bool light = counting && cut == ~0ull && drafted_bin == kRest;
+    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, !accepted ? 0 : light ? kIfKept : 1, static_cast<int32_t>(token)};
   }
 }
 
 // ---- verify: the sequences ------------------------------------------------------------------------
 
+// Whether top-k keeps a row's drafted token: whether fewer than k are before it (by a whole wave).  (Rare: u times the draft's
+// probability, was below 2^-51.  In the row's own launch this code took 0.8 us of 64 bf16 rows of 131072 that do not need it.)
+template <int DT>
+__device__ __forceinline__ bool keeps_drafted(const SamplingParams& q, int row, int lane) {
+  const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
+  const int64_t d = q.tokens[row + 1];
+  if (d < 0 || d >= q.V) return false;  // (not in a row that was judged: sequences that do not ascend leave some out)
+  const int drafted = static_cast<int>(d), k = q.top_k ? q.top_k[row] : q.top_k_all;
+  const float its = x[drafted];
+  uint32_t before = 0;
+#pragma unroll 8
+  for (int i = lane; i < q.V; i += 64) {
+    const float l = x[i];
+    before += l > its || (l == its && i < drafted);
+  }
+  return wave_sum(before) < static_cast<uint32_t>(k);
+}
+
 // The rows of sequence b: the first whose drafted token is refused, or the last (by a whole wave; -1: no rows).
+template <int DT>
 __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, int& first, int& end, int& token) {
   auto clamp = [&](int64_t v, int lo) -> int { return v < lo ? lo : v > q.rows ? q.rows : static_cast<int>(v); };
   first = clamp(q.cu[b], 0);
@@ -1616,7 +1623,11 @@ __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, 
     const int i = i0 + lane;
     const Row* const r = q.rowres + (i < end ? i : end - 1);
     const int accepted = r->accepted, its = r->token;
-    const uint64_t stop = __ballot(i < end && (i + 1 == end || !accepted));
+    uint64_t stop = __ballot(i < end && (i + 1 == end || !accepted)), ask = __ballot(i + 1 < end && accepted == kIfKept);
+    for (; ask && (!stop || __builtin_ctzll(ask) < __builtin_ctzll(stop)); ask &= ask - 1) {  // uniform
+      const int at = __builtin_ctzll(ask);
+      if (!keeps_drafted<DT>(q, i0 + at, lane)) stop |= 1ull << at;
+    }
     if (stop) {
       const int at = __builtin_ctzll(stop);
       token = __builtin_amdgcn_readlane(its, at);
@@ -1628,11 +1639,12 @@ __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, 
 
 // The sequences, a wave each: without the draft's probabilities, and where no token is refused, the token of that row is
 // the next.
+template <int DT>
 __global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
   const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (b >= q.B) return;
   int first, end, token;
-  const int i = judged(q, b, lane, first, end, token);
+  const int i = judged<DT>(q, b, lane, first, end, token);
   if (lane != 0) return;
   q.accepted[b] = i < 0 ? 0 : i - first;
   q.token[b] = token;
@@ -1659,7 +1671,7 @@ __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.x / q.rest_chunks, chunk = blockIdx.x - b * q.rest_chunks;
   int first, end, token;
-  const int row = judged(q, b, lane, first, end, token);
+  const int row = judged<DT>(q, b, lane, first, end, token);
   const bool refused = row >= 0 && row + 1 < end;  // uniform
   if (chunk == 0 && tid == 0) {
     q.accepted[b] = row < 0 ? 0 : row - first;
@@ -1866,7 +1878,7 @@ int launch(const SamplingParams& q, hipStream_t s) {
   }
   if (q.mode == kVerify) {
     if (!q.probs) {
-      verify_kernel<<<static_cast<unsigned>((q.B + 3) / 4), 256, 0, s>>>(q);
+      verify_kernel<DT><<<static_cast<unsigned>((q.B + 3) / 4), 256, 0, s>>>(q);
     } else {
       rest_kernel<DT><<<static_cast<unsigned>(q.B) * static_cast<unsigned>(q.rest_chunks), 256, 0, s>>>(q);
       redraw_kernel<DT><<<static_cast<unsigned>(q.B), 256, 0, s>>>(q);
@@ -1999,7 +2011,7 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   q.token = next;
   if (T == 0) {  // no rows: sequences of nothing
     q.probs = nullptr;
-    verify_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, as_stream(stream)>>>(q);
+    verify_kernel<MZK_F32><<<static_cast<unsigned>((B + 3) / 4), 256, 0, as_stream(stream)>>>(q);
     MZK_LAUNCH_CHECK("verify");
     return MZK_OK;
   }

@@ -102,6 +102,29 @@ def test_verify_top_k_ends_among_light_tokens(dev, dtype, v, sequences, chunks, 
         assert (acc[b], nxt[b]) == (0, token), f"sequence {b}: place {at[b]} of {k[2 * b]} kept ones: {acc[b]}, {nxt[b]}"
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_light_tokens_one_after_another(dev, dtype, probs):
+    """Sequences of 150 tokens, each of which only its place says is kept: up to the first that is not, or is refused otherwise."""
+    v, n, k = 3000, 150, 40
+    g = torch.Generator().manual_seed(5)
+    row = torch.full((v,), -60.0)
+    row[torch.randperm(v, generator=g)[:2]] = 0.0
+    order = np.argsort(-row.numpy(), kind="stable")
+    x = row.expand(4 * n, v).to(dtype)
+    tokens = torch.from_numpy(order)[torch.randint(2, k, (4 * n,), generator=g)]
+    tokens[n + 71] = int(order[k])                    # behind top-k's end
+    tokens[2 * n + 100], tokens[2 * n + 101] = v, int(order[k])  # no token, before that
+    tokens[3 * n + 3] = int(order[-1])
+    u = torch.full((4 * n,), 0.5 if probs else 0.0)
+    q = torch.full((4 * n, v), 2.0 ** -140) if probs else None
+    acc, nxt = sampling.verify(x.to(dev), tokens.to(dev), torch.arange(0, 4 * n + 1, n, device=dev), u.to(dev), torch.full((4,), 0.75, device=dev),
+                               draft_probs=None if q is None else q.to(dev), top_k=k)
+    assert acc.tolist() == [n - 1, 70, 99, 2]
+    heavy = sorted(order[:2].tolist())
+    assert nxt.tolist() == [heavy[1]] * 4             # by the order and by the index alike: equal ones
+
+
 # ---- temperatures at the ends of float32 ------------------------------------------------------
 
 ENDS = [1.401298464324817e-45, 1e-30, 1e-3, 0.01, 1e30, 3.4028234663852886e38, float("inf")]
