@@ -585,6 +585,11 @@ constexpr int kRowThreads = kBins / 2;
 constexpr int kMostChunks = 64;
 constexpr int kDigits = 1024;  // of a selection's step
 constexpr int kByValue = 16384;  // longer rows of bf16 logits are counted by value
+// LDS of a row's workgroup: its own arrays, and behind them the list with the hot values' places, or a survey's bins.  The plan's
+// launch asks for no more than any kernel has, the others for what a compute unit has.
+constexpr int kRowStaticLds = 26 * 1024;
+constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2)) + 4 * kRowThreads, kBinsLds = 12 * (kCopies * kBins + kAside);
+static_assert(kBinsLds <= kRowLds && kBinsLds + kRowStaticLds <= 64 * 1024 && kRowLds + kRowStaticLds <= 160 * 1024, "LDS");
 
 // A row in one launch, or, where its chunks are surveyed and listed by workgroups of their own, in two: up to the bins
 // in which something is to be found, and from the list on.
@@ -614,6 +619,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   if (q.mode == kVerify && !sequence_of(q, row, lane, b, end)) return;  // uniform
   __shared__ uint4 edge[2];
   const P x(q.logits + row * q.stride, q.V, edge);
+  static_assert(sizeof(hist) + sizeof(counts) + sizeof(cw) + sizeof(cn) + sizeof(part) + sizeof(sel) + sizeof(last_ones) + sizeof(partn) +
+                        sizeof(number) + sizeof(found) + sizeof(lds) + sizeof(tops) + sizeof(edge) <= kRowStaticLds, "row_kernel's static LDS");
   x.edges(tid, edge);
   __syncthreads();
   const Settings z = settings(q, row);
@@ -1595,7 +1602,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
 // ---- verify: the sequences ------------------------------------------------------------------------
 
 // Whether top-k keeps a row's drafted token: whether fewer than k are before it (by a whole wave).  (Rare: u times the draft's
-// probability, was below 2^-51.  In the row's own launch this code took 0.8 us of 64 bf16 rows of 131072 that do not need it.)
+// probability was below 2^-51.  In the row's own launch this code took 0.8 us of 64 bf16 rows of 131072 that do not need it.)
 template <int DT>
 __device__ __forceinline__ bool keeps_drafted(const SamplingParams& q, int row, int lane) {
   const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
@@ -1839,9 +1846,6 @@ int64_t lay(SamplingParams& q, uint8_t* ws) {
   }
   return at;
 }
-
-constexpr int kRowLds = kCap * static_cast<int>(sizeof(uint2)) + 4 * kRowThreads, kBinsLds = 12 * (kCopies * kBins + kAside);
-static_assert(kBinsLds <= kRowLds && kBinsLds + 20 * 1024 <= 64 * 1024, "LDS");
 
 // The dynamic-LDS limit is a per-device function attribute: set once per device.
 template <typename K>
