@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   uint32_t my_cn[2];
   {
     // (by value the sums are there)
-    const int at = kBins * row;
+    const int64_t at = static_cast<int64_t>(kBins) * row;
     uint64_t w = 0;
     uint32_t m = 0;
     if (PART != kFinishPart && !by_value) {

@@ -244,3 +244,68 @@ def test_verify_finds_a_rows_sequence_in_few_steps(dev):
     print(f"verify {verify:.0f} us, sample {sample:.0f} us", flush=True)
     assert verify < 3 * sample
     assert torch.equal(sampling.verify(x, tokens, cu, u, u, top_p=0.9)[1], sampling.sample(x, u, top_p=0.9)[0])
+
+
+# ---- the most rows, the longest rows --------------------------------------------------------------
+
+MOST = (1 << 22) - 1
+
+
+def test_the_most_rows(dev):
+    """2^22 - 1 rows of 3 logits; one more is refused."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(MOST, 3, device=dev, generator=g)
+    u = torch.rand(MOST, device=dev, generator=g)
+    tokens, lp = sampling.sample(x, u, temperature=0.7)
+    w, order = (x.double() / float(np.float32(0.7))).softmax(1).sort(1, descending=True)
+    sums = w.cumsum(1)
+    at = (sums <= u.double()[:, None]).sum(1).clamp(max=2)
+    clear = (sums[:, :2] - u.double()[:, None]).abs().amin(1) > 2.0 ** -28
+    assert int(clear.sum()) > MOST - 20
+    assert torch.equal(tokens[clear], order.gather(1, at[:, None])[:, 0][clear])
+    want = w.gather(1, at[:, None])[:, 0].log()
+    assert bool(((lp.double() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -30)[clear].all())
+    with pytest.raises(RuntimeError, match="too many rows"):
+        sampling.sample(torch.zeros(MOST + 1, 3, device=dev), torch.zeros(MOST + 1, device=dev))
+
+    # sequences of 3 rows, and beams, of all rows as of the second half alone
+    drafted = torch.randint(0, 3, (MOST,), device=dev, generator=g)
+    cu = torch.arange(0, MOST + 1, 3, device=dev)
+    batch = cu.shape[0] - 1
+    half = batch // 2
+    draw = torch.rand(batch, device=dev, generator=g)
+    q = torch.randn(MOST, 3, device=dev, generator=g).softmax(1)
+    for probs in (None, q):
+        acc, nxt = sampling.verify(x, drafted, cu, u, draw, draft_probs=probs)
+        part = sampling.verify(x[3 * half:], drafted[3 * half:], cu[half:] - 3 * half, u[3 * half:], draw[half:],
+                               draft_probs=None if probs is None else probs[3 * half:])
+        assert torch.equal(acc[half:], part[0]) and torch.equal(nxt[half:], part[1])
+        assert acc.unique().tolist() == [0, 1, 2] and nxt.unique().tolist() == [0, 1, 2]
+    got = sampling.beams(x, -u, 3)
+    part = sampling.beams(x[3 * half:], -u[3 * half:], 3)
+    assert torch.equal(got[0][3 * half:], part[0] + 3 * half) and torch.equal(got[1][3 * half:], part[1]) and torch.equal(got[2][3 * half:], part[2])
+
+
+@pytest.mark.parametrize("dtype,rows,chunks", [(torch.float32, 2, True), (torch.float32, 140, False), (torch.bfloat16, 2, True),
+                                               (torch.bfloat16, 70, False), (torch.float16, 2, True), (torch.float16, 140, False)])
+def test_the_longest_rows(dev, dtype, rows, chunks):
+    """Of 2^20 logits, the last of which the largest; two rows of it are looked at, of which one begins masked."""
+    v = 1 << 20
+    assert _in_chunks(rows, v, dtype) == chunks
+    g = torch.Generator().manual_seed(rows)
+    x = (torch.randn(2, v, generator=g) * 2.0).to(dtype)
+    x[1, :v // 2] = -float("inf")
+    x[:, v - 1] = 17.0
+    there = x[torch.arange(rows) % 2].to(dev)
+    u = torch.rand(rows, generator=g)
+    for f in (dict(top_p=0.9), dict(top_k=2000, temperature=1.4), dict(min_p=1e-4), dict()):
+        print(f"{rows} rows of {v} {dtype} {f}", flush=True)
+        token, lp = [r.tolist() for r in sampling.sample(there, u.to(dev), **f)]
+        for i in range(2):
+            want, want_lp, clear = R.sample(x[i].float().numpy(), u[i].item(), **f)
+            assert clear, f"row {i}: a border is near"
+            assert token[i] == want, f"row {i}: {token[i]}, expected {want}"
+            # float32's half step, and the logarithm of W, which is off by less than 2^-29 of itself
+            assert abs(lp[i] - want_lp) <= 2.0 ** -24 * abs(want_lp) + 2.0 ** -29, f"row {i}: {lp[i]} {want_lp}"
+    with pytest.raises(RuntimeError, match="at most"):
+        sampling.sample(torch.zeros(1, v + 1, device=dev), torch.zeros(1, device=dev))
