@@ -7,6 +7,8 @@ import torch
 
 from mzoo_amd import sampling
 from tests import sampling_ref as R
+from tests.test_gpu_sampling import _u
+from tests.test_gpu_sampling_rows import MANY, _check_near, _hard
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -309,3 +311,33 @@ def test_the_longest_rows(dev, dtype, rows, chunks):
             assert abs(lp[i] - want_lp) <= 2.0 ** -24 * abs(want_lp) + 2.0 ** -29, f"row {i}: {lp[i]} {want_lp}"
     with pytest.raises(RuntimeError, match="at most"):
         sampling.sample(torch.zeros(1, v + 1, device=dev), torch.zeros(1, device=dev))
+
+
+# ---- hard rows, each way they are read ------------------------------------------------------------
+
+EACH_WAY = [(torch.float32, 20000, 73, False), (torch.float32, 150000, 21, True), (torch.float32, 150000, 146, False),
+            (torch.float16, 20000, 73, False), (torch.float16, 70000, 21, True), (torch.float16, 70000, 146, False),
+            (torch.float16, 150000, 21, True), (torch.float16, 150000, 146, False),
+            (torch.bfloat16, 16384, 73, False), (torch.bfloat16, 20000, 73, False), (torch.bfloat16, 150000, 21, True),
+            (torch.bfloat16, 150000, 73, False)]
+
+
+def _hard_filters(v):
+    return dict(), dict(top_k=1000), dict(min_p=0.3), dict(temperature=0.0), dict(top_k=v - v // 20, temperature=1.5)
+
+
+def _hard_case(v, dtype, rows):
+    x, plain = _hard(v, dtype)
+    of = torch.arange(rows) % MANY
+    return x[of], plain[:21], _u(rows, v + 70)
+
+
+@pytest.mark.parametrize("dtype,v,rows,chunks", EACH_WAY)
+def test_hard_rows_each_way(dev, dtype, v, rows, chunks):
+    """Masks, ties, the ends of the type, values whose number passes 16 bits: a workgroup a row, and in chunks, of each type."""
+    assert _in_chunks(rows, v, dtype) == chunks
+    x, plain, u = _hard_case(v, dtype, rows)
+    for f in _hard_filters(v):
+        print(f"{rows} rows of {v} {dtype} {f}", flush=True)
+        token, lp = sampling.sample(x.to(dev), u.to(dev), **f)
+        _check_near([token[:21].cpu(), lp[:21].cpu()], plain, u[:21], f)
