@@ -57,7 +57,7 @@ struct Row {
   double kept;    // W, in units of 2^-scale
   uint64_t cut;   // key and index of the last token that top-k and top-p keep
   float max, origin;
-  int32_t top, accepted, token;
+  int32_t top, accepted, token, drafted;
 };
 // Accepted if top-k keeps it: the drafted token is too light for the sums, and top-k may end among such ones.
 constexpr int kIfKept = 2;
@@ -1595,7 +1595,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     q.logprob[row] = lp > -0x1p-40 ? 0.0f : static_cast<float>(lp);
   } else {
     const bool light = counting && cut == ~0ull && drafted_bin == kRest;
-    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, !accepted ? 0 : light ? kIfKept : 1, static_cast<int32_t>(token)};
+    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, !accepted ? 0 : light ? kIfKept : 1, static_cast<int32_t>(token),
+                        static_cast<int32_t>(drafted)};
   }
 }
 
@@ -1606,9 +1607,8 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
 template <int DT>
 __device__ __forceinline__ bool keeps_drafted(const SamplingParams& q, int row, int lane) {
   const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
-  const int64_t d = q.tokens[row + 1];
-  if (d < 0 || d >= q.V) return false;  // (not in a row that was judged: sequences that do not ascend leave some out)
-  const int drafted = static_cast<int>(d), k = q.top_k ? q.top_k[row] : q.top_k_all;
+  const int drafted = q.rowres[row].drafted, k = q.top_k ? q.top_k[row] : q.top_k_all;
+  if (drafted < 0 || drafted >= q.V) return false;  // (not of a row that was judged: sequences that do not ascend leave some out)
   const float its = x[drafted];
   uint32_t before = 0;
 #pragma unroll 8

@@ -127,6 +127,24 @@ def test_verify_light_tokens_one_after_another(dev, dtype, probs):
     assert nxt.tolist() == [heavy[1]] * 4             # by the order and by the index alike: equal ones
 
 
+def test_verify_next_tokens_over_the_tokens(dev):
+    """A call's next tokens may be written where its tokens were: 64 sequences of a drafted token that only its place says is kept,
+    or not, over and over."""
+    v, k, n = 5000, 20, 64
+    x = torch.full((2 * n, v), -60.0)
+    x[:, 7] = 0.0
+    order = torch.argsort(-x[0], stable=True)
+    tokens = order[torch.arange(2 * n) // 2 % (2 * k) + 1].to(dev)  # the places 1 .. 2 k of the order
+    want = [1 if i % (2 * k) + 1 < k else 0 for i in range(n)]
+    cu, zero = torch.arange(0, 2 * n + 1, 2, device=dev), torch.zeros(2 * n, device=dev)
+    there, acc = x.to(dev), torch.empty(n, dtype=torch.int64, device=dev)
+    for _ in range(20):
+        mine = tokens.clone()
+        sampling.verify(there, mine, cu, zero, zero[:n], top_k=k, out=(acc, mine[n // 2:n // 2 + n]))
+        assert acc.tolist() == want
+        assert mine[n // 2:n // 2 + n].tolist() == [7] * n
+
+
 # ---- temperatures at the ends of float32 ------------------------------------------------------
 
 ENDS = [1.401298464324817e-45, 1e-30, 1e-3, 0.01, 1e30, 3.4028234663852886e38, float("inf")]
