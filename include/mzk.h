@@ -726,7 +726,8 @@ int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, int64_t row_
 
 /* A step of a beam search: of each group of `width` rows the `keep` best continuations by scores[row] + logit -
  * log sum exp, best first, equal ones by row and token (width * keep at most 4096).  parents: their rows, tokens,
- * out_scores; -1, -1 and -inf where a group has fewer.  A row whose score is -inf or NaN has none. */
+ * out_scores; -1, -1 and -inf where a group has fewer.  A row whose score is -inf or NaN has none.  out_scores may be scores with
+ * keep == width, and overlaps it no other way. */
 int mzk_beams_workspace_bytes(int64_t rows, int64_t V, int dtype, int keep, int64_t* bytes);
 int mzk_beams(const void* logits, int dtype, int64_t rows, int64_t V, int64_t row_stride, const float* scores, int width,
               int keep, int32_t* parents, int64_t* tokens, float* out_scores, void* workspace, int64_t workspace_bytes,

@@ -2043,6 +2043,11 @@ extern "C" int mzk_beams(const void* logits, int dtype, int64_t rows, int64_t V,
   MZK_CHECK_ARG(rows % width == 0, "beams: %lld rows are no groups of %d", (long long)rows, width);
   if (rows == 0) return MZK_OK;
   MZK_CHECK_ARG(scores && parents && tokens && out_scores, "beams: null pointer");
+  // (a group's workgroup reads its scores and then writes its new ones)
+  const uintptr_t from = reinterpret_cast<uintptr_t>(scores), to = reinterpret_cast<uintptr_t>(out_scores);
+  MZK_CHECK_ARG((from == to && keep == width) || to >= from + 4u * static_cast<uintptr_t>(rows) ||
+                    from >= to + 4u * static_cast<uintptr_t>(rows / width * keep),
+                "beams: the out scores are the scores themselves, as many, or overlap none of them");
   q.scores = scores;
   q.width = width;
   q.keep = keep;

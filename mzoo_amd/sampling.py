@@ -190,7 +190,7 @@ def beams(logits: torch.Tensor, scores: torch.Tensor, width: int, keep: int | No
     continue -- ``paged.fork``'s parents --, their tokens and log probabilities; -1, -1 and -inf where a
     group has fewer.  A beam of score -inf or NaN has no continuation: a search starts with 0 and -inf.
     ``out=(parents, tokens, scores)`` and ``workspace`` (``beams_workspace_bytes``) as in ``sample``; the out scores may
-    be ``scores`` itself."""
+    be ``scores`` itself, if as many, and overlap it no other way."""
     _one_device("beams", logits, scores, workspace)
     logits, rows, v, stride = _logits("beams", logits)
     if not isinstance(width, int) or width < 1 or rows % width:
@@ -203,6 +203,9 @@ def beams(logits: torch.Tensor, scores: torch.Tensor, width: int, keep: int | No
     n = rows // width * keep
     parents, tokens, new = _out("beams", out, ("parents", "tokens", "scores"),
                                 (((n,), torch.int32), ((n,), torch.int64), ((n,), torch.float32)), logits.device)
+    at, to = scores.data_ptr(), new.data_ptr()
+    if not (at == to and keep == width) and at < to + 4 * n and to < at + 4 * rows:
+        raise ValueError("beams: the out scores are the scores themselves, as many, or overlap none of them")
     if rows:
         need = beams_workspace_bytes(rows, v, keep, logits.dtype)
         ws = _workspace("beams", workspace, need, logits.device)
