@@ -8,8 +8,13 @@
 // shortest.  The token drawn is the first whose running sum exceeds u times the kept sum W.  (T <= 0: the
 // first of the order.)  NaN and -inf are no tokens; +inf counts as its type's largest finite number, -0 as 0.
 //
-// Tokens are whole numbers, so a token beside a border of the running sum has to come out right: weights
-// are computed in 64 bits to about 2^-50 of themselves, and summed as whole numbers, in any order the same.
+// Tokens are whole numbers, so a token beside a border of the running sum has to come out right: weights are computed in 64 bits
+// and summed as whole numbers, in any order the same.  A running sum's share of W is off by less than 2^-29:
+//   bins      2^-44 of a weight for its second factor, and |t| 2^-52 ln 2 / 20 for its place t, at most 2^27 bins from
+//             the origin: 2^-29.8, half of which can reach a share of W; half a unit of 1023 bins, 2^-33; what is too small to count,
+//             2^20 tokens of 2^-51 each.  (Mostly t is below 2^10, and all of it some 2^-40.)
+//   by value  2^-49 of a weight; half a unit of 2^-scale of each of at most 2^16 values, 2^-30 for rows of up to 2^17 tokens; each
+//             doubling of a row's length doubles that, to 2^-27 for 2^20.
 //
 // No row is sorted.  What is to be found lies in few places of the order, and those are found from sums:
 //   bins      weights are summed in bins of 1/20 octave, from the largest down, by atomic sums in LDS (survey);
@@ -149,7 +154,8 @@ __device__ __forceinline__ uint64_t whole_exp2(double r) {
   return w[0];
 }
 
-// log2 x for x >= 2^-190: the hardware's, and what it leaves, 1 + d with |d| < 2^-20, by the series.
+// log2 x for x >= 2^-190: the hardware's, a float32 of at most 128 and so off by some 2^-17, and what it leaves, 1 + d, by the series,
+// whose first term left out is d^4 / 4 < 2^-68.
 __device__ __forceinline__ double log2_of(double x) {
   const double y = static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(x * 0x1p64))) - 64.0;
   const double d = x * exp2_of(-y) - 1.0;

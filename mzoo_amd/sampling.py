@@ -8,8 +8,9 @@ What stands between a step of ``mzoo_amd.paged`` and the next one:
 * ``beams``   which continuations a beam search keeps: ``fork``'s parents, and their tokens.
 
 Random numbers are inputs, and so everything is reproducible: the same call gives the same bits.  The same row gives the
-same token in any batch, unless its random number times the sum is within 2^-29 of the sum from a border between
-two tokens: how many rows there are decides how weights are summed.  Calls read lengths and settings on the device and never synchronise, so a step is captured once::
+same token in any batch, unless its random number times the sum is within 2^-29 of the sum (bf16 rows of more than 2^17
+logits: 2^-27) from a border between two tokens: how many rows there are decides how weights are summed.  Calls read
+lengths and settings on the device and never synchronise, so a step is captured once::
 
     o, lse = paged.attend(q, pool, tables, lens, cu=cu)          # the newest tokens, drafted ones among them
     accepted, token = sampling.verify(head(o), tokens, cu, u, draw, temperature=0.8, top_p=0.95)

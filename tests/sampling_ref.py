@@ -1,11 +1,10 @@
 """Plain restatements, on the CPU in 64 bits and more, of what ``mzoo_amd.sampling`` computes.
 
-Tokens are whole numbers and have to be equal.  The kernels' weights are off by at most 2^-49 of
-themselves, weights below 2^-50 of the largest count as 0, and bins of them are rounded to whole numbers of which 2^42 or
-more stand for the largest weight: with N tokens a running sum is off by less than N 2^-50 + 512 2^-43 of the
-largest weight, below 2^-29 for the 2^20 tokens of the longest row, and 2^-33 for 2^17.  ``Rows.clear`` says whether
-no border of a row lies within 2^-28 of what is looked for; random inputs of a fixed seed are (a border among
-N at distance 2^-28 has probability N 2^-28 at most).  Where all weights are equal, sums of them are exact on both sides.
+Tokens are whole numbers and have to be equal.  The kernels' running sums, as shares of a row's sum W, are off by less than
+2^-29 (``csrc/sampling.hip`` adds up of what): 2^-44 of each weight, 2^-52 ln 2 / 20 of its distance in bins from where the row's bins are
+counted from, half a unit of each bin or value, of which 2^42 and more are the largest weight, and what is below 2^-51 of
+that.  ``clear`` says whether no border of a row lies within 2^-28 W of what is looked for; random inputs of a fixed seed are (a
+border among N at distance 2^-28 has probability N 2^-28 at most).  Where all weights are equal, sums of them are exact on both sides.
 """
 
 import numpy as np
