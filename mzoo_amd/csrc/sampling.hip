@@ -25,10 +25,10 @@
 // 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
 // row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
 //
-// Measured: fp32, 1 row of 131072: 6.9 + 9.7 + 4.5 + 10.3 us in four launches, of which reading would be 0.1 us: bound
+// Measured: fp32, 1 row of 131072: 6.9 + 9.5 + 4.5 + 10.4 us in four launches, of which reading would be 0.1 us: bound
 // by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
-// turns: 107 us: the first reading 55, at 3.7 TB/s near what memory gives (4.0), the second 24, from the caches.  bf16, 64
-// rows of 131072: 44 us, of which the count 12; 160 drafted rows: 50.  fp16, 16 rows of 32000: 22 us.
+// turns: 105 us a call: the first reading 58, at 3.5 TB/s near what memory gives (4.0), the second 23, from the caches.  bf16, 64
+// rows of 131072: 43.5 us, of which the count 12.3 and the second reading 6.5; 160 drafted rows: 49.  fp16, 16 rows of 32000: 22 us.
 #include "common.h"
 #include "sampling_numbers.h"
 
@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
   Surveyed r{kNoTop, -__builtin_huge_valf(), 0.0f};
   bool by_value = false;  // bf16 logits: the counts of their values say where to look
   // ---- bf16 logits: how many tokens have each value ----
-  // (4096 logits: 25.6 us by value, 24.4 with bins; 32768: 31.1 and 33.8; 131072: 46.4 and 60.6, 64 rows)
+  // (64 rows, by value and with bins: of 8192 logits 25.4 and 23.5 us, 16384 26.2 and 27.2, 32768 30.6 and 34.2, 131072 45.5 and 63.2)
   // Two counters a word, the negative value's above the positive's, from the order's first 128 values (a block) on:
   // block j is thread j's.  A counter that passes 2^16 is found out by the sum of all.
   uint32_t* const tally = reinterpret_cast<uint32_t*>(smem);
@@ -1817,9 +1817,10 @@ __global__ void __launch_bounds__(1024) beams_kernel(const SamplingParams q, int
 
 // Up to how many rows of V their chunks have workgroups of their own.  Four launches cost some 29 us and 2e-6 us an
 // element of all rows; one launch some 20 us and 3.2e-4 us an element of a row, of bf16 by value 25 us and 1.45e-4 us.
-// So the borders' two sides, split and whole: fp32, 131072: 52.9 and 62.6 us with 64 rows, 68.7 and 63.8 with 128;
-// 65536: 31.5 and 41.1 with 32, 52.6 and 42.7 with 128, 32768: 28.8 and 30.0 with 1; fp16, 65536: 38.5 and 43.4 with 64, 49.5 and 44.9 with 128;
-// bf16, 131072: 39.6 and 45.9 with 32, 48.4 and 46.4 with 64; 65536: 31.7 and 36.0 with 32, 38.4 and 36.3 with 64.
+// So the borders' two sides, split and whole: fp32, 131072: 59.3 and 63.8 us with 96 rows, 70.0 and 64.6 with 128; 65536: 32.9 and 42.1
+// with 32, 42.6 and 41.9 with 96; 32768: 30.0 and 29.5 with 8; fp16, 131072: 50.8 and 60.2 with 96, 63.1 and 62.2 with 160;
+// 65536: 39.2 and 41.3 with 64, 40.7 and 41.8 with 96, 50.2 and 42.1 with 128; bf16, 131072: 41.3 and 45.1 with 48, 48.7 and 45.2 with
+// 64; 65536: 30.5 and 36.0 with 8, 38.7 and 35.7 with 64; 32768: 29.9 and 30.2 with 8, 31.5 and 30.6 with 64.
 int64_t split_rows(int64_t V, int dtype) { return dtype == MZK_BF16 ? 72 - (3 << 20) / V : 144 - (5 << 20) / V; }
 
 int64_t up(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
