@@ -62,10 +62,8 @@ struct Row {
   double kept;    // W, in units of 2^-scale
   uint64_t cut;   // key and index of the last token that top-k and top-p keep
   float max, origin;
-  int32_t top, accepted, token, drafted;
+  int32_t top, accepted, token;
 };
-// Accepted if top-k keeps it: the drafted token is too light for the sums, and top-k may end among such ones.
-constexpr int kIfKept = 2;
 
 struct Filter {
   const float* f;  // one for each row, or null: `all` for every row
@@ -1567,31 +1565,40 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     }
     if (q.mode == kBeams) break;  // uniform
   }
-  if (q.mode == kBeams) {
+  // Beams keep the tokens up to the cut.  And top-k may end among tokens too light for the sums, without a cut: a drafted one of those is
+  // accepted if fewer than k are before it.  (With a walk of its own among the steps above, 64 bf16 rows of 131072 that do not need it
+  // took 0.8 us more, with this one 0.5.)
+  const bool light = accepted && counting && cut == ~0ull && drafted_bin == kRest;
+  if (q.mode == kBeams || light) {  // uniform
+    const uint64_t upto_here = light ? order_of(drafted_key, drafted) : cut;
     __syncthreads();
     if (tid == 0) number[1] = 0;
     __syncthreads();
     auto take = [&](uint32_t k, uint32_t i) {
       const uint32_t to = atomicAdd(&number[1], 1u);
-      if (to < static_cast<uint32_t>(q.keep)) q.best[static_cast<int64_t>(row) * q.keep + to] = uint2{k, i};
+      if (!light && to < static_cast<uint32_t>(q.keep)) q.best[static_cast<int64_t>(row) * q.keep + to] = uint2{k, i};
     };
-    if (in_list) {
+    if (in_list && !light) {
       for (int i = tid; i < n; i += NT) {
         const uint32_t idx = list[i].y & 0xfffffu;
-        if (order_of(list[i].x, idx) <= cut) take(list[i].x, idx);
+        if (order_of(list[i].x, idx) <= upto_here) take(list[i].x, idx);
       }
     } else {
       x.template walk<NT>(tid, [&](int i, float l) __attribute__((always_inline)) {
         const uint32_t k = key_of(l);
-        if (order_of(k, static_cast<uint32_t>(i)) <= cut) take(k, static_cast<uint32_t>(i));
+        if (order_of(k, static_cast<uint32_t>(i)) <= upto_here) take(k, static_cast<uint32_t>(i));
       });
     }
     __syncthreads();
-    if (tid == 0) {
-      q.nbest[row] = min(number[1], static_cast<uint32_t>(q.keep));
-      q.rowres[row] = Row{log_of(total), 0, r.max, g.origin, r.top, 0, 0};
+    if (light) {
+      accepted = number[1] <= static_cast<uint32_t>(z.k);  // (itself among them)
+    } else {
+      if (tid == 0) {
+        q.nbest[row] = min(number[1], static_cast<uint32_t>(q.keep));
+        q.rowres[row] = Row{log_of(total), 0, r.max, g.origin, r.top, 0, 0};
+      }
+      return;
     }
-    return;
   }
   if (tid != 0) return;
   if (q.mode == kSample) {
@@ -1600,33 +1607,13 @@ __global__ void __launch_bounds__(kRowThreads) row_kernel(const SamplingParams q
     const double lp = (static_cast<double>(drawn) - static_cast<double>(r.max)) * z.s * (kLn2D / kPerOctave) - log_of(kept);
     q.logprob[row] = lp > -0x1p-40 ? 0.0f : static_cast<float>(lp);
   } else {
-    const bool light = counting && cut == ~0ull && drafted_bin == kRest;
-    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, !accepted ? 0 : light ? kIfKept : 1, static_cast<int32_t>(token),
-                        static_cast<int32_t>(drafted)};
+    q.rowres[row] = Row{kept, cut, r.max, g.origin, r.top, accepted ? 1 : 0, static_cast<int32_t>(token)};
   }
 }
 
 // ---- verify: the sequences ------------------------------------------------------------------------
 
-// Whether top-k keeps a row's drafted token: whether fewer than k are before it (by a whole wave).  (Rare: u times the draft's
-// probability was below 2^-51.  In the row's own launch this code took 0.8 us of 64 bf16 rows of 131072 that do not need it.)
-template <int DT>
-__device__ __forceinline__ bool keeps_drafted(const SamplingParams& q, int row, int lane) {
-  const Pieces<DT> x(q.logits + row * q.stride, q.V, nullptr);
-  const int drafted = q.rowres[row].drafted, k = q.top_k ? q.top_k[row] : q.top_k_all;
-  if (drafted < 0 || drafted >= q.V) return false;  // (not of a row that was judged: sequences that do not ascend leave some out)
-  const float its = x[drafted];
-  uint32_t before = 0;
-#pragma unroll 8
-  for (int i = lane; i < q.V; i += 64) {
-    const float l = x[i];
-    before += l > its || (l == its && i < drafted);
-  }
-  return wave_sum(before) < static_cast<uint32_t>(k);
-}
-
 // The rows of sequence b: the first whose drafted token is refused, or the last (by a whole wave; -1: no rows).
-template <int DT>
 __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, int& first, int& end, int& token) {
   auto clamp = [&](int64_t v, int lo) -> int { return v < lo ? lo : v > q.rows ? q.rows : static_cast<int>(v); };
   first = clamp(q.cu[b], 0);
@@ -1636,11 +1623,7 @@ __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, 
     const int i = i0 + lane;
     const Row* const r = q.rowres + (i < end ? i : end - 1);
     const int accepted = r->accepted, its = r->token;
-    uint64_t stop = __ballot(i < end && (i + 1 == end || !accepted)), ask = __ballot(i + 1 < end && accepted == kIfKept);
-    for (; ask && (!stop || __builtin_ctzll(ask) < __builtin_ctzll(stop)); ask &= ask - 1) {  // uniform
-      const int at = __builtin_ctzll(ask);
-      if (!keeps_drafted<DT>(q, i0 + at, lane)) stop |= 1ull << at;
-    }
+    const uint64_t stop = __ballot(i < end && (i + 1 == end || !accepted));
     if (stop) {
       const int at = __builtin_ctzll(stop);
       token = __builtin_amdgcn_readlane(its, at);
@@ -1652,12 +1635,11 @@ __device__ __forceinline__ int judged(const SamplingParams& q, int b, int lane, 
 
 // The sequences, a wave each: without the draft's probabilities, and where no token is refused, the token of that row is
 // the next.
-template <int DT>
 __global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
   const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (b >= q.B) return;
   int first, end, token;
-  const int i = judged<DT>(q, b, lane, first, end, token);
+  const int i = judged(q, b, lane, first, end, token);
   if (lane != 0) return;
   q.accepted[b] = i < 0 ? 0 : i - first;
   q.token[b] = token;
@@ -1684,7 +1666,7 @@ __global__ void __launch_bounds__(256) rest_kernel(const SamplingParams q) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.x / q.rest_chunks, chunk = blockIdx.x - b * q.rest_chunks;
   int first, end, token;
-  const int row = judged<DT>(q, b, lane, first, end, token);
+  const int row = judged(q, b, lane, first, end, token);
   const bool refused = row >= 0 && row + 1 < end;  // uniform
   if (chunk == 0 && tid == 0) {
     q.accepted[b] = row < 0 ? 0 : row - first;
@@ -1889,7 +1871,7 @@ int launch(const SamplingParams& q, hipStream_t s) {
   }
   if (q.mode == kVerify) {
     if (!q.probs) {
-      verify_kernel<DT><<<static_cast<unsigned>((q.B + 3) / 4), 256, 0, s>>>(q);
+      verify_kernel<<<static_cast<unsigned>((q.B + 3) / 4), 256, 0, s>>>(q);
     } else {
       rest_kernel<DT><<<static_cast<unsigned>(q.B) * static_cast<unsigned>(q.rest_chunks), 256, 0, s>>>(q);
       redraw_kernel<DT><<<static_cast<unsigned>(q.B), 256, 0, s>>>(q);
@@ -2022,7 +2004,7 @@ extern "C" int mzk_verify(const void* logits, int dtype, int64_t T, int64_t V, i
   q.token = next;
   if (T == 0) {  // no rows: sequences of nothing
     q.probs = nullptr;
-    verify_kernel<MZK_F32><<<static_cast<unsigned>((B + 3) / 4), 256, 0, as_stream(stream)>>>(q);
+    verify_kernel<<<static_cast<unsigned>((B + 3) / 4), 256, 0, as_stream(stream)>>>(q);
     MZK_LAUNCH_CHECK("verify");
     return MZK_OK;
   }
