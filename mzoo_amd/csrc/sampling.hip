@@ -25,9 +25,9 @@
 // 28 bytes a ns that one of them loads and by its arithmetic, and four launches share the work: bins of chunks of the
 // row (survey_kernel), joined and searched (row_kernel), chunks listed (list_kernel), the selection (row_kernel).
 //
-// Measured: fp32, 1 row of 131072: 6.9 + 9.5 + 4.5 + 10.4 us in four launches, of which reading would be 0.1 us: bound
+// Measured: fp32, 1 row of 131072: 6.9 + 9.7 + 4.5 + 10.6 us in four launches, of which reading would be 0.1 us: bound
 // by dependent steps, barriers and code that is executed once.  256 rows of 200019, with top-k, top-p and min-p by
-// turns: 105 us a call: the first reading 58, at 3.5 TB/s near what memory gives (4.0), the second 23, from the caches.  bf16, 64
+// turns: 106 us a call: the first reading 58, at 3.5 TB/s near what memory gives (4.0), the second 23, from the caches.  bf16, 64
 // rows of 131072: 43.5 us, of which the count 12.3 and the second reading 6.5; 160 drafted rows: 49.  fp16, 16 rows of 32000: 22 us.
 #include "common.h"
 #include "sampling_numbers.h"
