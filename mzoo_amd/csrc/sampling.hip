@@ -1656,13 +1656,15 @@ __global__ void __launch_bounds__(256) verify_kernel(const SamplingParams q) {
   q.token[b] = token;
 }
 
-// What the target has above the draft at token i, 2^52 a probability of 1.
+// What the target has above the draft at token i, 2^52 a probability of 1.  (Of tokens too light for the sums, a unit or two at most; nothing where
+// top-k may end among them, whose place nobody knows.)
 template <int DT>
 __device__ __forceinline__ uint64_t above(const SamplingParams& q, const Settings& z, const Row& r, int row, float l, int i) {
   constexpr int KS = DT == MZK_F32 ? 0 : DT == MZK_BF16 ? 16 : 13;
   const uint64_t me = static_cast<uint64_t>(key_of(l) >> KS) << 20 | static_cast<uint32_t>(i);
   if (!(l > -__builtin_huge_valf()) || me > r.cut || (static_cast<double>(l) - static_cast<double>(r.max)) * z.s < z.f) return 0;
-  const double t = Grid{r.origin, z.s}.place(l) - static_cast<double>(r.top);
+  const double place = Grid{r.origin, z.s}.place(l), t = place - static_cast<double>(r.top);
+  if (r.cut == ~0ull && z.k > 0 && static_cast<double>(r.top) - __builtin_rint(place) >= static_cast<double>(kRest)) return 0;
   const double p = exp2_of(t / kPerOctave) * __builtin_ldexp(1.0, q.scale) / r.kept;
   const double d = p - static_cast<double>(fmaxf(q.probs[row * q.probs_stride + i], 0.0f));
   return d > 0.0 ? static_cast<uint64_t>(d * 0x1p52) : 0;

@@ -104,6 +104,30 @@ def test_verify_top_k_ends_among_light_tokens(dev, dtype, v, sequences, chunks, 
         assert (acc[b], nxt[b]) == (0, token), f"sequence {b}: place {at[b]} of {k[2 * b]} kept ones: {acc[b]}, {nxt[b]}"
 
 
+@pytest.mark.parametrize("dtype,v,sequences,chunks", [
+    (torch.float32, 1000, 6, False), (torch.float32, 9001, 80, False), (torch.float32, 70001, 8, True), (torch.float16, 700, 6, False),
+    (torch.float16, 70001, 8, True), (torch.bfloat16, 700, 6, False), (torch.bfloat16, 70001, 8, True), (torch.bfloat16, 20001, 80, False),
+    (torch.bfloat16, 131072, 80, False)])
+def test_verify_nothing_above_the_draft_but_light_tokens(dev, dtype, v, sequences, chunks):
+    """One token holds the sum; the others are each 1 to 2 units of what a target has above a draft, and top-k keeps some of them, of which
+    the draft is sure: what is left is nothing, and the next token is the one that holds the sum."""
+    assert _in_chunks(2 * sequences, v, dtype) == chunks
+    light = -35.5                                     # e^-35.5 = 1.72 2^-52: below what is counted, above 2^-52
+    x = torch.full((2 * sequences, v), light)
+    x[:, 7] = 0.0
+    order = torch.argsort(-x[0], stable=True)
+    k = torch.tensor([2, 3, 40, 500])[torch.arange(2 * sequences) // 2 % 4].int()
+    q = torch.zeros(2 * sequences, v)
+    for row in range(2 * sequences):
+        q[row, order[:k[row]]] = 1.0
+    tokens = torch.full((2 * sequences,), v)          # no token: refused
+    cu = torch.arange(0, 2 * sequences + 1, 2)
+    u, draw = torch.rand(2 * sequences, generator=torch.Generator().manual_seed(v)), torch.rand(sequences, generator=torch.Generator().manual_seed(v + 1))
+    acc, nxt = sampling.verify(x.to(dtype).to(dev), tokens.to(dev), cu.to(dev), u.to(dev), draw.to(dev), draft_probs=q.to(dev), top_k=k.to(dev))
+    assert acc.tolist() == [0] * sequences
+    assert nxt.tolist() == [7] * sequences
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("probs", [False, True])
 def test_verify_light_tokens_one_after_another(dev, dtype, probs):
